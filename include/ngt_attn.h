@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define NGT_ABI_VERSION 11
+#define NGT_ABI_VERSION 12
 
 #define NGT_F32 0
 #define NGT_BF16 1
@@ -430,6 +430,84 @@ int ngt_adj_weights_workspace_bytes(int64_t n_entries, int64_t n_nodes, size_t* 
 int ngt_adj_weights(const int64_t* edge_index, const float* ppr_val, int64_t n_entries,
                     int64_t n_nodes, int32_t* xadj, int32_t* adjncy, int32_t* eweights,
                     int64_t* info, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Attention over packed windows: n_windows sequences of different lengths back
+ * to back, q [n_q, H, d] and k, v [n_k, H_kv, d] in NGT_F32 or NGT_BF16, d a
+ * multiple of 8 up to 128, H a multiple of H_kv (query head h reads key head
+ * h / (H / H_kv)).  Per window and head, over its own rows:
+ *   S = scale q k^T (+ table[bucket(i, j)][h]);  out = softmax_j(S) v
+ * causal: query i sees the keys j <= i + (keys - queries) of its window.
+ * A query that sees no key gets a zero row and gives no gradient.  q, k and v
+ * may have rows further apart than heads * d: *_stride is in elements, rows
+ * 16-byte aligned.  Values of unseen keys enter with weight 0, so they must be
+ * finite where any query of their window is not to see a NaN.
+ *
+ * The plan.  ngt_packed_plan writes the windows' offsets and work lists for
+ * ngt_packed_plan_bytes bytes at device, which the caller then copies there
+ * from host, and fills *out (host memory; its pointers point into device).
+ * Lengths are host arrays, 0 <= length <= 2^30.  Neither call touches the GPU.
+ *
+ * The bias.  table [n_buckets, H] has the element type of q, 1 <= n_buckets
+ * <= 255.  ngt_packed_buckets lays the pairs' bucket ids out once for all
+ * heads, layers and steps: ids holds the windows' [queries, keys] matrices
+ * back to back (n_pairs elements of 1 (unsigned), 4 or 8 bytes (signed)),
+ * buckets_q and buckets_k take bucket_bytes_q and bucket_bytes_k bytes,
+ * 16-byte aligned.  A pair whose id is not in [0, n_buckets) is not seen.
+ * Table entries may be -infinity (never seen) or the type's lowest value (seen
+ * where nothing greater is).
+ *
+ * out_f32 and lse [H, n_q] (log2 units) are what the backward needs (both
+ * nullable in a forward without one): out again in fp32, and each row's
+ * softmax statistic.  The backward writes grad_q [n_q, H, d], grad_k and
+ * grad_v [n_k, H_kv, d] and, where grad_table is not null, grad_table
+ * [n_buckets, H]; grad_out is contiguous.  All sums are fp32 in a fixed order.
+ * workspace: ngt_packed_workspace_bytes with the same dtype, windows and heads;
+ * n_buckets there is the table's for a backward that writes grad_table, else 0.
+ */
+typedef struct ngt_packed_windows {
+  int32_t n_windows;
+  int32_t causal;
+  int32_t max_q; /* longest window, queries and keys */
+  int32_t max_k;
+  int64_t n_q;
+  int64_t n_k;
+  int64_t n_pairs;
+  int64_t bucket_bytes_q;
+  int64_t bucket_bytes_k;
+  const int64_t* q_start; /* [n_windows + 1] each, device */
+  const int64_t* k_start;
+  const int64_t* p_start;
+  const int64_t* b_start;
+  const int64_t* bt_start;
+  const int32_t* items_q[3]; /* {window, first row} of blocks of 32, 64 and 128 rows, device */
+  const int32_t* items_k[3];
+  int32_t n_items_q[3];
+  int32_t n_items_k[3];
+} ngt_packed_windows;
+
+int ngt_packed_plan_bytes(int32_t n_windows, const int32_t* q_len, const int32_t* k_len,
+                          size_t* bytes);
+int ngt_packed_plan(int32_t n_windows, const int32_t* q_len, const int32_t* k_len, int32_t causal,
+                    void* host, size_t bytes, void* device, ngt_packed_windows* out);
+int ngt_packed_buckets(const ngt_packed_windows* windows, const void* ids, int32_t id_bytes,
+                       uint8_t* buckets_q, uint8_t* buckets_k, void* stream);
+int ngt_packed_workspace_bytes(int dtype, const ngt_packed_windows* windows, int32_t n_heads,
+                               int32_t n_kv_heads, int32_t head_dim, int32_t n_buckets,
+                               size_t* fwd_bytes, size_t* bwd_bytes);
+int ngt_packed_fwd(int dtype, const void* q, const void* k, const void* v, int64_t q_stride,
+                   int64_t k_stride, int64_t v_stride, const ngt_packed_windows* windows,
+                   int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, float scale,
+                   const void* table, int32_t n_buckets, const uint8_t* buckets_q, void* out,
+                   float* out_f32, float* lse, void* workspace, size_t workspace_bytes,
+                   void* stream);
+int ngt_packed_bwd(int dtype, const void* q, const void* k, const void* v, int64_t q_stride,
+                   int64_t k_stride, int64_t v_stride, const float* out_f32, const void* grad_out,
+                   const float* lse, const ngt_packed_windows* windows, int32_t n_heads,
+                   int32_t n_kv_heads, int32_t head_dim, float scale, const void* table,
+                   int32_t n_buckets, const uint8_t* buckets_q, const uint8_t* buckets_k,
+                   void* grad_q, void* grad_k, void* grad_v, void* grad_table, void* workspace,
+                   size_t workspace_bytes, void* stream);
 
 /*
  * Row gather dst[r, :] = src[idx[r], :] for r < n_rows (row_bytes a multiple

@@ -7,6 +7,8 @@ install(model)           swap a model's local_attn modules for CoreAttention
 sparse_attention(...)    functional masked attention over a window edge_index
 window_attention(...)    the same over a built WindowAdjacency (C++ autograd node)
 dense_attention(...)     functional full-window attention
+packed_attention(...)    attention over a PackedWindows batch (grouped heads, causal, bucket bias)
+PackedWindows            plan of windows of different lengths back to back
 WindowAdjacency          device CSR/transposed CSR/work lists of one window
 """
 from .attention import (CoreAttention, DenseAttentionBiasFunction, DenseAttentionFunction,
@@ -14,6 +16,7 @@ from .attention import (CoreAttention, DenseAttentionBiasFunction, DenseAttentio
                         dense_attention_bias, install, sparse_attention, window_attention)
 from .csr import (AdjacencyCache, WindowAdjacency, chunk_for_heads, default_cache, pack_q_adaptive,
                   small_for_heads)
+from .packed import PackedAttentionFunction, PackedWindows, PairBuckets, packed_attention
 
 __all__ = [
     "CoreAttention",
@@ -26,6 +29,10 @@ __all__ = [
     "DenseAttentionFunction",
     "DenseAttentionBiasFunction",
     "dense_attention_bias",
+    "packed_attention",
+    "PackedAttentionFunction",
+    "PackedWindows",
+    "PairBuckets",
     "WindowAdjacency",
     "AdjacencyCache",
     "chunk_for_heads",

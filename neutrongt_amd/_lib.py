@@ -13,7 +13,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libngt_attn.so"
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 NGT_F32 = 0
 NGT_BF16 = 1
@@ -79,11 +79,37 @@ class WindowCSR(C.Structure):
     ]
 
 
+class PackedWindowsC(C.Structure):
+    """Mirror of ``ngt_packed_windows``."""
+
+    _fields_ = [
+        ("n_windows", C.c_int32),
+        ("causal", C.c_int32),
+        ("max_q", C.c_int32),
+        ("max_k", C.c_int32),
+        ("n_q", C.c_int64),
+        ("n_k", C.c_int64),
+        ("n_pairs", C.c_int64),
+        ("bucket_bytes_q", C.c_int64),
+        ("bucket_bytes_k", C.c_int64),
+        ("q_start", C.c_void_p),
+        ("k_start", C.c_void_p),
+        ("p_start", C.c_void_p),
+        ("b_start", C.c_void_p),
+        ("bt_start", C.c_void_p),
+        ("items_q", C.c_void_p * 3),
+        ("items_k", C.c_void_p * 3),
+        ("n_items_q", C.c_int32 * 3),
+        ("n_items_k", C.c_int32 * 3),
+    ]
+
+
 _i32, _i64, _f32, _vp, _sz = C.c_int32, C.c_int64, C.c_float, C.c_void_p, C.c_size_t
 _u64 = C.c_uint64
 _pi32 = C.POINTER(C.c_int32)
 _psz = C.POINTER(C.c_size_t)
 _pcsr = C.POINTER(WindowCSR)
+_ppw = C.POINTER(PackedWindowsC)
 
 # name -> argtypes (restype is int unless listed in _RESTYPES)
 SIGNATURES = {
@@ -123,6 +149,14 @@ SIGNATURES = {
                       _vp, _vp, _vp, _vp, _sz, _vp],
     "ngt_dense_bwd": [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _f32, _f32,
                       _u64, _vp, _vp, _vp, _vp, _vp, _sz, _vp],
+    "ngt_packed_plan_bytes": [_i32, _vp, _vp, _psz],
+    "ngt_packed_plan": [_i32, _vp, _vp, _i32, _vp, _sz, _vp, _ppw],
+    "ngt_packed_buckets": [_ppw, _vp, _i32, _vp, _vp, _vp],
+    "ngt_packed_workspace_bytes": [_i32, _ppw, _i32, _i32, _i32, _i32, _psz, _psz],
+    "ngt_packed_fwd": [_i32, _vp, _vp, _vp, _i64, _i64, _i64, _ppw, _i32, _i32, _i32, _f32, _vp,
+                       _i32, _vp, _vp, _vp, _vp, _vp, _sz, _vp],
+    "ngt_packed_bwd": [_i32, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _ppw, _i32, _i32,
+                       _i32, _f32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp],
     "ngt_layernorm_fwd": [_i32, _vp, _i64, _i32, _vp, _vp, _f32, _i32, _vp, _vp, _vp, _vp],
     "ngt_layernorm_bwd_workspace_bytes": [_i64, _i32, _psz],
     "ngt_layernorm_bwd": [_i32, _vp, _i32, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,

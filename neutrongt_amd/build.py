@@ -45,6 +45,8 @@ HIPCC_FLAGS = [
 FILE_FLAGS = {
     "ngt_dense_mfma.hip": ["-fno-honor-nans", "-mno-amdgpu-ieee"],
     "ngt_dense_fx.hip": ["-fno-honor-nans", "-mno-amdgpu-ieee"],
+    "ngt_packed.hip": ["-fno-honor-nans", "-mno-amdgpu-ieee"],
+    "ngt_packed_bwd.hip": ["-fno-honor-nans", "-mno-amdgpu-ieee"],
 }
 
 

@@ -1,0 +1,273 @@
+// Tiles of the packed-window attention: 64 (or 32) rows of one head in LDS,
+// read both as rows and as columns by the 32 x 32 matrix instructions.
+//
+// Lane layouts of the instructions (half = lane / 32, l = lane % 32):
+//   D (32 x 32): lane holds D[8*(i/4) + 4*half + i%4][l], i < 16
+//   bf16, K = 16: lane holds A[l][8*half + e] and B[8*half + e][l], e < 8
+//   fp32, K = 2:  lane holds A[l][half] and B[half][l]
+// A contraction may take its indices in any order as long as A and B agree,
+// and the rows of A may be any 32 rows of the tile.  Both freedoms are used:
+//  * row m of A is tile row 32t + 16*((m/4)%2) + 4*(m/8) + m%4, so that a lane
+//    holds the scores of 16 CONSECUTIVE tile rows 32t + 16*half + i: its 16
+//    bucket ids are one 16-byte load, and
+//  * registers 8c .. 8c+7 of such a score tile are the B operand of K step c of
+//    the next product as they are; its A operand is columns of the same tile
+//    rows 32t + 16*half + 8c + e, which ds_read_b64_tr_b16 reads out of the
+//    row-major tile (bf16) or plain 4-byte reads do (fp32: K = 2, one register
+//    a step).
+// So one copy of a tile in LDS serves Q K^T, P V and every product of the
+// backward, and no score leaves the registers.
+//
+// The 16-byte pieces of a row are permuted by tile_swz(row): the 8 lanes that
+// a 16-byte read serves at once (rows r .. r+3 and r+16 .. r+19, one piece)
+// and the 16 lanes of an 8-byte column read (4 rows, two pieces) fall on
+// distinct banks, without padding.
+#pragma once
+
+#include "ngt_common.h"
+
+namespace ngt {
+namespace packed {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// Work-item and work-group ids as register reads: with the IEEE mode bit off
+// (see build.py) the functions behind threadIdx and blockIdx are not inlined.
+__device__ __forceinline__ int tid_x() { return static_cast<int>(__builtin_amdgcn_workitem_id_x()); }
+__device__ __forceinline__ int wg_x() { return static_cast<int>(__builtin_amdgcn_workgroup_id_x()); }
+
+__device__ __forceinline__ f32x16 fill16(float v) {
+  f32x16 r;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) r[i] = v;
+  return r;
+}
+
+// c += A B over one 32-byte chunk of both rows: 16 bf16 or 8 fp32 elements.
+template <typename T>
+__device__ __forceinline__ f32x16 mma_rows(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (sizeof(T) == 2) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0,
+                                               0, 0);
+    return c;
+  }
+}
+
+// The two wave halves' values of a row, joined: v_permlane32_swap leaves the
+// lower half's value in r[0] and the upper half's in r[1] of both.
+__device__ __forceinline__ float max_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// DP: the head size rounded up to 32, 64 or 128; T: float or bf16_t.
+template <typename T, int DP>
+struct Tile {
+  static constexpr int kEs = static_cast<int>(sizeof(T));
+  static constexpr int kPitch = DP * kEs;     // bytes of a row
+  static constexpr int kPieces = kPitch / 16;  // 16-byte pieces of a row
+  static constexpr int kChunks = kPitch / 32;  // mma_rows steps of a row
+  static constexpr int kCols = DP / 32;        // 32-column blocks of a row
+
+  __device__ static __forceinline__ int swz(int row) {
+    if constexpr (kPieces == 4)
+      return (((row >> 1) & 1) << 1) | ((row >> 4) & 1);
+    else
+      return ((row & 3) << 1) | ((row >> 4) & 1);
+  }
+  __device__ static __forceinline__ int offset(int row, int piece) {
+    return row * kPitch + ((piece ^ swz(row)) << 4);
+  }
+  // Row operand A of rows 32t ..: lane l's row (without 32t).
+  __device__ static __forceinline__ int a_row(int l) {
+    return 16 * ((l >> 2) & 1) + 4 * (l >> 3) + (l & 3);
+  }
+  __device__ static __forceinline__ u32x4 load_a(const char* tile, int t, int c, int l, int half) {
+    return *reinterpret_cast<const u32x4*>(tile + 32 * t * kPitch + offset(a_row(l), 2 * c + half));
+  }
+
+  // acc[dt] (rows = columns 32dt .. of the tile) += tile^T p over tile rows
+  // 32t .. 32t+31, p the lane's 16 values of those rows.
+  __device__ static __forceinline__ void mma_cols(const char* tile, int t, const f32x16& p,
+                                                  f32x16 (&acc)[kCols], int lane) {
+    const int half = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      const int j = lane & 15;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        u32x4 b;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = pack2_bf16(p[8 * c + 2 * e], p[8 * c + 2 * e + 1]);
+        // rows 4-aligned + j / 4: swz() depends on the lane alone
+        const int row = 16 * half + (j >> 2);
+        const int piece = 2 * ((lane >> 4) & 1) + ((j & 3) >> 1);
+        const int at = (piece ^ swz(row)) * 16 + 8 * (j & 1) + row * kPitch;
+#pragma unroll
+        for (int dt = 0; dt < kCols; ++dt) {
+          // pieces 4 further on: bit 2 of the piece flips with dt's low bit
+          const int off = (kPieces > 4 ? (at ^ ((dt & 1) << 6)) + (dt >> 1) * 128 : at) +
+                          (32 * t + 8 * c) * kPitch;
+          typedef __attribute__((address_space(3))) s16x4* lds4_t;
+          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(tile + off));
+          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(tile + off + 4 * kPitch));
+          const uint2 lw = __builtin_bit_cast(uint2, lo), hw = __builtin_bit_cast(uint2, hi);
+          const u32x4 a = {lw.x, lw.y, hw.x, hw.y};
+          acc[dt] = mma_rows<T>(a, b, acc[dt]);
+        }
+      }
+    } else {
+      const int l = lane & 31;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int row = 16 * half + i;
+#pragma unroll
+        for (int dt = 0; dt < kCols; ++dt) {
+          const float a = *reinterpret_cast<const float*>(
+              tile + 32 * t * kPitch + offset(row, 8 * dt + (l >> 2)) + 4 * (l & 3));
+          acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[i], acc[dt], 0, 0, 0);
+        }
+      }
+    }
+  }
+};
+
+// A lane's row of one head as the chunks it supplies to mma_rows: 16 bytes at
+// 32c + 16*half, zero behind the row's d elements or where the row is not there.
+template <typename T, int DP>
+struct RowFrag {
+  static constexpr int NC = Tile<T, DP>::kChunks;
+  u32x4 w[NC];
+  __device__ __forceinline__ void load(const T* __restrict__ row, bool ok, int d, int half) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      w[c] = u32x4{0u, 0u, 0u, 0u};
+      if (ok && 32 * c + 16 * half < d * static_cast<int>(sizeof(T)))
+        w[c] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(row) + 32 * c +
+                                               16 * half);
+    }
+  }
+};
+
+// The 16-byte pieces of ROWS rows of one head that one of N threads moves from
+// memory to an LDS tile; rows behind the window's end and columns behind d are zero.
+template <typename T, int DP, int ROWS, int N>
+struct Stage {
+  using L = Tile<T, DP>;
+  static constexpr int NV = (ROWS * L::kPieces) / N;
+  static_assert(NV * N == ROWS * L::kPieces, "whole pieces per thread");
+  u32x4 w[NV];
+  __device__ __forceinline__ static u32x4 piece(const T* __restrict__ base, int64_t stride, int row0,
+                                                int n_rows, int d, int e) {
+    const int r = e / L::kPieces, p = e % L::kPieces;
+    u32x4 x = {0u, 0u, 0u, 0u};
+    if (row0 + r < n_rows && 16 * p < d * L::kEs)
+      x = *reinterpret_cast<const u32x4*>(
+          reinterpret_cast<const char*>(base) + int64_t(row0 + r) * stride + 16 * p);
+    return x;
+  }
+  __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, int n_rows, int d,
+                                       int tid) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) w[i] = piece(base, stride, row0, n_rows, d, tid + i * N);
+  }
+  __device__ __forceinline__ void store(char* tile, int tid) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = tid + i * N;
+      *reinterpret_cast<u32x4*>(tile + L::offset(e / L::kPieces, e % L::kPieces)) = w[i];
+    }
+  }
+};
+
+// 4 consecutive values of a row.
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
+  if constexpr (sizeof(T) == 2)
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack2_bf16(a, b), pack2_bf16(c, d));
+  else
+    *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+}
+
+// Bucket ids of a lane's 16 tile rows, and the bias table of one head in LDS:
+// entries in log2 units, -inf (not attended) behind the n_buckets there are.
+// Finite entries stay finite: a table of the type's lowest values still gives
+// every pair the same weight instead of none.
+constexpr int kTable = 256;
+template <typename T>
+__device__ __forceinline__ void load_table(float* tab, const T* __restrict__ table, int n_buckets,
+                                           int n_heads, int h, int tid, int n_threads) {
+  for (int b = tid; b < kTable; b += n_threads) {
+    float x = -INFINITY;
+    if (b < n_buckets) {
+      x = elem<T>::load(table + int64_t(b) * n_heads + h);
+      const uint32_t mag = __float_as_uint(x) & 0x7fffffffu;
+      if (mag < 0x7f800000u) x = fminf(fmaxf(x * kLog2e, -3.0e38f), 3.0e38f);
+    }
+    tab[b] = x;
+  }
+}
+__device__ __forceinline__ int bucket_of(const u32x4& ids, int i) {
+  return static_cast<int>((ids[i >> 2] >> (8 * (i & 3))) & 255u);
+}
+
+}  // namespace packed
+}  // namespace ngt
+
+namespace ngt {
+namespace packed {
+
+// ------------------------------------------------------- the backward's launch
+struct BwdArgs {
+  const int64_t* q_start;
+  const int64_t* k_start;
+  const int64_t* b_start;
+  const int64_t* bt_start;
+  const int2* items;
+  int n_items;
+  int H, Hkv, d, causal, n_buckets;
+  float scale;
+  int64_t sq, sk, sv;  // bytes between rows
+  int64_t n_q;
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* go;
+  const float* out32;
+  const float* lse;
+  float* dsum;  // [H, n_q]: written by the dQ pass, read by the dK/dV pass
+  const void* table;
+  const uint8_t* ids;
+  const uint8_t* ids_t;
+  float* part_table;  // [H, items, n_buckets]
+  void* gq;
+  void* gk;
+  void* gv;
+  void* grad_table;
+};
+struct BwdPlan {
+  const int2* items_q;
+  const int2* items_k;
+  int n_items_q, dq_waves, dkv_waves;
+  int64_t dq_blocks, dkv_blocks;
+};
+int packed_bwd(int dtype, const BwdPlan& p, const BwdArgs& a, hipStream_t st);
+
+}  // namespace packed
+}  // namespace ngt

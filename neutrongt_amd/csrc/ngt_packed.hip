@@ -1,0 +1,841 @@
+// Attention over packed windows: sequences of different lengths back to back,
+// grouped heads, causal order, a learned bias per pair bucket.  Forward.
+#include "ngt_packed.h"
+
+#include <string.h>
+
+#include <algorithm>
+#include <new>
+#include <vector>
+
+namespace ngt {
+namespace packed {
+namespace {
+
+constexpr int kKeys = 64;       // keys of one stage
+constexpr float kRebase = 8.f;  // weights stay below 2^8 of a row's base
+
+struct FwdArgs {
+  const int64_t* q_start;
+  const int64_t* k_start;
+  const int64_t* b_start;
+  const int2* items;
+  int H, Hkv, d, causal, n_buckets;
+  float scale;
+  int64_t sq, sk, sv;  // bytes between rows
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* table;
+  const uint8_t* ids;
+  void* out;
+  float* out32;
+  float* lse;  // [H, n_q], log2 units; +inf for a row that attends to nothing
+  int64_t n_q;
+};
+
+// One online-softmax step of a lane's row over its 16 * NT scores x (log2
+// units times 1 / c2): the weights are exp2((x - m) c2).  The base m moves
+// only when some row exceeds it by more than kRebase, so that most tiles
+// rescale nothing; weights and sums share the base, so this is exact.
+template <int NT, int NC>
+__device__ __forceinline__ void softmax_step(f32x16 (&x)[NT], float c2, float step, float& m,
+                                             float& thr, float& l, f32x16 (&acc)[NC]) {
+  float mx = x[0][0];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[t][i]);
+  if (__any(mx > thr)) {  // thr: -inf before a row's first key, m + step after it
+    const float up = fmaxf(m, max_halves(mx));
+    const float f = up == m ? 1.f : __builtin_amdgcn_exp2f((m - up) * c2);
+    m = up;
+    thr = m == -INFINITY ? m : m + step;
+    l *= f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[c][i] *= f;
+  }
+  const float base = m == -INFINITY ? 0.f : m * c2;
+  float s = 0.f;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      x[t][i] = __builtin_amdgcn_exp2f(fmaf(x[t][i], c2, -base));
+      s += x[t][i];
+    }
+  l += s;
+}
+
+// One block: NW * 32 query rows of one window and head, a wave 32 of them; the
+// window's keys pass through LDS 64 at a time.
+template <typename T, int DP, bool BIAS, int NW>
+__global__ __launch_bounds__(64 * NW) void k_packed_fwd(FwdArgs a) {
+  using L = Tile<T, DP>;
+  constexpr int N = 64 * NW;
+  // registers for the next stage's pieces, where they are few enough
+  constexpr bool kAhead = (kKeys * L::kPieces / N) * 8 <= 64;
+  __shared__ __align__(16) char ks[kKeys * L::kPitch];
+  __shared__ __align__(16) char vs[kKeys * L::kPitch];
+  __shared__ float tab[BIAS ? kTable : 1];
+  const int tid = tid_x(), lane = tid & 63, wave = tid >> 6, half = lane >> 5, l32 = lane & 31;
+  // the heads that share K and V follow each other H_kv blocks apart: with 8
+  // key heads all blocks of one of them run on one XCD, whose L2 holds them
+  const int bid = wg_x();
+  const int kvh = bid % a.Hkv, grp = (bid / a.Hkv) % (a.H / a.Hkv);
+  const int h = kvh * (a.H / a.Hkv) + grp;
+  const int2 item = a.items[bid / a.H];
+  const int64_t q0 = a.q_start[item.x], k0 = a.k_start[item.x];
+  const int nq = static_cast<int>(a.q_start[item.x + 1] - q0);
+  const int nk = static_cast<int>(a.k_start[item.x + 1] - k0);
+  const int ahead = nk - nq;
+  const int qi = item.y + wave * 32 + l32;  // this lane's query
+  const int qc = min(qi, nq - 1);
+  const int lim = a.causal ? min(qc + ahead, nk - 1) : nk - 1;  // its last key
+  const int first_lim = a.causal ? min(item.y + wave * 32 + ahead, nk - 1) : nk - 1;
+  const int last_q = min(item.y + wave * 32 + 31, nq - 1);
+  const int wave_end = item.y + wave * 32 >= nq ? 0 : a.causal ? min(last_q + ahead + 1, nk) : nk;
+  const int block_end = a.causal ? min(min(item.y + 32 * NW, nq) + ahead, nk) : nk;
+  const T* kb = reinterpret_cast<const T*>(reinterpret_cast<const char*>(a.k) + k0 * a.sk) +
+                int64_t(kvh) * a.d;
+  const T* vb = reinterpret_cast<const T*>(reinterpret_cast<const char*>(a.v) + k0 * a.sv) +
+                int64_t(kvh) * a.d;
+  RowFrag<T, DP> q;
+  q.load(reinterpret_cast<const T*>(reinterpret_cast<const char*>(a.q) + (q0 + qc) * a.sq) +
+             int64_t(h) * a.d,
+         qi < nq, a.d, half);
+  const uint8_t* ids = nullptr;
+  if constexpr (BIAS) {
+    load_table(tab, reinterpret_cast<const T*>(a.table), a.n_buckets, a.H, h, tid, N);
+    ids = a.ids + a.b_start[item.x] + int64_t(qc) * ((nk + 63) & ~63) + 16 * half;
+  }
+  const float s2 = a.scale * kLog2e;
+  const float c2 = BIAS ? 1.f : s2;
+  const float step = kRebase / c2;
+  float m = -INFINITY, thr = -INFINITY, l = 0.f;
+  f32x16 acc[L::kCols];
+#pragma unroll
+  for (int c = 0; c < L::kCols; ++c) acc[c] = fill16(0.f);
+
+  Stage<T, DP, kKeys, N> pk, pv;
+  u32x4 idw[2];
+  if constexpr (kAhead) {
+    pk.load(kb, a.sk, 0, nk, a.d, tid);
+    pv.load(vb, a.sv, 0, nk, a.d, tid);
+  }
+  for (int kt = 0; kt < block_end; kt += kKeys) {
+    if constexpr (BIAS) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) idw[t] = *reinterpret_cast<const u32x4*>(ids + kt + 32 * t);
+    }
+    __syncthreads();
+    if constexpr (!kAhead) {
+      pk.load(kb, a.sk, kt, nk, a.d, tid);
+      pk.store(ks, tid);
+      pv.load(vb, a.sv, kt, nk, a.d, tid);
+      pv.store(vs, tid);
+    } else {
+      pk.store(ks, tid);
+      pv.store(vs, tid);
+    }
+    __syncthreads();
+    if constexpr (kAhead) {
+      if (kt + kKeys < block_end) {
+        pk.load(kb, a.sk, kt + kKeys, nk, a.d, tid);
+        pv.load(vb, a.sv, kt + kKeys, nk, a.d, tid);
+      }
+    }
+    if (kt >= wave_end) continue;
+    f32x16 x[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      x[t] = fill16(0.f);
+#pragma unroll
+      for (int c = 0; c < L::kChunks; ++c)
+        x[t] = mma_rows<T>(L::load_a(ks, t, c, l32, half), q.w[c], x[t]);
+      if constexpr (BIAS) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[t][i] = fmaf(x[t][i], s2, tab[bucket_of(idw[t], i)]);
+      }
+    }
+    if (kt + kKeys - 1 > first_lim) {  // some key of the tile is behind some row's last one
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (kt + 32 * t + 16 * half + i > lim) x[t][i] = -INFINITY;
+    }
+    softmax_step<2>(x, c2, step, m, thr, l, acc);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) L::mma_cols(vs, t, x[t], acc, lane);
+  }
+
+  l = sum_halves(l);
+  if (qi < nq) {
+    const float r = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+    T* o = reinterpret_cast<T*>(a.out) + ((q0 + qi) * a.H + h) * int64_t(a.d);
+    float* o32 = a.out32 ? a.out32 + ((q0 + qi) * a.H + h) * int64_t(a.d) : nullptr;
+#pragma unroll
+    for (int c = 0; c < L::kCols; ++c)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int at = 32 * c + 8 * g + 4 * half;
+        if (at < a.d) {
+          store4(o + at, acc[c][4 * g] * r, acc[c][4 * g + 1] * r, acc[c][4 * g + 2] * r,
+                 acc[c][4 * g + 3] * r);
+          if (o32)
+            store4(o32 + at, acc[c][4 * g] * r, acc[c][4 * g + 1] * r, acc[c][4 * g + 2] * r,
+                   acc[c][4 * g + 3] * r);
+        }
+      }
+    if (a.lse && half == 0)
+      a.lse[int64_t(h) * a.n_q + q0 + qi] = l == 0.f ? INFINITY : m * c2 + __builtin_amdgcn_logf(l);
+  }
+}
+
+// ------------------------------------------------------- a few rows per window
+struct FewArgs {
+  FwdArgs f;
+  int splits;
+  float* part_ml;   // [windows * H_kv, splits, 32, 2]: base (log2 units) and sum
+  float* part_acc;  // [windows * H_kv, splits, 32, DP]
+};
+
+// The rows of one window and key head: row r is query r % nq of the group's
+// head r / nq.  One block: the keys of one split, each wave its own tiles of
+// 32 keys straight from memory (nothing is shared between waves but the end).
+template <typename T, int DP, bool BIAS>
+__global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
+  using L = Tile<T, DP>;
+  const FwdArgs& a = fa.f;
+  constexpr int kTileBytes = 32 * L::kPitch;
+  constexpr int kJoin = 36;  // floats per row of the join's buffer
+  constexpr int kBytes = 4 * kTileBytes > 4 * 32 * kJoin * 4 ? 4 * kTileBytes : 4 * 32 * kJoin * 4;
+  __shared__ __align__(16) char buf[kBytes];
+  __shared__ float ml[4][32][2];
+  extern __shared__ float tabs[];  // [group][kTable] with a bias
+  const int tid = tid_x(), lane = tid & 63, wave = tid >> 6, half = lane >> 5, l32 = lane & 31;
+  const int bid = wg_x();
+  const int kvh = bid % a.Hkv, split = (bid / a.Hkv) % fa.splits, w = bid / (a.Hkv * fa.splits);
+  const int G = a.H / a.Hkv;
+  const int64_t q0 = a.q_start[w], k0 = a.k_start[w];
+  const int nq = static_cast<int>(a.q_start[w + 1] - q0);
+  const int nk = static_cast<int>(a.k_start[w + 1] - k0);
+  if (nq == 0) return;
+  const int rows = nq * G;
+  const int r = min(l32, rows - 1), grp = r / nq, qi = r - grp * nq, h = kvh * G + grp;
+  const int lim = a.causal ? min(qi + nk - nq, nk - 1) : nk - 1;
+  const int first_lim = a.causal ? min(nk - nq, nk - 1) : nk - 1;
+  const int tiles = (nk + 31) >> 5;
+  const int t_begin = static_cast<int>(int64_t(tiles) * split / fa.splits);
+  const int t_end = static_cast<int>(int64_t(tiles) * (split + 1) / fa.splits);
+  const T* kb = reinterpret_cast<const T*>(reinterpret_cast<const char*>(a.k) + k0 * a.sk) +
+                int64_t(kvh) * a.d;
+  const T* vb = reinterpret_cast<const T*>(reinterpret_cast<const char*>(a.v) + k0 * a.sv) +
+                int64_t(kvh) * a.d;
+  RowFrag<T, DP> q;
+  q.load(reinterpret_cast<const T*>(reinterpret_cast<const char*>(a.q) + (q0 + qi) * a.sq) +
+             int64_t(h) * a.d,
+         l32 < rows, a.d, half);
+  const uint8_t* ids = nullptr;
+  const float* tab = nullptr;
+  if constexpr (BIAS) {
+    for (int g = 0; g < G; ++g)
+      load_table(tabs + g * kTable, reinterpret_cast<const T*>(a.table), a.n_buckets, a.H,
+                 kvh * G + g, tid, 256);
+    ids = a.ids + a.b_start[w] + int64_t(qi) * ((nk + 63) & ~63) + 16 * half;
+    tab = tabs + grp * kTable;
+    __syncthreads();
+  }
+  const float s2 = a.scale * kLog2e;
+  const float c2 = BIAS ? 1.f : s2;
+  const float step = kRebase / c2;
+  float m = -INFINITY, thr = -INFINITY, l = 0.f;
+  f32x16 acc[L::kCols];
+#pragma unroll
+  for (int c = 0; c < L::kCols; ++c) acc[c] = fill16(0.f);
+  char* vs = buf + wave * kTileBytes;
+
+  Stage<T, DP, 32, 64> pv;
+  RowFrag<T, DP> pk;
+  u32x4 idw = {0u, 0u, 0u, 0u};
+  const int a_row = L::a_row(l32);
+  auto fetch = [&](int t) {
+    const int kt = 32 * t;
+    pk.load(reinterpret_cast<const T*>(reinterpret_cast<const char*>(kb) +
+                                       int64_t(kt + a_row) * a.sk),
+            kt + a_row < nk, a.d, half);
+    pv.load(vb, a.sv, kt, nk, a.d, lane);
+    if constexpr (BIAS) idw = *reinterpret_cast<const u32x4*>(ids + kt);
+  };
+  int t = t_begin + wave;
+  if (t < t_end) fetch(t);
+  while (t < t_end) {
+    const int kt = 32 * t;
+    f32x16 x[1] = {fill16(0.f)};
+#pragma unroll
+    for (int c = 0; c < L::kChunks; ++c) x[0] = mma_rows<T>(pk.w[c], q.w[c], x[0]);
+    if constexpr (BIAS) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[0][i] = fmaf(x[0][i], s2, tab[bucket_of(idw, i)]);
+    }
+    pv.store(vs, lane);
+    t += 4;
+    if (t < t_end) fetch(t);
+    if (kt + 31 > first_lim) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (kt + 16 * half + i > lim) x[0][i] = -INFINITY;
+    }
+    softmax_step<1>(x, c2, step, m, thr, l, acc);
+    // the wave's own tile: its writes above, then its reads
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    L::mma_cols(vs, 0, x[0], acc, lane);
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+
+  // join the four waves, in wave order
+  l = sum_halves(l);
+  if (half == 0) {
+    ml[wave][l32][0] = m * c2;
+    ml[wave][l32][1] = l;
+  }
+  __syncthreads();
+  const int jr = tid >> 3, jd = (tid & 7) * 4;
+  float top = -INFINITY, f[4], sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = fmaxf(top, ml[i][jr][0]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[i] = ml[i][jr][1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[i][jr][0] - top);
+    sum += ml[i][jr][1] * f[i];
+  }
+  const int64_t slot = (int64_t(w) * a.Hkv + kvh) * fa.splits + split;
+  const int jg = jr / nq, jq = jr - jg * nq, jh = kvh * G + jg;
+  const float inv = fa.splits > 1 ? 1.f : sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+  float* jb = reinterpret_cast<float*>(buf);
+#pragma unroll
+  for (int c = 0; c < L::kCols; ++c) {
+    if (c) __syncthreads();
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      store4(jb + (wave * 32 + l32) * kJoin + 8 * g + 4 * half, acc[c][4 * g], acc[c][4 * g + 1],
+             acc[c][4 * g + 2], acc[c][4 * g + 3]);
+    __syncthreads();
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 y = *reinterpret_cast<const float4*>(jb + (i * 32 + jr) * kJoin + jd);
+      if (f[i] != 0.f) {
+        o[0] = fmaf(y.x, f[i], o[0]);
+        o[1] = fmaf(y.y, f[i], o[1]);
+        o[2] = fmaf(y.z, f[i], o[2]);
+        o[3] = fmaf(y.w, f[i], o[3]);
+      }
+    }
+    const int at = 32 * c + jd;
+    if (jr < rows) {
+      if (fa.splits > 1) {
+        store4(fa.part_acc + (slot * 32 + jr) * DP + at, o[0], o[1], o[2], o[3]);
+      } else if (at < a.d) {
+        const int64_t row = ((q0 + jq) * a.H + jh) * int64_t(a.d) + at;
+        store4(reinterpret_cast<T*>(a.out) + row, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+        if (a.out32) store4(a.out32 + row, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+      }
+    }
+  }
+  if (jr < rows && jd == 0) {
+    if (fa.splits > 1) {
+      fa.part_ml[(slot * 32 + jr) * 2] = top;
+      fa.part_ml[(slot * 32 + jr) * 2 + 1] = sum;
+    } else if (a.lse) {
+      a.lse[int64_t(jh) * a.n_q + q0 + jq] =
+          sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+    }
+  }
+}
+
+// Joins the splits of k_packed_few, in split order: 8 threads a row.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void k_packed_few_join(FewArgs fa) {
+  const FwdArgs& a = fa.f;
+  const int tid = tid_x(), jr = tid >> 3, jd = (tid & 7) * 4;
+  const int kvh = wg_x() % a.Hkv, w = wg_x() / a.Hkv, G = a.H / a.Hkv;
+  const int64_t q0 = a.q_start[w];
+  const int nq = static_cast<int>(a.q_start[w + 1] - q0);
+  if (nq == 0 || jr >= nq * G) return;
+  const int jg = jr / nq, jq = jr - jg * nq, jh = kvh * G + jg;
+  const int64_t slot = (int64_t(w) * a.Hkv + kvh) * fa.splits;
+  float top = -INFINITY, sum = 0.f, o[DP / 8];
+#pragma unroll
+  for (int i = 0; i < DP / 8; ++i) o[i] = 0.f;
+  for (int s = 0; s < fa.splits; ++s)
+    if (fa.part_ml[((slot + s) * 32 + jr) * 2 + 1] != 0.f)
+      top = fmaxf(top, fa.part_ml[((slot + s) * 32 + jr) * 2]);
+  for (int s = 0; s < fa.splits; ++s) {
+    const float* ml = fa.part_ml + ((slot + s) * 32 + jr) * 2;
+    if (ml[1] == 0.f) continue;
+    const float f = __builtin_amdgcn_exp2f(ml[0] - top);
+    sum = fmaf(ml[1], f, sum);
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c) {
+      const float4 y =
+          *reinterpret_cast<const float4*>(fa.part_acc + ((slot + s) * 32 + jr) * DP + 32 * c + jd);
+      o[4 * c] = fmaf(y.x, f, o[4 * c]);
+      o[4 * c + 1] = fmaf(y.y, f, o[4 * c + 1]);
+      o[4 * c + 2] = fmaf(y.z, f, o[4 * c + 2]);
+      o[4 * c + 3] = fmaf(y.w, f, o[4 * c + 3]);
+    }
+  }
+  const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+#pragma unroll
+  for (int c = 0; c < DP / 32; ++c) {
+    const int at = 32 * c + jd;
+    if (at >= a.d) continue;
+    const int64_t row = ((q0 + jq) * a.H + jh) * int64_t(a.d) + at;
+    store4(reinterpret_cast<T*>(a.out) + row, o[4 * c] * inv, o[4 * c + 1] * inv,
+           o[4 * c + 2] * inv, o[4 * c + 3] * inv);
+    if (a.out32)
+      store4(a.out32 + row, o[4 * c] * inv, o[4 * c + 1] * inv, o[4 * c + 2] * inv,
+             o[4 * c + 3] * inv);
+  }
+  if (a.lse && jd == 0)
+    a.lse[int64_t(jh) * a.n_q + q0 + jq] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+}
+
+// The windows' bucket ids as the kernels read them: one byte a pair, rows padded
+// to 64 with 255, by queries and by keys.  One block: 64 queries of a window.
+template <typename I>
+__global__ __launch_bounds__(256) void k_packed_buckets(const I* __restrict__ ids,
+                                                        const int64_t* __restrict__ q_start,
+                                                        const int64_t* __restrict__ k_start,
+                                                        const int64_t* __restrict__ p_start,
+                                                        const int64_t* __restrict__ b_start,
+                                                        const int64_t* __restrict__ bt_start,
+                                                        const int2* __restrict__ items,
+                                                        uint8_t* __restrict__ out,
+                                                        uint8_t* __restrict__ out_t) {
+  __shared__ uint8_t t[64][68];
+  const int tid = tid_x();
+  const int2 item = items[wg_x()];
+  const int nq = static_cast<int>(q_start[item.x + 1] - q_start[item.x]);
+  const int nk = static_cast<int>(k_start[item.x + 1] - k_start[item.x]);
+  const int ldq = (nk + 63) & ~63, ldk = (nq + 63) & ~63;
+  const I* src = ids + p_start[item.x];
+  uint8_t* dst = out + b_start[item.x];
+  uint8_t* dst_t = out_t + bt_start[item.x];
+  for (int kt = 0; kt < ldq; kt += 64) {
+    __syncthreads();
+    for (int e = tid; e < 64 * 64; e += 256) {
+      const int r = e >> 6, c = e & 63;
+      int64_t x = 255;
+      if (item.y + r < nq && kt + c < nk) x = int64_t(src[int64_t(item.y + r) * nk + kt + c]);
+      t[r][c] = static_cast<uint8_t>(x < 0 || x > 255 ? 255 : x);
+    }
+    __syncthreads();
+    const int r = tid >> 2, c0 = (tid & 3) * 16;
+    uint32_t w[4], wt[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = wt[i] = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        w[i] |= uint32_t(t[r][c0 + 4 * i + j]) << (8 * j);
+        wt[i] |= uint32_t(t[c0 + 4 * i + j][r]) << (8 * j);
+      }
+    }
+    if (item.y + r < nq)
+      *reinterpret_cast<u32x4*>(dst + int64_t(item.y + r) * ldq + kt + c0) =
+          u32x4{w[0], w[1], w[2], w[3]};
+    if (kt + r < nk)
+      *reinterpret_cast<u32x4*>(dst_t + int64_t(kt + r) * ldk + item.y + c0) =
+          u32x4{wt[0], wt[1], wt[2], wt[3]};
+  }
+}
+
+// ------------------------------------------------------------------ host side
+constexpr int kTargetBlocks = 512;  // two blocks for each of the 256 compute units
+
+inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+// Index of the work list of 32 << i rows.
+inline int waves_of(int i) { return 1 << i; }
+
+// How many waves (32 rows each) a block has: as many as the longest window
+// fills, up to 4, and fewer where the grid would leave compute units without a
+// block: more rows a block share each staged tile, more blocks fill the chip.
+int pick_list(int32_t longest, const int32_t n_items[3], int heads, int most) {
+  int i = longest <= 32 ? 0 : longest <= 64 ? 1 : 2;
+  if (i > most) i = most;
+  while (i > 0 && int64_t(n_items[i]) * heads < kTargetBlocks) --i;
+  return i;
+}
+
+struct FewPlan {
+  bool use;
+  int splits;
+  size_t acc, total;
+};
+FewPlan few_plan(const ngt_packed_windows& w, int H, int Hkv, int dp) {
+  FewPlan p{};
+  // all heads of a group and all queries of a window in one 32-row tile, and
+  // keys enough for four waves
+  p.use = int64_t(w.max_q) * (H / Hkv) <= 32 && w.max_k > 128;
+  if (!p.use) return p;
+  const int64_t blocks = int64_t(w.n_windows) * Hkv;
+  const int tiles = (w.max_k + 31) / 32;
+  p.splits = static_cast<int>(std::min<int64_t>((kTargetBlocks + blocks - 1) / blocks,
+                                                std::max(1, tiles / 8)));
+  p.splits = std::max(1, std::min(p.splits, 64));
+  if (p.splits > 1) {
+    const size_t rows = size_t(blocks) * p.splits * 32;
+    p.acc = align256(rows * 8);
+    p.total = p.acc + align256(rows * dp * 4);
+  }
+  return p;
+}
+
+int dp_of(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+
+int check_call(const char* fn, int dtype, const ngt_packed_windows* w, int H, int Hkv, int d,
+               float scale, const void* table, int n_buckets, const uint8_t* ids) {
+  if (!w) return set_error(NGT_ERR_ARG, "%s: null windows", fn);
+  if (dtype != NGT_F32 && dtype != NGT_BF16)
+    return set_error(NGT_ERR_ARG, "%s: unknown dtype %d", fn, dtype);
+  if (H < 1 || Hkv < 1 || H > 65535 || H % Hkv)
+    return set_error(NGT_ERR_ARG, "%s: %d heads over %d key heads", fn, H, Hkv);
+  if (d < 8 || d > 128 || d % 8)
+    return set_error(NGT_ERR_UNSUPPORTED, "%s: head_dim=%d (a multiple of 8 up to 128)", fn, d);
+  if (!(scale > 0.f) || !(scale < INFINITY))
+    return set_error(NGT_ERR_ARG, "%s: scale must be finite and > 0", fn);
+  if (w->n_windows < 0 || w->n_q < 0 || w->n_k < 0 || w->max_q < 0 || w->max_k < 0)
+    return set_error(NGT_ERR_ARG, "%s: bad windows", fn);
+  for (int i = 0; i < 3; ++i)
+    if (w->n_items_q[i] < 0 || w->n_items_k[i] < 0 ||
+        int64_t(std::max(w->n_items_q[i], w->n_items_k[i])) * H > 0x7fffffff)
+      return set_error(NGT_ERR_UNSUPPORTED, "%s: too many rows for one launch", fn);
+  if ((table != nullptr) != (ids != nullptr))
+    return set_error(NGT_ERR_ARG, "%s: a bias takes a table and bucket ids", fn);
+  if (table && (n_buckets < 1 || n_buckets > 255))
+    return set_error(NGT_ERR_ARG, "%s: n_buckets=%d (1 to 255)", fn, n_buckets);
+  if (table && !(w->b_start && w->bt_start))
+    return set_error(NGT_ERR_ARG, "%s: null bucket offsets", fn);
+  return NGT_OK;
+}
+
+int check_stride(const char* fn, const char* name, const void* p, int64_t stride, int heads, int d,
+                 int es) {
+  if (stride < int64_t(heads) * d || (stride * es) % 16 || reinterpret_cast<uintptr_t>(p) % 16)
+    return set_error(NGT_ERR_ARG,
+                     "%s: %s rows must be at least heads * head_dim apart and 16-byte aligned", fn,
+                     name);
+  return NGT_OK;
+}
+
+template <typename T, int DP, bool BIAS>
+int run_fwd(const ngt_packed_windows& w, const FewPlan& fp, FwdArgs a, void* ws, hipStream_t st) {
+  if (fp.use) {
+    FewArgs fa{a, fp.splits, nullptr, nullptr};
+    if (fp.splits > 1) {
+      fa.part_ml = static_cast<float*>(ws);
+      fa.part_acc = reinterpret_cast<float*>(static_cast<char*>(ws) + fp.acc);
+    }
+    const int64_t blocks = int64_t(w.n_windows) * a.Hkv;
+    {
+      KernelTimer timer_("packed_few", st);
+      hipLaunchKernelGGL((k_packed_few<T, DP, BIAS>), dim3(unsigned(blocks * fp.splits)), dim3(256),
+                         BIAS ? (a.H / a.Hkv) * kTable * sizeof(float) : 0, st, fa);
+      NGT_HIP_CHECK(hipGetLastError());
+    }
+    if (fp.splits > 1) {
+      KernelTimer timer_("packed_few_join", st);
+      hipLaunchKernelGGL((k_packed_few_join<T, DP>), dim3(unsigned(blocks)), dim3(256), 0, st, fa);
+      NGT_HIP_CHECK(hipGetLastError());
+    }
+    return NGT_OK;
+  }
+  const int i = pick_list(w.max_q, w.n_items_q, a.H, 2);
+  const unsigned blocks = unsigned(w.n_items_q[i]) * unsigned(a.H);
+  if (!blocks) return NGT_OK;
+  a.items = reinterpret_cast<const int2*>(w.items_q[i]);
+  KernelTimer timer_("packed_fwd", st);
+  if (i == 2) hipLaunchKernelGGL((k_packed_fwd<T, DP, BIAS, 4>), dim3(blocks), dim3(256), 0, st, a);
+  else if (i == 1) hipLaunchKernelGGL((k_packed_fwd<T, DP, BIAS, 2>), dim3(blocks), dim3(128), 0, st, a);
+  else hipLaunchKernelGGL((k_packed_fwd<T, DP, BIAS, 1>), dim3(blocks), dim3(64), 0, st, a);
+  NGT_HIP_CHECK(hipGetLastError());
+  return NGT_OK;
+}
+
+template <typename T>
+int run_fwd_d(int dp, const ngt_packed_windows& w, const FewPlan& fp, const FwdArgs& a, void* ws,
+              hipStream_t st) {
+  if (a.table)
+    return dp == 32   ? run_fwd<T, 32, true>(w, fp, a, ws, st)
+           : dp == 64 ? run_fwd<T, 64, true>(w, fp, a, ws, st)
+                      : run_fwd<T, 128, true>(w, fp, a, ws, st);
+  return dp == 32   ? run_fwd<T, 32, false>(w, fp, a, ws, st)
+         : dp == 64 ? run_fwd<T, 64, false>(w, fp, a, ws, st)
+                    : run_fwd<T, 128, false>(w, fp, a, ws, st);
+}
+
+struct BwdLayout {
+  size_t part, total;
+  int list_q, list_k;
+};
+BwdLayout bwd_layout(int dtype, const ngt_packed_windows& w, int H, int Hkv, int d, int n_buckets) {
+  BwdLayout L{};
+  const int es = dtype == NGT_F32 ? 4 : 2;
+  int most = 2;
+  // with a table gradient a wave holds 64 sums per bucket beside the block's two tiles
+  const size_t fixed = 2 * size_t(64) * dp_of(d) * es + 2048;
+  while (most > 0 && fixed + size_t(waves_of(most)) * (n_buckets + 1) * 256 > 160 * 1024) --most;
+  L.list_q = pick_list(w.max_q, w.n_items_q, H, most);
+  L.list_k = pick_list(w.max_k, w.n_items_k, Hkv, 2);
+  L.part = align256(size_t(w.n_q) * H * 4);
+  L.total = L.part + align256(size_t(w.n_items_q[L.list_q]) * H * n_buckets * 4);
+  return L;
+}
+
+// The plan's arrays, in the order in which they lie in its buffer.
+struct PlanLayout {
+  int64_t items[2][3];
+  size_t start[5], list[2][3], total;
+};
+PlanLayout plan_layout(int32_t n, const int32_t* q_len, const int32_t* k_len) {
+  PlanLayout L{};
+  for (int32_t w = 0; w < n; ++w)
+    for (int i = 0; i < 3; ++i) {
+      L.items[0][i] += (int64_t(q_len[w]) + (32 << i) - 1) / (32 << i);
+      L.items[1][i] += (int64_t(k_len[w]) + (32 << i) - 1) / (32 << i);
+    }
+  size_t at = 0;
+  for (int s = 0; s < 5; ++s) L.start[s] = at, at += align256((size_t(n) + 1) * 8);
+  for (int o = 0; o < 2; ++o)
+    for (int i = 0; i < 3; ++i) L.list[o][i] = at, at += align256(size_t(L.items[o][i]) * 8);
+  L.total = at;
+  return L;
+}
+
+int check_lengths(const char* fn, int32_t n, const int32_t* q_len, const int32_t* k_len) {
+  if (n < 0 || (n > 0 && (!q_len || !k_len)))
+    return set_error(NGT_ERR_ARG, "%s: bad window count or null lengths", fn);
+  int64_t tq = 0, tk = 0;
+  for (int32_t w = 0; w < n; ++w) {
+    if (q_len[w] < 0 || k_len[w] < 0)
+      return set_error(NGT_ERR_ARG, "%s: window %d has a negative length", fn, w);
+    if (q_len[w] > (1 << 30) || k_len[w] > (1 << 30))
+      return set_error(NGT_ERR_UNSUPPORTED, "%s: window %d is longer than 2^30", fn, w);
+    tq += (q_len[w] + 31) / 32;
+    tk += (k_len[w] + 31) / 32;
+  }
+  if (tq > 0x7fffffff || tk > 0x7fffffff)
+    return set_error(NGT_ERR_UNSUPPORTED, "%s: too many rows", fn);
+  return NGT_OK;
+}
+
+}  // namespace
+}  // namespace packed
+}  // namespace ngt
+
+using namespace ngt;
+using namespace ngt::packed;
+
+extern "C" int ngt_packed_plan_bytes(int32_t n_windows, const int32_t* q_len, const int32_t* k_len,
+                                     size_t* bytes) {
+  NGT_CHECK_OK(check_lengths("ngt_packed_plan_bytes", n_windows, q_len, k_len));
+  if (!bytes) return set_error(NGT_ERR_ARG, "ngt_packed_plan_bytes: null bytes");
+  *bytes = plan_layout(n_windows, q_len, k_len).total;
+  return NGT_OK;
+}
+
+extern "C" int ngt_packed_plan(int32_t n_windows, const int32_t* q_len, const int32_t* k_len,
+                               int32_t causal, void* host, size_t bytes, void* device,
+                               ngt_packed_windows* out) {
+  NGT_CHECK_OK(check_lengths("ngt_packed_plan", n_windows, q_len, k_len));
+  if (!out) return set_error(NGT_ERR_ARG, "ngt_packed_plan: null windows");
+  const PlanLayout L = plan_layout(n_windows, q_len, k_len);
+  if (!host || !device || bytes < L.total)
+    return set_error(NGT_ERR_WORKSPACE, "ngt_packed_plan: buffer %zu < %zu", bytes, L.total);
+  char* base = static_cast<char*>(host);
+  char* dev = static_cast<char*>(device);
+  memset(out, 0, sizeof(*out));
+  memset(base, 0, L.total);
+  out->n_windows = n_windows;
+  out->causal = causal != 0;
+  int64_t* s[5];
+  for (int i = 0; i < 5; ++i) s[i] = reinterpret_cast<int64_t*>(base + L.start[i]);
+  for (int32_t w = 0; w < n_windows; ++w) {
+    const int64_t nq = q_len[w], nk = k_len[w];
+    s[0][w + 1] = s[0][w] + nq;
+    s[1][w + 1] = s[1][w] + nk;
+    s[2][w + 1] = s[2][w] + nq * nk;
+    s[3][w + 1] = s[3][w] + nq * ((nk + 63) & ~int64_t(63));
+    s[4][w + 1] = s[4][w] + nk * ((nq + 63) & ~int64_t(63));
+    out->max_q = std::max(out->max_q, q_len[w]);
+    out->max_k = std::max(out->max_k, k_len[w]);
+  }
+  out->n_q = s[0][n_windows];
+  out->n_k = s[1][n_windows];
+  out->n_pairs = s[2][n_windows];
+  out->bucket_bytes_q = s[3][n_windows];
+  out->bucket_bytes_k = s[4][n_windows];
+  out->q_start = reinterpret_cast<const int64_t*>(dev + L.start[0]);
+  out->k_start = reinterpret_cast<const int64_t*>(dev + L.start[1]);
+  out->p_start = reinterpret_cast<const int64_t*>(dev + L.start[2]);
+  out->b_start = reinterpret_cast<const int64_t*>(dev + L.start[3]);
+  out->bt_start = reinterpret_cast<const int64_t*>(dev + L.start[4]);
+  try {
+    // the work lists, the items with the most rows on the other side first (a
+    // counting sort by 64-row steps): the last blocks to start are short ones
+    for (int o = 0; o < 2; ++o)
+      for (int i = 0; i < 3; ++i) {
+        const int rows = 32 << i;
+        int32_t* list = reinterpret_cast<int32_t*>(base + L.list[o][i]);
+        auto steps = [&](int32_t w, int32_t row) {
+          const int64_t nq = q_len[w], nk = k_len[w], mine = o ? nk : nq, other = o ? nq : nk;
+          int64_t seen = other;
+          if (causal) {
+            const int64_t last = std::min<int64_t>(row + rows, mine);
+            seen = o ? nq - std::max<int64_t>(0, row - (nk - nq)) : std::min(last + nk - nq, nk);
+          }
+          return std::max<int64_t>(0, std::min(seen, other) + 63) / 64;
+        };
+        const int64_t top = ((o ? out->max_q : out->max_k) + 63) / 64;
+        std::vector<int64_t> at(size_t(top) + 2, 0);
+        for (int32_t w = 0; w < n_windows; ++w)
+          for (int32_t r = 0; r < (o ? k_len[w] : q_len[w]); r += rows) ++at[size_t(top - steps(w, r)) + 1];
+        for (size_t j = 1; j < at.size(); ++j) at[j] += at[j - 1];
+        for (int32_t w = 0; w < n_windows; ++w)
+          for (int32_t r = 0; r < (o ? k_len[w] : q_len[w]); r += rows) {
+            const int64_t j = at[size_t(top - steps(w, r))]++;
+            list[2 * j] = w;
+            list[2 * j + 1] = r;
+          }
+        const int32_t* d = reinterpret_cast<const int32_t*>(dev + L.list[o][i]);
+        if (o) out->n_items_k[i] = static_cast<int32_t>(L.items[1][i]), out->items_k[i] = d;
+        else out->n_items_q[i] = static_cast<int32_t>(L.items[0][i]), out->items_q[i] = d;
+      }
+  } catch (const std::bad_alloc&) {
+    return set_error(NGT_ERR_HIP, "ngt_packed_plan: out of host memory");
+  }
+  return NGT_OK;
+}
+
+extern "C" int ngt_packed_buckets(const ngt_packed_windows* w, const void* ids, int32_t id_bytes,
+                                  uint8_t* buckets_q, uint8_t* buckets_k, void* stream) {
+  if (!w) return set_error(NGT_ERR_ARG, "ngt_packed_buckets: null windows");
+  if (id_bytes != 1 && id_bytes != 4 && id_bytes != 8)
+    return set_error(NGT_ERR_ARG, "ngt_packed_buckets: ids of %d bytes (1, 4 or 8)", id_bytes);
+  if (w->n_pairs == 0) return NGT_OK;
+  if (!ids || !buckets_q || !buckets_k)
+    return set_error(NGT_ERR_ARG, "ngt_packed_buckets: null ids or buckets");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  KernelTimer timer_("packed_buckets", st);
+  auto run = [&](auto kernel, auto* p) {
+    hipLaunchKernelGGL(kernel, dim3(unsigned(w->n_items_q[1])), dim3(256), 0, st, p, w->q_start,
+                       w->k_start, w->p_start, w->b_start, w->bt_start,
+                       reinterpret_cast<const int2*>(w->items_q[1]), buckets_q, buckets_k);
+  };
+  if (id_bytes == 1) run(k_packed_buckets<uint8_t>, static_cast<const uint8_t*>(ids));
+  else if (id_bytes == 4) run(k_packed_buckets<int32_t>, static_cast<const int32_t*>(ids));
+  else run(k_packed_buckets<int64_t>, static_cast<const int64_t*>(ids));
+  NGT_HIP_CHECK(hipGetLastError());
+  return NGT_OK;
+}
+
+extern "C" int ngt_packed_workspace_bytes(int dtype, const ngt_packed_windows* w, int32_t n_heads,
+                                          int32_t n_kv_heads, int32_t head_dim, int32_t n_buckets,
+                                          size_t* fwd_bytes, size_t* bwd_bytes) {
+  NGT_CHECK_OK(check_call("ngt_packed_workspace_bytes", dtype, w, n_heads, n_kv_heads, head_dim,
+                          1.f, nullptr, 0, nullptr));
+  if (n_buckets < 0 || n_buckets > 255)
+    return set_error(NGT_ERR_ARG, "ngt_packed_workspace_bytes: n_buckets=%d", n_buckets);
+  if (fwd_bytes) *fwd_bytes = few_plan(*w, n_heads, n_kv_heads, dp_of(head_dim)).total;
+  if (bwd_bytes)
+    *bwd_bytes = bwd_layout(dtype, *w, n_heads, n_kv_heads, head_dim, n_buckets).total;
+  return NGT_OK;
+}
+
+extern "C" int ngt_packed_fwd(int dtype, const void* q, const void* k, const void* v,
+                              int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                              const ngt_packed_windows* w, int32_t n_heads, int32_t n_kv_heads,
+                              int32_t head_dim, float scale, const void* table, int32_t n_buckets,
+                              const uint8_t* buckets_q, void* out, float* out_f32, float* lse,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "ngt_packed_fwd";
+  NGT_CHECK_OK(check_call(fn, dtype, w, n_heads, n_kv_heads, head_dim, scale, table, n_buckets,
+                          buckets_q));
+  if (w->n_q == 0) return NGT_OK;
+  const int es = dtype == NGT_F32 ? 4 : 2;
+  if (!q || !out) return set_error(NGT_ERR_ARG, "%s: null q or out", fn);
+  if (w->n_k > 0 && (!k || !v)) return set_error(NGT_ERR_ARG, "%s: null k or v", fn);
+  NGT_CHECK_OK(check_stride(fn, "q", q, q_stride, n_heads, head_dim, es));
+  if (w->n_k > 0) {
+    NGT_CHECK_OK(check_stride(fn, "k", k, k_stride, n_kv_heads, head_dim, es));
+    NGT_CHECK_OK(check_stride(fn, "v", v, v_stride, n_kv_heads, head_dim, es));
+  }
+  const int dp = dp_of(head_dim);
+  const FewPlan fp = few_plan(*w, n_heads, n_kv_heads, dp);
+  if (fp.total && (!workspace || workspace_bytes < fp.total))
+    return set_error(NGT_ERR_WORKSPACE, "%s: workspace %zu < %zu", fn, workspace_bytes, fp.total);
+  if (fp.use && int64_t(w->n_windows) * n_kv_heads * fp.splits > 0x7fffffff)
+    return set_error(NGT_ERR_UNSUPPORTED, "%s: too many windows for one launch", fn);
+  FwdArgs a{w->q_start, w->k_start, w->b_start, nullptr, n_heads, n_kv_heads, head_dim, w->causal,
+            n_buckets, scale, q_stride * es, k_stride * es, v_stride * es, q, k, v, table,
+            buckets_q, out, out_f32, lse, w->n_q};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return dtype == NGT_F32 ? run_fwd_d<float>(dp, *w, fp, a, workspace, st)
+                          : run_fwd_d<bf16_t>(dp, *w, fp, a, workspace, st);
+}
+
+extern "C" int ngt_packed_bwd(int dtype, const void* q, const void* k, const void* v,
+                              int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                              const float* out_f32, const void* grad_out, const float* lse,
+                              const ngt_packed_windows* w, int32_t n_heads, int32_t n_kv_heads,
+                              int32_t head_dim, float scale, const void* table, int32_t n_buckets,
+                              const uint8_t* buckets_q, const uint8_t* buckets_k, void* grad_q,
+                              void* grad_k, void* grad_v, void* grad_table, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  const char* fn = "ngt_packed_bwd";
+  NGT_CHECK_OK(check_call(fn, dtype, w, n_heads, n_kv_heads, head_dim, scale, table, n_buckets,
+                          buckets_q));
+  const int es = dtype == NGT_F32 ? 4 : 2;
+  if (table && !buckets_k) return set_error(NGT_ERR_ARG, "%s: null buckets_k", fn);
+  if (grad_table && !table) return set_error(NGT_ERR_ARG, "%s: grad_table without a table", fn);
+  if (w->n_q > 0 && (!q || !out_f32 || !grad_out || !lse || !grad_q))
+    return set_error(NGT_ERR_ARG, "%s: null query-side pointer", fn);
+  if (w->n_k > 0 && (!k || !v || !grad_k || !grad_v))
+    return set_error(NGT_ERR_ARG, "%s: null key-side pointer", fn);
+  if (w->n_q > 0) NGT_CHECK_OK(check_stride(fn, "q", q, q_stride, n_heads, head_dim, es));
+  if (w->n_k > 0) {
+    NGT_CHECK_OK(check_stride(fn, "k", k, k_stride, n_kv_heads, head_dim, es));
+    NGT_CHECK_OK(check_stride(fn, "v", v, v_stride, n_kv_heads, head_dim, es));
+  }
+  const int hist = grad_table ? n_buckets : 0;
+  const BwdLayout L = bwd_layout(dtype, *w, n_heads, n_kv_heads, head_dim, hist);
+  if (L.total && (!workspace || workspace_bytes < L.total))
+    return set_error(NGT_ERR_WORKSPACE, "%s: workspace %zu < %zu", fn, workspace_bytes, L.total);
+  char* ws = static_cast<char*>(workspace);
+  BwdArgs a{};
+  a.q_start = w->q_start, a.k_start = w->k_start, a.b_start = w->b_start, a.bt_start = w->bt_start;
+  a.H = n_heads, a.Hkv = n_kv_heads, a.d = head_dim, a.causal = w->causal, a.n_buckets = n_buckets;
+  a.scale = scale, a.sq = q_stride * es, a.sk = k_stride * es, a.sv = v_stride * es, a.n_q = w->n_q;
+  a.q = q, a.k = k, a.v = v, a.go = grad_out, a.out32 = out_f32, a.lse = lse;
+  a.dsum = reinterpret_cast<float*>(ws);
+  a.table = table, a.ids = buckets_q, a.ids_t = buckets_k;
+  a.part_table = reinterpret_cast<float*>(ws + L.part);
+  a.gq = grad_q, a.gk = grad_k, a.gv = grad_v, a.grad_table = grad_table;
+  BwdPlan p{};
+  p.items_q = reinterpret_cast<const int2*>(w->items_q[L.list_q]);
+  p.items_k = reinterpret_cast<const int2*>(w->items_k[L.list_k]);
+  p.n_items_q = w->n_items_q[L.list_q];
+  p.dq_waves = waves_of(L.list_q);
+  p.dkv_waves = waves_of(L.list_k);
+  p.dq_blocks = int64_t(p.n_items_q) * n_heads;
+  p.dkv_blocks = int64_t(w->n_items_k[L.list_k]) * n_kv_heads;
+  return packed_bwd(dtype, p, a, static_cast<hipStream_t>(stream));
+}
