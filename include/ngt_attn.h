@@ -744,6 +744,31 @@ int ngt_colsum_bf16(const void* dy, int64_t n_rows, int32_t n_cols, float* out, 
 int ngt_chunk_sum_f32(const float* in, int32_t n_chunks, int64_t n, float* out, void* stream);
 
 /*
+ * Linear layer with its epilogue, bf16: y = act(x W^T + bias) + residual from
+ * x [n_rows, n_in] (rows x_stride elements apart), W [n_out, n_in], bias [n_out]
+ * and residual [n_rows, n_out] (both nullable), summed in fp32 and rounded
+ * once; any sizes >= 1 and 2-byte alignment (16-byte accesses where sizes and
+ * addresses are multiples of 8 elements).  z, where not null, receives
+ * x W^T + bias for the backward.  residual may be y.
+ * ngt_linear_bwd: dz = dy act'(z) (with an activation: z and dz [n_rows, n_out],
+ * 16-byte aligned like dy; without one dz is dy, and z and dz are not used) and
+ * dx = dz W (dx nullable).  dW and dbias are ngt_wgrad_bf16 of x and dz; the
+ * residual's gradient is dy.  workspace (16-byte aligned) holds W^T.
+ * The encoder's FFN and output projection with the activation and residual
+ * that follow them, NeutronGT/models/graphormer_dist_node_level.py:18-30, 176-206.
+ */
+#define NGT_ACT_NONE 0
+#define NGT_ACT_RELU 1
+#define NGT_ACT_GELU 2 /* z (1 + erf(z / sqrt 2)) / 2 */
+int ngt_linear_fwd(const void* x, int64_t x_stride, const void* w, const void* bias,
+                   const void* residual, int64_t n_rows, int32_t n_out, int32_t n_in,
+                   int32_t activation, void* y, void* z, void* stream);
+int ngt_linear_bwd_workspace_bytes(int64_t n_rows, int32_t n_out, int32_t n_in, size_t* bytes);
+int ngt_linear_bwd(const void* dy, const void* z, const void* w, int64_t n_rows, int32_t n_out,
+                   int32_t n_in, int32_t activation, void* dz, void* dx, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/*
  * Weight and bias gradient of a bf16 linear layer: dw[o][i] = sum_k dy[k][o]
  * x[k][i] and db[o] = sum_k dy[k][o], both fp32, from x [n_rows, n_in] and dy
  * [n_rows, n_out] (bf16, row-major, any widths and 2-byte alignment).  db may

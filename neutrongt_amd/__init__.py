@@ -9,6 +9,7 @@ window_attention(...)    the same over a built WindowAdjacency (C++ autograd nod
 dense_attention(...)     functional full-window attention
 packed_attention(...)    attention over a PackedWindows batch (grouped heads, causal, bucket bias)
 PackedWindows            plan of windows of different lengths back to back
+linear_epilogue(...)     act(x W^T + b) + residual as one kernel, differentiable
 WindowAdjacency          device CSR/transposed CSR/work lists of one window
 """
 from .attention import (CoreAttention, DenseAttentionBiasFunction, DenseAttentionFunction,
@@ -16,6 +17,7 @@ from .attention import (CoreAttention, DenseAttentionBiasFunction, DenseAttentio
                         dense_attention_bias, install, sparse_attention, window_attention)
 from .csr import (AdjacencyCache, WindowAdjacency, chunk_for_heads, default_cache, pack_q_adaptive,
                   small_for_heads)
+from .linear import LinearEpilogueFunction, linear_epilogue
 from .packed import PackedAttentionFunction, PackedWindows, PairBuckets, packed_attention
 
 __all__ = [
@@ -33,6 +35,8 @@ __all__ = [
     "PackedAttentionFunction",
     "PackedWindows",
     "PairBuckets",
+    "linear_epilogue",
+    "LinearEpilogueFunction",
     "WindowAdjacency",
     "AdjacencyCache",
     "chunk_for_heads",

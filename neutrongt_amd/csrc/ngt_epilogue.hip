@@ -1,0 +1,390 @@
+// Linear layer with its epilogue: y = act(x W^T + b) + r in bf16, fp32 inside,
+// and its backward up to the weight's gradient (ngt_wgrad.hip).  The encoder's
+// FFN and output projections (NeutronGT/models/graphormer_dist_node_level.py:
+// 18-30, 176-206) read and write their activations once instead of three times.
+//
+// x [M, K] and W [N, K] both have the contraction along their rows, so an MFMA
+// takes W's rows as A and x's as B as they lie in LDS (16 bytes a lane), and D
+// has outputs n in its registers: with the row order of ngt_packed.h a lane
+// ends up with 16 consecutive outputs of one row, so bias, residual and result
+// are 16-byte accesses.
+#include "ngt_packed.h"
+
+namespace ngt {
+namespace {
+
+using packed::f32x16;
+using packed::fill16;
+using packed::mma_rows;
+using packed::tid_x;
+using packed::u32x4;
+using packed::wg_x;
+
+constexpr int kActNone = NGT_ACT_NONE, kActRelu = NGT_ACT_RELU, kActGelu = NGT_ACT_GELU;
+constexpr int kStage = 64;  // contraction per LDS stage: rows of 128 bytes
+using L = packed::Tile<bf16_t, kStage>;
+
+struct GemmArgs {
+  const uint16_t* x;  // [M, K], rows x_stride apart
+  const uint16_t* w;  // [N, K]
+  const uint16_t* bias;
+  const uint16_t* r;  // [M, N]
+  uint16_t* y;        // [M, N]
+  uint16_t* z;        // [M, N] or null: before the activation
+  int64_t x_stride;
+  int32_t M, N, K, act;
+  int32_t tiles_m, tiles_n;
+};
+
+// gelu(z) = z (1 + erf(z / sqrt 2)) / 2
+__device__ __forceinline__ float act_of(float z, int act) {
+  if (act == kActRelu) return z > 0.f ? z : (z != z ? z : 0.f);
+  if (act == kActGelu) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+  return z;
+}
+__device__ __forceinline__ float act_grad(float z, int act) {
+  if (act == kActRelu) return z > 0.f ? 1.f : 0.f;
+  if (act == kActGelu)
+    return 0.5f * (1.f + erff(z * 0.70710678118654752f)) +
+           z * 0.39894228040143268f * __expf(-0.5f * z * z);
+  return 1.f;
+}
+
+struct __attribute__((packed, aligned(2))) Loose16 {
+  u32x4 w;
+};
+
+// 8 elements at column c of a row of n: whole pieces in one access (any 2-byte
+// alignment without ALIGNED), what is behind the row as zeros.
+template <bool ALIGNED>
+__device__ __forceinline__ u32x4 load8(const uint16_t* __restrict__ row, int c, int n) {
+  if constexpr (ALIGNED) {
+    if (c < n) return *reinterpret_cast<const u32x4*>(row + c);
+    return u32x4{0u, 0u, 0u, 0u};
+  } else {
+    if (c + 8 <= n) return reinterpret_cast<const Loose16*>(row + c)->w;
+    u32x4 v = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < n) v[i / 2] |= uint32_t(row[c + i]) << (16 * (i & 1));
+    return v;
+  }
+}
+
+__device__ __forceinline__ float half_of(const u32x4& v, int i) {
+  const uint32_t w = v[i / 2];
+  return __uint_as_float((i & 1) ? (w & 0xffff0000u) : (w << 16));
+}
+
+// 8 outputs n .. n+7 of row m from their sums.
+template <bool ALIGNED>
+__device__ __forceinline__ void finish8(const GemmArgs& a, int m, int n, const float (&s)[8]) {
+  if (m >= a.M || n >= a.N) return;
+  const int64_t at = int64_t(m) * a.N + n;
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = s[i];
+  if (a.bias) {
+    const u32x4 b = load8<ALIGNED>(a.bias, n, a.N);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += half_of(b, i);
+  }
+  u32x4 z, y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) z[i] = pack2_bf16(v[2 * i], v[2 * i + 1]);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = act_of(v[i], a.act);
+  if (a.r) {
+    const u32x4 r = load8<ALIGNED>(a.r + int64_t(m) * a.N, n, a.N);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += half_of(r, i);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = pack2_bf16(v[2 * i], v[2 * i + 1]);
+  if (ALIGNED || n + 8 <= a.N) {
+    if constexpr (ALIGNED) {
+      *reinterpret_cast<u32x4*>(a.y + at) = y;
+      if (a.z) *reinterpret_cast<u32x4*>(a.z + at) = z;
+    } else {
+      reinterpret_cast<Loose16*>(a.y + at)->w = y;
+      if (a.z) reinterpret_cast<Loose16*>(a.z + at)->w = z;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (n + i < a.N) {
+        a.y[at + i] = static_cast<uint16_t>(y[i / 2] >> (16 * (i & 1)));
+        if (a.z) a.z[at + i] = static_cast<uint16_t>(z[i / 2] >> (16 * (i & 1)));
+      }
+  }
+}
+
+// One block: BM rows by BN outputs, 2 x 2 waves.
+template <int BM, int BN, bool ALIGNED>
+__global__ __launch_bounds__(256) void k_gemm(GemmArgs a) {
+  constexpr int FM = BM / 64, FN = BN / 64;  // 32 x 32 tiles of a wave
+  constexpr int NX = BM * 8 / 256, NW = BN * 8 / 256;  // 16-byte pieces per thread
+  __shared__ __align__(16) char xs[BM * 128];
+  __shared__ __align__(16) char ws[BN * 128];
+  const int tid = tid_x(), lane = tid & 63, wave = tid >> 6, half = lane >> 5, l32 = lane & 31;
+  // each XCD (block number mod 8) takes a contiguous run of tiles, the tiles
+  // of a row of x one after another: its L2 holds W and each row once
+  const int total = a.tiles_m * a.tiles_n, per = (total + 7) / 8;
+  const int id = (wg_x() % 8) * per + wg_x() / 8;
+  if (wg_x() / 8 >= per || id >= total) return;  // block-uniform
+  const int m0 = id / a.tiles_n * BM, n0 = id % a.tiles_n * BN;
+  const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
+  f32x16 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = fill16(0.f);
+  u32x4 px[NX], pw[NW];
+  auto fetch = [&](int k) {
+#pragma unroll
+    for (int i = 0; i < NX; ++i) {
+      const int e = tid + i * 256, row = m0 + e / 8;
+      px[i] = u32x4{0u, 0u, 0u, 0u};
+      if (row < a.M) px[i] = load8<ALIGNED>(a.x + row * a.x_stride, k + 8 * (e % 8), a.K);
+    }
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      const int e = tid + i * 256, row = n0 + e / 8;
+      pw[i] = u32x4{0u, 0u, 0u, 0u};
+      if (row < a.N) pw[i] = load8<ALIGNED>(a.w + int64_t(row) * a.K, k + 8 * (e % 8), a.K);
+    }
+  };
+  fetch(0);
+  for (int k = 0; k < a.K; k += kStage) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NX; ++i) {
+      const int e = tid + i * 256;
+      *reinterpret_cast<u32x4*>(xs + L::offset(e / 8, e % 8)) = px[i];
+    }
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      const int e = tid + i * 256;
+      *reinterpret_cast<u32x4*>(ws + L::offset(e / 8, e % 8)) = pw[i];
+    }
+    __syncthreads();
+    if (k + kStage < a.K) fetch(k + kStage);
+#pragma unroll
+    for (int c = 0; c < L::kChunks; ++c) {
+      u32x4 fx[FM], fw[FN];
+#pragma unroll
+      for (int i = 0; i < FM; ++i) fx[i] = L::load_a(xs + wm * 128, i, c, l32, half);
+#pragma unroll
+      for (int j = 0; j < FN; ++j) fw[j] = L::load_a(ws + wn * 128, j, c, l32, half);
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mma_rows<bf16_t>(fw[j], fx[i], acc[i][j]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float s[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) s[t] = acc[i][j][8 * e + t];
+        finish8<ALIGNED>(a, m0 + wm + 32 * i + L::a_row(l32), n0 + wn + 32 * j + 16 * half + 8 * e,
+                         s);
+      }
+}
+
+// Few outputs: one block 32 rows by 32 outputs straight from memory, its four
+// waves a quarter of the contraction each; their sums are added in wave order.
+template <bool ALIGNED>
+__global__ __launch_bounds__(256) void k_gemm_few(GemmArgs a) {
+  constexpr int kPitch = 36;  // floats
+  __shared__ __align__(16) float red[4][32][kPitch];
+  const int tid = tid_x(), lane = tid & 63, wave = tid >> 6, half = lane >> 5, l32 = lane & 31;
+  const int m0 = wg_x() / a.tiles_n * 32, n0 = wg_x() % a.tiles_n * 32;
+  const int row = L::a_row(l32);
+  const bool mx = m0 + l32 < a.M, nx = n0 + row < a.N;
+  const uint16_t* xr = a.x + (mx ? (m0 + l32) * a.x_stride : 0);
+  const uint16_t* wr = a.w + (nx ? int64_t(n0 + row) * a.K : 0);
+  f32x16 acc = fill16(0.f);
+  for (int k = 64 * wave; k < a.K; k += 256) {
+    u32x4 fx[4], fw[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      fx[c] = fw[c] = u32x4{0u, 0u, 0u, 0u};
+      if (mx) fx[c] = load8<ALIGNED>(xr, k + 16 * c + 8 * half, a.K);
+      if (nx) fw[c] = load8<ALIGNED>(wr, k + 16 * c + 8 * half, a.K);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc = mma_rows<bf16_t>(fw[c], fx[c], acc);
+  }
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    *reinterpret_cast<float4*>(&red[wave][l32][16 * half + 4 * g]) =
+        make_float4(acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]);
+  __syncthreads();
+  if (tid < 128) {
+    const int m = tid >> 2, n = (tid & 3) * 8;
+    float s[8];
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+      s[t] = ((red[0][m][n + t] + red[1][m][n + t]) + red[2][m][n + t]) + red[3][m][n + t];
+    finish8<ALIGNED>(a, m0 + m, n0 + n, s);
+  }
+}
+
+// dz = dy act'(z), 8 elements a thread.
+__global__ __launch_bounds__(256) void k_act_grad(const uint16_t* __restrict__ dy,
+                                                  const uint16_t* __restrict__ z, int64_t n,
+                                                  int act, uint16_t* __restrict__ dz) {
+  const int64_t step = int64_t(__builtin_amdgcn_grid_size_x()) * 8;
+  for (int64_t i = (int64_t(wg_x()) * 256 + tid_x()) * 8; i < n; i += step) {
+    if (i + 8 <= n) {
+      const u32x4 g = *reinterpret_cast<const u32x4*>(dy + i);
+      const u32x4 v = *reinterpret_cast<const u32x4*>(z + i);
+      u32x4 o;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        o[t] = pack2_bf16(half_of(g, 2 * t) * act_grad(half_of(v, 2 * t), act),
+                          half_of(g, 2 * t + 1) * act_grad(half_of(v, 2 * t + 1), act));
+      *reinterpret_cast<u32x4*>(dz + i) = o;
+    } else {
+      for (int64_t t = i; t < n; ++t)
+        dz[t] = f32_to_bf16(bf16_to_f32(dy[t]) * act_grad(bf16_to_f32(z[t]), act));
+    }
+  }
+}
+
+// out[c][r] = in[r][c], 64 x 64 elements a block.
+__global__ __launch_bounds__(256) void k_transpose(const uint16_t* __restrict__ in, int rows,
+                                                   int cols, int tiles_c,
+                                                   uint16_t* __restrict__ out) {
+  __shared__ uint16_t t[64][66];
+  const int r0 = wg_x() / tiles_c * 64, c0 = wg_x() % tiles_c * 64;
+  for (int e = tid_x(); e < 4096; e += 256) {
+    const int r = r0 + e / 64, c = c0 + e % 64;
+    if (r < rows && c < cols) t[e / 64][e % 64] = in[int64_t(r) * cols + c];
+  }
+  __syncthreads();
+  for (int e = tid_x(); e < 4096; e += 256) {
+    const int c = c0 + e / 64, r = r0 + e % 64;
+    if (r < rows && c < cols) out[int64_t(c) * rows + r] = t[e % 64][e / 64];
+  }
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+int launch_gemm(GemmArgs a, hipStream_t st) {
+  KernelTimer timer_("linear_gemm", st);
+  const bool al = a.K % 8 == 0 && a.N % 8 == 0 && a.x_stride % 8 == 0 && aligned16(a.x) &&
+                  aligned16(a.w) && aligned16(a.bias) && aligned16(a.r) && aligned16(a.y) &&
+                  aligned16(a.z);
+  auto tiles = [&](int bm, int bn) {
+    a.tiles_m = (a.M + bm - 1) / bm;
+    a.tiles_n = (a.N + bn - 1) / bn;
+    return int64_t(a.tiles_m) * a.tiles_n;
+  };
+  if (tiles(128, 128) < 128) {
+    const int64_t n = tiles(32, 32);
+    if (al) hipLaunchKernelGGL(k_gemm_few<true>, dim3(unsigned(n)), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(k_gemm_few<false>, dim3(unsigned(n)), dim3(256), 0, st, a);
+  } else if (tiles(256, 128) < 256) {
+    const int64_t n = (tiles(128, 128) + 7) / 8 * 8;
+    if (al) hipLaunchKernelGGL((k_gemm<128, 128, true>), dim3(unsigned(n)), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_gemm<128, 128, false>), dim3(unsigned(n)), dim3(256), 0, st, a);
+  } else {
+    const int64_t n = (tiles(256, 128) + 7) / 8 * 8;
+    if (al) hipLaunchKernelGGL((k_gemm<256, 128, true>), dim3(unsigned(n)), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_gemm<256, 128, false>), dim3(unsigned(n)), dim3(256), 0, st, a);
+  }
+  NGT_HIP_CHECK(hipGetLastError());
+  return NGT_OK;
+}
+
+int check_sizes(const char* fn, int64_t M, int32_t N, int32_t K, int act) {
+  if (M < 0 || N < 1 || K < 1)
+    return set_error(NGT_ERR_ARG, "%s: bad sizes rows=%lld n_out=%d n_in=%d", fn,
+                     static_cast<long long>(M), N, K);
+  if (act < kActNone || act > kActGelu) return set_error(NGT_ERR_ARG, "%s: activation %d", fn, act);
+  // 32-bit rows, and fewer than 2^24 blocks of 256 threads for each of the tile
+  // grids: y, dx and W's transpose
+  auto blocks = [](int64_t r, int64_t c, int t) { return (r + t - 1) / t * ((c + t - 1) / t); };
+  constexpr int64_t kMost = (1 << 24) - 8;
+  if (M > (1 << 30) || blocks(M, N, 128) > kMost || blocks(M, K, 128) > kMost ||
+      blocks(N, K, 64) > kMost)
+    return set_error(NGT_ERR_UNSUPPORTED, "%s: rows=%lld n_out=%d n_in=%d exceed the grid", fn,
+                     static_cast<long long>(M), N, K);
+  return NGT_OK;
+}
+
+}  // namespace
+}  // namespace ngt
+
+using namespace ngt;
+
+extern "C" int ngt_linear_fwd(const void* x, int64_t x_stride, const void* w, const void* bias,
+                              const void* residual, int64_t n_rows, int32_t n_out, int32_t n_in,
+                              int32_t activation, void* y, void* z, void* stream) {
+  const char* fn = "ngt_linear_fwd";
+  NGT_CHECK_OK(check_sizes(fn, n_rows, n_out, n_in, activation));
+  if (n_rows == 0) return NGT_OK;
+  if (!x || !w || !y) return set_error(NGT_ERR_ARG, "%s: null x, w or y", fn);
+  if (x_stride < n_in) return set_error(NGT_ERR_ARG, "%s: x rows overlap", fn);
+  GemmArgs a{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(w),
+             static_cast<const uint16_t*>(bias), static_cast<const uint16_t*>(residual),
+             static_cast<uint16_t*>(y), static_cast<uint16_t*>(z), x_stride,
+             static_cast<int32_t>(n_rows), n_out, n_in, activation, 0, 0};
+  return launch_gemm(a, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int ngt_linear_bwd_workspace_bytes(int64_t n_rows, int32_t n_out, int32_t n_in,
+                                              size_t* bytes) {
+  NGT_CHECK_OK(check_sizes("ngt_linear_bwd_workspace_bytes", n_rows, n_out, n_in, kActNone));
+  if (!bytes) return set_error(NGT_ERR_ARG, "ngt_linear_bwd_workspace_bytes: null bytes");
+  *bytes = size_t(n_out) * n_in * 2;
+  return NGT_OK;
+}
+
+extern "C" int ngt_linear_bwd(const void* dy, const void* z, const void* w, int64_t n_rows,
+                              int32_t n_out, int32_t n_in, int32_t activation, void* dz, void* dx,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "ngt_linear_bwd";
+  NGT_CHECK_OK(check_sizes(fn, n_rows, n_out, n_in, activation));
+  if (n_rows == 0) return NGT_OK;
+  if (!dy || (activation != kActNone && (!z || !dz)))
+    return set_error(NGT_ERR_ARG, "%s: null dy, z or dz", fn);
+  if (activation != kActNone && !(aligned16(dy) && aligned16(z) && aligned16(dz)))
+    return set_error(NGT_ERR_ARG, "%s: dy, z and dz must be 16-byte aligned", fn);
+  const size_t need = size_t(n_out) * n_in * 2;
+  if (dx && !w) return set_error(NGT_ERR_ARG, "%s: null w", fn);
+  if (dx && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return set_error(NGT_ERR_WORKSPACE, "%s: workspace %zu < %zu or not 16-byte aligned", fn,
+                     workspace_bytes, need);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (activation != kActNone) {
+    KernelTimer timer_("linear_act_grad", st);
+    const int64_t n = n_rows * n_out, blocks = (n + 2047) / 2048;
+    hipLaunchKernelGGL(k_act_grad, dim3(unsigned(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st,
+                       static_cast<const uint16_t*>(dy), static_cast<const uint16_t*>(z), n,
+                       activation, static_cast<uint16_t*>(dz));
+    NGT_HIP_CHECK(hipGetLastError());
+    dy = dz;
+  }
+  if (!dx) return NGT_OK;
+  {
+    KernelTimer timer_("linear_transpose", st);
+    const int tc = (n_in + 63) / 64;
+    const int64_t blocks = int64_t((n_out + 63) / 64) * tc;
+    hipLaunchKernelGGL(k_transpose, dim3(unsigned(blocks)), dim3(256), 0, st,
+                       static_cast<const uint16_t*>(w), n_out, n_in, tc,
+                       static_cast<uint16_t*>(workspace));
+    NGT_HIP_CHECK(hipGetLastError());
+  }
+  // dx = dz W: rows of W^T are the other operand
+  GemmArgs a{static_cast<const uint16_t*>(dy), static_cast<const uint16_t*>(workspace), nullptr,
+             nullptr, static_cast<uint16_t*>(dx), nullptr, n_out, static_cast<int32_t>(n_rows),
+             n_in, n_out, kActNone, 0, 0};
+  return launch_gemm(a, st);
+}

@@ -27,6 +27,7 @@ import ctypes as C
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -304,3 +305,98 @@ class WgradLinear(nn.Linear):
                 return ext.linear(x, self.weight, self.bias)
             return _WgradLinearFn.apply(x, self.weight, self.bias)
         return super().forward(x)
+
+
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2}
+
+
+class LinearEpilogueFunction(torch.autograd.Function):
+    """act(x2 W^T + b) + r of bf16 rows x2 [M, n_in] (ngt_linear_fwd /
+    ngt_linear_bwd / ngt_wgrad_bf16); the gradients of weight and bias come in
+    their own type, from fp32 sums."""
+
+    @staticmethod
+    def forward(ctx, x2, weight, bias, residual, act, want_grad):
+        m, n_in = x2.shape
+        n_out, dev = weight.shape[0], x2.device
+        w16 = weight.to(torch.bfloat16).contiguous()
+        b16 = bias.to(torch.bfloat16).contiguous() if bias is not None else None
+        y = torch.empty(m, n_out, dtype=torch.bfloat16, device=dev)
+        z = torch.empty_like(y) if want_grad and act else None
+        with torch.cuda.device(dev):
+            _lib.check(_lib.load().ngt_linear_fwd(
+                x2.data_ptr(), x2.stride(0) if m > 1 else n_in, w16.data_ptr(),
+                b16.data_ptr() if b16 is not None else None,
+                residual.data_ptr() if residual is not None else None, m, n_out, n_in, act,
+                y.data_ptr(), z.data_ptr() if z is not None else None, _lib.stream_ptr(dev)))
+        if want_grad:
+            ctx.save_for_backward(x2, w16, z)
+            ctx.act, ctx.dtypes = act, (weight.dtype, bias.dtype if bias is not None else None)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        x2, w16, z = ctx.saved_tensors
+        (m, n_in), n_out, dev = x2.shape, w16.shape[0], x2.device
+        want_x, want_w, want_b, want_r = ctx.needs_input_grad[:4]
+        g = gy.to(torch.bfloat16)
+        if not g.is_contiguous() or g.data_ptr() % 16:
+            g = g.clone(memory_format=torch.contiguous_format)
+        dx = torch.empty(m, n_in, dtype=torch.bfloat16, device=dev) if want_x else None
+        dz = g
+        if want_x or want_w or want_b:
+            dz = torch.empty_like(g) if ctx.act else g
+            nb = C.c_size_t()
+            _lib.check(_lib.load().ngt_linear_bwd_workspace_bytes(m, n_out, n_in, C.byref(nb)))
+            ws = torch.empty(nb.value if want_x else 0, dtype=torch.uint8, device=dev)
+            with torch.cuda.device(dev):
+                _lib.check(_lib.load().ngt_linear_bwd(
+                    g.data_ptr(), z.data_ptr() if z is not None else None, w16.data_ptr(), m, n_out,
+                    n_in, ctx.act, dz.data_ptr(), dx.data_ptr() if want_x else None,
+                    ws.data_ptr() if want_x else None, ws.numel(), _lib.stream_ptr(dev)))
+        dw = db = None
+        with torch.cuda.device(dev):
+            if want_w:
+                dw, db = linear_grads(x2, dz, want_b)
+                dw = dw.to(ctx.dtypes[0])
+            elif want_b:
+                db = colsum_bf16(dz)
+        if want_b:
+            db = db.to(ctx.dtypes[1])
+        return dx, dw, db, g if want_r else None, None, None
+
+
+def linear_epilogue(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
+                    activation: str | None = None, residual: torch.Tensor | None = None):
+    """act(x W^T + b) + residual as one kernel in bf16: x [..., n_in], weight
+    [n_out, n_in] and bias [n_out] as nn.Linear holds them, activation None,
+    "relu" or "gelu" (the erf form, nn.GELU()'s default), residual
+    [..., n_out].  fp32 inputs are rounded to bf16 as autocast does; the sums,
+    the activation and the residual's addition are fp32 and the result is
+    rounded once.  The gradients have the inputs' types; those of weight and
+    bias are fp32 sums in a fixed order.  Differentiable once."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
+    ts = [t for t in (x, weight, bias, residual) if t is not None]
+    if any(not t.is_cuda for t in ts):
+        raise ValueError("linear_epilogue takes GPU tensors (there is no CPU path)")
+    if any(t.device != x.device for t in ts):
+        raise ValueError("x, weight, bias and residual must be on one device")
+    if any(t.dtype not in (torch.bfloat16, torch.float32) for t in ts):
+        raise TypeError("linear_epilogue takes bfloat16 or float32 tensors")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
+    n_out, n_in = weight.shape
+    shape = (*x.shape[:-1], n_out)
+    if bias is not None and tuple(bias.shape) != (n_out,):
+        raise ValueError(f"bias must be [{n_out}], got {tuple(bias.shape)}")
+    if residual is not None and tuple(residual.shape) != shape:
+        raise ValueError(f"residual must be {shape}, got {tuple(residual.shape)}")
+    x2 = x.to(torch.bfloat16).reshape(-1, n_in)
+    if (n_in > 1 and x2.stride(1) != 1) or (x2.shape[0] > 1 and x2.stride(0) < n_in):
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    r2 = residual.to(torch.bfloat16).reshape(-1, n_out).contiguous() if residual is not None else None
+    want_grad = torch.is_grad_enabled() and any(t.requires_grad for t in ts)
+    return LinearEpilogueFunction.apply(x2, weight, bias, r2, ACTIVATIONS[activation],
+                                        want_grad).view(shape)
