@@ -475,6 +475,8 @@ typedef struct ngt_packed_windows {
   int64_t n_pairs;
   int64_t bucket_bytes_q;
   int64_t bucket_bytes_k;
+  int64_t steps_q; /* steps of 64 keys of all 32-query items, and the other way round */
+  int64_t steps_k;
   const int64_t* q_start; /* [n_windows + 1] each, device */
   const int64_t* k_start;
   const int64_t* p_start;

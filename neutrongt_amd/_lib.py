@@ -92,6 +92,8 @@ class PackedWindowsC(C.Structure):
         ("n_pairs", C.c_int64),
         ("bucket_bytes_q", C.c_int64),
         ("bucket_bytes_k", C.c_int64),
+        ("steps_q", C.c_int64),
+        ("steps_k", C.c_int64),
         ("q_start", C.c_void_p),
         ("k_start", C.c_void_p),
         ("p_start", C.c_void_p),

@@ -26,6 +26,8 @@
 
 #include "ngt_common.h"
 
+#include <type_traits>
+
 namespace ngt {
 namespace packed {
 
@@ -41,6 +43,10 @@ constexpr float kLn2 = 0.6931471805599453f;
 // (see build.py) the functions behind threadIdx and blockIdx are not inlined.
 __device__ __forceinline__ int tid_x() { return static_cast<int>(__builtin_amdgcn_workitem_id_x()); }
 __device__ __forceinline__ int wg_x() { return static_cast<int>(__builtin_amdgcn_workgroup_id_x()); }
+
+// The wave's number in its block, known to be the same in all its lanes: what
+// depends on it alone is decided once, on the scalar unit.
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(tid_x() >> 6); }
 
 __device__ __forceinline__ f32x16 fill16(float v) {
   f32x16 r;
@@ -196,6 +202,44 @@ struct Stage {
   }
 };
 
+// A block is RW x KS waves: RW waves of 32 rows each, KS of them on the same
+// rows, each on its own 64 of the 64 * KS rows of the other side that a stage
+// holds.  More row waves share a stage's tile among more rows; more sets
+// shorten the longest block and fill the chip where rows are few.  At the end
+// the sets' sums of a row wave are added in set order.
+template <int RW, int KS>
+struct Block {
+  static constexpr int kThreads = 64 * RW * KS;
+  static constexpr int kStage = 64 * KS;                        // rows of a stage
+  static constexpr int kJoinBytes = (KS - 1) * RW * 64 * 16 * 4;  // of one accumulator
+};
+
+// Adds the sets' accumulators into set 0's; buf holds kJoinBytes.  Every wave
+// calls it; the block's earlier reads of buf are done (a barrier is passed here).
+template <int RW, int KS>
+__device__ __forceinline__ void join_sets(f32x16& acc, char* buf, int rw, int set, int lane) {
+  if constexpr (KS > 1) {
+    float4* b = reinterpret_cast<float4*>(buf);
+    __syncthreads();
+    if (set > 0) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        b[(((set - 1) * RW + rw) * 4 + g) * 64 + lane] =
+            make_float4(acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]);
+    }
+    __syncthreads();
+    if (set == 0) {
+#pragma unroll
+      for (int s = 0; s < KS - 1; ++s)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4 y = b[((s * RW + rw) * 4 + g) * 64 + lane];
+          acc[4 * g] += y.x, acc[4 * g + 1] += y.y, acc[4 * g + 2] += y.z, acc[4 * g + 3] += y.w;
+        }
+    }
+  }
+}
+
 // 4 consecutive values of a row.
 template <typename T>
 __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
@@ -207,8 +251,8 @@ __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d)
 
 // Bucket ids of a lane's 16 tile rows, and the bias table of one head in LDS:
 // entries in log2 units, -inf (not attended) behind the n_buckets there are.
-// Finite entries stay finite: a table of the type's lowest values still gives
-// every pair the same weight instead of none.
+// Finite entries act as if within +-2^60: a row of the type's lowest values
+// still gives every pair the same weight instead of none.
 constexpr int kTable = 256;
 template <typename T>
 __device__ __forceinline__ void load_table(float* tab, const T* __restrict__ table, int n_buckets,
@@ -218,7 +262,7 @@ __device__ __forceinline__ void load_table(float* tab, const T* __restrict__ tab
     if (b < n_buckets) {
       x = elem<T>::load(table + int64_t(b) * n_heads + h);
       const uint32_t mag = __float_as_uint(x) & 0x7fffffffu;
-      if (mag < 0x7f800000u) x = fminf(fmaxf(x * kLog2e, -3.0e38f), 3.0e38f);
+      if (mag < 0x7f800000u) x = fminf(fmaxf(x * kLog2e, -0x1p60f), 0x1p60f);
     }
     tab[b] = x;
   }
@@ -232,6 +276,29 @@ __device__ __forceinline__ int bucket_of(const u32x4& ids, int i) {
 
 namespace ngt {
 namespace packed {
+
+// The blocks there are: row waves and sets (Block).
+struct Shape {
+  int rw, ks;
+};
+// The most sets of a kernel: by the LDS of its tiles, and for the dK/dV pass,
+// whose two accumulators and two operands fill a wave's registers, by those.
+constexpr int most_sets(int pitch, bool dkv) {
+  return pitch <= 128 ? 4 : pitch <= 256 && !dkv ? 2 : 1;
+}
+template <int MOST, typename F>
+int with_shape(Shape s, F&& f) {
+  using std::integral_constant;
+  if (s.rw == 1) return f(integral_constant<int, 1>(), integral_constant<int, 1>());
+  if constexpr (MOST >= 2) {
+    if (s.ks == 2 && s.rw == 4) return f(integral_constant<int, 4>(), integral_constant<int, 2>());
+    if (s.ks == 2) return f(integral_constant<int, 2>(), integral_constant<int, 2>());
+  }
+  if constexpr (MOST >= 4)
+    if (s.ks == 4) return f(integral_constant<int, 2>(), integral_constant<int, 4>());
+  if (s.rw == 4) return f(integral_constant<int, 4>(), integral_constant<int, 1>());
+  return f(integral_constant<int, 2>(), integral_constant<int, 1>());
+}
 
 // ------------------------------------------------------- the backward's launch
 struct BwdArgs {
@@ -251,7 +318,7 @@ struct BwdArgs {
   const void* go;
   const float* out32;
   const float* lse;
-  float* dsum;  // [H, n_q]: written by the dQ pass, read by the dK/dV pass
+  float* dsum;  // [H, n_q]: -D, written by the dQ pass, read by the dK/dV pass
   const void* table;
   const uint8_t* ids;
   const uint8_t* ids_t;
@@ -264,7 +331,8 @@ struct BwdArgs {
 struct BwdPlan {
   const int2* items_q;
   const int2* items_k;
-  int n_items_q, dq_waves, dkv_waves;
+  int n_items_q;
+  Shape dq, dkv;
   int64_t dq_blocks, dkv_blocks;
 };
 int packed_bwd(int dtype, const BwdPlan& p, const BwdArgs& a, hipStream_t st);

@@ -12,7 +12,6 @@ namespace ngt {
 namespace packed {
 namespace {
 
-constexpr int kKeys = 64;       // keys of one stage
 constexpr float kRebase = 8.f;  // weights stay below 2^8 of a row's base
 
 struct FwdArgs {
@@ -34,53 +33,76 @@ struct FwdArgs {
   int64_t n_q;
 };
 
-// One online-softmax step of a lane's row over its 16 * NT scores x (log2
-// units times 1 / c2): the weights are exp2((x - m) c2).  The base m moves
-// only when some row exceeds it by more than kRebase, so that most tiles
-// rescale nothing; weights and sums share the base, so this is exact.
-template <int NT, int NC>
-__device__ __forceinline__ void softmax_step(f32x16 (&x)[NT], float c2, float step, float& m,
-                                             float& thr, float& l, f32x16 (&acc)[NC]) {
-  float mx = x[0][0];
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[t][i]);
-  if (__any(mx > thr)) {  // thr: -inf before a row's first key, m + step after it
-    const float up = fmaxf(m, max_halves(mx));
-    const float f = up == m ? 1.f : __builtin_amdgcn_exp2f((m - up) * c2);
-    m = up;
-    thr = m == -INFINITY ? m : m + step;
-    l *= f;
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[c][i] *= f;
-  }
-  const float base = m == -INFINITY ? 0.f : m * c2;
-  float s = 0.f;
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      x[t][i] = __builtin_amdgcn_exp2f(fmaf(x[t][i], c2, -base));
-      s += x[t][i];
-    }
-  l += s;
-}
+// The running softmax of a lane's row.  Scores x (log2 units times 1 / c2) come
+// relative to the row's base m: the first product of a tile starts from -m
+// (`start`, in product units) instead of 0, so that a weight costs a multiply
+// and an exponential.  The base moves only when some row exceeds it by kRebase,
+// so most tiles rescale nothing; weights and sums share the base, so this is
+// exact.
+struct RowSoftmax {
+  float c2, per, step;  // per: product units per unit of x
+  float m = 0.f;
+  float thr = -INFINITY;  // -inf before the row's first key
+  float l = 0.f;
+  f32x16 start = fill16(0.f);
+  __device__ __forceinline__ RowSoftmax(float c2_, float per_) : c2(c2_), per(per_), step(kRebase / c2_) {}
 
-// One block: NW * 32 query rows of one window and head, a wave 32 of them; the
-// window's keys pass through LDS 64 at a time.
-template <typename T, int DP, bool BIAS, int NW>
-__global__ __launch_bounds__(64 * NW) void k_packed_fwd(FwdArgs a) {
+  template <int NT, int NC>
+  __device__ __forceinline__ void weights(f32x16 (&x)[NT], f32x16 (&acc)[NC]) {
+    float mx = x[0][0];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[t][i]);
+    if (__any(mx > thr)) {
+      mx = max_halves(mx);
+      const bool first = thr == -INFINITY;
+      const float up = !first ? fmaxf(mx, 0.f) : mx == -INFINITY ? 0.f : mx;
+      const float f = first ? 0.f : __builtin_amdgcn_exp2f(-up * c2);
+      if (mx > -INFINITY) thr = step;
+      m += up;
+      l *= f;
+      start = fill16(-m * per);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[t][i] -= up;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[c][i] *= f;
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        x[t][i] = __builtin_amdgcn_exp2f(x[t][i] * c2);
+        s += x[t][i];
+      }
+    l += s;
+  }
+  // the row's base in log2 units, -inf where it has seen no key
+  __device__ __forceinline__ float base() const { return thr == -INFINITY ? thr : m * c2; }
+};
+
+// One block: RW * 32 query rows of one window and head; the window's keys pass
+// through LDS 64 * KS at a time.
+template <typename T, int DP, bool BIAS, int RW, int KS>
+__global__ __launch_bounds__(64 * RW * KS) void k_packed_fwd(FwdArgs a) {
   using L = Tile<T, DP>;
-  constexpr int N = 64 * NW;
+  using B = Block<RW, KS>;
+  constexpr int N = B::kThreads, kKeys = B::kStage;
+  constexpr int kTileBytes = kKeys * L::kPitch;
   // registers for the next stage's pieces, where they are few enough
   constexpr bool kAhead = (kKeys * L::kPieces / N) * 8 <= 64;
-  __shared__ __align__(16) char ks[kKeys * L::kPitch];
-  __shared__ __align__(16) char vs[kKeys * L::kPitch];
+  __shared__ __align__(16) char
+      buf[2 * kTileBytes > B::kJoinBytes ? 2 * kTileBytes : B::kJoinBytes];
   __shared__ float tab[BIAS ? kTable : 1];
-  const int tid = tid_x(), lane = tid & 63, wave = tid >> 6, half = lane >> 5, l32 = lane & 31;
+  __shared__ float ml[KS > 1 ? KS * RW : 1][2][64];
+  char *const ks = buf, *const vs = buf + kTileBytes;
+  const int tid = tid_x(), lane = tid & 63, half = lane >> 5, l32 = lane & 31;
+  const int wid = tid >> 6, wave = wid % RW, set = wid / RW;
   // the heads that share K and V follow each other H_kv blocks apart: with 8
   // key heads all blocks of one of them run on one XCD, whose L2 holds them
   const int bid = wg_x();
@@ -97,7 +119,7 @@ __global__ __launch_bounds__(64 * NW) void k_packed_fwd(FwdArgs a) {
   const int first_lim = a.causal ? min(item.y + wave * 32 + ahead, nk - 1) : nk - 1;
   const int last_q = min(item.y + wave * 32 + 31, nq - 1);
   const int wave_end = item.y + wave * 32 >= nq ? 0 : a.causal ? min(last_q + ahead + 1, nk) : nk;
-  const int block_end = a.causal ? min(min(item.y + 32 * NW, nq) + ahead, nk) : nk;
+  const int block_end = a.causal ? min(min(item.y + 32 * RW, nq) + ahead, nk) : nk;
   const T* kb = reinterpret_cast<const T*>(reinterpret_cast<const char*>(a.k) + k0 * a.sk) +
                 int64_t(kvh) * a.d;
   const T* vb = reinterpret_cast<const T*>(reinterpret_cast<const char*>(a.v) + k0 * a.sv) +
@@ -112,24 +134,26 @@ __global__ __launch_bounds__(64 * NW) void k_packed_fwd(FwdArgs a) {
     ids = a.ids + a.b_start[item.x] + int64_t(qc) * ((nk + 63) & ~63) + 16 * half;
   }
   const float s2 = a.scale * kLog2e;
-  const float c2 = BIAS ? 1.f : s2;
-  const float step = kRebase / c2;
-  float m = -INFINITY, thr = -INFINITY, l = 0.f;
+  RowSoftmax sm(BIAS ? 1.f : s2, BIAS ? 1.f / s2 : 1.f);
   f32x16 acc[L::kCols];
 #pragma unroll
   for (int c = 0; c < L::kCols; ++c) acc[c] = fill16(0.f);
 
   Stage<T, DP, kKeys, N> pk, pv;
-  u32x4 idw[2];
+  u32x4 idw[2], id_next[2];
+  auto fetch_ids = [&](int k1) {  // of keys that are there
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      if (BIAS && k1 < nk) id_next[t] = *reinterpret_cast<const u32x4*>(ids + k1 + 32 * t);
+  };
+  fetch_ids(64 * set);
   if constexpr (kAhead) {
     pk.load(kb, a.sk, 0, nk, a.d, tid);
     pv.load(vb, a.sv, 0, nk, a.d, tid);
   }
+  const char* kt_tile = ks + 64 * set * L::kPitch;
+  const char* vt_tile = vs + 64 * set * L::kPitch;
   for (int kt = 0; kt < block_end; kt += kKeys) {
-    if constexpr (BIAS) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) idw[t] = *reinterpret_cast<const u32x4*>(ids + kt + 32 * t);
-    }
     __syncthreads();
     if constexpr (!kAhead) {
       pk.load(kb, a.sk, kt, nk, a.d, tid);
@@ -141,38 +165,63 @@ __global__ __launch_bounds__(64 * NW) void k_packed_fwd(FwdArgs a) {
       pv.store(vs, tid);
     }
     __syncthreads();
+    idw[0] = id_next[0], idw[1] = id_next[1];
+    fetch_ids(kt + kKeys + 64 * set);
     if constexpr (kAhead) {
       if (kt + kKeys < block_end) {
         pk.load(kb, a.sk, kt + kKeys, nk, a.d, tid);
         pv.load(vb, a.sv, kt + kKeys, nk, a.d, tid);
       }
     }
-    if (kt >= wave_end) continue;
-    f32x16 x[2];
+    const int k1 = kt + 64 * set;  // this set's first key
+    if (k1 >= wave_end) continue;
+    f32x16 x[2] = {sm.start, sm.start};
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      x[t] = fill16(0.f);
+    for (int c = 0; c < L::kChunks; ++c)
 #pragma unroll
-      for (int c = 0; c < L::kChunks; ++c)
-        x[t] = mma_rows<T>(L::load_a(ks, t, c, l32, half), q.w[c], x[t]);
-      if constexpr (BIAS) {
+      for (int t = 0; t < 2; ++t)
+        x[t] = mma_rows<T>(L::load_a(kt_tile, t, c, l32, half), q.w[c], x[t]);
+    if constexpr (BIAS) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[t][i] = fmaf(x[t][i], s2, tab[bucket_of(idw[t], i)]);
-      }
     }
-    if (kt + kKeys - 1 > first_lim) {  // some key of the tile is behind some row's last one
+    if (k1 + 63 > first_lim) {  // some key of the tile is behind some row's last one
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (kt + 32 * t + 16 * half + i > lim) x[t][i] = -INFINITY;
+          if (k1 + 32 * t + 16 * half + i > lim) x[t][i] = -INFINITY;
     }
-    softmax_step<2>(x, c2, step, m, thr, l, acc);
+    sm.weights(x, acc);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) L::mma_cols(vs, t, x[t], acc, lane);
+    for (int t = 0; t < 2; ++t) L::mma_cols(vt_tile, t, x[t], acc, lane);
   }
 
-  l = sum_halves(l);
+  float base = sm.base(), l = sum_halves(sm.l);
+  if constexpr (KS > 1) {
+    ml[set * RW + wave][0][lane] = base;
+    ml[set * RW + wave][1][lane] = l;
+    __syncthreads();
+    const float mine = base;
+    float sum = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) base = fmaxf(base, ml[s * RW + wave][0][lane]);
+    auto factor = [&](float b) { return b == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(b - base); };
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      sum = fmaf(ml[s * RW + wave][1][lane], factor(ml[s * RW + wave][0][lane]), sum);
+    const float f = factor(mine);
+    l = sum;
+#pragma unroll
+    for (int c = 0; c < L::kCols; ++c) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[c][i] *= f;
+      join_sets<RW, KS>(acc[c], buf, wave, set, lane);
+    }
+    if (set > 0) return;
+  }
   if (qi < nq) {
     const float r = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
     T* o = reinterpret_cast<T*>(a.out) + ((q0 + qi) * a.H + h) * int64_t(a.d);
@@ -191,7 +240,7 @@ __global__ __launch_bounds__(64 * NW) void k_packed_fwd(FwdArgs a) {
         }
       }
     if (a.lse && half == 0)
-      a.lse[int64_t(h) * a.n_q + q0 + qi] = l == 0.f ? INFINITY : m * c2 + __builtin_amdgcn_logf(l);
+      a.lse[int64_t(h) * a.n_q + q0 + qi] = l == 0.f ? INFINITY : base + __builtin_amdgcn_logf(l);
   }
 }
 
@@ -216,7 +265,8 @@ __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
   __shared__ __align__(16) char buf[kBytes];
   __shared__ float ml[4][32][2];
   extern __shared__ float tabs[];  // [group][kTable] with a bias
-  const int tid = tid_x(), lane = tid & 63, wave = tid >> 6, half = lane >> 5, l32 = lane & 31;
+  const int tid = tid_x(), lane = tid & 63, half = lane >> 5, l32 = lane & 31;
+  const int wave = wave_id();
   const int bid = wg_x();
   const int kvh = bid % a.Hkv, split = (bid / a.Hkv) % fa.splits, w = bid / (a.Hkv * fa.splits);
   const int G = a.H / a.Hkv;
@@ -250,9 +300,7 @@ __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
     __syncthreads();
   }
   const float s2 = a.scale * kLog2e;
-  const float c2 = BIAS ? 1.f : s2;
-  const float step = kRebase / c2;
-  float m = -INFINITY, thr = -INFINITY, l = 0.f;
+  RowSoftmax sm(BIAS ? 1.f : s2, BIAS ? 1.f / s2 : 1.f);
   f32x16 acc[L::kCols];
 #pragma unroll
   for (int c = 0; c < L::kCols; ++c) acc[c] = fill16(0.f);
@@ -274,7 +322,7 @@ __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
   if (t < t_end) fetch(t);
   while (t < t_end) {
     const int kt = 32 * t;
-    f32x16 x[1] = {fill16(0.f)};
+    f32x16 x[1] = {sm.start};
 #pragma unroll
     for (int c = 0; c < L::kChunks; ++c) x[0] = mma_rows<T>(pk.w[c], q.w[c], x[0]);
     if constexpr (BIAS) {
@@ -289,7 +337,7 @@ __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
       for (int i = 0; i < 16; ++i)
         if (kt + 16 * half + i > lim) x[0][i] = -INFINITY;
     }
-    softmax_step<1>(x, c2, step, m, thr, l, acc);
+    sm.weights(x, acc);
     // the wave's own tile: its writes above, then its reads
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -299,9 +347,9 @@ __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
   }
 
   // join the four waves, in wave order
-  l = sum_halves(l);
+  const float l = sum_halves(sm.l);
   if (half == 0) {
-    ml[wave][l32][0] = m * c2;
+    ml[wave][l32][0] = sm.base();
     ml[wave][l32][1] = l;
   }
   __syncthreads();
@@ -311,7 +359,7 @@ __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
   for (int i = 0; i < 4; ++i) top = fmaxf(top, ml[i][jr][0]);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    f[i] = ml[i][jr][1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[i][jr][0] - top);
+    f[i] = ml[i][jr][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[i][jr][0] - top);
     sum += ml[i][jr][1] * f[i];
   }
   const int64_t slot = (int64_t(w) * a.Hkv + kvh) * fa.splits + split;
@@ -374,11 +422,10 @@ __global__ __launch_bounds__(256) void k_packed_few_join(FewArgs fa) {
 #pragma unroll
   for (int i = 0; i < DP / 8; ++i) o[i] = 0.f;
   for (int s = 0; s < fa.splits; ++s)
-    if (fa.part_ml[((slot + s) * 32 + jr) * 2 + 1] != 0.f)
-      top = fmaxf(top, fa.part_ml[((slot + s) * 32 + jr) * 2]);
+    top = fmaxf(top, fa.part_ml[((slot + s) * 32 + jr) * 2]);
   for (int s = 0; s < fa.splits; ++s) {
     const float* ml = fa.part_ml + ((slot + s) * 32 + jr) * 2;
-    if (ml[1] == 0.f) continue;
+    if (ml[0] == -INFINITY) continue;
     const float f = __builtin_amdgcn_exp2f(ml[0] - top);
     sum = fmaf(ml[1], f, sum);
 #pragma unroll
@@ -459,20 +506,33 @@ __global__ __launch_bounds__(256) void k_packed_buckets(const I* __restrict__ id
 
 // ------------------------------------------------------------------ host side
 constexpr int kTargetBlocks = 512;  // two blocks for each of the 256 compute units
+constexpr int kSimds = 1024;
+constexpr size_t kLds = 160 * 1024;
 
 inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
-// Index of the work list of 32 << i rows.
-inline int waves_of(int i) { return 1 << i; }
+inline int list_of(Shape s) { return s.rw == 4 ? 2 : s.rw == 2 ? 1 : 0; }
 
-// How many waves (32 rows each) a block has: as many as the longest window
-// fills, up to 4, and fewer where the grid would leave compute units without a
-// block: more rows a block share each staged tile, more blocks fill the chip.
-int pick_list(int32_t longest, const int32_t n_items[3], int heads, int most) {
-  int i = longest <= 32 ? 0 : longest <= 64 ? 1 : 2;
-  if (i > most) i = most;
-  while (i > 0 && int64_t(n_items[i]) * heads < kTargetBlocks) --i;
-  return i;
+// The block's shape.  Row waves: as many as the longest window fills, up to 4.
+// Sets: a wave's path is the stages it passes through, `path` for the longest
+// window; with `steps` of them over all waves a SIMD's share is steps / 1024, and
+// a path of more than 0.7 of that share leaves the chip waiting for the longest
+// blocks: then 2 or 4 sets take turns.  (us, 1 / 2 / 4 sets: dK/dV of 6 windows up
+// to 4,096, 4 heads a group, path 2.5 shares, 340 / 265 / 181; fp32 3,001 rows, 8
+// heads, 1.4 shares, 592 / 544 / 610 for the three passes; 24 windows up to 1,500, 8
+// heads, 0.6 shares, 114 / 120 / 145.)
+// stage: LDS bytes of 64 rows of both tiles; wave: bytes of each wave beside them.
+Shape pick_shape(int32_t longest, int64_t path, int64_t steps, size_t stage, size_t wave,
+                 int most) {
+  if (longest <= 32) return Shape{1, 1};
+  Shape s{longest <= 64 ? 2 : 4, 1};
+  auto over = [&](int ks) { return path * 10 * kSimds > 7 * ks * steps && ks * 2 <= path; };
+  if (most >= 2 && over(1)) s.ks = 2;
+  if (most >= 4 && s.ks == 2 && over(2)) s = Shape{2, 4};
+  auto bytes = [&] { return s.ks * stage + size_t(s.rw) * s.ks * wave + 6 * 1024; };
+  while (bytes() > kLds && s.ks > 1) s = Shape{2, s.ks / 2};
+  while (bytes() > kLds && s.rw > 1) s.rw /= 2;
+  return s;
 }
 
 struct FewPlan {
@@ -512,7 +572,8 @@ int check_call(const char* fn, int dtype, const ngt_packed_windows* w, int H, in
     return set_error(NGT_ERR_UNSUPPORTED, "%s: head_dim=%d (a multiple of 8 up to 128)", fn, d);
   if (!(scale > 0.f) || !(scale < INFINITY))
     return set_error(NGT_ERR_ARG, "%s: scale must be finite and > 0", fn);
-  if (w->n_windows < 0 || w->n_q < 0 || w->n_k < 0 || w->max_q < 0 || w->max_k < 0)
+  if (w->n_windows < 0 || w->n_q < 0 || w->n_k < 0 || w->max_q < 0 || w->max_k < 0 || w->steps_q < 0 ||
+      w->steps_k < 0)
     return set_error(NGT_ERR_ARG, "%s: bad windows", fn);
   for (int i = 0; i < 3; ++i)
     if (w->n_items_q[i] < 0 || w->n_items_k[i] < 0 ||
@@ -558,16 +619,21 @@ int run_fwd(const ngt_packed_windows& w, const FewPlan& fp, FwdArgs a, void* ws,
     }
     return NGT_OK;
   }
-  const int i = pick_list(w.max_q, w.n_items_q, a.H, 2);
+  constexpr int kMost = most_sets(Tile<T, DP>::kPitch, false);
+  const Shape shape =
+      pick_shape(w.max_q, (w.max_k + 63) / 64, w.steps_q * a.H, 128 * Tile<T, DP>::kPitch, 512,
+                 kMost);
+  const int i = list_of(shape);
   const unsigned blocks = unsigned(w.n_items_q[i]) * unsigned(a.H);
   if (!blocks) return NGT_OK;
   a.items = reinterpret_cast<const int2*>(w.items_q[i]);
   KernelTimer timer_("packed_fwd", st);
-  if (i == 2) hipLaunchKernelGGL((k_packed_fwd<T, DP, BIAS, 4>), dim3(blocks), dim3(256), 0, st, a);
-  else if (i == 1) hipLaunchKernelGGL((k_packed_fwd<T, DP, BIAS, 2>), dim3(blocks), dim3(128), 0, st, a);
-  else hipLaunchKernelGGL((k_packed_fwd<T, DP, BIAS, 1>), dim3(blocks), dim3(64), 0, st, a);
-  NGT_HIP_CHECK(hipGetLastError());
-  return NGT_OK;
+  return with_shape<kMost>(shape, [&](auto rw, auto ks) {
+    hipLaunchKernelGGL((k_packed_fwd<T, DP, BIAS, rw.value, ks.value>), dim3(blocks),
+                       dim3(64 * rw.value * ks.value), 0, st, a);
+    NGT_HIP_CHECK(hipGetLastError());
+    return int(NGT_OK);
+  });
 }
 
 template <typename T>
@@ -584,19 +650,18 @@ int run_fwd_d(int dp, const ngt_packed_windows& w, const FewPlan& fp, const FwdA
 
 struct BwdLayout {
   size_t part, total;
-  int list_q, list_k;
+  Shape dq, dkv;
 };
 BwdLayout bwd_layout(int dtype, const ngt_packed_windows& w, int H, int Hkv, int d, int n_buckets) {
   BwdLayout L{};
-  const int es = dtype == NGT_F32 ? 4 : 2;
-  int most = 2;
-  // with a table gradient a wave holds 64 sums per bucket beside the block's two tiles
-  const size_t fixed = 2 * size_t(64) * dp_of(d) * es + 2048;
-  while (most > 0 && fixed + size_t(waves_of(most)) * (n_buckets + 1) * 256 > 160 * 1024) --most;
-  L.list_q = pick_list(w.max_q, w.n_items_q, H, most);
-  L.list_k = pick_list(w.max_k, w.n_items_k, Hkv, 2);
+  const int row = dp_of(d) * (dtype == NGT_F32 ? 4 : 2);  // bytes of a tile's row
+  // with a table gradient a wave holds 64 sums per bucket
+  L.dq = pick_shape(w.max_q, (w.max_k + 63) / 64, w.steps_q * H, size_t(128) * row,
+                    n_buckets ? size_t(n_buckets + 1) * 256 : 0, most_sets(row, false));
+  L.dkv = pick_shape(w.max_k, int64_t((w.max_q + 63) / 64) * (H / Hkv), w.steps_k * H,
+                     size_t(128) * row, 0, most_sets(row, true));
   L.part = align256(size_t(w.n_q) * H * 4);
-  L.total = L.part + align256(size_t(w.n_items_q[L.list_q]) * H * n_buckets * 4);
+  L.total = L.part + align256(size_t(w.n_items_q[list_of(L.dq)]) * H * n_buckets * 4);
   return L;
 }
 
@@ -707,7 +772,10 @@ extern "C" int ngt_packed_plan(int32_t n_windows, const int32_t* q_len, const in
         const int64_t top = ((o ? out->max_q : out->max_k) + 63) / 64;
         std::vector<int64_t> at(size_t(top) + 2, 0);
         for (int32_t w = 0; w < n_windows; ++w)
-          for (int32_t r = 0; r < (o ? k_len[w] : q_len[w]); r += rows) ++at[size_t(top - steps(w, r)) + 1];
+          for (int32_t r = 0; r < (o ? k_len[w] : q_len[w]); r += rows) {
+          ++at[size_t(top - steps(w, r)) + 1];
+          if (i == 0) (o ? out->steps_k : out->steps_q) += steps(w, r);
+        }
         for (size_t j = 1; j < at.size(); ++j) at[j] += at[j - 1];
         for (int32_t w = 0; w < n_windows; ++w)
           for (int32_t r = 0; r < (o ? k_len[w] : q_len[w]); r += rows) {
@@ -830,12 +898,11 @@ extern "C" int ngt_packed_bwd(int dtype, const void* q, const void* k, const voi
   a.part_table = reinterpret_cast<float*>(ws + L.part);
   a.gq = grad_q, a.gk = grad_k, a.gv = grad_v, a.grad_table = grad_table;
   BwdPlan p{};
-  p.items_q = reinterpret_cast<const int2*>(w->items_q[L.list_q]);
-  p.items_k = reinterpret_cast<const int2*>(w->items_k[L.list_k]);
-  p.n_items_q = w->n_items_q[L.list_q];
-  p.dq_waves = waves_of(L.list_q);
-  p.dkv_waves = waves_of(L.list_k);
+  p.dq = L.dq, p.dkv = L.dkv;
+  p.items_q = reinterpret_cast<const int2*>(w->items_q[list_of(L.dq)]);
+  p.items_k = reinterpret_cast<const int2*>(w->items_k[list_of(L.dkv)]);
+  p.n_items_q = w->n_items_q[list_of(L.dq)];
   p.dq_blocks = int64_t(p.n_items_q) * n_heads;
-  p.dkv_blocks = int64_t(w->n_items_k[L.list_k]) * n_kv_heads;
+  p.dkv_blocks = int64_t(w->n_items_k[list_of(L.dkv)]) * n_kv_heads;
   return packed_bwd(dtype, p, a, static_cast<hipStream_t>(stream));
 }

@@ -5,24 +5,38 @@ namespace ngt {
 namespace packed {
 namespace {
 
-constexpr int kRows = 64;  // rows of one stage
+// Adds a lane's 16 values to the wave's running sums of their buckets, in the
+// lane's column: hist[bucket][l % 32], doubles.  LDS adds a double in 9 clocks
+// a wave instruction where a float takes 193 (3 a lane); reading, adding and
+// writing back takes 10 and seven compares and selects a value.  Only the two
+// halves of one row share a column.
+__device__ __forceinline__ void add_to_buckets(double* hist, const u32x4& ids, const f32x16& x,
+                                               int n_buckets) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    unsafeAtomicAdd(hist + min(bucket_of(ids, i), n_buckets) * 32, static_cast<double>(x[i]));
+}
 
-// dQ, D = G . out and the bias's gradient.  One block: NW * 32 query rows of
-// one window and head, a wave 32 of them (lane = query); the window's keys pass
-// through LDS 64 at a time.
+// dQ, D = G . out and the bias's gradient.  One block: RW * 32 query rows of
+// one window and head (lane = query); the window's keys pass through LDS
+// 64 * KS at a time.
 //   S^T = K Q^T, dP^T = V G^T, P = exp2(S - lse), dS = P (dP - D), dQ^T += K^T dS^T
-// HIST: the wave keeps 64 running sums per bucket, one a lane, so that every
+// HIST: the wave keeps 32 running sums per bucket, one a row, so that every
 // sum has a fixed order; the block adds them up at its end.
-template <typename T, int DP, bool BIAS, bool HIST, int NW>
-__global__ __launch_bounds__(64 * NW) void k_packed_dq(BwdArgs a) {
+template <typename T, int DP, bool BIAS, bool HIST, int RW, int KS>
+__global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
   using L = Tile<T, DP>;
-  constexpr int N = 64 * NW;
+  using B = Block<RW, KS>;
+  constexpr int N = B::kThreads, kRows = B::kStage;
+  constexpr int kTileBytes = kRows * L::kPitch;
   constexpr bool kAhead = (kRows * L::kPieces / N) * 8 <= 32;
-  __shared__ __align__(16) char ks[kRows * L::kPitch];
-  __shared__ __align__(16) char vs[kRows * L::kPitch];
+  __shared__ __align__(16) char
+      buf[2 * kTileBytes > B::kJoinBytes ? 2 * kTileBytes : B::kJoinBytes];
   __shared__ float tab[BIAS ? kTable : 1];
-  extern __shared__ float hist[];  // HIST: [NW][n_buckets + 1][64]
-  const int tid = tid_x(), lane = tid & 63, wave = tid >> 6, half = lane >> 5, l32 = lane & 31;
+  extern __shared__ __align__(8) double hist[];  // HIST: [RW * KS][n_buckets + 1][32]
+  char *const ks = buf, *const vs = buf + kTileBytes;
+  const int tid = tid_x(), lane = tid & 63, half = lane >> 5, l32 = lane & 31;
+  const int wid = wave_id(), wave = wid % RW, set = wid / RW;
   const int bid = wg_x();
   const int kvh = bid % a.Hkv, grp = (bid / a.Hkv) % (a.H / a.Hkv);
   const int h = kvh * (a.H / a.Hkv) + grp;
@@ -38,7 +52,7 @@ __global__ __launch_bounds__(64 * NW) void k_packed_dq(BwdArgs a) {
   const int first_lim = a.causal ? min(item.y + wave * 32 + ahead, nk - 1) : nk - 1;
   const int last_q = min(item.y + wave * 32 + 31, nq - 1);
   const int wave_end = item.y + wave * 32 >= nq ? 0 : a.causal ? min(last_q + ahead + 1, nk) : nk;
-  const int block_end = a.causal ? min(min(item.y + 32 * NW, nq) + ahead, nk) : nk;
+  const int block_end = a.causal ? min(min(item.y + 32 * RW, nq) + ahead, nk) : nk;
   const T* kb = reinterpret_cast<const T*>(reinterpret_cast<const char*>(a.k) + k0 * a.sk) +
                 int64_t(kvh) * a.d;
   const T* vb = reinterpret_cast<const T*>(reinterpret_cast<const char*>(a.v) + k0 * a.sv) +
@@ -77,34 +91,40 @@ __global__ __launch_bounds__(64 * NW) void k_packed_dq(BwdArgs a) {
   D = sum_halves(D);
   // a lane without a row has no weight anywhere
   const float lse = qi < nq ? a.lse[int64_t(h) * a.n_q + q0 + qi] : INFINITY;
-  if (qi < nq && half == 0) a.dsum[int64_t(h) * a.n_q + q0 + qi] = D;
+  if (qi < nq && half == 0 && set == 0) a.dsum[int64_t(h) * a.n_q + q0 + qi] = -D;
 
   const uint8_t* ids = nullptr;
-  float* my_hist = nullptr;
+  double* my_hist = nullptr;
   if constexpr (BIAS) {
     load_table(tab, reinterpret_cast<const T*>(a.table), a.n_buckets, a.H, h, tid, N);
     ids = a.ids + a.b_start[item.x] + int64_t(qc) * ((nk + 63) & ~63) + 16 * half;
   }
   if constexpr (HIST) {
-    for (int i = tid; i < NW * (a.n_buckets + 1) * 64; i += N) hist[i] = 0.f;
-    my_hist = hist + wave * (a.n_buckets + 1) * 64 + lane;
+    for (int i = tid; i < RW * KS * (a.n_buckets + 1) * 32; i += N) hist[i] = 0.;
+    my_hist = hist + wid * (a.n_buckets + 1) * 32 + l32;
   }
   const float s2 = a.scale * kLog2e;
+  // the products start from -lse (with a bias; in their units) and -D
+  const f32x16 s_start = fill16(BIAS ? -lse / s2 : 0.f), dp_start = fill16(-D);
   f32x16 acc[L::kCols];
 #pragma unroll
   for (int c = 0; c < L::kCols; ++c) acc[c] = fill16(0.f);
 
   Stage<T, DP, kRows, N> pk, pv;
-  u32x4 idw[2];
+  u32x4 idw[2], id_next[2];
+  auto fetch_ids = [&](int k1) {  // of keys that are there
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      if (BIAS && k1 < nk) id_next[t] = *reinterpret_cast<const u32x4*>(ids + k1 + 32 * t);
+  };
+  fetch_ids(64 * set);
   if constexpr (kAhead) {
     pk.load(kb, a.sk, 0, nk, a.d, tid);
     pv.load(vb, a.sv, 0, nk, a.d, tid);
   }
+  const char* k_tile = ks + 64 * set * L::kPitch;
+  const char* v_tile = vs + 64 * set * L::kPitch;
   for (int kt = 0; kt < block_end; kt += kRows) {
-    if constexpr (BIAS) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) idw[t] = *reinterpret_cast<const u32x4*>(ids + kt + 32 * t);
-    }
     __syncthreads();
     if constexpr (!kAhead) {
       pk.load(kb, a.sk, kt, nk, a.d, tid);
@@ -116,44 +136,42 @@ __global__ __launch_bounds__(64 * NW) void k_packed_dq(BwdArgs a) {
       pv.store(vs, tid);
     }
     __syncthreads();
+    idw[0] = id_next[0], idw[1] = id_next[1];
+    fetch_ids(kt + kRows + 64 * set);
     if constexpr (kAhead) {
       if (kt + kRows < block_end) {
         pk.load(kb, a.sk, kt + kRows, nk, a.d, tid);
         pv.load(vb, a.sv, kt + kRows, nk, a.d, tid);
       }
     }
-    if (kt >= wave_end) continue;
+    const int k1 = kt + 64 * set;  // this set's first key
+    if (k1 >= wave_end) continue;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      if (t == 1 && kt + 32 >= wave_end) break;
-      f32x16 s = fill16(0.f), dp = fill16(-D);
+      if (t == 1 && k1 + 32 >= wave_end) break;
+      f32x16 s = s_start, dp = dp_start;
 #pragma unroll
       for (int c = 0; c < L::kChunks; ++c) {
-        s = mma_rows<T>(L::load_a(ks, t, c, l32, half), q.w[c], s);
-        dp = mma_rows<T>(L::load_a(vs, t, c, l32, half), g.w[c], dp);
+        s = mma_rows<T>(L::load_a(k_tile, t, c, l32, half), q.w[c], s);
+        dp = mma_rows<T>(L::load_a(v_tile, t, c, l32, half), g.w[c], dp);
       }
-      const bool cut = kt + 32 * t + 31 > first_lim;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float x;
-        if constexpr (BIAS)
-          x = fmaf(s[i], s2, tab[bucket_of(idw[t], i)]) - lse;
-        else
-          x = fmaf(s[i], s2, -lse);
-        if (cut && kt + 32 * t + 16 * half + i > lim) x = -INFINITY;
-        s[i] = __builtin_amdgcn_exp2f(x) * dp[i];
-      }
-      if constexpr (HIST) {
+      for (int i = 0; i < 16; ++i)
+        s[i] = fmaf(s[i], s2, BIAS ? tab[bucket_of(idw[t], i)] : -lse);
+      if (k1 + 32 * t + 31 > first_lim) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int b = min(bucket_of(idw[t], i), a.n_buckets);
-          atomicAdd(my_hist + b * 64, s[i]);  // the lane's own word: no other writes it
-        }
+        for (int i = 0; i < 16; ++i)
+          if (k1 + 32 * t + 16 * half + i > lim) s[i] = -INFINITY;
       }
-      L::mma_cols(ks, t, s, acc, lane);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i]) * dp[i];
+      if constexpr (HIST) add_to_buckets(my_hist, idw[t], s, a.n_buckets);
+      L::mma_cols(k_tile, t, s, acc, lane);
     }
   }
-  if (qi < nq) {
+#pragma unroll
+  for (int c = 0; c < L::kCols; ++c) join_sets<RW, KS>(acc[c], buf, wave, set, lane);
+  if (qi < nq && set == 0) {
     T* o = reinterpret_cast<T*>(a.gq) + ((q0 + qi) * a.H + h) * int64_t(a.d);
 #pragma unroll
     for (int c = 0; c < L::kCols; ++c)
@@ -168,33 +186,38 @@ __global__ __launch_bounds__(64 * NW) void k_packed_dq(BwdArgs a) {
   if constexpr (HIST) {
     __syncthreads();
     for (int b = tid; b < a.n_buckets; b += N) {
-      float sum = 0.f;
-      for (int w = 0; w < NW; ++w) {
-        const float* hw = hist + (w * (a.n_buckets + 1) + b) * 64;
-        float s = 0.f;
-        for (int i = 0; i < 64; ++i) s += hw[(i + b) & 63];  // from its own place: no bank twice
-        sum += s;
+      double sum = 0.;
+      for (int w = 0; w < RW * KS; ++w) {
+        const double* hw = hist + (w * (a.n_buckets + 1) + b) * 32;
+        for (int i = 0; i < 32; ++i) sum += hw[(i + b) & 31];  // from its own place: no bank twice
       }
-      a.part_table[(int64_t(h) * a.n_items + it) * a.n_buckets + b] = sum;
+      a.part_table[(int64_t(h) * a.n_items + it) * a.n_buckets + b] = static_cast<float>(sum);
     }
   }
 }
 
-// dK and dV.  One block: NW * 32 keys of one window and key head, a wave 32 of
-// them (lane = key); the rows of the group's heads that see them pass through
-// LDS 64 at a time, head after head: dK and dV of shared heads are one sum.
+// dK and dV.  One block: RW * 32 keys of one window and key head (lane = key);
+// the rows of the group's heads that see them pass through LDS 64 * KS at a
+// time, head after head: dK and dV of shared heads are one sum.
 //   S = Q K^T, dP = G V^T, P = exp2(S - lse), dS = P (dP - D)
 //   dV^T += G^T P, dK^T += Q^T dS
-template <typename T, int DP, bool BIAS, int NW>
-__global__ __launch_bounds__(64 * NW) void k_packed_dkv(BwdArgs a) {
+// With a bias, whose table lookups it waits for, three waves a SIMD where the
+// registers allow it: 32 heads of 24, 8,556 rows, 379 -> 343 us (without, 42 -> 45).
+template <typename T, int DP, bool BIAS, int RW, int KS>
+__global__ __launch_bounds__(64 * RW * KS, BIAS && DP == 32 && sizeof(T) == 2 ? 3 : 1) void
+k_packed_dkv(BwdArgs a) {
   using L = Tile<T, DP>;
-  constexpr int N = 64 * NW;
+  using B = Block<RW, KS>;
+  constexpr int N = B::kThreads, kRows = B::kStage;
+  constexpr int kTileBytes = kRows * L::kPitch;
   constexpr bool kAhead = (kRows * L::kPieces / N) * 8 <= 32;
-  __shared__ __align__(16) char qs[kRows * L::kPitch];
-  __shared__ __align__(16) char gs[kRows * L::kPitch];
+  __shared__ __align__(16) char
+      buf[2 * kTileBytes > B::kJoinBytes ? 2 * kTileBytes : B::kJoinBytes];
   __shared__ __align__(16) float ls[kRows], ds[kRows];
   __shared__ float tab[BIAS ? kTable : 1];
-  const int tid = tid_x(), lane = tid & 63, wave = tid >> 6, half = lane >> 5, l32 = lane & 31;
+  char *const qs = buf, *const gs = buf + kTileBytes;
+  const int tid = tid_x(), lane = tid & 63, half = lane >> 5, l32 = lane & 31;
+  const int wid = wave_id(), wave = wid % RW, set = wid / RW;
   const int kvh = wg_x() % a.Hkv;
   const int2 item = a.items[wg_x() / a.Hkv];
   const int G = a.H / a.Hkv;
@@ -206,7 +229,7 @@ __global__ __launch_bounds__(64 * NW) void k_packed_dkv(BwdArgs a) {
   const int kc = min(kj, nk - 1);
   // the first query that sees this key, the block's first key, the wave's last one
   const int lim = a.causal ? kc - ahead : 0;
-  const int block_begin = a.causal ? max(0, item.y - ahead) & ~(kRows - 1) : 0;
+  const int block_begin = a.causal ? max(0, item.y - ahead) & ~63 : 0;
   const int wave_begin = a.causal ? max(0, item.y + wave * 32 - ahead) : 0;
   const int last_lim = a.causal ? item.y + wave * 32 + 31 - ahead : 0;
   RowFrag<T, DP> k, v;
@@ -225,7 +248,11 @@ __global__ __launch_bounds__(64 * NW) void k_packed_dkv(BwdArgs a) {
   for (int c = 0; c < L::kCols; ++c) ak[c] = fill16(0.f), av[c] = fill16(0.f);
 
   Stage<T, DP, kRows, N> pq, pg;
+  const float lse_per = -1.f / s2;  // into product units
   float pl = 0.f, pd = 0.f;
+  u32x4 idw[2], id_next[2];
+  const char* q_tile = qs + 64 * set * L::kPitch;
+  const char* g_tile = gs + 64 * set * L::kPitch;
   for (int grp = 0; grp < G; ++grp) {
     const int h = kvh * G + grp;
     const T* qb = reinterpret_cast<const T*>(reinterpret_cast<const char*>(a.q) + q0 * a.sq) +
@@ -235,6 +262,10 @@ __global__ __launch_bounds__(64 * NW) void k_packed_dkv(BwdArgs a) {
     const float* lse = a.lse + int64_t(h) * a.n_q + q0;
     const float* dsum = a.dsum + int64_t(h) * a.n_q + q0;
     auto fetch = [&](int qt) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)  // of queries that are there
+        if (BIAS && qt + 64 * set < nq)
+          id_next[t] = *reinterpret_cast<const u32x4*>(ids + qt + 64 * set + 32 * t);
       if (tid < kRows) {  // a row that is not there has no weight
         pl = qt + tid < nq ? lse[qt + tid] : INFINITY;
         pd = qt + tid < nq ? dsum[qt + tid] : 0.f;
@@ -250,11 +281,6 @@ __global__ __launch_bounds__(64 * NW) void k_packed_dkv(BwdArgs a) {
     }
     fetch(block_begin);
     for (int qt = block_begin; qt < nq; qt += kRows) {
-      u32x4 idw[2];
-      if constexpr (BIAS) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) idw[t] = *reinterpret_cast<const u32x4*>(ids + qt + 32 * t);
-      }
       __syncthreads();
       if constexpr (!kAhead) {
         pq.load(qb, a.sq, qt, nq, a.d, tid);
@@ -265,47 +291,52 @@ __global__ __launch_bounds__(64 * NW) void k_packed_dkv(BwdArgs a) {
         pq.store(qs, tid);
         pg.store(gs, tid);
       }
-      if (tid < kRows) ls[tid] = pl, ds[tid] = pd;
+      if (tid < kRows) ls[tid] = pl * lse_per, ds[tid] = pd;
       __syncthreads();
+      idw[0] = id_next[0], idw[1] = id_next[1];
       if (qt + kRows < nq) fetch(qt + kRows);
-      if (qt + kRows <= wave_begin || item.y + wave * 32 >= nk) continue;
+      const int q1 = qt + 64 * set;  // this set's first query
+      if (q1 + 64 <= wave_begin || q1 >= nq || item.y + wave * 32 >= nk) continue;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        f32x16 s = fill16(0.f), dp;
+        f32x16 s, dp;  // start from -lse, in product units, and -D of the rows
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float4 y = *reinterpret_cast<const float4*>(ds + 32 * t + 16 * half + 4 * i);
-          dp[4 * i] = -y.x, dp[4 * i + 1] = -y.y, dp[4 * i + 2] = -y.z, dp[4 * i + 3] = -y.w;
+          const int at = 64 * set + 32 * t + 16 * half + 4 * i;
+          const float4 x = *reinterpret_cast<const float4*>(ls + at);
+          const float4 y = *reinterpret_cast<const float4*>(ds + at);
+          s[4 * i] = x.x, s[4 * i + 1] = x.y, s[4 * i + 2] = x.z, s[4 * i + 3] = x.w;
+          dp[4 * i] = y.x, dp[4 * i + 1] = y.y, dp[4 * i + 2] = y.z, dp[4 * i + 3] = y.w;
         }
 #pragma unroll
         for (int c = 0; c < L::kChunks; ++c) {
-          s = mma_rows<T>(L::load_a(qs, t, c, l32, half), k.w[c], s);
-          dp = mma_rows<T>(L::load_a(gs, t, c, l32, half), v.w[c], dp);
+          s = mma_rows<T>(L::load_a(q_tile, t, c, l32, half), k.w[c], s);
+          dp = mma_rows<T>(L::load_a(g_tile, t, c, l32, half), v.w[c], dp);
         }
-        const bool cut = qt + 32 * t < last_lim;
 #pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-          const float4 y = *reinterpret_cast<const float4*>(ls + 32 * t + 16 * half + 4 * i4);
-          const float lv[4] = {y.x, y.y, y.z, y.w};
+        for (int i = 0; i < 16; ++i)
+          s[i] = BIAS ? fmaf(s[i], s2, tab[bucket_of(idw[t], i)]) : s[i] * s2;
+        if (q1 + 32 * t < last_lim) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int i = 4 * i4 + j;
-            float x;
-            if constexpr (BIAS)
-              x = fmaf(s[i], s2, tab[bucket_of(idw[t], i)]) - lv[j];
-            else
-              x = fmaf(s[i], s2, -lv[j]);
-            if (cut && qt + 32 * t + 16 * half + i < lim) x = -INFINITY;
-            s[i] = __builtin_amdgcn_exp2f(x);
-            dp[i] *= s[i];
-          }
+          for (int i = 0; i < 16; ++i)
+            if (q1 + 32 * t + 16 * half + i < lim) s[i] = -INFINITY;
         }
-        L::mma_cols(gs, t, s, av, lane);
-        L::mma_cols(qs, t, dp, ak, lane);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          s[i] = __builtin_amdgcn_exp2f(s[i]);
+          dp[i] *= s[i];
+        }
+        L::mma_cols(g_tile, t, s, av, lane);
+        L::mma_cols(q_tile, t, dp, ak, lane);
       }
     }
   }
-  if (kj < nk) {
+#pragma unroll
+  for (int c = 0; c < L::kCols; ++c) {
+    join_sets<RW, KS>(ak[c], buf, wave, set, lane);
+    join_sets<RW, KS>(av[c], buf, wave, set, lane);
+  }
+  if (kj < nk && set == 0) {
     const int64_t row = ((k0 + kj) * a.Hkv + kvh) * int64_t(a.d);
     T* ok = reinterpret_cast<T*>(a.gk) + row;
     T* ov = reinterpret_cast<T*>(a.gv) + row;
@@ -347,19 +378,29 @@ __global__ __launch_bounds__(1024) void k_packed_table_grad(const float* __restr
 }
 
 template <typename T, int DP, bool BIAS, bool HIST>
-int launch_dq(const BwdArgs& a, int nw, int64_t blocks, size_t lds, hipStream_t st) {
+int launch_dq(const BwdArgs& a, const BwdPlan& p, size_t lds, hipStream_t st) {
   KernelTimer timer_("packed_dq", st);
-  auto run = [&](auto kernel) {
+  return with_shape<most_sets(Tile<T, DP>::kPitch, false)>(p.dq, [&](auto rw, auto ks) {
+    auto kernel = k_packed_dq<T, DP, BIAS, HIST, rw.value, ks.value>;
     if (lds)
       NGT_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                         hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)));
-    hipLaunchKernelGGL(kernel, dim3(unsigned(blocks)), dim3(64 * nw), lds, st, a);
+    hipLaunchKernelGGL(kernel, dim3(unsigned(p.dq_blocks)), dim3(64 * rw.value * ks.value), lds, st,
+                       a);
     NGT_HIP_CHECK(hipGetLastError());
     return int(NGT_OK);
-  };
-  if (nw == 4) return run(k_packed_dq<T, DP, BIAS, HIST, 4>);
-  if (nw == 2) return run(k_packed_dq<T, DP, BIAS, HIST, 2>);
-  return run(k_packed_dq<T, DP, BIAS, HIST, 1>);
+  });
+}
+
+template <typename T, int DP, bool BIAS>
+int launch_dkv(const BwdArgs& a, const BwdPlan& p, hipStream_t st) {
+  KernelTimer timer_("packed_dkv", st);
+  return with_shape<most_sets(Tile<T, DP>::kPitch, true)>(p.dkv, [&](auto rw, auto ks) {
+    hipLaunchKernelGGL((k_packed_dkv<T, DP, BIAS, rw.value, ks.value>), dim3(unsigned(p.dkv_blocks)),
+                       dim3(64 * rw.value * ks.value), 0, st, a);
+    NGT_HIP_CHECK(hipGetLastError());
+    return int(NGT_OK);
+  });
 }
 
 template <typename T, int DP>
@@ -369,27 +410,14 @@ int bwd(const BwdPlan& p, const BwdArgs& base, hipStream_t st) {
   if (p.dq_blocks > 0) {
     a.items = p.items_q;
     a.n_items = p.n_items_q;
-    const size_t lds = hist ? size_t(p.dq_waves) * (a.n_buckets + 1) * 256 : 0;
-    NGT_CHECK_OK(hist   ? (launch_dq<T, DP, true, true>(a, p.dq_waves, p.dq_blocks, lds, st))
-                 : bias ? (launch_dq<T, DP, true, false>(a, p.dq_waves, p.dq_blocks, 0, st))
-                        : (launch_dq<T, DP, false, false>(a, p.dq_waves, p.dq_blocks, 0, st)));
+    const size_t lds = size_t(p.dq.rw) * p.dq.ks * (a.n_buckets + 1) * 256;
+    NGT_CHECK_OK(hist   ? (launch_dq<T, DP, true, true>(a, p, lds, st))
+                 : bias ? (launch_dq<T, DP, true, false>(a, p, 0, st))
+                        : (launch_dq<T, DP, false, false>(a, p, 0, st)));
   }
   if (p.dkv_blocks > 0) {
-    KernelTimer timer_("packed_dkv", st);
     a.items = p.items_k;
-    auto run = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(unsigned(p.dkv_blocks)), dim3(64 * p.dkv_waves), 0, st, a);
-    };
-    if (bias) {
-      if (p.dkv_waves == 4) run(k_packed_dkv<T, DP, true, 4>);
-      else if (p.dkv_waves == 2) run(k_packed_dkv<T, DP, true, 2>);
-      else run(k_packed_dkv<T, DP, true, 1>);
-    } else {
-      if (p.dkv_waves == 4) run(k_packed_dkv<T, DP, false, 4>);
-      else if (p.dkv_waves == 2) run(k_packed_dkv<T, DP, false, 2>);
-      else run(k_packed_dkv<T, DP, false, 1>);
-    }
-    NGT_HIP_CHECK(hipGetLastError());
+    NGT_CHECK_OK(bias ? (launch_dkv<T, DP, true>(a, p, st)) : (launch_dkv<T, DP, false>(a, p, st)));
   }
   if (hist) {
     KernelTimer timer_("packed_table_grad", st);
