@@ -265,9 +265,10 @@ def autograd_ext():
                     # prototypes the extension was compiled with
                     raise RuntimeError(f"{EXT_PATH.name} was built against ABI version {ext_abi}, "
                                        f"the library is {lib.ngt_abi_version()}; rebuild it")
-                if mod.csr_struct_bytes() != C.sizeof(WindowCSR):
+                if (mod.csr_struct_bytes() != C.sizeof(WindowCSR)
+                        or mod.packed_struct_bytes() != C.sizeof(PackedWindowsC)):
                     raise RuntimeError(f"{EXT_PATH.name} was built against another "
-                                       "ngt_window_csr; rebuild it")
+                                       "ngt_window_csr or ngt_packed_windows; rebuild it")
                 addr = lambda fn: C.cast(fn, C.c_void_p).value
                 mod.init({name: addr(getattr(lib, name)) for name in SIGNATURES})
                 _ext = mod

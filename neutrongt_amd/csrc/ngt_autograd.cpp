@@ -29,10 +29,16 @@
 // launches, 1.4 ms of kernels) took 4.0 ms and take 2.9, a GPH_Large block
 // over 10,007 queries 1.37 -> 0.97 ms, and the core alone over a small window
 // 113 -> 91 us (74 -> 60 us on a faster host).
+//
+// PackedAttention and LinearEpilogue are PackedAttentionFunction (packed.py) and
+// LinearEpilogueFunction (linear.py).  Their entries return nothing where an
+// argument is not one that they take: Python then checks it and says why.
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <c10/hip/HIPStream.h>
 
+#include <cmath>
 #include <map>
 #include <string>
 
@@ -58,6 +64,12 @@ decltype(&ngt_layernorm_bwd_workspace_bytes) g_ln_bwd_ws = nullptr;
 decltype(&ngt_layernorm_bwd) g_ln_bwd = nullptr;
 decltype(&ngt_add_layernorm_fwd) g_add_ln_fwd = nullptr;
 decltype(&ngt_add_layernorm_bwd) g_add_ln_bwd = nullptr;
+decltype(&ngt_packed_workspace_bytes) g_packed_ws = nullptr;
+decltype(&ngt_packed_fwd) g_packed_fwd = nullptr;
+decltype(&ngt_packed_bwd) g_packed_bwd = nullptr;
+decltype(&ngt_linear_fwd) g_linear_fwd = nullptr;
+decltype(&ngt_linear_bwd_workspace_bytes) g_linear_bwd_ws = nullptr;
+decltype(&ngt_linear_bwd) g_linear_bwd = nullptr;
 
 void check(int rc) {
   if (rc != NGT_OK) {
@@ -552,6 +564,293 @@ std::tuple<Tensor, Tensor> add_layernorm(Tensor x, Tensor y, Tensor weight, Tens
   return {r[0], r[1]};
 }
 
+// ------------------------------------------------------------ packed windows
+// Gradients of a backward that cannot itself be differentiated: under
+// create_graph they carry a node that says so.
+tensor_list once(const char* name, tensor_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  tensor_list given;
+  for (auto& g : grads)
+    if (g.defined()) {
+      Tensor t = g.detach();
+      t.set_requires_grad(true);
+      given.push_back(t);
+    }
+  if (given.empty()) return grads;
+  const auto n = static_cast<int64_t>(given.size());
+  auto node = std::make_shared<torch::autograd::DelayedError>(
+      std::string(name) + " is differentiable once", n);
+  given = (*node)(std::move(given));
+  size_t i = 0;
+  for (auto& g : grads)
+    if (g.defined()) g = given[i++];
+  return grads;
+}
+
+// rows [n, heads, d] that the kernels read where they are
+Tensor packed_rows(const Tensor& t) {
+  const int64_t es = t.element_size();
+  if (t.size(0) == 0 ||
+      (t.stride(2) == 1 && t.stride(1) == t.size(2) && t.stride(0) >= t.size(1) * t.size(2) &&
+       t.stride(0) * es % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0))
+    return t;
+  return t.clone(at::MemoryFormat::Contiguous);
+}
+
+const ngt_packed_windows* windows_of(const Tensor& bytes) {
+  return reinterpret_cast<const ngt_packed_windows*>(bytes.data_ptr());
+}
+
+struct PackedForward {
+  Tensor out, out32, lse;
+};
+
+PackedForward packed_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table,
+                             const Tensor& win, const Tensor& by_query, double scale,
+                             bool want_grad) {
+  const int64_t n_q = q.size(0), H = q.size(1), d = q.size(2);
+  const auto f32 = q.options().dtype(at::kFloat);
+  PackedForward r;
+  r.out = at::empty({n_q, H, d}, q.options());
+  if (want_grad) {
+    r.out32 = q.scalar_type() == at::kFloat ? r.out : at::empty({n_q, H, d}, f32);
+    r.lse = at::empty({H, n_q}, f32);
+  }
+  const int dt = dtype_code(q);
+  const auto h = static_cast<int32_t>(H), hkv = static_cast<int32_t>(k.size(1));
+  size_t bytes = 0;
+  check(g_packed_ws(dt, windows_of(win), h, hkv, static_cast<int32_t>(d), 0, &bytes, nullptr));
+  const Tensor ws = bytes ? workspace(static_cast<int64_t>(bytes), q) : Tensor();
+  check(g_packed_fwd(dt, q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), k.stride(0),
+                     v.stride(0), windows_of(win), h, hkv, static_cast<int32_t>(d),
+                     static_cast<float>(scale), table.defined() ? table.data_ptr() : nullptr,
+                     table.defined() ? static_cast<int32_t>(table.size(0)) : 0,
+                     table.defined() ? by_query.data_ptr<uint8_t>() : nullptr, r.out.data_ptr(),
+                     want_grad && !r.out32.is_same(r.out) ? r.out32.data_ptr<float>() : nullptr,
+                     want_grad ? r.lse.data_ptr<float>() : nullptr,
+                     bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)));
+  return r;
+}
+
+struct PackedAttention : public torch::autograd::Function<PackedAttention> {
+  static Tensor forward(AutogradContext* ctx, Tensor q, Tensor k, Tensor v,
+                        std::optional<Tensor> table_opt, Tensor win, Tensor win_mem,
+                        std::optional<Tensor> by_query, std::optional<Tensor> by_key,
+                        double scale) {
+    q = packed_rows(q), k = packed_rows(k), v = packed_rows(v);
+    const Tensor table = table_opt.has_value() ? table_opt->contiguous() : Tensor();
+    const Tensor bq = by_query.value_or(Tensor()), bk = by_key.value_or(Tensor());
+    const auto r = packed_forward(q, k, v, table, win, bq, scale, true);
+    ctx->save_for_backward({q, k, v, table, r.out32, r.lse});
+    ctx->saved_data["win"] = win;
+    ctx->saved_data["win_mem"] = win_mem;
+    ctx->saved_data["by_query"] = bq;
+    ctx->saved_data["by_key"] = bk;
+    ctx->saved_data["scale"] = scale;
+    return r.out;
+  }
+
+  static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &table = saved[3], &out32 = saved[4],
+                 &lse = saved[5];
+    const at::DeviceGuard guard(q.device());
+    const Tensor win = ctx->saved_data["win"].toTensor();
+    const bool bias = table.defined();
+    const Tensor bq = ctx->saved_data["by_query"].toTensor();
+    const Tensor bk = ctx->saved_data["by_key"].toTensor();
+    const int64_t H = q.size(1), d = q.size(2);
+    const Tensor g = rows16(grads[0].to(q.scalar_type()));
+    tensor_list res(9);
+    res[0] = at::empty(q.sizes(), q.options());
+    res[1] = at::empty(k.sizes(), k.options());
+    res[2] = at::empty(v.sizes(), v.options());
+    const bool want_table = bias && ctx->needs_input_grad(3);
+    if (want_table) res[3] = at::empty_like(table);
+    const int dt = dtype_code(q);
+    const auto h = static_cast<int32_t>(H), hkv = static_cast<int32_t>(k.size(1)),
+               nb = bias ? static_cast<int32_t>(table.size(0)) : 0;
+    size_t bytes = 0;
+    check(g_packed_ws(dt, windows_of(win), h, hkv, static_cast<int32_t>(d), want_table ? nb : 0,
+                      nullptr, &bytes));
+    const Tensor ws = workspace(static_cast<int64_t>(bytes), q);
+    check(g_packed_bwd(dt, q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), k.stride(0),
+                       v.stride(0), out32.data_ptr<float>(), g.data_ptr(), lse.data_ptr<float>(),
+                       windows_of(win), h, hkv, static_cast<int32_t>(d),
+                       static_cast<float>(ctx->saved_data["scale"].toDouble()),
+                       bias ? table.data_ptr() : nullptr, nb,
+                       bias ? bq.data_ptr<uint8_t>() : nullptr,
+                       bias ? bk.data_ptr<uint8_t>() : nullptr, res[0].data_ptr(),
+                       res[1].data_ptr(), res[2].data_ptr(),
+                       want_table ? res[3].data_ptr() : nullptr, ws.data_ptr(), bytes,
+                       stream_of(q)));
+    return once("packed_attention", res);
+  }
+};
+
+// The checks of packed.py's packed_attention, without their messages: nothing
+// where one of them fails.
+std::optional<Tensor> packed_attention(const Tensor& q, const Tensor& k, const Tensor& v,
+                                       const std::optional<Tensor>& table, const Tensor& win,
+                                       const Tensor& win_mem,
+                                       const std::optional<Tensor>& by_query,
+                                       const std::optional<Tensor>& by_key, double scale) {
+  const ngt_packed_windows* w = windows_of(win);
+  if (q.dim() != 3 || k.dim() != 3 || v.dim() != 3) return std::nullopt;
+  const int64_t H = q.size(1), hkv = k.size(1), d = q.size(2);
+  const auto type = q.scalar_type();
+  if (q.size(0) != w->n_q || k.size(0) != w->n_k || k.sizes() != v.sizes() || k.size(2) != d ||
+      H < 1 || hkv < 1 || H % hkv || d < 8 || d > 128 || d % 8 ||
+      (type != at::kFloat && type != at::kBFloat16) || k.scalar_type() != type ||
+      v.scalar_type() != type || q.device() != win_mem.device() ||
+      k.device() != win_mem.device() || v.device() != win_mem.device() || !(scale > 0.) ||
+      !std::isfinite(scale) || !q.has_storage() || !k.has_storage() || !v.has_storage())
+    return std::nullopt;
+  if (table.has_value() != by_query.has_value()) return std::nullopt;
+  if (table.has_value() &&
+      (table->dim() != 2 || table->size(1) != H || table->size(0) < 1 || table->size(0) > 255 ||
+       table->scalar_type() != type || table->device() != q.device()))
+    return std::nullopt;
+  const at::DeviceGuard guard(q.device());
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
+                                     (table.has_value() && table->requires_grad())))
+    return PackedAttention::apply(q, k, v, table, win, win_mem, by_query, by_key, scale);
+  return packed_forward(packed_rows(q), packed_rows(k), packed_rows(v),
+                        table.has_value() ? table->contiguous() : Tensor(), win,
+                        by_query.value_or(Tensor()), scale, false)
+      .out;
+}
+
+// ------------------------------------------------------ linear with epilogue
+struct EpilogueForward {
+  Tensor x2, w16, y, z;
+};
+
+EpilogueForward epilogue_forward(const Tensor& x, const Tensor& weight,
+                                 const std::optional<Tensor>& bias,
+                                 const std::optional<Tensor>& residual, int64_t act,
+                                 bool want_grad) {
+  NoAutocast off;
+  const int64_t n_out = weight.size(0), n_in = weight.size(1);
+  EpilogueForward r;
+  r.x2 = bf16(x).reshape({-1, n_in});
+  const int64_t m = r.x2.size(0);
+  if ((n_in > 1 && r.x2.stride(1) != 1) || (m > 1 && r.x2.stride(0) < n_in))
+    r.x2 = r.x2.clone(at::MemoryFormat::Contiguous);
+  r.w16 = bf16(weight).contiguous();
+  const Tensor b = bias.has_value() ? bf16(*bias).contiguous() : Tensor();
+  const Tensor res =
+      residual.has_value() ? bf16(*residual).reshape({-1, n_out}).contiguous() : Tensor();
+  auto shape = x.sizes().vec();
+  shape.back() = n_out;
+  r.y = at::empty(shape, r.x2.options());
+  if (want_grad && act) r.z = at::empty({m, n_out}, r.x2.options());
+  check(g_linear_fwd(r.x2.data_ptr(), m > 1 ? r.x2.stride(0) : n_in, r.w16.data_ptr(),
+                     b.defined() ? b.data_ptr() : nullptr,
+                     res.defined() ? res.data_ptr() : nullptr, m, static_cast<int32_t>(n_out),
+                     static_cast<int32_t>(n_in), static_cast<int32_t>(act), r.y.data_ptr(),
+                     r.z.defined() ? r.z.data_ptr() : nullptr, stream_of(x)));
+  return r;
+}
+
+struct LinearEpilogue : public torch::autograd::Function<LinearEpilogue> {
+  static Tensor forward(AutogradContext* ctx, Tensor x, Tensor weight, std::optional<Tensor> bias,
+                        std::optional<Tensor> residual, int64_t act) {
+    const auto r = epilogue_forward(x, weight, bias, residual, act, true);
+    ctx->save_for_backward({r.x2, r.w16, r.z});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["x_type"] = x.scalar_type();
+    ctx->saved_data["w_type"] = weight.scalar_type();
+    ctx->saved_data["b_type"] =
+        static_cast<int64_t>(bias.has_value() ? static_cast<int>(bias->scalar_type()) : -1);
+    ctx->saved_data["r_type"] =
+        static_cast<int64_t>(residual.has_value() ? static_cast<int>(residual->scalar_type()) : -1);
+    ctx->saved_data["shape"] = x.sizes().vec();
+    return r.y;
+  }
+
+  static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+    NoAutocast off;
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x2 = saved[0], &w16 = saved[1], &z = saved[2];
+    const at::DeviceGuard guard(x2.device());
+    const int64_t m = x2.size(0), n_in = x2.size(1), n_out = w16.size(0);
+    const int64_t act = ctx->saved_data["act"].toInt();
+    const int64_t b_type = ctx->saved_data["b_type"].toInt();
+    const int64_t r_type = ctx->saved_data["r_type"].toInt();
+    // the node's edges are numbered over the tensors that were given
+    const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+    const bool want_b = b_type >= 0 && ctx->needs_input_grad(2);
+    const bool want_r = r_type >= 0 && ctx->needs_input_grad(b_type >= 0 ? 3 : 2);
+    const Tensor g = rows16(bf16(grads[0]));
+    tensor_list res(5);
+    Tensor dx, dz = g.view({m, n_out});
+    if (want_x || want_w || want_b) {
+      const Tensor gz = dz;
+      if (act) dz = at::empty({m, n_out}, g.options());
+      if (want_x) dx = at::empty({m, n_in}, g.options());
+      size_t bytes = 0;
+      check(g_linear_bwd_ws(m, static_cast<int32_t>(n_out), static_cast<int32_t>(n_in), &bytes));
+      const Tensor ws = want_x ? workspace(static_cast<int64_t>(bytes), g) : Tensor();
+      check(g_linear_bwd(gz.data_ptr(), z.defined() ? z.data_ptr() : nullptr, w16.data_ptr(), m,
+                         static_cast<int32_t>(n_out), static_cast<int32_t>(n_in),
+                         static_cast<int32_t>(act), dz.data_ptr(),
+                         want_x ? dx.data_ptr() : nullptr, want_x ? ws.data_ptr() : nullptr, bytes,
+                         stream_of(x2)));
+    }
+    if (want_x)
+      res[0] = dx.view(ctx->saved_data["shape"].toIntVector())
+                   .to(ctx->saved_data["x_type"].toScalarType());
+    if (want_w) {
+      const Tensor xc = x2.contiguous();
+      const auto opt = x2.options().dtype(at::kFloat);
+      Tensor dw = at::empty({n_out, n_in}, opt), db = want_b ? at::empty({n_out}, opt) : Tensor();
+      size_t bytes = 0;
+      check(g_wgrad_ws(m, static_cast<int32_t>(n_out), static_cast<int32_t>(n_in), &bytes));
+      const Tensor ws = workspace(static_cast<int64_t>(bytes), x2);
+      check(g_wgrad(xc.data_ptr(), dz.data_ptr(), m, static_cast<int32_t>(n_out),
+                    static_cast<int32_t>(n_in), dw.data_ptr<float>(),
+                    want_b ? db.data_ptr<float>() : nullptr, ws.data_ptr(), bytes, stream_of(x2)));
+      res[1] = dw.to(ctx->saved_data["w_type"].toScalarType());
+      if (want_b) res[2] = db;
+    } else if (want_b) {
+      res[2] = colsum(dz);
+    }
+    if (want_b) res[2] = res[2].to(static_cast<at::ScalarType>(b_type));
+    if (want_r) res[3] = grads[0].to(static_cast<at::ScalarType>(r_type));
+    return once("linear_epilogue", res);
+  }
+};
+
+bool linear_type(const Tensor& t, const Tensor& x) {
+  return (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat) &&
+         t.device() == x.device() && t.has_storage();
+}
+
+// The checks of linear.py's linear_epilogue, without their messages: nothing
+// where one of them fails.
+std::optional<Tensor> linear_epilogue(const Tensor& x, const Tensor& weight,
+                                      const std::optional<Tensor>& bias,
+                                      const std::optional<Tensor>& residual, int64_t act) {
+  if (!x.is_cuda() || !linear_type(x, x) || !linear_type(weight, x) || weight.dim() != 2 ||
+      x.dim() < 1 || x.size(-1) != weight.size(1) || weight.numel() == 0)
+    return std::nullopt;
+  if (bias.has_value() &&
+      (!linear_type(*bias, x) || bias->dim() != 1 || bias->size(0) != weight.size(0)))
+    return std::nullopt;
+  if (residual.has_value() &&
+      (!linear_type(*residual, x) || residual->dim() != x.dim() ||
+       residual->size(-1) != weight.size(0) ||
+       residual->sizes().slice(0, x.dim() - 1) != x.sizes().slice(0, x.dim() - 1)))
+    return std::nullopt;
+  const at::DeviceGuard guard(x.device());
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || weight.requires_grad() || (bias.has_value() && bias->requires_grad()) ||
+       (residual.has_value() && residual->requires_grad())))
+    return LinearEpilogue::apply(x, weight, bias, residual, act);
+  return epilogue_forward(x, weight, bias, residual, act, false).y;
+}
+
 template <typename F>
 void entry(F*& fn, const std::map<std::string, int64_t>& addr, const char* name) {
   const auto it = addr.find(name);
@@ -574,6 +873,12 @@ void init(const std::map<std::string, int64_t>& addr) {
   entry(g_ln_bwd, addr, "ngt_layernorm_bwd");
   entry(g_add_ln_fwd, addr, "ngt_add_layernorm_fwd");
   entry(g_add_ln_bwd, addr, "ngt_add_layernorm_bwd");
+  entry(g_packed_ws, addr, "ngt_packed_workspace_bytes");
+  entry(g_packed_fwd, addr, "ngt_packed_fwd");
+  entry(g_packed_bwd, addr, "ngt_packed_bwd");
+  entry(g_linear_fwd, addr, "ngt_linear_fwd");
+  entry(g_linear_bwd_ws, addr, "ngt_linear_bwd_workspace_bytes");
+  entry(g_linear_bwd, addr, "ngt_linear_bwd");
 }
 
 }  // namespace
@@ -595,4 +900,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("add_layernorm", &add_layernorm,
         "(x, y, weight, bias, eps, p, seed tensor or None, out_bf16) -> (s, out): layernorm.py's "
         "_AddLayerNormFn");
+  m.def("packed_struct_bytes", []() { return static_cast<int64_t>(sizeof(ngt_packed_windows)); });
+  m.def("packed_attention", &packed_attention,
+        "(q, k, v, table, windows, windows_mem, by_query, by_key, scale) -> out or None: "
+        "packed.py's PackedAttentionFunction; windows: the bytes of one ngt_packed_windows");
+  m.def("linear_epilogue", &linear_epilogue,
+        "(x, weight, bias, residual, activation) -> y or None: linear.py's LinearEpilogueFunction");
 }

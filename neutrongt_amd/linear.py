@@ -378,6 +378,10 @@ def linear_epilogue(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | 
     bias are fp32 sums in a fixed order.  Differentiable once."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
+    ext = _lib.node_ext()
+    y = ext and ext.linear_epilogue(x, weight, bias, residual, ACTIVATIONS[activation])
+    if y is not None:
+        return y
     ts = [t for t in (x, weight, bias, residual) if t is not None]
     if any(not t.is_cuda for t in ts):
         raise ValueError("linear_epilogue takes GPU tensors (there is no CPU path)")

@@ -67,6 +67,9 @@ class PackedWindows:
                                        C.byref(self.struct)))
         self.mem.copy_(host)
         self.device = dev
+        self.stream = _stream(dev)  # the memory's own
+        # the struct's bytes, for the C++ node
+        self.struct_bytes = torch.frombuffer(bytearray(self.struct), dtype=torch.uint8)
         self.q_lengths, self.k_lengths = ql.tolist(), kl.tolist()
         self.causal = bool(causal)
 
@@ -84,6 +87,14 @@ class PackedWindows:
 
     def ptr(self):
         return C.byref(self.struct)
+
+    def on_current_stream(self, *more: torch.Tensor) -> None:
+        """Keeps the plan's memory (and ``more``, allocated with it) from being
+        reused before the work that the current stream is about to get has run."""
+        if _stream(self.device) != self.stream:
+            cur = torch.cuda.current_stream(self.device)
+            for t in (self.mem, *more):
+                t.record_stream(cur)
 
     def workspace_bytes(self, dtype: int, heads: int, kv_heads: int, dim: int, n_buckets: int = 0):
         f, b = C.c_size_t(), C.c_size_t()
@@ -121,6 +132,7 @@ class PairBuckets:
     def __init__(self, windows: PackedWindows, ids: torch.Tensor):
         s, dev = windows.struct, windows.device
         self.windows = windows
+        windows.on_current_stream(ids)
         self.by_query = torch.empty(max(s.bucket_bytes_q, 1), dtype=torch.uint8, device=dev)
         self.by_key = torch.empty(max(s.bucket_bytes_k, 1), dtype=torch.uint8, device=dev)
         with torch.cuda.device(dev):
@@ -220,6 +232,18 @@ def packed_attention(q, k, v, windows: PackedWindows, scale: float | None = None
     gives zeros.  Differentiable once, in q, k, v and bias_table; deterministic."""
     if not isinstance(windows, PackedWindows):
         raise TypeError("windows must be a PackedWindows")
+    if buckets is not None and (not isinstance(buckets, PairBuckets)
+                                or buckets.windows is not windows):
+        raise ValueError("buckets must come from these windows' pack_buckets")
+    by = (buckets.by_query, buckets.by_key) if buckets is not None else (None, None)
+    if q.is_cuda and q.dim() == 3:
+        windows.on_current_stream(*(t for t in by if t is not None))
+        ext = _lib.node_ext()
+        out = ext and ext.packed_attention(
+            q, k, v, bias_table, windows.struct_bytes, windows.mem, *by,
+            1.0 / math.sqrt(max(q.shape[2], 1)) if scale is None else float(scale))
+        if out is not None:
+            return out
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError(f"q and k must be [rows, heads, d], got {tuple(q.shape)} {tuple(k.shape)}")
     H, d = q.shape[1:]
@@ -240,8 +264,6 @@ def packed_attention(q, k, v, windows: PackedWindows, scale: float | None = None
     if (bias_table is None) != (buckets is None):
         raise ValueError("bias_table and buckets go together")
     if bias_table is not None:
-        if not isinstance(buckets, PairBuckets) or buckets.windows is not windows:
-            raise ValueError("buckets must come from these windows' pack_buckets")
         if (bias_table.dim() != 2 or bias_table.shape[1] != H
                 or not 1 <= bias_table.shape[0] <= 255 or bias_table.dtype != q.dtype
                 or bias_table.device != q.device):

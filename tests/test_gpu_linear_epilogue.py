@@ -219,3 +219,20 @@ def test_refusals(dev):
     g, = torch.autograd.grad(linear_epilogue(xg, w).sum(), xg, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("act", list(ACTIVATIONS))
+@pytest.mark.parametrize("w_type", [BF16, F32])
+def test_the_cpp_node_and_the_python_class_give_the_same_bits(dev, act, w_type, monkeypatch):
+    assert _lib.autograd_ext() is not None
+    x, w, b, r, gy = (t.to(dev) for t in _inputs(300, 56, 104, True, True, 9))
+    leaves = [t.requires_grad_() for t in (x.float(), w.to(w_type), b.to(w_type), r.float())]
+
+    def step():
+        y = linear_epilogue(leaves[0].view(3, 100, 104), *leaves[1:3], act,
+                            leaves[3].view(3, 100, 56))
+        return [y.detach(), *torch.autograd.grad(y, leaves, gy.view(3, 100, 56))]
+
+    a = step()
+    monkeypatch.setattr(_lib, "node_ext", lambda: None)
+    assert all(torch.equal(p, q) and p.dtype == q.dtype for p, q in zip(a, step()))

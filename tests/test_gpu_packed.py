@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from neutrongt_amd import PackedWindows, packed_attention
+from neutrongt_amd import PackedWindows, _lib, packed_attention
 from oracle import packed as OP
 
 pytestmark = pytest.mark.gpu
@@ -348,3 +348,72 @@ def test_second_derivatives_are_refused(dev):
     g, = torch.autograd.grad(packed_attention(q, k, v, win).sum(), q, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), k)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("buckets", [0, 13])
+def test_the_cpp_node_and_the_python_class_give_the_same_bits(dev, dtype, buckets, monkeypatch):
+    assert _lib.autograd_ext() is not None
+    ql = [70, 33, 1]
+    q, k, v, go, table, ids = _inputs(ql, ql, 4, 2, 24, dtype, buckets, seed=30)
+    win = PackedWindows(ql, causal=True, device=dev)
+    a = _run(dev, q, k, v, go, table, ids, win)
+    monkeypatch.setattr(_lib, "node_ext", lambda: None)
+    b = _run(dev, q, k, v, go, table, ids, win)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    g, = torch.autograd.grad(
+        packed_attention(x := q.to(dev).requires_grad_(), k.to(dev), v.to(dev), win).sum(), x,
+        create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+def test_refusals_on_the_gpu(dev):
+    win = PackedWindows([5, 3], device=dev)
+    q = torch.zeros(8, 4, 16, device=dev)
+    k = torch.zeros(8, 2, 16, device=dev)
+    b = win.pack_buckets(torch.zeros(34, dtype=torch.uint8, device=dev))
+    t = torch.zeros(3, 4, device=dev)
+    other = PackedWindows([5, 3], device=dev)
+    bad = [((q[:7], k, k), {}, ValueError), ((q, k[:7], k[:7]), {}, ValueError),
+           ((q, k, k[:, :1]), {}, ValueError), ((q, k.bfloat16(), k.bfloat16()), {}, TypeError),
+           ((q.half(), k.half(), k.half()), {}, TypeError), ((q[:, :3], k, k), {}, ValueError),
+           ((q[..., :12], k[..., :12], k[..., :12]), {}, ValueError),
+           ((q, k.cpu(), k.cpu()), {}, ValueError), ((q, k, k), dict(scale=0.0), ValueError),
+           ((q, k, k), dict(scale=math.inf), ValueError),
+           ((q, k, k), dict(bias_table=t), ValueError), ((q, k, k), dict(buckets=b), ValueError),
+           ((q, k, k), dict(bias_table=t.bfloat16(), buckets=b), ValueError),
+           ((q, k, k), dict(bias_table=t[:, :2], buckets=b), ValueError),
+           ((q, k, k), dict(bias_table=torch.zeros(256, 4, device=dev), buckets=b), ValueError),
+           ((q, k, k), dict(bias_table=t[:0], buckets=b), ValueError)]
+    for args, more, err in bad:
+        with pytest.raises(err):
+            packed_attention(*args, win, **more)
+    with pytest.raises(ValueError, match="pack_buckets"):
+        packed_attention(q, k, k, other, bias_table=t, buckets=b)
+    for ids, err in ((torch.zeros(33, dtype=torch.uint8, device=dev), ValueError),
+                     (torch.zeros(34, device=dev), TypeError),
+                     (torch.zeros(34, dtype=torch.uint8), ValueError)):
+        with pytest.raises(err):
+            win.pack_buckets(ids)
+
+
+def test_a_plan_made_and_dropped_on_another_stream(dev):
+    """The plan's memory outlives the work that another stream still has to do."""
+    ql = [300] * 20
+    q, k, v, go, _, _ = _inputs(ql, ql, 4, 4, 32, BF16, seed=31)
+    want = _run(dev, q, k, v, go, None, None, PackedWindows(ql, device=dev))
+    q, k, v = q.to(dev), k.to(dev), v.to(dev)
+    side = torch.cuda.Stream(dev)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        win = PackedWindows(ql, device=dev)
+        n = win.mem.numel()
+        with torch.cuda.stream(side), torch.no_grad():
+            for _ in range(10):
+                out = packed_attention(q, k, v, win)
+        del win
+        junk = [torch.full((n,), 255, dtype=torch.uint8, device=dev) for _ in range(4)]
+        side.synchronize()
+        assert torch.equal(out, want[0])
+        del junk
