@@ -18,10 +18,12 @@
 // So one copy of a tile in LDS serves Q K^T, P V and every product of the
 // backward, and no score leaves the registers.
 //
-// The 16-byte pieces of a row are permuted by tile_swz(row): the 8 lanes that
-// a 16-byte read serves at once (rows r .. r+3 and r+16 .. r+19, one piece)
-// and the 16 lanes of an 8-byte column read (4 rows, two pieces) fall on
-// distinct banks, without padding.
+// The 16-byte pieces of a row are permuted by swz(row), without padding.  LDS
+// serves a 16-byte read in groups of lanes that are not 8 neighbours, so the
+// bits were chosen by the conflict counter: with bits 1, 2 and 4 of the row
+// (and 0 where a row fills all 64 banks) row reads and ds_read_b64_tr_b16 reads
+// of every row size have none; with bits 0, 1 and 4 a row read took 12 clocks
+// instead of 8.
 #pragma once
 
 #include "ngt_common.h"
@@ -93,10 +95,10 @@ struct Tile {
   static constexpr int kCols = DP / 32;        // 32-column blocks of a row
 
   __device__ static __forceinline__ int swz(int row) {
-    if constexpr (kPieces == 4)
-      return (((row >> 1) & 1) << 1) | ((row >> 4) & 1);
-    else
-      return ((row & 3) << 1) | ((row >> 4) & 1);
+    int f = (row >> 1 & 2) | (row >> 4 & 1);
+    if constexpr (kPieces >= 8) f |= row << 1 & 4;
+    if constexpr (kPieces >= 16) f |= row << 3 & 8;
+    return f;
   }
   __device__ static __forceinline__ int offset(int row, int piece) {
     return row * kPitch + ((piece ^ swz(row)) << 4);
@@ -121,18 +123,18 @@ struct Tile {
         u32x4 b;
 #pragma unroll
         for (int e = 0; e < 4; ++e) b[e] = pack2_bf16(p[8 * c + 2 * e], p[8 * c + 2 * e + 1]);
-        // rows 4-aligned + j / 4: swz() depends on the lane alone
+        // rows j / 4 and then 4 further: of swz() only bit 1 depends on more than the lane
         const int row = 16 * half + (j >> 2);
         const int piece = 2 * ((lane >> 4) & 1) + ((j & 3) >> 1);
         const int at = (piece ^ swz(row)) * 16 + 8 * (j & 1) + row * kPitch;
 #pragma unroll
         for (int dt = 0; dt < kCols; ++dt) {
-          // pieces 4 further on: bit 2 of the piece flips with dt's low bit
-          const int off = (kPieces > 4 ? (at ^ ((dt & 1) << 6)) + (dt >> 1) * 128 : at) +
-                          (32 * t + 8 * c) * kPitch;
+          // the column block is bits 2 and 3 of the piece
+          const int off = (at ^ (dt << 6)) + (32 * t + 8 * c) * kPitch;
+          const int off4 = (at ^ (dt << 6) ^ 32) + (32 * t + 8 * c + 4) * kPitch;
           typedef __attribute__((address_space(3))) s16x4* lds4_t;
           const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(tile + off));
-          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(tile + off + 4 * kPitch));
+          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(tile + off4));
           const uint2 lw = __builtin_bit_cast(uint2, lo), hw = __builtin_bit_cast(uint2, hi);
           const u32x4 a = {lw.x, lw.y, hw.x, hw.y};
           acc[dt] = mma_rows<T>(a, b, acc[dt]);
