@@ -440,13 +440,14 @@ int ngt_adj_weights(const int64_t* edge_index, const float* ppr_val, int64_t n_e
  * causal: query i sees the keys j <= i + (keys - queries) of its window.
  * A query that sees no key gets a zero row and gives no gradient.  q, k and v
  * may have rows further apart than heads * d: *_stride is in elements, rows
- * 16-byte aligned.  Values of unseen keys enter with weight 0, so they must be
+ * 16-byte aligned and less than 8 MB apart.  Values of unseen keys enter with weight 0, so they must be
  * finite where any query of their window is not to see a NaN.
  *
  * The plan.  ngt_packed_plan writes the windows' offsets and work lists for
  * ngt_packed_plan_bytes bytes at device, which the caller then copies there
  * from host, and fills *out (host memory; its pointers point into device).
- * Lengths are host arrays, 0 <= length <= 2^30.  Neither call touches the GPU.
+ * Lengths are host arrays, 0 <= length <= 2^28 (2^23
+ * with a bias).  Neither call touches the GPU.
  *
  * The bias.  table [n_buckets, H] has the element type of q, 1 <= n_buckets
  * <= 255.  ngt_packed_buckets lays the pairs' bucket ids out once for all

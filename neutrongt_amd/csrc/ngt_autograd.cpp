@@ -592,7 +592,8 @@ Tensor packed_rows(const Tensor& t) {
   const int64_t es = t.element_size();
   if (t.size(0) == 0 ||
       (t.stride(2) == 1 && t.stride(1) == t.size(2) && t.stride(0) >= t.size(1) * t.size(2) &&
-       t.stride(0) * es % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0))
+       t.stride(0) * es % 16 == 0 && t.stride(0) * es < (1 << 23) &&
+       reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0))
     return t;
   return t.clone(at::MemoryFormat::Contiguous);
 }

@@ -173,27 +173,48 @@ struct RowFrag {
   }
 };
 
+// Reads through a buffer descriptor: 16 or 4 bytes at a byte offset of a base that
+// is the same in all lanes; what lies at or behind `bytes` reads as zero, so a
+// tile's missing rows cost neither a branch nor a select.
+using Buffer = __amdgpu_buffer_rsrc_t;
+constexpr int kMostBytes = 0x7fffff00;
+constexpr int kNowhere = 0x7ffffff0;  // an offset behind every buffer's end
+__device__ __forceinline__ Buffer make_buffer(const void* base, int64_t bytes) {
+  const int n = bytes > kMostBytes ? kMostBytes : bytes < 0 ? 0 : static_cast<int>(bytes);
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, n, 0x00027000);
+}
+__device__ __forceinline__ u32x4 read16(Buffer b, int offset) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b, offset, 0, 0));
+}
+__device__ __forceinline__ float read4(Buffer b, int offset) {
+  return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, offset, 0, 0));
+}
+
 // The 16-byte pieces of ROWS rows of one head that one of N threads moves from
-// memory to an LDS tile; rows behind the window's end and columns behind d are zero.
+// memory to an LDS tile; rows behind the window's end and columns behind d are
+// zero.  ROWS rows span less than 2^31 bytes (kMostRowBytes).
+constexpr int64_t kMostRowBytes = (1 << 23) - 1;  // of 256 rows, and room for a last row
 template <typename T, int DP, int ROWS, int N>
 struct Stage {
   using L = Tile<T, DP>;
   static constexpr int NV = (ROWS * L::kPieces) / N;
   static_assert(NV * N == ROWS * L::kPieces, "whole pieces per thread");
   u32x4 w[NV];
-  __device__ __forceinline__ static u32x4 piece(const T* __restrict__ base, int64_t stride, int row0,
-                                                int n_rows, int d, int e) {
-    const int r = e / L::kPieces, p = e % L::kPieces;
-    u32x4 x = {0u, 0u, 0u, 0u};
-    if (row0 + r < n_rows && 16 * p < d * L::kEs)
-      x = *reinterpret_cast<const u32x4*>(
-          reinterpret_cast<const char*>(base) + int64_t(row0 + r) * stride + 16 * p);
-    return x;
-  }
-  __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, int n_rows, int d,
-                                       int tid) {
+  int at[NV];
+  __device__ __forceinline__ Stage(int64_t stride, int d, int tid) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) w[i] = piece(base, stride, row0, n_rows, d, tid + i * N);
+    for (int i = 0; i < NV; ++i) {
+      const int r = (tid + i * N) / L::kPieces, p = (tid + i * N) % L::kPieces;
+      at[i] = 16 * p < d * L::kEs ? r * static_cast<int>(stride) + 16 * p : kNowhere;
+    }
+  }
+  // rows row0 .. of the n_rows at base, `stride` bytes apart
+  __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, int n_rows, int d) {
+    const Buffer b =
+        make_buffer(reinterpret_cast<const char*>(base) + int64_t(row0) * stride,
+                    row0 < n_rows ? int64_t(n_rows - row0 - 1) * stride + d * L::kEs : 0);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) w[i] = read16(b, at[i]);
   }
   __device__ __forceinline__ void store(char* tile, int tid) const {
 #pragma unroll
@@ -271,6 +292,16 @@ __device__ __forceinline__ void load_table(float* tab, const T* __restrict__ tab
 }
 __device__ __forceinline__ int bucket_of(const u32x4& ids, int i) {
   return static_cast<int>((ids[i >> 2] >> (8 * (i & 3))) & 255u);
+}
+
+// The table's values for a lane's 16 ids.  All reads are under way before what
+// follows (left to itself the compiler waits for each: 16 latencies a tile).
+__device__ __forceinline__ f32x16 look_up(const float* tab, const u32x4& ids) {
+  f32x16 v;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = tab[bucket_of(ids, i)];
+  __builtin_amdgcn_sched_barrier(0);
+  return v;
 }
 
 }  // namespace packed

@@ -128,10 +128,11 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_fwd(FwdArgs a) {
   q.load(reinterpret_cast<const T*>(reinterpret_cast<const char*>(a.q) + (q0 + qc) * a.sq) +
              int64_t(h) * a.d,
          qi < nq, a.d, half);
-  const uint8_t* ids = nullptr;
+  const int ld = (nk + 63) & ~63;
+  const uint8_t* ids = nullptr;  // of the block's first query
   if constexpr (BIAS) {
     load_table(tab, reinterpret_cast<const T*>(a.table), a.n_buckets, a.H, h, tid, N);
-    ids = a.ids + a.b_start[item.x] + int64_t(qc) * ((nk + 63) & ~63) + 16 * half;
+    ids = a.ids + a.b_start[item.x] + int64_t(item.y) * ld;
   }
   const float s2 = a.scale * kLog2e;
   RowSoftmax sm(BIAS ? 1.f : s2, BIAS ? 1.f / s2 : 1.f);
@@ -139,26 +140,29 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_fwd(FwdArgs a) {
 #pragma unroll
   for (int c = 0; c < L::kCols; ++c) acc[c] = fill16(0.f);
 
-  Stage<T, DP, kKeys, N> pk, pv;
+  Stage<T, DP, kKeys, N> pk(a.sk, a.d, tid), pv(a.sv, a.d, tid);
   u32x4 idw[2], id_next[2];
-  auto fetch_ids = [&](int k1) {  // of keys that are there
+  const Buffer id_buf = make_buffer(ids, int64_t(min(32 * RW, nq - item.y)) * ld);
+  const int id_at = (qc - item.y) * ld + 16 * half;
+  auto fetch_ids = [&](int k1) {
+    if constexpr (BIAS) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-      if (BIAS && k1 < nk) id_next[t] = *reinterpret_cast<const u32x4*>(ids + k1 + 32 * t);
+      for (int t = 0; t < 2; ++t) id_next[t] = read16(id_buf, id_at + k1 + 32 * t);
+    }
   };
   fetch_ids(64 * set);
   if constexpr (kAhead) {
-    pk.load(kb, a.sk, 0, nk, a.d, tid);
-    pv.load(vb, a.sv, 0, nk, a.d, tid);
+    pk.load(kb, a.sk, 0, nk, a.d);
+    pv.load(vb, a.sv, 0, nk, a.d);
   }
   const char* kt_tile = ks + 64 * set * L::kPitch;
   const char* vt_tile = vs + 64 * set * L::kPitch;
   for (int kt = 0; kt < block_end; kt += kKeys) {
     __syncthreads();
     if constexpr (!kAhead) {
-      pk.load(kb, a.sk, kt, nk, a.d, tid);
+      pk.load(kb, a.sk, kt, nk, a.d);
       pk.store(ks, tid);
-      pv.load(vb, a.sv, kt, nk, a.d, tid);
+      pv.load(vb, a.sv, kt, nk, a.d);
       pv.store(vs, tid);
     } else {
       pk.store(ks, tid);
@@ -169,12 +173,14 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_fwd(FwdArgs a) {
     fetch_ids(kt + kKeys + 64 * set);
     if constexpr (kAhead) {
       if (kt + kKeys < block_end) {
-        pk.load(kb, a.sk, kt + kKeys, nk, a.d, tid);
-        pv.load(vb, a.sv, kt + kKeys, nk, a.d, tid);
+        pk.load(kb, a.sk, kt + kKeys, nk, a.d);
+        pv.load(vb, a.sv, kt + kKeys, nk, a.d);
       }
     }
     const int k1 = kt + 64 * set;  // this set's first key
     if (k1 >= wave_end) continue;
+    f32x16 bias[2];
+    if constexpr (BIAS) bias[0] = look_up(tab, idw[0]), bias[1] = look_up(tab, idw[1]);
     f32x16 x[2] = {sm.start, sm.start};
 #pragma unroll
     for (int c = 0; c < L::kChunks; ++c)
@@ -185,7 +191,7 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_fwd(FwdArgs a) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[t][i] = fmaf(x[t][i], s2, tab[bucket_of(idw[t], i)]);
+        for (int i = 0; i < 16; ++i) x[t][i] = fmaf(x[t][i], s2, bias[t][i]);
     }
     if (k1 + 63 > first_lim) {  // some key of the tile is behind some row's last one
 #pragma unroll
@@ -289,13 +295,14 @@ __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
   q.load(reinterpret_cast<const T*>(reinterpret_cast<const char*>(a.q) + (q0 + qi) * a.sq) +
              int64_t(h) * a.d,
          l32 < rows, a.d, half);
+  const int ld = (nk + 63) & ~63;
   const uint8_t* ids = nullptr;
   const float* tab = nullptr;
   if constexpr (BIAS) {
     for (int g = 0; g < G; ++g)
       load_table(tabs + g * kTable, reinterpret_cast<const T*>(a.table), a.n_buckets, a.H,
                  kvh * G + g, tid, 256);
-    ids = a.ids + a.b_start[w] + int64_t(qi) * ((nk + 63) & ~63) + 16 * half;
+    ids = a.ids + a.b_start[w];
     tab = tabs + grp * kTable;
     __syncthreads();
   }
@@ -306,28 +313,34 @@ __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
   for (int c = 0; c < L::kCols; ++c) acc[c] = fill16(0.f);
   char* vs = buf + wave * kTileBytes;
 
-  Stage<T, DP, 32, 64> pv;
-  RowFrag<T, DP> pk;
+  Stage<T, DP, 32, 64> pv(a.sv, a.d, lane);
+  u32x4 pk[L::kChunks];
   u32x4 idw = {0u, 0u, 0u, 0u};
-  const int a_row = L::a_row(l32);
+  const int k_at = L::a_row(l32) * static_cast<int>(a.sk) + 16 * half;
+  const Buffer id_buf = make_buffer(ids, int64_t(nq) * ld);
+  const int id_at = qi * ld + 16 * half;
   auto fetch = [&](int t) {
     const int kt = 32 * t;
-    pk.load(reinterpret_cast<const T*>(reinterpret_cast<const char*>(kb) +
-                                       int64_t(kt + a_row) * a.sk),
-            kt + a_row < nk, a.d, half);
-    pv.load(vb, a.sv, kt, nk, a.d, lane);
-    if constexpr (BIAS) idw = *reinterpret_cast<const u32x4*>(ids + kt);
+    const Buffer kbuf = make_buffer(reinterpret_cast<const char*>(kb) + int64_t(kt) * a.sk,
+                                    int64_t(nk - kt - 1) * a.sk + a.d * L::kEs);
+#pragma unroll
+    for (int c = 0; c < L::kChunks; ++c)
+      pk[c] = read16(kbuf, 32 * c + 16 * half < a.d * L::kEs ? k_at + 32 * c : kNowhere);
+    pv.load(vb, a.sv, kt, nk, a.d);
+    if constexpr (BIAS) idw = read16(id_buf, id_at + kt);
   };
   int t = t_begin + wave;
   if (t < t_end) fetch(t);
   while (t < t_end) {
     const int kt = 32 * t;
+    f32x16 bias;
+    if constexpr (BIAS) bias = look_up(tab, idw);
     f32x16 x[1] = {sm.start};
 #pragma unroll
-    for (int c = 0; c < L::kChunks; ++c) x[0] = mma_rows<T>(pk.w[c], q.w[c], x[0]);
+    for (int c = 0; c < L::kChunks; ++c) x[0] = mma_rows<T>(pk[c], q.w[c], x[0]);
     if constexpr (BIAS) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[0][i] = fmaf(x[0][i], s2, tab[bucket_of(idw, i)]);
+      for (int i = 0; i < 16; ++i) x[0][i] = fmaf(x[0][i], s2, bias[i]);
     }
     pv.store(vs, lane);
     t += 4;
@@ -508,6 +521,8 @@ __global__ __launch_bounds__(256) void k_packed_buckets(const I* __restrict__ id
 constexpr int kTargetBlocks = 512;  // two blocks for each of the 256 compute units
 constexpr int kSimds = 1024;
 constexpr size_t kLds = 160 * 1024;
+constexpr int kMostIds = 1 << 23;      // of a window with a bias
+constexpr int32_t kMostRows = 1 << 28;  // of a window
 
 inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
@@ -583,6 +598,12 @@ int check_call(const char* fn, int dtype, const ngt_packed_windows* w, int H, in
     return set_error(NGT_ERR_ARG, "%s: a bias takes a table and bucket ids", fn);
   if (table && (n_buckets < 1 || n_buckets > 255))
     return set_error(NGT_ERR_ARG, "%s: n_buckets=%d (1 to 255)", fn, n_buckets);
+  // 32-bit offsets within a block's rows
+  if (table && (w->max_q > kMostIds || w->max_k > kMostIds))
+    return set_error(NGT_ERR_UNSUPPORTED, "%s: a bias over windows of more than %d rows", fn,
+                     kMostIds);
+  if (int64_t(H) * d * (dtype == NGT_F32 ? 4 : 2) > kMostRowBytes)
+    return set_error(NGT_ERR_UNSUPPORTED, "%s: %d heads of %d", fn, H, d);
   if (table && !(w->b_start && w->bt_start))
     return set_error(NGT_ERR_ARG, "%s: null bucket offsets", fn);
   return NGT_OK;
@@ -590,6 +611,8 @@ int check_call(const char* fn, int dtype, const ngt_packed_windows* w, int H, in
 
 int check_stride(const char* fn, const char* name, const void* p, int64_t stride, int heads, int d,
                  int es) {
+  if (stride > kMostRowBytes / es)
+    return set_error(NGT_ERR_UNSUPPORTED, "%s: %s rows more than 8 MB apart", fn, name);
   if (stride < int64_t(heads) * d || (stride * es) % 16 || reinterpret_cast<uintptr_t>(p) % 16)
     return set_error(NGT_ERR_ARG,
                      "%s: %s rows must be at least heads * head_dim apart and 16-byte aligned", fn,
@@ -692,8 +715,8 @@ int check_lengths(const char* fn, int32_t n, const int32_t* q_len, const int32_t
   for (int32_t w = 0; w < n; ++w) {
     if (q_len[w] < 0 || k_len[w] < 0)
       return set_error(NGT_ERR_ARG, "%s: window %d has a negative length", fn, w);
-    if (q_len[w] > (1 << 30) || k_len[w] > (1 << 30))
-      return set_error(NGT_ERR_UNSUPPORTED, "%s: window %d is longer than 2^30", fn, w);
+    if (q_len[w] > kMostRows || k_len[w] > kMostRows)
+      return set_error(NGT_ERR_UNSUPPORTED, "%s: window %d is longer than 2^28", fn, w);
     tq += (q_len[w] + 31) / 32;
     tk += (k_len[w] + 31) / 32;
   }

@@ -93,11 +93,12 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
   const float lse = qi < nq ? a.lse[int64_t(h) * a.n_q + q0 + qi] : INFINITY;
   if (qi < nq && half == 0 && set == 0) a.dsum[int64_t(h) * a.n_q + q0 + qi] = -D;
 
-  const uint8_t* ids = nullptr;
+  const int ld = (nk + 63) & ~63;
+  const uint8_t* ids = nullptr;  // of the block's first query
   double* my_hist = nullptr;
   if constexpr (BIAS) {
     load_table(tab, reinterpret_cast<const T*>(a.table), a.n_buckets, a.H, h, tid, N);
-    ids = a.ids + a.b_start[item.x] + int64_t(qc) * ((nk + 63) & ~63) + 16 * half;
+    ids = a.ids + a.b_start[item.x] + int64_t(item.y) * ld;
   }
   if constexpr (HIST) {
     for (int i = tid; i < RW * KS * (a.n_buckets + 1) * 32; i += N) hist[i] = 0.;
@@ -110,26 +111,29 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
 #pragma unroll
   for (int c = 0; c < L::kCols; ++c) acc[c] = fill16(0.f);
 
-  Stage<T, DP, kRows, N> pk, pv;
+  Stage<T, DP, kRows, N> pk(a.sk, a.d, tid), pv(a.sv, a.d, tid);
   u32x4 idw[2], id_next[2];
-  auto fetch_ids = [&](int k1) {  // of keys that are there
+  const Buffer id_buf = make_buffer(ids, int64_t(min(32 * RW, nq - item.y)) * ld);
+  const int id_at = (qc - item.y) * ld + 16 * half;
+  auto fetch_ids = [&](int k1) {
+    if constexpr (BIAS) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-      if (BIAS && k1 < nk) id_next[t] = *reinterpret_cast<const u32x4*>(ids + k1 + 32 * t);
+      for (int t = 0; t < 2; ++t) id_next[t] = read16(id_buf, id_at + k1 + 32 * t);
+    }
   };
   fetch_ids(64 * set);
   if constexpr (kAhead) {
-    pk.load(kb, a.sk, 0, nk, a.d, tid);
-    pv.load(vb, a.sv, 0, nk, a.d, tid);
+    pk.load(kb, a.sk, 0, nk, a.d);
+    pv.load(vb, a.sv, 0, nk, a.d);
   }
   const char* k_tile = ks + 64 * set * L::kPitch;
   const char* v_tile = vs + 64 * set * L::kPitch;
   for (int kt = 0; kt < block_end; kt += kRows) {
     __syncthreads();
     if constexpr (!kAhead) {
-      pk.load(kb, a.sk, kt, nk, a.d, tid);
+      pk.load(kb, a.sk, kt, nk, a.d);
       pk.store(ks, tid);
-      pv.load(vb, a.sv, kt, nk, a.d, tid);
+      pv.load(vb, a.sv, kt, nk, a.d);
       pv.store(vs, tid);
     } else {
       pk.store(ks, tid);
@@ -140,8 +144,8 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
     fetch_ids(kt + kRows + 64 * set);
     if constexpr (kAhead) {
       if (kt + kRows < block_end) {
-        pk.load(kb, a.sk, kt + kRows, nk, a.d, tid);
-        pv.load(vb, a.sv, kt + kRows, nk, a.d, tid);
+        pk.load(kb, a.sk, kt + kRows, nk, a.d);
+        pv.load(vb, a.sv, kt + kRows, nk, a.d);
       }
     }
     const int k1 = kt + 64 * set;  // this set's first key
@@ -149,6 +153,8 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       if (t == 1 && k1 + 32 >= wave_end) break;
+      f32x16 bias;
+      if constexpr (BIAS) bias = look_up(tab, idw[t]);
       f32x16 s = s_start, dp = dp_start;
 #pragma unroll
       for (int c = 0; c < L::kChunks; ++c) {
@@ -157,7 +163,7 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        s[i] = fmaf(s[i], s2, BIAS ? tab[bucket_of(idw[t], i)] : -lse);
+        s[i] = fmaf(s[i], s2, BIAS ? bias[i] : -lse);
       if (k1 + 32 * t + 31 > first_lim) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -239,15 +245,18 @@ k_packed_dkv(BwdArgs a) {
   v.load(reinterpret_cast<const T*>(reinterpret_cast<const char*>(a.v) + (k0 + kc) * a.sv) +
              int64_t(kvh) * a.d,
          kj < nk, a.d, half);
-  const uint8_t* ids = nullptr;
-  if constexpr (BIAS)
-    ids = a.ids_t + a.bt_start[item.x] + int64_t(kc) * ((nq + 63) & ~63) + 16 * half;
+  const int ld = (nq + 63) & ~63;
+  const uint8_t* ids = nullptr;  // of the block's first key
+  if constexpr (BIAS) ids = a.ids_t + a.bt_start[item.x] + int64_t(item.y) * ld;
+  const Buffer id_buf = make_buffer(ids, int64_t(min(32 * RW, nk - item.y)) * ld);
+  const int id_at = (kc - item.y) * ld + 16 * half;
   const float s2 = a.scale * kLog2e;
   f32x16 ak[L::kCols], av[L::kCols];
 #pragma unroll
   for (int c = 0; c < L::kCols; ++c) ak[c] = fill16(0.f), av[c] = fill16(0.f);
 
-  Stage<T, DP, kRows, N> pq, pg;
+  const int64_t sg = int64_t(a.H) * a.d * L::kEs;
+  Stage<T, DP, kRows, N> pq(a.sq, a.d, tid), pg(sg, a.d, tid);
   const float lse_per = -1.f / s2;  // into product units
   float pl = 0.f, pd = 0.f;
   u32x4 idw[2], id_next[2];
@@ -258,21 +267,21 @@ k_packed_dkv(BwdArgs a) {
     const T* qb = reinterpret_cast<const T*>(reinterpret_cast<const char*>(a.q) + q0 * a.sq) +
                   int64_t(h) * a.d;
     const T* gb = reinterpret_cast<const T*>(a.go) + (q0 * a.H + h) * int64_t(a.d);
-    const int64_t sg = int64_t(a.H) * a.d * L::kEs;
-    const float* lse = a.lse + int64_t(h) * a.n_q + q0;
-    const float* dsum = a.dsum + int64_t(h) * a.n_q + q0;
+    const Buffer lse = make_buffer(a.lse + int64_t(h) * a.n_q + q0, int64_t(nq) * 4);
+    const Buffer dsum = make_buffer(a.dsum + int64_t(h) * a.n_q + q0, int64_t(nq) * 4);
     auto fetch = [&](int qt) {
+      if constexpr (BIAS) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)  // of queries that are there
-        if (BIAS && qt + 64 * set < nq)
-          id_next[t] = *reinterpret_cast<const u32x4*>(ids + qt + 64 * set + 32 * t);
-      if (tid < kRows) {  // a row that is not there has no weight
-        pl = qt + tid < nq ? lse[qt + tid] : INFINITY;
-        pd = qt + tid < nq ? dsum[qt + tid] : 0.f;
+        for (int t = 0; t < 2; ++t)
+          id_next[t] = read16(id_buf, id_at + qt + 64 * set + 32 * t);
       }
+      // (a row that is not there has no weight)
+      pl = read4(lse, 4 * (qt + tid));
+      pl = qt + tid < nq ? pl : INFINITY;
+      pd = read4(dsum, 4 * (qt + tid));
       if constexpr (kAhead) {
-        pq.load(qb, a.sq, qt, nq, a.d, tid);
-        pg.load(gb, sg, qt, nq, a.d, tid);
+        pq.load(qb, a.sq, qt, nq, a.d);
+        pg.load(gb, sg, qt, nq, a.d);
       }
     };
     if constexpr (BIAS) {
@@ -283,9 +292,9 @@ k_packed_dkv(BwdArgs a) {
     for (int qt = block_begin; qt < nq; qt += kRows) {
       __syncthreads();
       if constexpr (!kAhead) {
-        pq.load(qb, a.sq, qt, nq, a.d, tid);
+        pq.load(qb, a.sq, qt, nq, a.d);
         pq.store(qs, tid);
-        pg.load(gb, sg, qt, nq, a.d, tid);
+        pg.load(gb, sg, qt, nq, a.d);
         pg.store(gs, tid);
       } else {
         pq.store(qs, tid);
@@ -299,6 +308,8 @@ k_packed_dkv(BwdArgs a) {
       if (q1 + 64 <= wave_begin || q1 >= nq || item.y + wave * 32 >= nk) continue;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
+        f32x16 bias;
+        if constexpr (BIAS) bias = look_up(tab, idw[t]);
         f32x16 s, dp;  // start from -lse, in product units, and -D of the rows
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -315,7 +326,7 @@ k_packed_dkv(BwdArgs a) {
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          s[i] = BIAS ? fmaf(s[i], s2, tab[bucket_of(idw[t], i)]) : s[i] * s2;
+          s[i] = BIAS ? fmaf(s[i], s2, bias[i]) : s[i] * s2;
         if (q1 + 32 * t < last_lim) {
 #pragma unroll
           for (int i = 0; i < 16; ++i)

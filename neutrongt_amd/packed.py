@@ -33,8 +33,8 @@ def _lengths(x, name: str) -> torch.Tensor:
     t = torch.as_tensor(x if len(x) else torch.empty(0, dtype=torch.int32), device="cpu")
     if t.dim() != 1 or t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
         raise ValueError(f"{name} must be a 1-D sequence of integers, got {tuple(t.shape)} {t.dtype}")
-    if t.numel() and (int(t.min()) < 0 or int(t.max()) > 1 << 30):
-        raise ValueError(f"{name} must lie in [0, 2^30]")
+    if t.numel() and (int(t.min()) < 0 or int(t.max()) > 1 << 28):
+        raise ValueError(f"{name} must lie in [0, 2^28]")
     return t.to(torch.int32).contiguous()
 
 
@@ -212,7 +212,7 @@ def _rows(t: torch.Tensor, name: str, n: int, dim: int) -> torch.Tensor:
         raise ValueError(f"{name} must be [{n}, heads, {dim}], got {tuple(t.shape)}")
     es = t.element_size()
     if n and (t.stride(2) != 1 or t.stride(1) != dim or t.stride(0) < t.shape[1] * dim
-              or t.stride(0) * es % 16 or t.data_ptr() % 16):
+              or t.stride(0) * es % 16 or t.stride(0) * es >= 1 << 23 or t.data_ptr() % 16):
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 

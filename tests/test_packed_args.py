@@ -59,7 +59,7 @@ def test_plan(ql, kl, causal):
 
 def test_plan_refusals():
     lib = _lib.load()
-    one, neg, big = (np.array([x], np.int32) for x in (4, -1, (1 << 30) + 1))
+    one, neg, big = (np.array([x], np.int32) for x in (4, -1, (1 << 28) + 1))
     nb, st = C.c_size_t(), _lib.PackedWindowsC()
     assert lib.ngt_packed_plan_bytes(1, neg.ctypes.data, one.ctypes.data, C.byref(nb)) == 1
     assert lib.ngt_packed_plan_bytes(1, one.ctypes.data, big.ctypes.data, C.byref(nb)) == 2
@@ -89,10 +89,13 @@ def test_call_refusals_touch_no_gpu():
                       (dict(scale=0.0), 1), (dict(scale=float("nan")), 1),
                       (dict(scale=float("inf")), 1), (dict(q=None), 1), (dict(k=None), 1),
                       (dict(v=None), 1), (dict(out=None), 1), (dict(sq=31), 1), (dict(sk=36), 1),
-                      (dict(q=p + 8), 1), (dict(table=p), 1), (dict(ids=p), 1),
+                      (dict(q=p + 8), 1),
+                      (dict(sk=1 << 22), 2), (dict(H=40000, hkv=40000, d=128), 2), (dict(table=p), 1), (dict(ids=p), 1),
                       (dict(table=p, ids=p, nb=0), 1), (dict(table=p, ids=p, nb=256), 1)):
         assert fwd(**bad) == code, bad
         assert b"ngt_packed_fwd" in lib.ngt_last_error()
+    long, _ = _plan([4], [(1 << 23) + 1], 0)
+    assert fwd(win=C.byref(long), table=p, ids=p, nb=3) == 2
     few, _ = _plan([1], [100000], 1)  # splits its keys: needs a workspace
     fb = C.c_size_t()
     assert lib.ngt_packed_workspace_bytes(1, C.byref(few), 2, 2, 16, 0, C.byref(fb), None) == 0
@@ -109,7 +112,7 @@ def test_call_refusals_touch_no_gpu():
 
 
 def test_python_refusals():
-    for bad in ([[1, 2]], [1.5], [-1], [(1 << 30) + 1], [True]):
+    for bad in ([[1, 2]], [1.5], [-1], [(1 << 28) + 1], [True]):
         with pytest.raises(ValueError):
             PackedWindows(bad, device="cuda:0")
     with pytest.raises(ValueError, match="key lengths"):
