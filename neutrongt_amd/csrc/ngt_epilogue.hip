@@ -15,7 +15,6 @@ namespace {
 
 using packed::f32x16;
 using packed::fill16;
-using packed::mma_rows;
 using packed::tid_x;
 using packed::u32x4;
 using packed::wg_x;
@@ -198,7 +197,7 @@ __global__ __launch_bounds__(256) void k_gemm(GemmArgs a) {
     if (k + kStage < a.K) fetch(k + kStage);
 #pragma unroll
     for (int c = 0; c < L::kChunks; ++c) {
-      u32x4 fx[FM], fw[FN];
+      L::Op fx[FM], fw[FN];
 #pragma unroll
       for (int i = 0; i < FM; ++i) fx[i] = L::load_a(xs + wm * 128, i, c, l32, half);
 #pragma unroll
@@ -206,7 +205,7 @@ __global__ __launch_bounds__(256) void k_gemm(GemmArgs a) {
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = mma_rows<bf16_t>(fw[j], fx[i], acc[i][j]);
+        for (int j = 0; j < FN; ++j) acc[i][j] = L::mma(fw[j], fx[i], acc[i][j]);
     }
   }
 #pragma unroll
@@ -245,7 +244,7 @@ __global__ __launch_bounds__(256) void k_gemm_few(GemmArgs a) {
       if (nx) fw[c] = load8<ALIGNED>(wr, k + 16 * c + 8 * half, a.K);
     }
 #pragma unroll
-    for (int c = 0; c < 4; ++c) acc = mma_rows<bf16_t>(fw[c], fx[c], acc);
+    for (int c = 0; c < 4; ++c) acc = L::mma({{fw[c]}}, {{fx[c]}}, acc);
   }
 #pragma unroll
   for (int g = 0; g < 4; ++g)

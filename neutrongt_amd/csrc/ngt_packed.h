@@ -57,21 +57,6 @@ __device__ __forceinline__ f32x16 fill16(float v) {
   return r;
 }
 
-// c += A B over one 32-byte chunk of both rows: 16 bf16 or 8 fp32 elements.
-template <typename T>
-__device__ __forceinline__ f32x16 mma_rows(u32x4 a, u32x4 b, f32x16 c) {
-  if constexpr (sizeof(T) == 2) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
-                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0,
-                                               0, 0);
-    return c;
-  }
-}
-
 // The two wave halves' values of a row, joined: v_permlane32_swap leaves the
 // lower half's value in r[0] and the upper half's in r[1] of both.
 __device__ __forceinline__ float max_halves(float x) {
@@ -85,14 +70,52 @@ __device__ __forceinline__ float sum_halves(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// DP: the head size rounded up to 32, 64 or 128; T: float or bf16_t.
+// fp32 operands as three bf16 pieces: x = hi + mid + lo, each the rounding of
+// what the ones before it leave.  Six of the nine products of two such operands
+// reach fp32 precision (the three left out are below 2^-24 of the first), and
+// the bf16 matrix instructions are 16 times as fast as the fp32 ones.  What lies
+// below 2^-110 keeps fewer bits (its lower pieces fall below the type).
+struct Pieces2 {
+  uint32_t hi, mid, lo;
+};
+template <bool FINITE>
+__device__ __forceinline__ Pieces2 split2(float a, float b) {
+  auto low = [](uint32_t w) { return __uint_as_float(w << 16); };
+  auto high = [](uint32_t w) { return __uint_as_float(w & 0xffff0000u); };
+  Pieces2 r;
+  r.hi = pack2_bf16(a, b);
+  a -= low(r.hi), b -= high(r.hi);
+  if constexpr (!FINITE) {  // an infinity is its first piece
+    if ((r.hi & 0x7f80u) == 0x7f80u) a = 0.f;
+    if ((r.hi & 0x7f800000u) == 0x7f800000u) b = 0.f;
+  }
+  r.mid = pack2_bf16(a, b);
+  r.lo = pack2_bf16(a - low(r.mid), b - high(r.mid));
+  return r;
+}
+
+// DP: the head size rounded up to 32, 64 or 128; T: float or bf16_t.  fp32
+// tiles up to 64 wide hold three planes of bf16 pieces, 32 rows of a plane side
+// by side; wider ones (whose operands would fill the registers three times over)
+// are fp32 and run on the fp32 instructions.
 template <typename T, int DP>
 struct Tile {
   static constexpr int kEs = static_cast<int>(sizeof(T));
-  static constexpr int kPitch = DP * kEs;     // bytes of a row
-  static constexpr int kPieces = kPitch / 16;  // 16-byte pieces of a row
-  static constexpr int kChunks = kPitch / 32;  // mma_rows steps of a row
+  static constexpr bool kSplit = kEs == 4 && DP <= 64;
+  static constexpr int kPlanes = kSplit ? 3 : 1;
+  static constexpr int kPitch = DP * (kSplit ? 2 : kEs);  // bytes of a row of a plane
+  static constexpr int kRow = kPitch * kPlanes;           // bytes of a row in LDS
+  static constexpr int kPieces = kPitch / 16;  // 16-byte pieces of a plane's row
+  static constexpr int kChunks = kPitch / 32;  // mma steps of a row
   static constexpr int kCols = DP / 32;        // 32-column blocks of a row
+  static constexpr int kMemPieces = DP * kEs / 16;  // 16-byte pieces of a row in memory
+  static constexpr int kRaw = kSplit ? 2 : 1;  // of them in one lane's share of a chunk
+
+  // One lane's share of a chunk of an operand's row: 16 bytes at 32c + 16*half
+  // of each plane.
+  struct Op {
+    u32x4 p[kPlanes];
+  };
 
   __device__ static __forceinline__ int swz(int row) {
     int f = (row >> 1 & 2) | (row >> 4 & 1);
@@ -100,15 +123,69 @@ struct Tile {
     if constexpr (kPieces >= 16) f |= row << 3 & 8;
     return f;
   }
+  // of a row's piece in the first plane
   __device__ static __forceinline__ int offset(int row, int piece) {
-    return row * kPitch + ((piece ^ swz(row)) << 4);
+    return (kPlanes > 1 ? (row >> 5) * 32 * kRow + (row & 31) * kPitch : row * kPitch) +
+           ((piece ^ swz(row)) << 4);
   }
   // Row operand A of rows 32t ..: lane l's row (without 32t).
   __device__ static __forceinline__ int a_row(int l) {
     return 16 * ((l >> 2) & 1) + 4 * (l >> 3) + (l & 3);
   }
-  __device__ static __forceinline__ u32x4 load_a(const char* tile, int t, int c, int l, int half) {
-    return *reinterpret_cast<const u32x4*>(tile + 32 * t * kPitch + offset(a_row(l), 2 * c + half));
+  __device__ static __forceinline__ Op load_a(const char* tile, int t, int c, int l, int half) {
+    Op r;
+#pragma unroll
+    for (int n = 0; n < kPlanes; ++n)
+      r.p[n] = *reinterpret_cast<const u32x4*>(tile + 32 * t * kRow + 32 * n * kPitch +
+                                               offset(a_row(l), 2 * c + half));
+    return r;
+  }
+  // An operand from a row's bytes in memory: kRaw times 16.
+  __device__ static __forceinline__ Op op_of(const u32x4 (&raw)[kRaw]) {
+    Op r;
+    if constexpr (kSplit) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const Pieces2 x = split2<false>(__uint_as_float(raw[i / 2][2 * (i & 1)]),
+                                        __uint_as_float(raw[i / 2][2 * (i & 1) + 1]));
+        r.p[0][i] = x.hi, r.p[1][i] = x.mid, r.p[2][i] = x.lo;
+      }
+    } else {
+      r.p[0] = raw[0];
+    }
+    return r;
+  }
+  // Writes one 16-byte piece of a row in memory to the tile.
+  __device__ static __forceinline__ void put(char* tile, int row, int piece, const u32x4& w) {
+    if constexpr (kSplit) {
+      const Pieces2 a = split2<false>(__uint_as_float(w[0]), __uint_as_float(w[1]));
+      const Pieces2 b = split2<false>(__uint_as_float(w[2]), __uint_as_float(w[3]));
+      char* at = tile + offset(row, piece >> 1) + 8 * (piece & 1);
+      *reinterpret_cast<uint2*>(at) = make_uint2(a.hi, b.hi);
+      *reinterpret_cast<uint2*>(at + 32 * kPitch) = make_uint2(a.mid, b.mid);
+      *reinterpret_cast<uint2*>(at + 64 * kPitch) = make_uint2(a.lo, b.lo);
+    } else {
+      *reinterpret_cast<u32x4*>(tile + offset(row, piece)) = w;
+    }
+  }
+
+  // c += A B over one chunk of both rows (16 elements; 8 of whole fp32).
+  __device__ static __forceinline__ f32x16 mma(const Op& a, const Op& b, f32x16 c) {
+    if constexpr (kEs == 4 && !kSplit) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.p[0][i]),
+                                                 __uint_as_float(b.p[0][i]), c, 0, 0, 0);
+      return c;
+    } else {
+      auto step = [&](int i, int j) {
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a.p[i]),
+                                                    __builtin_bit_cast(bf16x8, b.p[j]), c, 0, 0, 0);
+      };
+      if constexpr (kSplit) step(2, 0), step(0, 2), step(1, 1), step(1, 0), step(0, 1);
+      step(0, 0);
+      return c;
+    }
   }
 
   // acc[dt] (rows = columns 32dt .. of the tile) += tile^T p over tile rows
@@ -116,28 +193,40 @@ struct Tile {
   __device__ static __forceinline__ void mma_cols(const char* tile, int t, const f32x16& p,
                                                   f32x16 (&acc)[kCols], int lane) {
     const int half = lane >> 5;
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (kEs == 2 || kSplit) {
       const int j = lane & 15;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        u32x4 b;
+        Op b;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) b[e] = pack2_bf16(p[8 * c + 2 * e], p[8 * c + 2 * e + 1]);
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (kSplit) {
+            const Pieces2 x = split2<true>(p[8 * c + 2 * e], p[8 * c + 2 * e + 1]);
+            b.p[0][e] = x.hi, b.p[1][e] = x.mid, b.p[2][e] = x.lo;
+          } else {
+            b.p[0][e] = pack2_bf16(p[8 * c + 2 * e], p[8 * c + 2 * e + 1]);
+          }
+        }
         // rows j / 4 and then 4 further: of swz() only bit 1 depends on more than the lane
         const int row = 16 * half + (j >> 2);
         const int piece = 2 * ((lane >> 4) & 1) + ((j & 3) >> 1);
         const int at = (piece ^ swz(row)) * 16 + 8 * (j & 1) + row * kPitch;
 #pragma unroll
         for (int dt = 0; dt < kCols; ++dt) {
-          // the column block is bits 2 and 3 of the piece
-          const int off = (at ^ (dt << 6)) + (32 * t + 8 * c) * kPitch;
-          const int off4 = (at ^ (dt << 6) ^ 32) + (32 * t + 8 * c + 4) * kPitch;
-          typedef __attribute__((address_space(3))) s16x4* lds4_t;
-          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(tile + off));
-          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(tile + off4));
-          const uint2 lw = __builtin_bit_cast(uint2, lo), hw = __builtin_bit_cast(uint2, hi);
-          const u32x4 a = {lw.x, lw.y, hw.x, hw.y};
-          acc[dt] = mma_rows<T>(a, b, acc[dt]);
+          Op a;
+#pragma unroll
+          for (int n = 0; n < kPlanes; ++n) {
+            // the column block is bits 2 and 3 of the piece
+            const char* base = tile + 32 * t * kRow + (32 * n + 8 * c) * kPitch;
+            typedef __attribute__((address_space(3))) s16x4* lds4_t;
+            const s16x4 lo =
+                __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(base + (at ^ (dt << 6))));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds4_t)(base + 4 * kPitch + (at ^ (dt << 6) ^ 32)));
+            const uint2 lw = __builtin_bit_cast(uint2, lo), hw = __builtin_bit_cast(uint2, hi);
+            a.p[n] = u32x4{lw.x, lw.y, hw.x, hw.y};
+          }
+          acc[dt] = mma(a, b, acc[dt]);
         }
       }
     } else {
@@ -156,19 +245,24 @@ struct Tile {
   }
 };
 
-// A lane's row of one head as the chunks it supplies to mma_rows: 16 bytes at
-// 32c + 16*half, zero behind the row's d elements or where the row is not there.
+// A lane's row of one head as the operands it supplies to mma, zero behind the
+// row's d elements or where the row is not there.
 template <typename T, int DP>
 struct RowFrag {
-  static constexpr int NC = Tile<T, DP>::kChunks;
-  u32x4 w[NC];
+  using L = Tile<T, DP>;
+  typename L::Op w[L::kChunks];
   __device__ __forceinline__ void load(const T* __restrict__ row, bool ok, int d, int half) {
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      w[c] = u32x4{0u, 0u, 0u, 0u};
-      if (ok && 32 * c + 16 * half < d * static_cast<int>(sizeof(T)))
-        w[c] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(row) + 32 * c +
-                                               16 * half);
+    for (int c = 0; c < L::kChunks; ++c) {
+      const int at = (2 * c + half) * 16 * L::kRaw;  // bytes
+      u32x4 raw[L::kRaw];
+#pragma unroll
+      for (int i = 0; i < L::kRaw; ++i) {
+        raw[i] = u32x4{0u, 0u, 0u, 0u};
+        if (ok && at < d * L::kEs)
+          raw[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(row) + at + 16 * i);
+      }
+      w[c] = L::op_of(raw);
     }
   }
 };
@@ -197,14 +291,14 @@ constexpr int64_t kMostRowBytes = (1 << 23) - 1;  // of 256 rows, and room for a
 template <typename T, int DP, int ROWS, int N>
 struct Stage {
   using L = Tile<T, DP>;
-  static constexpr int NV = (ROWS * L::kPieces) / N;
-  static_assert(NV * N == ROWS * L::kPieces, "whole pieces per thread");
+  static constexpr int NV = (ROWS * L::kMemPieces) / N;
+  static_assert(NV * N == ROWS * L::kMemPieces, "whole pieces per thread");
   u32x4 w[NV];
   int at[NV];
   __device__ __forceinline__ Stage(int64_t stride, int d, int tid) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int r = (tid + i * N) / L::kPieces, p = (tid + i * N) % L::kPieces;
+      const int r = (tid + i * N) / L::kMemPieces, p = (tid + i * N) % L::kMemPieces;
       at[i] = 16 * p < d * L::kEs ? r * static_cast<int>(stride) + 16 * p : kNowhere;
     }
   }
@@ -220,7 +314,7 @@ struct Stage {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int e = tid + i * N;
-      *reinterpret_cast<u32x4*>(tile + L::offset(e / L::kPieces, e % L::kPieces)) = w[i];
+      L::put(tile, e / L::kMemPieces, e % L::kMemPieces, w[i]);
     }
   }
 };
@@ -264,6 +358,16 @@ __device__ __forceinline__ void join_sets(f32x16& acc, char* buf, int rw, int se
 }
 
 // 4 consecutive values of a row.
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p) {
+  if constexpr (sizeof(T) == 2) {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u),
+                       __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+  } else {
+    return *reinterpret_cast<const float4*>(p);
+  }
+}
 template <typename T>
 __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
   if constexpr (sizeof(T) == 2)
@@ -316,8 +420,8 @@ struct Shape {
 };
 // The most sets of a kernel: by the LDS of its tiles, and for the dK/dV pass,
 // whose two accumulators and two operands fill a wave's registers, by those.
-constexpr int most_sets(int pitch, bool dkv) {
-  return pitch <= 128 ? 4 : pitch <= 256 && !dkv ? 2 : 1;
+constexpr int most_sets(int row, bool dkv) {
+  return row <= 192 ? 4 : row <= 384 && !dkv ? 2 : 1;
 }
 template <int MOST, typename F>
 int with_shape(Shape s, F&& f) {

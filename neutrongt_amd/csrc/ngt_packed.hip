@@ -93,9 +93,9 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_fwd(FwdArgs a) {
   using L = Tile<T, DP>;
   using B = Block<RW, KS>;
   constexpr int N = B::kThreads, kKeys = B::kStage;
-  constexpr int kTileBytes = kKeys * L::kPitch;
+  constexpr int kTileBytes = kKeys * L::kRow;
   // registers for the next stage's pieces, where they are few enough
-  constexpr bool kAhead = (kKeys * L::kPieces / N) * 8 <= 64;
+  constexpr bool kAhead = (kKeys * L::kMemPieces / N) * 8 <= 64;
   __shared__ __align__(16) char
       buf[2 * kTileBytes > B::kJoinBytes ? 2 * kTileBytes : B::kJoinBytes];
   __shared__ float tab[BIAS ? kTable : 1];
@@ -155,8 +155,8 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_fwd(FwdArgs a) {
     pk.load(kb, a.sk, 0, nk, a.d);
     pv.load(vb, a.sv, 0, nk, a.d);
   }
-  const char* kt_tile = ks + 64 * set * L::kPitch;
-  const char* vt_tile = vs + 64 * set * L::kPitch;
+  const char* kt_tile = ks + 64 * set * L::kRow;
+  const char* vt_tile = vs + 64 * set * L::kRow;
   for (int kt = 0; kt < block_end; kt += kKeys) {
     __syncthreads();
     if constexpr (!kAhead) {
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_fwd(FwdArgs a) {
     for (int c = 0; c < L::kChunks; ++c)
 #pragma unroll
       for (int t = 0; t < 2; ++t)
-        x[t] = mma_rows<T>(L::load_a(kt_tile, t, c, l32, half), q.w[c], x[t]);
+        x[t] = L::mma(L::load_a(kt_tile, t, c, l32, half), q.w[c], x[t]);
     if constexpr (BIAS) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -265,7 +265,7 @@ template <typename T, int DP, bool BIAS>
 __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
   using L = Tile<T, DP>;
   const FwdArgs& a = fa.f;
-  constexpr int kTileBytes = 32 * L::kPitch;
+  constexpr int kTileBytes = 32 * L::kRow;
   constexpr int kJoin = 36;  // floats per row of the join's buffer
   constexpr int kBytes = 4 * kTileBytes > 4 * 32 * kJoin * 4 ? 4 * kTileBytes : 4 * 32 * kJoin * 4;
   __shared__ __align__(16) char buf[kBytes];
@@ -314,9 +314,9 @@ __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
   char* vs = buf + wave * kTileBytes;
 
   Stage<T, DP, 32, 64> pv(a.sv, a.d, lane);
-  u32x4 pk[L::kChunks];
+  u32x4 pk[L::kChunks][L::kRaw];
   u32x4 idw = {0u, 0u, 0u, 0u};
-  const int k_at = L::a_row(l32) * static_cast<int>(a.sk) + 16 * half;
+  const int k_at = L::a_row(l32) * static_cast<int>(a.sk);
   const Buffer id_buf = make_buffer(ids, int64_t(nq) * ld);
   const int id_at = qi * ld + 16 * half;
   auto fetch = [&](int t) {
@@ -325,7 +325,11 @@ __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
                                     int64_t(nk - kt - 1) * a.sk + a.d * L::kEs);
 #pragma unroll
     for (int c = 0; c < L::kChunks; ++c)
-      pk[c] = read16(kbuf, 32 * c + 16 * half < a.d * L::kEs ? k_at + 32 * c : kNowhere);
+#pragma unroll
+      for (int i = 0; i < L::kRaw; ++i) {
+        const int at = ((2 * c + half) * L::kRaw + i) * 16;
+        pk[c][i] = read16(kbuf, at < a.d * L::kEs ? k_at + at : kNowhere);
+      }
     pv.load(vb, a.sv, kt, nk, a.d);
     if constexpr (BIAS) idw = read16(id_buf, id_at + kt);
   };
@@ -337,7 +341,7 @@ __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
     if constexpr (BIAS) bias = look_up(tab, idw);
     f32x16 x[1] = {sm.start};
 #pragma unroll
-    for (int c = 0; c < L::kChunks; ++c) x[0] = mma_rows<T>(pk[c], q.w[c], x[0]);
+    for (int c = 0; c < L::kChunks; ++c) x[0] = L::mma(L::op_of(pk[c]), q.w[c], x[0]);
     if constexpr (BIAS) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[0][i] = fmaf(x[0][i], s2, bias[i]);
@@ -642,9 +646,9 @@ int run_fwd(const ngt_packed_windows& w, const FewPlan& fp, FwdArgs a, void* ws,
     }
     return NGT_OK;
   }
-  constexpr int kMost = most_sets(Tile<T, DP>::kPitch, false);
+  constexpr int kMost = most_sets(Tile<T, DP>::kRow, false);
   const Shape shape =
-      pick_shape(w.max_q, (w.max_k + 63) / 64, w.steps_q * a.H, 128 * Tile<T, DP>::kPitch, 512,
+      pick_shape(w.max_q, (w.max_k + 63) / 64, w.steps_q * a.H, 128 * Tile<T, DP>::kRow, 512,
                  kMost);
   const int i = list_of(shape);
   const unsigned blocks = unsigned(w.n_items_q[i]) * unsigned(a.H);
@@ -677,7 +681,10 @@ struct BwdLayout {
 };
 BwdLayout bwd_layout(int dtype, const ngt_packed_windows& w, int H, int Hkv, int d, int n_buckets) {
   BwdLayout L{};
-  const int row = dp_of(d) * (dtype == NGT_F32 ? 4 : 2);  // bytes of a tile's row
+  const int dp = dp_of(d);  // bytes of a tile's row in LDS:
+  const int row = dtype != NGT_F32 ? Tile<bf16_t, 32>::kRow * (dp / 32)
+                  : dp == 128      ? Tile<float, 128>::kRow
+                                   : Tile<float, 32>::kRow * (dp / 32);
   // with a table gradient a wave holds 64 sums per bucket
   L.dq = pick_shape(w.max_q, (w.max_k + 63) / 64, w.steps_q * H, size_t(128) * row,
                     n_buckets ? size_t(n_buckets + 1) * 256 : 0, most_sets(row, false));

@@ -28,8 +28,8 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
   using L = Tile<T, DP>;
   using B = Block<RW, KS>;
   constexpr int N = B::kThreads, kRows = B::kStage;
-  constexpr int kTileBytes = kRows * L::kPitch;
-  constexpr bool kAhead = (kRows * L::kPieces / N) * 8 <= 32;
+  constexpr int kTileBytes = kRows * L::kRow;
+  constexpr bool kAhead = (kRows * L::kMemPieces / N) * 8 <= 32;
   __shared__ __align__(16) char
       buf[2 * kTileBytes > B::kJoinBytes ? 2 * kTileBytes : B::kJoinBytes];
   __shared__ float tab[BIAS ? kTable : 1];
@@ -63,29 +63,14 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
              int64_t(h) * a.d,
          qi < nq, a.d, half);
   g.load(reinterpret_cast<const T*>(a.go) + row, qi < nq, a.d, half);
-  // D: this half's chunks of the row, then both halves
+  // D: every other 4 elements of the row, then both halves
   float D = 0.f;
-#pragma unroll
-  for (int c = 0; c < L::kChunks; ++c) {
-    constexpr int kE = 16 / L::kEs;  // elements of a lane's 16 bytes
-    const int at = (2 * c + half) * kE;
-    if (at < a.d) {
-#pragma unroll
-      for (int e = 0; e < kE; e += 4) {
-        const float4 o = *reinterpret_cast<const float4*>(a.out32 + row + at + e);
-        float x[4];
-        if constexpr (L::kEs == 4) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(g.w[c][i]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t w = g.w[c][(e + i) / 2];
-            x[i] = __uint_as_float((i & 1) ? (w & 0xffff0000u) : (w << 16));
-          }
-        }
-        D = fmaf(x[0], o.x, fmaf(x[1], o.y, fmaf(x[2], o.z, fmaf(x[3], o.w, D))));
-      }
+  if (qi < nq) {
+    const T* gr = reinterpret_cast<const T*>(a.go) + row;
+    for (int at = 4 * half; at < a.d; at += 8) {
+      const float4 o = *reinterpret_cast<const float4*>(a.out32 + row + at);
+      const float4 x = load4(gr + at);
+      D = fmaf(x.x, o.x, fmaf(x.y, o.y, fmaf(x.z, o.z, fmaf(x.w, o.w, D))));
     }
   }
   D = sum_halves(D);
@@ -126,8 +111,8 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
     pk.load(kb, a.sk, 0, nk, a.d);
     pv.load(vb, a.sv, 0, nk, a.d);
   }
-  const char* k_tile = ks + 64 * set * L::kPitch;
-  const char* v_tile = vs + 64 * set * L::kPitch;
+  const char* k_tile = ks + 64 * set * L::kRow;
+  const char* v_tile = vs + 64 * set * L::kRow;
   for (int kt = 0; kt < block_end; kt += kRows) {
     __syncthreads();
     if constexpr (!kAhead) {
@@ -158,8 +143,8 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
       f32x16 s = s_start, dp = dp_start;
 #pragma unroll
       for (int c = 0; c < L::kChunks; ++c) {
-        s = mma_rows<T>(L::load_a(k_tile, t, c, l32, half), q.w[c], s);
-        dp = mma_rows<T>(L::load_a(v_tile, t, c, l32, half), g.w[c], dp);
+        s = L::mma(L::load_a(k_tile, t, c, l32, half), q.w[c], s);
+        dp = L::mma(L::load_a(v_tile, t, c, l32, half), g.w[c], dp);
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i)
@@ -215,8 +200,8 @@ k_packed_dkv(BwdArgs a) {
   using L = Tile<T, DP>;
   using B = Block<RW, KS>;
   constexpr int N = B::kThreads, kRows = B::kStage;
-  constexpr int kTileBytes = kRows * L::kPitch;
-  constexpr bool kAhead = (kRows * L::kPieces / N) * 8 <= 32;
+  constexpr int kTileBytes = kRows * L::kRow;
+  constexpr bool kAhead = (kRows * L::kMemPieces / N) * 8 <= 32;
   __shared__ __align__(16) char
       buf[2 * kTileBytes > B::kJoinBytes ? 2 * kTileBytes : B::kJoinBytes];
   __shared__ __align__(16) float ls[kRows], ds[kRows];
@@ -260,8 +245,8 @@ k_packed_dkv(BwdArgs a) {
   const float lse_per = -1.f / s2;  // into product units
   float pl = 0.f, pd = 0.f;
   u32x4 idw[2], id_next[2];
-  const char* q_tile = qs + 64 * set * L::kPitch;
-  const char* g_tile = gs + 64 * set * L::kPitch;
+  const char* q_tile = qs + 64 * set * L::kRow;
+  const char* g_tile = gs + 64 * set * L::kRow;
   for (int grp = 0; grp < G; ++grp) {
     const int h = kvh * G + grp;
     const T* qb = reinterpret_cast<const T*>(reinterpret_cast<const char*>(a.q) + q0 * a.sq) +
@@ -321,8 +306,8 @@ k_packed_dkv(BwdArgs a) {
         }
 #pragma unroll
         for (int c = 0; c < L::kChunks; ++c) {
-          s = mma_rows<T>(L::load_a(q_tile, t, c, l32, half), k.w[c], s);
-          dp = mma_rows<T>(L::load_a(g_tile, t, c, l32, half), v.w[c], dp);
+          s = L::mma(L::load_a(q_tile, t, c, l32, half), k.w[c], s);
+          dp = L::mma(L::load_a(g_tile, t, c, l32, half), v.w[c], dp);
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -391,7 +376,7 @@ __global__ __launch_bounds__(1024) void k_packed_table_grad(const float* __restr
 template <typename T, int DP, bool BIAS, bool HIST>
 int launch_dq(const BwdArgs& a, const BwdPlan& p, size_t lds, hipStream_t st) {
   KernelTimer timer_("packed_dq", st);
-  return with_shape<most_sets(Tile<T, DP>::kPitch, false)>(p.dq, [&](auto rw, auto ks) {
+  return with_shape<most_sets(Tile<T, DP>::kRow, false)>(p.dq, [&](auto rw, auto ks) {
     auto kernel = k_packed_dq<T, DP, BIAS, HIST, rw.value, ks.value>;
     if (lds)
       NGT_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
@@ -406,7 +391,7 @@ int launch_dq(const BwdArgs& a, const BwdPlan& p, size_t lds, hipStream_t st) {
 template <typename T, int DP, bool BIAS>
 int launch_dkv(const BwdArgs& a, const BwdPlan& p, hipStream_t st) {
   KernelTimer timer_("packed_dkv", st);
-  return with_shape<most_sets(Tile<T, DP>::kPitch, true)>(p.dkv, [&](auto rw, auto ks) {
+  return with_shape<most_sets(Tile<T, DP>::kRow, true)>(p.dkv, [&](auto rw, auto ks) {
     hipLaunchKernelGGL((k_packed_dkv<T, DP, BIAS, rw.value, ks.value>), dim3(unsigned(p.dkv_blocks)),
                        dim3(64 * rw.value * ks.value), 0, st, a);
     NGT_HIP_CHECK(hipGetLastError());
