@@ -94,7 +94,7 @@ __device__ __forceinline__ Pieces2 split2(float a, float b) {
   return r;
 }
 
-// DP: the head size rounded up to 32, 64 or 128; T: float or bf16_t.  fp32
+// DP: the head size rounded up to 16, 32, 64 or 128; T: float or bf16_t.  fp32
 // tiles up to 64 wide hold three planes of bf16 pieces, 32 rows of a plane side
 // by side; wider ones (whose operands would fill the registers three times over)
 // are fp32 and run on the fp32 instructions.
@@ -107,7 +107,7 @@ struct Tile {
   static constexpr int kRow = kPitch * kPlanes;           // bytes of a row in LDS
   static constexpr int kPieces = kPitch / 16;  // 16-byte pieces of a plane's row
   static constexpr int kChunks = kPitch / 32;  // mma steps of a row
-  static constexpr int kCols = DP / 32;        // 32-column blocks of a row
+  static constexpr int kCols = DP < 32 ? 1 : DP / 32;  // 32-column blocks of a row
   static constexpr int kMemPieces = DP * kEs / 16;  // 16-byte pieces of a row in memory
   static constexpr int kRaw = kSplit ? 2 : 1;  // of them in one lane's share of a chunk
 
@@ -118,7 +118,8 @@ struct Tile {
   };
 
   __device__ static __forceinline__ int swz(int row) {
-    int f = (row >> 1 & 2) | (row >> 4 & 1);
+    int f = row >> 4 & 1;
+    if constexpr (kPieces >= 4) f |= row >> 1 & 2;
     if constexpr (kPieces >= 8) f |= row << 1 & 4;
     if constexpr (kPieces >= 16) f |= row << 3 & 8;
     return f;
@@ -209,7 +210,9 @@ struct Tile {
         }
         // rows j / 4 and then 4 further: of swz() only bit 1 depends on more than the lane
         const int row = 16 * half + (j >> 2);
-        const int piece = 2 * ((lane >> 4) & 1) + ((j & 3) >> 1);
+        // (of a 16-wide tile columns 16 .. 31 are 0 .. 15 again: nobody reads those sums)
+        const int piece = (DP < 32 ? 0 : 2 * ((lane >> 4) & 1)) + ((j & 3) >> 1);
+        constexpr int kFlip = kPieces >= 4 ? 32 : 0;
         const int at = (piece ^ swz(row)) * 16 + 8 * (j & 1) + row * kPitch;
 #pragma unroll
         for (int dt = 0; dt < kCols; ++dt) {
@@ -222,7 +225,7 @@ struct Tile {
             const s16x4 lo =
                 __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(base + (at ^ (dt << 6))));
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds4_t)(base + 4 * kPitch + (at ^ (dt << 6) ^ 32)));
+                (lds4_t)(base + 4 * kPitch + (at ^ (dt << 6) ^ kFlip)));
             const uint2 lw = __builtin_bit_cast(uint2, lo), hw = __builtin_bit_cast(uint2, hi);
             a.p[n] = u32x4{lw.x, lw.y, hw.x, hw.y};
           }
@@ -291,8 +294,8 @@ constexpr int64_t kMostRowBytes = (1 << 23) - 1;  // of 256 rows, and room for a
 template <typename T, int DP, int ROWS, int N>
 struct Stage {
   using L = Tile<T, DP>;
-  static constexpr int NV = (ROWS * L::kMemPieces) / N;
-  static_assert(NV * N == ROWS * L::kMemPieces, "whole pieces per thread");
+  static constexpr int kTotal = ROWS * L::kMemPieces;
+  static constexpr int NV = (kTotal + N - 1) / N;
   u32x4 w[NV];
   int at[NV];
   __device__ __forceinline__ Stage(int64_t stride, int d, int tid) {
@@ -314,7 +317,7 @@ struct Stage {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int e = tid + i * N;
-      L::put(tile, e / L::kMemPieces, e % L::kMemPieces, w[i]);
+      if (kTotal % N == 0 || e < kTotal) L::put(tile, e / L::kMemPieces, e % L::kMemPieces, w[i]);
     }
   }
 };

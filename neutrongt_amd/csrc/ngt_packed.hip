@@ -255,7 +255,7 @@ struct FewArgs {
   FwdArgs f;
   int splits;
   float* part_ml;   // [windows * H_kv, splits, 32, 2]: base (log2 units) and sum
-  float* part_acc;  // [windows * H_kv, splits, 32, DP]
+  float* part_acc;  // [windows * H_kv, splits, 32, DP rounded up to 32]
 };
 
 // The rows of one window and key head: row r is query r % nq of the group's
@@ -405,7 +405,7 @@ __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
     const int at = 32 * c + jd;
     if (jr < rows) {
       if (fa.splits > 1) {
-        store4(fa.part_acc + (slot * 32 + jr) * DP + at, o[0], o[1], o[2], o[3]);
+        store4(fa.part_acc + (slot * 32 + jr) * (32 * L::kCols) + at, o[0], o[1], o[2], o[3]);
       } else if (at < a.d) {
         const int64_t row = ((q0 + jq) * a.H + jh) * int64_t(a.d) + at;
         store4(reinterpret_cast<T*>(a.out) + row, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
@@ -435,9 +435,10 @@ __global__ __launch_bounds__(256) void k_packed_few_join(FewArgs fa) {
   if (nq == 0 || jr >= nq * G) return;
   const int jg = jr / nq, jq = jr - jg * nq, jh = kvh * G + jg;
   const int64_t slot = (int64_t(w) * a.Hkv + kvh) * fa.splits;
-  float top = -INFINITY, sum = 0.f, o[DP / 8];
+  constexpr int kCols = Tile<T, DP>::kCols;
+  float top = -INFINITY, sum = 0.f, o[4 * kCols];
 #pragma unroll
-  for (int i = 0; i < DP / 8; ++i) o[i] = 0.f;
+  for (int i = 0; i < 4 * kCols; ++i) o[i] = 0.f;
   for (int s = 0; s < fa.splits; ++s)
     top = fmaxf(top, fa.part_ml[((slot + s) * 32 + jr) * 2]);
   for (int s = 0; s < fa.splits; ++s) {
@@ -446,9 +447,9 @@ __global__ __launch_bounds__(256) void k_packed_few_join(FewArgs fa) {
     const float f = __builtin_amdgcn_exp2f(ml[0] - top);
     sum = fmaf(ml[1], f, sum);
 #pragma unroll
-    for (int c = 0; c < DP / 32; ++c) {
-      const float4 y =
-          *reinterpret_cast<const float4*>(fa.part_acc + ((slot + s) * 32 + jr) * DP + 32 * c + jd);
+    for (int c = 0; c < kCols; ++c) {
+      const float4 y = *reinterpret_cast<const float4*>(
+          fa.part_acc + ((slot + s) * 32 + jr) * (32 * kCols) + 32 * c + jd);
       o[4 * c] = fmaf(y.x, f, o[4 * c]);
       o[4 * c + 1] = fmaf(y.y, f, o[4 * c + 1]);
       o[4 * c + 2] = fmaf(y.z, f, o[4 * c + 2]);
@@ -457,7 +458,7 @@ __global__ __launch_bounds__(256) void k_packed_few_join(FewArgs fa) {
   }
   const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
 #pragma unroll
-  for (int c = 0; c < DP / 32; ++c) {
+  for (int c = 0; c < kCols; ++c) {
     const int at = 32 * c + jd;
     if (at >= a.d) continue;
     const int64_t row = ((q0 + jq) * a.H + jh) * int64_t(a.d) + at;
@@ -536,19 +537,25 @@ inline int list_of(Shape s) { return s.rw == 4 ? 2 : s.rw == 2 ? 1 : 0; }
 // Sets: a wave's path is the stages it passes through, `path` for the longest
 // window; with `steps` of them over all waves a SIMD's share is steps / 1024, and
 // a path of more than 0.7 of that share leaves the chip waiting for the longest
-// blocks: then 2 or 4 sets take turns.  (us, 1 / 2 / 4 sets: dK/dV of 6 windows up
-// to 4,096, 4 heads a group, path 2.5 shares, 340 / 265 / 181; fp32 3,001 rows, 8
-// heads, 1.4 shares, 592 / 544 / 610 for the three passes; 24 windows up to 1,500, 8
-// heads, 0.6 shares, 114 / 120 / 145.)
-// stage: LDS bytes of 64 rows of both tiles; wave: bytes of each wave beside them.
-Shape pick_shape(int32_t longest, int64_t path, int64_t steps, size_t stage, size_t wave,
-                 int most) {
+// blocks: then 2 or 4 sets take turns.  (us, 1 / 2 / 4 sets: dK/dV of 6 causal
+// windows up to 4,096, 4 heads a group, path 2.5 shares, 340 / 265 / 181; fp32, 9
+// windows up to 1,777, 8 heads of 16, 0.85 shares, 233 / 209 / 249 for the three
+// passes; 3,001 rows, 8 heads of 8, 1.4 shares, 366 / 297 / 344; causal forward of the 6
+// windows, 0.64 shares, 87 / 106 / 153.)  Two sets go with four row waves where that
+// gives every compute unit at most one block (192 blocks 297, with two 347) and
+// with two where there are more (448 blocks 225, with two 209).
+// blocks: of four row waves; stage: LDS bytes of 64 rows of both tiles; wave: bytes of
+// each wave beside them.
+Shape pick_shape(int32_t longest, int64_t path, int64_t steps, int64_t blocks, size_t stage,
+                 size_t wave, int most) {
   if (longest <= 32) return Shape{1, 1};
   Shape s{longest <= 64 ? 2 : 4, 1};
   auto over = [&](int ks) { return path * 10 * kSimds > 7 * ks * steps && ks * 2 <= path; };
-  if (most >= 2 && over(1)) s.ks = 2;
+  if (most >= 2 && over(1)) s = Shape{s.rw == 4 && blocks <= kTargetBlocks / 2 ? 4 : 2, 2};
   if (most >= 4 && s.ks == 2 && over(2)) s = Shape{2, 4};
-  auto bytes = [&] { return s.ks * stage + size_t(s.rw) * s.ks * wave + 6 * 1024; };
+  auto bytes = [&] {
+    return std::max(s.ks * stage, size_t(s.ks - 1) * s.rw * 4096) + size_t(s.rw) * s.ks * wave + 6 * 1024;
+  };
   while (bytes() > kLds && s.ks > 1) s = Shape{2, s.ks / 2};
   while (bytes() > kLds && s.rw > 1) s.rw /= 2;
   return s;
@@ -573,12 +580,12 @@ FewPlan few_plan(const ngt_packed_windows& w, int H, int Hkv, int dp) {
   if (p.splits > 1) {
     const size_t rows = size_t(blocks) * p.splits * 32;
     p.acc = align256(rows * 8);
-    p.total = p.acc + align256(rows * dp * 4);
+    p.total = p.acc + align256(rows * std::max(dp, 32) * 4);
   }
   return p;
 }
 
-int dp_of(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+int dp_of(int d) { return d <= 16 ? 16 : d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 
 int check_call(const char* fn, int dtype, const ngt_packed_windows* w, int H, int Hkv, int d,
                float scale, const void* table, int n_buckets, const uint8_t* ids) {
@@ -648,8 +655,8 @@ int run_fwd(const ngt_packed_windows& w, const FewPlan& fp, FwdArgs a, void* ws,
   }
   constexpr int kMost = most_sets(Tile<T, DP>::kRow, false);
   const Shape shape =
-      pick_shape(w.max_q, (w.max_k + 63) / 64, w.steps_q * a.H, 128 * Tile<T, DP>::kRow, 512,
-                 kMost);
+      pick_shape(w.max_q, (w.max_k + 63) / 64, w.steps_q * a.H, int64_t(w.n_items_q[2]) * a.H,
+                 128 * Tile<T, DP>::kRow, 512, kMost);
   const int i = list_of(shape);
   const unsigned blocks = unsigned(w.n_items_q[i]) * unsigned(a.H);
   if (!blocks) return NGT_OK;
@@ -667,10 +674,12 @@ template <typename T>
 int run_fwd_d(int dp, const ngt_packed_windows& w, const FewPlan& fp, const FwdArgs& a, void* ws,
               hipStream_t st) {
   if (a.table)
-    return dp == 32   ? run_fwd<T, 32, true>(w, fp, a, ws, st)
+    return dp == 16   ? run_fwd<T, 16, true>(w, fp, a, ws, st)
+           : dp == 32 ? run_fwd<T, 32, true>(w, fp, a, ws, st)
            : dp == 64 ? run_fwd<T, 64, true>(w, fp, a, ws, st)
                       : run_fwd<T, 128, true>(w, fp, a, ws, st);
-  return dp == 32   ? run_fwd<T, 32, false>(w, fp, a, ws, st)
+  return dp == 16   ? run_fwd<T, 16, false>(w, fp, a, ws, st)
+         : dp == 32 ? run_fwd<T, 32, false>(w, fp, a, ws, st)
          : dp == 64 ? run_fwd<T, 64, false>(w, fp, a, ws, st)
                     : run_fwd<T, 128, false>(w, fp, a, ws, st);
 }
@@ -682,14 +691,15 @@ struct BwdLayout {
 BwdLayout bwd_layout(int dtype, const ngt_packed_windows& w, int H, int Hkv, int d, int n_buckets) {
   BwdLayout L{};
   const int dp = dp_of(d);  // bytes of a tile's row in LDS:
-  const int row = dtype != NGT_F32 ? Tile<bf16_t, 32>::kRow * (dp / 32)
-                  : dp == 128      ? Tile<float, 128>::kRow
-                                   : Tile<float, 32>::kRow * (dp / 32);
+  static_assert(Tile<bf16_t, 16>::kRow == 32 && Tile<float, 16>::kRow == 96 &&
+                    Tile<float, 128>::kRow == 512, "row below");
+  const int row = dtype != NGT_F32 ? 2 * dp : dp == 128 ? 4 * dp : 6 * dp;
   // with a table gradient a wave holds 64 sums per bucket
-  L.dq = pick_shape(w.max_q, (w.max_k + 63) / 64, w.steps_q * H, size_t(128) * row,
+  L.dq = pick_shape(w.max_q, (w.max_k + 63) / 64, w.steps_q * H, int64_t(w.n_items_q[2]) * H,
+                    size_t(128) * row,
                     n_buckets ? size_t(n_buckets + 1) * 256 : 0, most_sets(row, false));
   L.dkv = pick_shape(w.max_k, int64_t((w.max_q + 63) / 64) * (H / Hkv), w.steps_k * H,
-                     size_t(128) * row, 0, most_sets(row, true));
+                     int64_t(w.n_items_k[2]) * Hkv, size_t(128) * row, 0, most_sets(row, true));
   L.part = align256(size_t(w.n_q) * H * 4);
   L.total = L.part + align256(size_t(w.n_items_q[list_of(L.dq)]) * H * n_buckets * 4);
   return L;

@@ -428,12 +428,14 @@ int bwd(const BwdPlan& p, const BwdArgs& base, hipStream_t st) {
 }  // namespace
 
 int packed_bwd(int dtype, const BwdPlan& p, const BwdArgs& a, hipStream_t st) {
-  const int dp = a.d <= 32 ? 32 : a.d <= 64 ? 64 : 128;
-  if (dtype == NGT_F32)
-    return dp == 32 ? bwd<float, 32>(p, a, st) : dp == 64 ? bwd<float, 64>(p, a, st)
-                                                          : bwd<float, 128>(p, a, st);
-  return dp == 32 ? bwd<bf16_t, 32>(p, a, st) : dp == 64 ? bwd<bf16_t, 64>(p, a, st)
-                                                         : bwd<bf16_t, 128>(p, a, st);
+  auto run = [&](auto t) {
+    using T = decltype(t);
+    return a.d <= 16   ? bwd<T, 16>(p, a, st)
+           : a.d <= 32 ? bwd<T, 32>(p, a, st)
+           : a.d <= 64 ? bwd<T, 64>(p, a, st)
+                       : bwd<T, 128>(p, a, st);
+  };
+  return dtype == NGT_F32 ? run(float{}) : run(bf16_t{});
 }
 
 }  // namespace packed
