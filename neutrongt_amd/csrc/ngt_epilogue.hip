@@ -166,18 +166,41 @@ __global__ __launch_bounds__(256) void k_gemm(GemmArgs a) {
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = fill16(0.f);
   u32x4 px[NX], pw[NW];
+  // ALIGNED: pieces through buffer descriptors, rows that are not there as zeros;
+  // a piece behind the row's end (the last stage's) is sent behind the buffer's
+  int ax[NX], aw[NW];
+  const int col = 8 * (tid % 8);
+  if constexpr (ALIGNED) {
+#pragma unroll
+    for (int i = 0; i < NX; ++i)
+      ax[i] = 2 * ((tid + i * 256) / 8 * static_cast<int>(a.x_stride) + col);
+#pragma unroll
+    for (int i = 0; i < NW; ++i) aw[i] = 2 * ((tid + i * 256) / 8 * a.K + col);
+  }
   auto fetch = [&](int k) {
+    if constexpr (ALIGNED) {
+      const int over = k + col < a.K ? 0 : packed::kNowhere;
+      const packed::Buffer bx = packed::make_buffer(
+          a.x + m0 * a.x_stride + k, 2 * ((min(BM, a.M - m0) - 1) * a.x_stride + a.K - k));
+      const packed::Buffer bw = packed::make_buffer(
+          a.w + int64_t(n0) * a.K + k, 2 * ((min(BN, a.N - n0) - 1) * int64_t(a.K) + a.K - k));
 #pragma unroll
-    for (int i = 0; i < NX; ++i) {
-      const int e = tid + i * 256, row = m0 + e / 8;
-      px[i] = u32x4{0u, 0u, 0u, 0u};
-      if (row < a.M) px[i] = load8<ALIGNED>(a.x + row * a.x_stride, k + 8 * (e % 8), a.K);
-    }
+      for (int i = 0; i < NX; ++i) px[i] = packed::read16(bx, ax[i] | over);
 #pragma unroll
-    for (int i = 0; i < NW; ++i) {
-      const int e = tid + i * 256, row = n0 + e / 8;
-      pw[i] = u32x4{0u, 0u, 0u, 0u};
-      if (row < a.N) pw[i] = load8<ALIGNED>(a.w + int64_t(row) * a.K, k + 8 * (e % 8), a.K);
+      for (int i = 0; i < NW; ++i) pw[i] = packed::read16(bw, aw[i] | over);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        const int e = tid + i * 256, row = m0 + e / 8;
+        px[i] = u32x4{0u, 0u, 0u, 0u};
+        if (row < a.M) px[i] = load8<false>(a.x + row * a.x_stride, k + 8 * (e % 8), a.K);
+      }
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {
+        const int e = tid + i * 256, row = n0 + e / 8;
+        pw[i] = u32x4{0u, 0u, 0u, 0u};
+        if (row < a.N) pw[i] = load8<false>(a.w + int64_t(row) * a.K, k + 8 * (e % 8), a.K);
+      }
     }
   };
   fetch(0);
@@ -305,7 +328,9 @@ bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 
 int launch_gemm(GemmArgs a, hipStream_t st) {
   KernelTimer timer_("linear_gemm", st);
-  const bool al = a.K % 8 == 0 && a.N % 8 == 0 && a.x_stride % 8 == 0 && aligned16(a.x) &&
+  // 16-byte accesses, and 32-bit offsets within a tile's 256 rows
+  constexpr int64_t kFar = 1 << 21;
+  const bool al = a.K < kFar && a.x_stride < kFar && a.K % 8 == 0 && a.N % 8 == 0 && a.x_stride % 8 == 0 && aligned16(a.x) &&
                   aligned16(a.w) && aligned16(a.bias) && aligned16(a.r) && aligned16(a.y) &&
                   aligned16(a.z);
   auto tiles = [&](int bm, int bn) {
