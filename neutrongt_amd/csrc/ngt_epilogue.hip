@@ -97,36 +97,36 @@ __device__ __forceinline__ float half_of(const u32x4& v, int i) {
   return __uint_as_float((i & 1) ? (w & 0xffff0000u) : (w << 16));
 }
 
-// 8 outputs n .. n+7 of row m from their sums.
+// 8 results from their sums and their pieces of bias and residual (zeros where
+// there are none).
+__device__ __forceinline__ void results8(int act, const float (&s)[8], const u32x4& bias,
+                                         const u32x4& res, u32x4& y, u32x4& z) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = s[i] + half_of(bias, i);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) z[i] = pack2_bf16(v[2 * i], v[2 * i + 1]);
+  if (act == kActGelu) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = act_of<kActGelu>(v[i]);
+  } else if (act == kActRelu) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = act_of<kActRelu>(v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    y[i] = pack2_bf16(v[2 * i] + half_of(res, 2 * i), v[2 * i + 1] + half_of(res, 2 * i + 1));
+}
+
+// 8 outputs n .. n+7 of row m.
 template <bool ALIGNED>
 __device__ __forceinline__ void finish8(const GemmArgs& a, int m, int n, const float (&s)[8]) {
   if (m >= a.M || n >= a.N) return;
   const int64_t at = int64_t(m) * a.N + n;
-  float v[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = s[i];
-  if (a.bias) {
-    const u32x4 b = load8<ALIGNED>(a.bias, n, a.N);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += half_of(b, i);
-  }
-  u32x4 z, y;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) z[i] = pack2_bf16(v[2 * i], v[2 * i + 1]);
-  if (a.act == kActGelu) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = act_of<kActGelu>(v[i]);
-  } else if (a.act == kActRelu) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = act_of<kActRelu>(v[i]);
-  }
-  if (a.r) {
-    const u32x4 r = load8<ALIGNED>(a.r + int64_t(m) * a.N, n, a.N);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += half_of(r, i);
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) y[i] = pack2_bf16(v[2 * i], v[2 * i + 1]);
+  u32x4 b = {0u, 0u, 0u, 0u}, r = {0u, 0u, 0u, 0u}, y, z;
+  if (a.bias) b = load8<ALIGNED>(a.bias, n, a.N);
+  if (a.r) r = load8<ALIGNED>(a.r + int64_t(m) * a.N, n, a.N);
+  results8(a.act, s, b, r, y, z);
   if (ALIGNED || n + 8 <= a.N) {
     if constexpr (ALIGNED) {
       *reinterpret_cast<u32x4*>(a.y + at) = y;
@@ -217,7 +217,7 @@ __global__ __launch_bounds__(256) void k_gemm(GemmArgs a) {
       *reinterpret_cast<u32x4*>(ws + L::offset(e / 8, e % 8)) = pw[i];
     }
     __syncthreads();
-    if (k + kStage < a.K) fetch(k + kStage);
+    fetch(k + kStage);  // (behind the last stage: zeros)
 #pragma unroll
     for (int c = 0; c < L::kChunks; ++c) {
       L::Op fx[FM], fw[FN];
@@ -231,18 +231,60 @@ __global__ __launch_bounds__(256) void k_gemm(GemmArgs a) {
         for (int j = 0; j < FN; ++j) acc[i][j] = L::mma(fw[j], fx[i], acc[i][j]);
     }
   }
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
+  if constexpr (ALIGNED) {
+    // all pieces of bias and residual under way at once (waiting for each in its
+    // turn took 7 us a block); what is not there reads as zero and is not written
+    const int64_t base = int64_t(m0) * a.N + n0;
+    const int64_t bytes = 2 * (int64_t(min(BM, a.M - m0) - 1) * a.N + min(BN, a.N - n0));
+    const packed::Buffer br = packed::make_buffer(a.r + base, a.r ? bytes : 0);
+    const packed::Buffer bb = packed::make_buffer(a.bias + n0, a.bias ? 2 * (a.N - n0) : 0);
+    const packed::Buffer by = packed::make_buffer(a.y + base, bytes);
+    const packed::Buffer bz = packed::make_buffer(a.z + base, a.z ? bytes : 0);
+    auto at = [&](int i, int j, int e) {
+      const int c = wn + 32 * j + 16 * half + 8 * e;
+      return n0 + c < a.N ? 2 * ((wm + 32 * i + L::a_row(l32)) * a.N + c) : packed::kNowhere;
+    };
+    u32x4 bias[FN][2], res[FM][FN][2];
 #pragma unroll
     for (int j = 0; j < FN; ++j)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float s[8];
+      for (int e = 0; e < 2; ++e)
+        bias[j][e] = packed::read16(bb, 2 * (wn + 32 * j + 16 * half + 8 * e));
 #pragma unroll
-        for (int t = 0; t < 8; ++t) s[t] = acc[i][j][8 * e + t];
-        finish8<ALIGNED>(a, m0 + wm + 32 * i + L::a_row(l32), n0 + wn + 32 * j + 16 * half + 8 * e,
-                         s);
-      }
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          res[i][j][e] = a.r ? packed::read16(br, at(i, j, e)) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float s[8];
+          u32x4 y, z;
+#pragma unroll
+          for (int t = 0; t < 8; ++t) s[t] = acc[i][j][8 * e + t];
+          results8(a.act, s, bias[j][e], res[i][j][e], y, z);
+          __builtin_amdgcn_raw_buffer_store_b128(y, by, at(i, j, e), 0, 0);
+          if (a.z) __builtin_amdgcn_raw_buffer_store_b128(z, bz, at(i, j, e), 0, 0);
+        }
+  } else {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float s[8];
+#pragma unroll
+          for (int t = 0; t < 8; ++t) s[t] = acc[i][j][8 * e + t];
+          finish8<false>(a, m0 + wm + 32 * i + L::a_row(l32),
+                         n0 + wn + 32 * j + 16 * half + 8 * e, s);
+        }
+  }
 }
 
 // Few outputs: one block 32 rows by 32 outputs straight from memory, its four
@@ -330,7 +372,7 @@ int launch_gemm(GemmArgs a, hipStream_t st) {
   KernelTimer timer_("linear_gemm", st);
   // 16-byte accesses, and 32-bit offsets within a tile's 256 rows
   constexpr int64_t kFar = 1 << 21;
-  const bool al = a.K < kFar && a.x_stride < kFar && a.K % 8 == 0 && a.N % 8 == 0 && a.x_stride % 8 == 0 && aligned16(a.x) &&
+  const bool al = a.K < kFar && a.N < kFar && a.x_stride < kFar && a.K % 8 == 0 && a.N % 8 == 0 && a.x_stride % 8 == 0 && aligned16(a.x) &&
                   aligned16(a.w) && aligned16(a.bias) && aligned16(a.r) && aligned16(a.y) &&
                   aligned16(a.z);
   auto tiles = [&](int bm, int bn) {
