@@ -287,43 +287,77 @@ __global__ __launch_bounds__(256) void k_gemm(GemmArgs a) {
   }
 }
 
-// Few outputs: one block 32 rows by 32 outputs straight from memory, its four
-// waves a quarter of the contraction each; their sums are added in wave order.
-template <bool ALIGNED>
+// Few outputs: one block 32 F rows by 32 F outputs straight from memory, its
+// four waves every fourth 64 of the contraction each; their sums are added in
+// wave order.
+template <int F, bool ALIGNED>
 __global__ __launch_bounds__(256) void k_gemm_few(GemmArgs a) {
   constexpr int kPitch = 36;  // floats
   __shared__ __align__(16) float red[4][32][kPitch];
-  const int tid = tid_x(), lane = tid & 63, wave = tid >> 6, half = lane >> 5, l32 = lane & 31;
-  const int m0 = wg_x() / a.tiles_n * 32, n0 = wg_x() % a.tiles_n * 32;
+  const int tid = tid_x(), lane = tid & 63, half = lane >> 5, l32 = lane & 31;
+  const int wave = packed::wave_id();
+  const int m0 = wg_x() / a.tiles_n * (32 * F), n0 = wg_x() % a.tiles_n * (32 * F);
   const int row = L::a_row(l32);
-  const bool mx = m0 + l32 < a.M, nx = n0 + row < a.N;
-  const uint16_t* xr = a.x + (mx ? (m0 + l32) * a.x_stride : 0);
-  const uint16_t* wr = a.w + (nx ? int64_t(n0 + row) * a.K : 0);
-  f32x16 acc = fill16(0.f);
+  f32x16 acc[F][F];
+#pragma unroll
+  for (int i = 0; i < F; ++i)
+#pragma unroll
+    for (int j = 0; j < F; ++j) acc[i][j] = fill16(0.f);
+  packed::Buffer bx, bw;
+  if constexpr (ALIGNED) {
+    bx = packed::make_buffer(a.x + m0 * a.x_stride,
+                             2 * ((min(32 * F, a.M - m0) - 1) * a.x_stride + a.K));
+    bw = packed::make_buffer(a.w + int64_t(n0) * a.K, 2 * (min(32 * F, a.N - n0) * int64_t(a.K)));
+  }
   for (int k = 64 * wave; k < a.K; k += 256) {
-    u32x4 fx[4], fw[4];
+    u32x4 fx[F][4], fw[F][4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      fx[c] = fw[c] = u32x4{0u, 0u, 0u, 0u};
-      if (mx) fx[c] = load8<ALIGNED>(xr, k + 16 * c + 8 * half, a.K);
-      if (nx) fw[c] = load8<ALIGNED>(wr, k + 16 * c + 8 * half, a.K);
+      const int col = k + 16 * c + 8 * half;
+#pragma unroll
+      for (int i = 0; i < F; ++i) {
+        if constexpr (ALIGNED) {
+          const int over = col < a.K ? 0 : packed::kNowhere;
+          fx[i][c] =
+              packed::read16(bx, 2 * ((32 * i + l32) * static_cast<int>(a.x_stride) + col) | over);
+          fw[i][c] = packed::read16(bw, 2 * ((32 * i + row) * a.K + col) | over);
+        } else {
+          fx[i][c] = fw[i][c] = u32x4{0u, 0u, 0u, 0u};
+          if (m0 + 32 * i + l32 < a.M)
+            fx[i][c] = load8<false>(a.x + (m0 + 32 * i + l32) * a.x_stride, col, a.K);
+          if (n0 + 32 * i + row < a.N)
+            fw[i][c] = load8<false>(a.w + int64_t(n0 + 32 * i + row) * a.K, col, a.K);
+        }
+      }
     }
 #pragma unroll
-    for (int c = 0; c < 4; ++c) acc = L::mma({{fw[c]}}, {{fx[c]}}, acc);
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int i = 0; i < F; ++i)
+#pragma unroll
+        for (int j = 0; j < F; ++j)
+          acc[i][j] = L::mma({{fw[j][c]}}, {{fx[i][c]}}, acc[i][j]);
   }
 #pragma unroll
-  for (int g = 0; g < 4; ++g)
-    *reinterpret_cast<float4*>(&red[wave][l32][16 * half + 4 * g]) =
-        make_float4(acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]);
-  __syncthreads();
-  if (tid < 128) {
-    const int m = tid >> 2, n = (tid & 3) * 8;
-    float s[8];
+  for (int i = 0; i < F; ++i)
 #pragma unroll
-    for (int t = 0; t < 8; ++t)
-      s[t] = ((red[0][m][n + t] + red[1][m][n + t]) + red[2][m][n + t]) + red[3][m][n + t];
-    finish8<ALIGNED>(a, m0 + m, n0 + n, s);
-  }
+    for (int j = 0; j < F; ++j) {
+      if (i + j > 0) __syncthreads();
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<float4*>(&red[wave][l32][16 * half + 4 * g]) =
+            make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2],
+                        acc[i][j][4 * g + 3]);
+      __syncthreads();
+      if (tid < 128) {
+        const int m = tid >> 2, n = (tid & 3) * 8;
+        float s[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+          s[t] = ((red[0][m][n + t] + red[1][m][n + t]) + red[2][m][n + t]) + red[3][m][n + t];
+        finish8<ALIGNED>(a, m0 + 32 * i + m, n0 + 32 * j + n, s);
+      }
+    }
 }
 
 // dz = dy act'(z), 8 elements a thread.
@@ -372,26 +406,38 @@ int launch_gemm(GemmArgs a, hipStream_t st) {
   KernelTimer timer_("linear_gemm", st);
   // 16-byte accesses, and 32-bit offsets within a tile's 256 rows
   constexpr int64_t kFar = 1 << 21;
-  const bool al = a.K < kFar && a.N < kFar && a.x_stride < kFar && a.K % 8 == 0 && a.N % 8 == 0 && a.x_stride % 8 == 0 && aligned16(a.x) &&
-                  aligned16(a.w) && aligned16(a.bias) && aligned16(a.r) && aligned16(a.y) &&
-                  aligned16(a.z);
+  const bool al = a.K < kFar && a.N < kFar && a.x_stride < kFar && a.K % 8 == 0 &&
+                  a.N % 8 == 0 && a.x_stride % 8 == 0 && aligned16(a.x) && aligned16(a.w) &&
+                  aligned16(a.bias) && aligned16(a.r) && aligned16(a.y) && aligned16(a.z);
   auto tiles = [&](int bm, int bn) {
     a.tiles_m = (a.M + bm - 1) / bm;
     a.tiles_n = (a.N + bn - 1) / bn;
     return int64_t(a.tiles_m) * a.tiles_n;
   };
-  if (tiles(128, 128) < 128) {
-    const int64_t n = tiles(32, 32);
-    if (al) hipLaunchKernelGGL(k_gemm_few<true>, dim3(unsigned(n)), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(k_gemm_few<false>, dim3(unsigned(n)), dim3(256), 0, st, a);
-  } else if (tiles(256, 128) < 256) {
-    const int64_t n = (tiles(128, 128) + 7) / 8 * 8;
-    if (al) hipLaunchKernelGGL((k_gemm<128, 128, true>), dim3(unsigned(n)), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_gemm<128, 128, false>), dim3(unsigned(n)), dim3(256), 0, st, a);
+  auto run = [&](auto kernel, auto loose, int64_t n) {
+    if (al) hipLaunchKernelGGL(kernel, dim3(unsigned(n)), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(loose, dim3(unsigned(n)), dim3(256), 0, st, a);
+  };
+  auto eighths = [](int64_t n) { return (n + 7) / 8 * 8; };
+  // By the count of 128 x 128 tiles, for the card's 256 CUs (us with bias, GELU and
+  // residual: 32 | 64 | 128 | 256 rows a block).  32-row blocks while the wider ones
+  // leave most CUs without work: 4,096 x 1,024 at 40 rows (32 tiles) 6.6 | 11.3 | 18.3,
+  // 768 x 768 at 512 (24) 8.6 | 10.5 | 15.8; but at 1,024 (48) 11.8 | 10.9 | 15.7, and
+  // 4,096 x 1,024 at 256 (64) 18.2 | 13.9 | 18.7.  Then whole tiles through LDS:
+  // 768 x 768 at 2,048 (96) 21.9 | 19.9 | 16.2, 4,096 x 1,024 at 512 (128)
+  // 33.1 | 22.6 | 23.4.  Tiles of 256 rows read less through LDS, but take several
+  // blocks on every CU and a long contraction to fill: 4,096 x 1,024 at 4,096 (512 of
+  // them) 55.5 | 49.4, at 10,007 133 | 124, 1,024 x 4,096 at 32,768 352 | 313, but 768 x 768
+  // at 32,768 62.6 | 65.4, 1,024 x 4,096 at 10,007 (320) 113 | 126.
+  const int64_t t128 = tiles(128, 128);
+  if (t128 < 40) {
+    run(k_gemm_few<1, true>, k_gemm_few<1, false>, tiles(32, 32));
+  } else if (t128 < 80) {
+    run(k_gemm_few<2, true>, k_gemm_few<2, false>, tiles(64, 64));
+  } else if (a.K < 1024 || tiles(256, 128) < 512) {
+    run(k_gemm<128, 128, true>, k_gemm<128, 128, false>, eighths(tiles(128, 128)));
   } else {
-    const int64_t n = (tiles(256, 128) + 7) / 8 * 8;
-    if (al) hipLaunchKernelGGL((k_gemm<256, 128, true>), dim3(unsigned(n)), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_gemm<256, 128, false>), dim3(unsigned(n)), dim3(256), 0, st, a);
+    run(k_gemm<256, 128, true>, k_gemm<256, 128, false>, eighths(tiles(256, 128)));
   }
   NGT_HIP_CHECK(hipGetLastError());
   return NGT_OK;

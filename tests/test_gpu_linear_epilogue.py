@@ -101,6 +101,17 @@ def test_tiles(dev, M, N, K, act, bias, res):
     _case(dev, M, N, K, act, bias, res, seed=N)
 
 
+@pytest.mark.parametrize("M,N,K", [(1100, 700, 96), (1001, 770, 99), (40, 5200, 264),
+                                   (520, 1000, 1024)])
+def test_between_few_outputs_and_tiles(dev, M, N, K):
+    _case(dev, M, N, K, "gelu", seed=K)
+
+
+@pytest.mark.parametrize("M,N,K", [(32700, 513, 1032), (32700, 513, 1025), (32641, 520, 1024)])
+def test_many_tiles_of_a_long_contraction(dev, M, N, K):
+    _case(dev, M, N, K, "relu", seed=N)
+
+
 def test_fp32_parameters_and_inputs(dev):
     _case(dev, 700, 96, 160, "gelu", w_type=F32)
     x, w, b, r, gy = _inputs(50, 24, 40, True, True, 3)
