@@ -39,8 +39,8 @@ struct GemmArgs {
 // from Abramowitz and Stegun 7.1.26: for z < 0
 //   Phi(z) = erfc(x) / 2 = (a1 t + .. + a5 t^5) e^(-x^2) / 2, x = |z| / sqrt 2, t = 1 / (1 + p x)
 // and 1 - Phi(-z) above; off by at most 1.5e-7 / 2, far below a half step of bf16
-// and without cancellation below zero.  (The device library's erff costs more
-// than the products: 128 outputs a lane, 10,007 x 1,024 -> 4,096 169 us, see k_gemm.)
+// and without cancellation below zero.  (10,007 x 1,024 -> 4,096 with the device
+// library's erff 169 us, with this 135 us when it was put in.)
 struct Normal {
   float cdf, pdf;  // pdf times sqrt(2 pi)
 };
@@ -145,14 +145,42 @@ __device__ __forceinline__ void finish8(const GemmArgs& a, int m, int n, const f
   }
 }
 
-// One block: BM rows by BN outputs, 2 x 2 waves.
-template <int BM, int BN, bool ALIGNED>
+// 64 pieces of a wave from memory to LDS, one after another from `at`.
+__device__ __forceinline__ void to_lds(packed::Buffer b, int offset, char* at) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      b, (__attribute__((address_space(3))) void*)at, 16, offset, 0, 0, 0);
+}
+// Until at most N of this wave's reads from memory are under way.
+template <int N>
+__device__ __forceinline__ void wait_for_all_but() {
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);
+}
+
+// One block: BM rows by BN outputs, 2 x 2 waves of (BM / 2) x (BN / 2), stages of 64
+// of the contraction in LDS.  A 128 x 128 block's stage is 512 clocks of MFMA, 512 of
+// its CU's reads from LDS and 256 of writes to it, and as many from L2; the 256 x 128
+// block has three quarters of the traffic per MFMA.
+// BUFS = 1: read, wait, multiply; the 2 to 3 blocks of a CU fill each other's waits
+// (10,007 x 4,096 -> 1,024 88 us, 113 us with the pieces read into registers and
+// stored to LDS a stage later).
+// BUFS = 4: three stages under way while one is multiplied, for a grid of at most one
+// block a CU, where nothing else fills the waits (2,048 x 4,096 -> 1,024 41 us,
+// BUFS = 1 64 us).
+// What is left of it then is the wait for the stage's first fragments and, with GELU,
+// the epilogue: 100 clocks an output and SIMD, as much as 600 of the contraction.
+template <int BM, int BN, int BUFS, bool ALIGNED>
 __global__ __launch_bounds__(256) void k_gemm(GemmArgs a) {
   constexpr int FM = BM / 64, FN = BN / 64;  // 32 x 32 tiles of a wave
   constexpr int NX = BM * 8 / 256, NW = BN * 8 / 256;  // 16-byte pieces per thread
-  __shared__ __align__(16) char xs[BM * 128];
-  __shared__ __align__(16) char ws[BN * 128];
+  constexpr int kTiles = (BM + BN) * 128, kMore = BUFS > 1 ? kTiles : 16;
+  // arrays of their own, so that the compiler knows a read from one independent of
+  // what is on its way to another
+  __shared__ __align__(16) char s0[kTiles];
+  __shared__ __align__(16) char s1[kMore];
+  __shared__ __align__(16) char s2[kMore];
+  __shared__ __align__(16) char s3[kMore];
   const int tid = tid_x(), lane = tid & 63, wave = tid >> 6, half = lane >> 5, l32 = lane & 31;
+  const int in_wave_order = 1024 * packed::wave_id();
   // each XCD (block number mod 8) takes a contiguous run of tiles, the tiles
   // of a row of x one after another: its L2 holds W and each row once
   const int total = a.tiles_m * a.tiles_n, per = (total + 7) / 8;
@@ -165,30 +193,95 @@ __global__ __launch_bounds__(256) void k_gemm(GemmArgs a) {
   for (int i = 0; i < FM; ++i)
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = fill16(0.f);
-  u32x4 px[NX], pw[NW];
-  // ALIGNED: pieces through buffer descriptors, rows that are not there as zeros;
-  // a piece behind the row's end (the last stage's) is sent behind the buffer's
-  int ax[NX], aw[NW];
-  const int col = 8 * (tid % 8);
+
+  // the next chunk's fragments are read before a chunk's products
+  auto multiply = [&](const char* xs) {
+    const char* ws = xs + BM * 128;
+    L::Op fx[2][FM], fw[2][FN];
+    auto read = [&](int c) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i) fx[c & 1][i] = L::load_a(xs + wm * 128, i, c, l32, half);
+#pragma unroll
+      for (int j = 0; j < FN; ++j) fw[c & 1][j] = L::load_a(ws + wn * 128, j, c, l32, half);
+    };
+    read(0);
+#pragma unroll
+    for (int c = 0; c < L::kChunks; ++c) {
+      if (c + 1 < L::kChunks) read(c + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = L::mma(fw[c & 1][j], fx[c & 1][i], acc[i][j]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
   if constexpr (ALIGNED) {
+    // Rows that are not there read as zeros, a piece behind the row's end (the last
+    // stage's) is sent behind the buffer's.  A wave's pieces lie one after another
+    // in LDS, so the swizzle is in which piece of its row a thread reads.
+    int ax[NX], aw[NW];
+    auto piece = [&](int i) {
+      const int r = (tid + i * 256) / 8;
+      return 8 * (tid % 8 ^ L::swz(r));
+    };
 #pragma unroll
     for (int i = 0; i < NX; ++i)
-      ax[i] = 2 * ((tid + i * 256) / 8 * static_cast<int>(a.x_stride) + col);
+      ax[i] = 2 * ((tid + i * 256) / 8 * static_cast<int>(a.x_stride) + piece(i));
 #pragma unroll
-    for (int i = 0; i < NW; ++i) aw[i] = 2 * ((tid + i * 256) / 8 * a.K + col);
-  }
-  auto fetch = [&](int k) {
-    if constexpr (ALIGNED) {
-      const int over = k + col < a.K ? 0 : packed::kNowhere;
+    for (int i = 0; i < NW; ++i) aw[i] = 2 * ((tid + i * 256) / 8 * a.K + piece(i));
+    auto fetch = [&](int k, char* to) {
       const packed::Buffer bx = packed::make_buffer(
           a.x + m0 * a.x_stride + k, 2 * ((min(BM, a.M - m0) - 1) * a.x_stride + a.K - k));
       const packed::Buffer bw = packed::make_buffer(
           a.w + int64_t(n0) * a.K + k, 2 * ((min(BN, a.N - n0) - 1) * int64_t(a.K) + a.K - k));
 #pragma unroll
-      for (int i = 0; i < NX; ++i) px[i] = packed::read16(bx, ax[i] | over);
+      for (int i = 0; i < NX; ++i)
+        to_lds(bx, ax[i] | (k + piece(i) < a.K ? 0 : packed::kNowhere),
+               to + 4096 * i + in_wave_order);
 #pragma unroll
-      for (int i = 0; i < NW; ++i) pw[i] = packed::read16(bw, aw[i] | over);
+      for (int i = 0; i < NW; ++i)
+        to_lds(bw, aw[i] | (k + piece(i) < a.K ? 0 : packed::kNowhere),
+               to + BM * 128 + 4096 * i + in_wave_order);
+    };
+    if constexpr (BUFS == 1) {
+      for (int k = 0; k < a.K; k += kStage) {
+        __syncthreads();
+        fetch(k, s0);
+        wait_for_all_but<0>();
+        __syncthreads();
+        multiply(s0);
+      }
     } else {
+      auto step = [&](int k, char* to, const char* from) {
+        // this wave's pieces of stage k are there; behind the barrier all waves' are,
+        // and all have read what `to` held
+        wait_for_all_but<2 * (NX + NW)>();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        fetch(k + 3 * kStage, to);  // (behind the last stage: zeros)
+        multiply(from);
+      };
+      fetch(0, s0);
+      fetch(kStage, s1);
+      fetch(2 * kStage, s2);
+      for (int k = 0;;) {
+        step(k, s3, s0);
+        if ((k += kStage) >= a.K) break;
+        step(k, s0, s1);
+        if ((k += kStage) >= a.K) break;
+        step(k, s1, s2);
+        if ((k += kStage) >= a.K) break;
+        step(k, s2, s3);
+        if ((k += kStage) >= a.K) break;
+      }
+      wait_for_all_but<0>();  // nothing is on its way to LDS when the block ends
+    }
+  } else {
+    u32x4 px[NX], pw[NW];
+    auto fetch = [&](int k) {
 #pragma unroll
       for (int i = 0; i < NX; ++i) {
         const int e = tid + i * 256, row = m0 + e / 8;
@@ -201,34 +294,23 @@ __global__ __launch_bounds__(256) void k_gemm(GemmArgs a) {
         pw[i] = u32x4{0u, 0u, 0u, 0u};
         if (row < a.N) pw[i] = load8<false>(a.w + int64_t(row) * a.K, k + 8 * (e % 8), a.K);
       }
-    }
-  };
-  fetch(0);
-  for (int k = 0; k < a.K; k += kStage) {
-    __syncthreads();
+    };
+    fetch(0);
+    for (int k = 0; k < a.K; k += kStage) {
+      __syncthreads();
 #pragma unroll
-    for (int i = 0; i < NX; ++i) {
-      const int e = tid + i * 256;
-      *reinterpret_cast<u32x4*>(xs + L::offset(e / 8, e % 8)) = px[i];
-    }
+      for (int i = 0; i < NX; ++i) {
+        const int e = tid + i * 256;
+        *reinterpret_cast<u32x4*>(s0 + L::offset(e / 8, e % 8)) = px[i];
+      }
 #pragma unroll
-    for (int i = 0; i < NW; ++i) {
-      const int e = tid + i * 256;
-      *reinterpret_cast<u32x4*>(ws + L::offset(e / 8, e % 8)) = pw[i];
-    }
-    __syncthreads();
-    fetch(k + kStage);  // (behind the last stage: zeros)
-#pragma unroll
-    for (int c = 0; c < L::kChunks; ++c) {
-      L::Op fx[FM], fw[FN];
-#pragma unroll
-      for (int i = 0; i < FM; ++i) fx[i] = L::load_a(xs + wm * 128, i, c, l32, half);
-#pragma unroll
-      for (int j = 0; j < FN; ++j) fw[j] = L::load_a(ws + wn * 128, j, c, l32, half);
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = L::mma(fw[j], fx[i], acc[i][j]);
+      for (int i = 0; i < NW; ++i) {
+        const int e = tid + i * 256;
+        *reinterpret_cast<u32x4*>(s0 + BM * 128 + L::offset(e / 8, e % 8)) = pw[i];
+      }
+      __syncthreads();
+      fetch(k + kStage);  // (behind the last stage: zeros)
+      multiply(s0);
     }
   }
   if constexpr (ALIGNED) {
@@ -420,24 +502,26 @@ int launch_gemm(GemmArgs a, hipStream_t st) {
   };
   auto eighths = [](int64_t n) { return (n + 7) / 8 * 8; };
   // By the count of 128 x 128 tiles, for the card's 256 CUs (us with bias, GELU and
-  // residual: 32 | 64 | 128 | 256 rows a block).  32-row blocks while the wider ones
-  // leave most CUs without work: 4,096 x 1,024 at 40 rows (32 tiles) 6.6 | 11.3 | 18.3,
-  // 768 x 768 at 512 (24) 8.6 | 10.5 | 15.8; but at 1,024 (48) 11.8 | 10.9 | 15.7, and
-  // 4,096 x 1,024 at 256 (64) 18.2 | 13.9 | 18.7.  Then whole tiles through LDS:
-  // 768 x 768 at 2,048 (96) 21.9 | 19.9 | 16.2, 4,096 x 1,024 at 512 (128)
-  // 33.1 | 22.6 | 23.4.  Tiles of 256 rows read less through LDS, but take several
-  // blocks on every CU and a long contraction to fill: 4,096 x 1,024 at 4,096 (512 of
-  // them) 55.5 | 49.4, at 10,007 133 | 124, 1,024 x 4,096 at 32,768 352 | 313, but 768 x 768
-  // at 32,768 62.6 | 65.4, 1,024 x 4,096 at 10,007 (320) 113 | 126.
+  // residual: 32 | 64 rows a block | 128 in four buffers | 128 | 256).  Narrow blocks
+  // while wider ones leave most CUs without work: 4,096 x 1,024 at 40 rows (32 tiles)
+  // 6.6 | 11.3 | 15.1, 768 x 768 at 512 (24) 8.6 | 10.5 | 13.0; but at 1,024 (48)
+  // 11.8 | 10.9 | 13.1, and 4,096 x 1,024 at 256 (64) 18.2 | 13.9 | 15.8.  Then whole
+  // tiles through LDS: 768 x 768 at 2,048 (96) - | 19.9 | 13.3 | 15.0, and at 10,007 (474)
+  // - | 62 | 27.9 | 24.7.  Tiles of 256 rows need several blocks on every CU and a long
+  // contraction: 4,096 x 1,024 at 4,096 (512 of them) 52.2 | 47.3, at 32,768 404 | 387,
+  // 1,024 x 4,096 at 32,768 317 | 285, but at 10,007 (320) 87.7 | 108, and 768 x 768 at
+  // 32,768 57.0 | 63.1.
   const int64_t t128 = tiles(128, 128);
   if (t128 < 40) {
     run(k_gemm_few<1, true>, k_gemm_few<1, false>, tiles(32, 32));
   } else if (t128 < 80) {
     run(k_gemm_few<2, true>, k_gemm_few<2, false>, tiles(64, 64));
+  } else if (t128 <= 256) {
+    run(k_gemm<128, 128, 4, true>, k_gemm<128, 128, 1, false>, eighths(tiles(128, 128)));
   } else if (a.K < 1024 || tiles(256, 128) < 512) {
-    run(k_gemm<128, 128, true>, k_gemm<128, 128, false>, eighths(tiles(128, 128)));
+    run(k_gemm<128, 128, 1, true>, k_gemm<128, 128, 1, false>, eighths(tiles(128, 128)));
   } else {
-    run(k_gemm<256, 128, true>, k_gemm<256, 128, false>, eighths(tiles(256, 128)));
+    run(k_gemm<256, 128, 1, true>, k_gemm<256, 128, 1, false>, eighths(tiles(256, 128)));
   }
   NGT_HIP_CHECK(hipGetLastError());
   return NGT_OK;

@@ -107,6 +107,12 @@ def test_between_few_outputs_and_tiles(dev, M, N, K):
     _case(dev, M, N, K, "gelu", seed=K)
 
 
+# K of one stage, a part of one, and ends after each of the four buffers
+@pytest.mark.parametrize("K", [8, 64, 72, 128, 192, 200, 256, 320, 456, 512])
+def test_one_block_on_each_cu(dev, K):
+    _case(dev, 1800, 1024, K, "gelu", seed=K)
+
+
 @pytest.mark.parametrize("M,N,K", [(32700, 513, 1032), (32700, 513, 1025), (32641, 520, 1024)])
 def test_many_tiles_of_a_long_contraction(dev, M, N, K):
     _case(dev, M, N, K, "relu", seed=N)
