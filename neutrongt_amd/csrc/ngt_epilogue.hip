@@ -157,17 +157,19 @@ __device__ __forceinline__ void wait_for_all_but() {
 }
 
 // One block: BM rows by BN outputs, 2 x 2 waves of (BM / 2) x (BN / 2), stages of 64
-// of the contraction in LDS.  A 128 x 128 block's stage is 512 clocks of MFMA, 512 of
-// its CU's reads from LDS and 256 of writes to it, and as many from L2; the 256 x 128
-// block has three quarters of the traffic per MFMA.
+// of the contraction in LDS.  A 128 x 128 block's stage takes 512 clocks of the CU's
+// MFMA, 512 of its reads from LDS, 256 of the writes there and 512 of its path from L2
+// (32 KB at 64 bytes a clock); a 256 x 128 block has three quarters of that traffic per
+// MFMA.
 // BUFS = 1: read, wait, multiply; the 2 to 3 blocks of a CU fill each other's waits
 // (10,007 x 4,096 -> 1,024 88 us, 113 us with the pieces read into registers and
 // stored to LDS a stage later).
 // BUFS = 4: three stages under way while one is multiplied, for a grid of at most one
 // block a CU, where nothing else fills the waits (2,048 x 4,096 -> 1,024 41 us,
 // BUFS = 1 64 us).
-// What is left of it then is the wait for the stage's first fragments and, with GELU,
-// the epilogue: 100 clocks an output and SIMD, as much as 600 of the contraction.
+// What is left then is the wait for each stage's first fragments and, with GELU, the
+// epilogue: some 100 clocks for a wave's 64 outputs, 6,600 a block, the MFMA time of
+// 800 of the contraction (blocks on the same CU overlap it, a lone one does not).
 template <int BM, int BN, int BUFS, bool ALIGNED>
 __global__ __launch_bounds__(256) void k_gemm(GemmArgs a) {
   constexpr int FM = BM / 64, FN = BN / 64;  // 32 x 32 tiles of a wave

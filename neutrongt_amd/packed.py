@@ -88,13 +88,11 @@ class PackedWindows:
     def ptr(self):
         return C.byref(self.struct)
 
-    def on_current_stream(self, *more: torch.Tensor) -> None:
-        """Keeps the plan's memory (and ``more``, allocated with it) from being
-        reused before the work that the current stream is about to get has run."""
+    def on_current_stream(self) -> None:
+        """Keeps the plan's memory from being reused before the work that the
+        current stream is about to get has run."""
         if _stream(self.device) != self.stream:
-            cur = torch.cuda.current_stream(self.device)
-            for t in (self.mem, *more):
-                t.record_stream(cur)
+            self.mem.record_stream(torch.cuda.current_stream(self.device))
 
     def workspace_bytes(self, dtype: int, heads: int, kv_heads: int, dim: int, n_buckets: int = 0):
         f, b = C.c_size_t(), C.c_size_t()
@@ -132,13 +130,20 @@ class PairBuckets:
     def __init__(self, windows: PackedWindows, ids: torch.Tensor):
         s, dev = windows.struct, windows.device
         self.windows = windows
-        windows.on_current_stream(ids)
+        self.stream = _stream(dev)  # the memory's own
+        windows.on_current_stream()
         self.by_query = torch.empty(max(s.bucket_bytes_q, 1), dtype=torch.uint8, device=dev)
         self.by_key = torch.empty(max(s.bucket_bytes_k, 1), dtype=torch.uint8, device=dev)
         with torch.cuda.device(dev):
             _lib.check(_lib.load().ngt_packed_buckets(
                 windows.ptr(), ids.data_ptr(), ids.element_size(), self.by_query.data_ptr(),
-                self.by_key.data_ptr(), _stream(dev)))
+                self.by_key.data_ptr(), self.stream))
+
+    def on_current_stream(self) -> None:
+        """As PackedWindows.on_current_stream, of the ids."""
+        if _stream(self.windows.device) != self.stream:
+            for t in (self.by_query, self.by_key):
+                t.record_stream(torch.cuda.current_stream(self.windows.device))
 
 
 class PackedAttentionFunction(torch.autograd.Function):
@@ -237,7 +242,9 @@ def packed_attention(q, k, v, windows: PackedWindows, scale: float | None = None
         raise ValueError("buckets must come from these windows' pack_buckets")
     by = (buckets.by_query, buckets.by_key) if buckets is not None else (None, None)
     if q.is_cuda and q.dim() == 3:
-        windows.on_current_stream(*(t for t in by if t is not None))
+        windows.on_current_stream()
+        if buckets is not None:
+            buckets.on_current_stream()
         ext = _lib.node_ext()
         out = ext and ext.packed_attention(
             q, k, v, bias_table, windows.struct_bytes, windows.mem, *by,

@@ -417,3 +417,62 @@ def test_a_plan_made_and_dropped_on_another_stream(dev):
         side.synchronize()
         assert torch.equal(out, want[0])
         del junk
+
+
+def test_ids_laid_out_and_dropped_on_another_stream(dev):
+    """As above for the pairs' ids, whose memory is the side stream's."""
+    ql = [600] * 4
+    q, k, v, go, table, ids = _inputs(ql, ql, 4, 4, 16, BF16, 9, seed=32)
+    win = PackedWindows(ql, device=dev)
+    q, k, v, table, ids = (t.to(dev) for t in (q, k, v, table, ids))
+    with torch.no_grad():
+        want = packed_attention(q, k, v, win, bias_table=table, buckets=win.pack_buckets(ids))
+        side = torch.cuda.Stream(dev)
+        for _ in range(5):
+            side.wait_stream(torch.cuda.current_stream(dev))
+            with torch.cuda.stream(side):
+                b = win.pack_buckets(ids)
+            torch.cuda.current_stream(dev).wait_stream(side)
+            for _ in range(10):
+                out = packed_attention(q, k, v, win, bias_table=table, buckets=b)
+            n = b.by_query.numel()
+            del b
+            with torch.cuda.stream(side):
+                junk = [torch.zeros(n, dtype=torch.uint8, device=dev) for _ in range(4)]
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+            del junk
+
+
+def test_two_graphs_and_eager_calls_of_one_plan(dev):
+    """Two captured training steps of one plan, replayed in turn and side by side
+    on two streams, with eager steps in between."""
+    ql = [130, 7, 64]
+    win = PackedWindows(ql, device=dev)
+    sets = [[t.to(dev) for t in _inputs(ql, ql, 4, 2, 16, BF16, 12, seed=s)] for s in (40, 41)]
+    b = win.pack_buckets(sets[0][5])
+
+    def step(q, k, v, go, table, _):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, table)]
+        out = packed_attention(*leaves[:3], win, bias_table=leaves[3], buckets=b)
+        return [out.detach(), *torch.autograd.grad(out, leaves, go)]
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    graphs, static = [], []
+    for s in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            static.append(step(*s))
+    side = torch.cuda.Stream(dev)
+    for i in range(4):
+        for x in (*static[0], *static[1]):
+            x.zero_()
+        side.wait_stream(torch.cuda.current_stream(dev))
+        graphs[0].replay()
+        with torch.cuda.stream(side) if i % 2 else torch.cuda.stream(torch.cuda.current_stream(dev)):
+            graphs[1].replay()
+        eager = step(*sets[i % 2])
+        torch.cuda.synchronize()
+        for a, w in ((static[0], want[0]), (static[1], want[1]), (eager, want[i % 2])):
+            assert all(torch.equal(x, y) for x, y in zip(a, w))
