@@ -190,7 +190,9 @@ struct Tile {
   }
 
   // acc[dt] (rows = columns 32dt .. of the tile) += tile^T p over tile rows
-  // 32t .. 32t+31, p the lane's 16 values of those rows.
+  // 32t .. 32t+31, p the lane's 16 values of those rows; for bf16 rounded to it,
+  // or, with FINE, as two bf16 pieces (16 bits).
+  template <bool FINE = false>
   __device__ static __forceinline__ void mma_cols(const char* tile, int t, const f32x16& p,
                                                   f32x16 (&acc)[kCols], int lane) {
     const int half = lane >> 5;
@@ -198,10 +200,16 @@ struct Tile {
       const int j = lane & 15;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        Op b;
+        Op b, rest;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if constexpr (kSplit) {
+          if constexpr (FINE && !kSplit) {
+            const float x = p[8 * c + 2 * e], y = p[8 * c + 2 * e + 1];
+            const uint32_t hi = pack2_bf16(x, y);
+            b.p[0][e] = hi;
+            rest.p[0][e] = pack2_bf16(x - __uint_as_float(hi << 16),
+                                      y - __uint_as_float(hi & 0xffff0000u));
+          } else if constexpr (kSplit) {
             const Pieces2 x = split2<true>(p[8 * c + 2 * e], p[8 * c + 2 * e + 1]);
             b.p[0][e] = x.hi, b.p[1][e] = x.mid, b.p[2][e] = x.lo;
           } else {
@@ -229,6 +237,7 @@ struct Tile {
             const uint2 lw = __builtin_bit_cast(uint2, lo), hw = __builtin_bit_cast(uint2, hi);
             a.p[n] = u32x4{lw.x, lw.y, hw.x, hw.y};
           }
+          if constexpr (FINE && !kSplit) acc[dt] = mma(a, rest, acc[dt]);
           acc[dt] = mma(a, b, acc[dt]);
         }
       }
@@ -267,6 +276,14 @@ struct RowFrag {
       }
       w[c] = L::op_of(raw);
     }
+  }
+  // -x for every element where `odd`
+  __device__ __forceinline__ void negate(bool odd) {
+    const uint32_t m = !odd ? 0u : L::kEs == 2 || L::kSplit ? 0x80008000u : 0x80000000u;
+#pragma unroll
+    for (int c = 0; c < L::kChunks; ++c)
+#pragma unroll
+      for (int n = 0; n < L::kPlanes; ++n) w[c].p[n] ^= u32x4{m, m, m, m};
   }
 };
 

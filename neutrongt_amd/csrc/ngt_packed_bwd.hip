@@ -90,8 +90,17 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
     my_hist = hist + wid * (a.n_buckets + 1) * 32 + l32;
   }
   const float s2 = a.scale * kLog2e;
-  // the products start from -lse (with a bias; in their units) and -D
-  const f32x16 s_start = fill16(BIAS ? -lse / s2 : 0.f), dp_start = fill16(-D);
+  // The bf16 matrix instructions round their sums down, a row's dP - D by some 2^-25 of
+  // its terms; the bias's gradient adds up millions of them, so in fp32 odd rows take
+  // everything with the other sign there, and what was rounded down cancels (fp32, 3,001
+  // rows, 40 buckets: the gradient's error 2.8e-6 -> 4.3e-7 of its norm, no time).
+  constexpr bool kTurn = HIST && sizeof(T) == 4;
+  const float sign = kTurn && (l32 & 1) ? -1.f : 1.f;
+  if constexpr (kTurn) g.negate(l32 & 1), D *= sign;
+  // bf16 with a bias: the products start from -lse, in their units, and -D; in fp32
+  // -lse would cost them bits there
+  constexpr bool kFromLse = BIAS && sizeof(T) == 2;
+  const f32x16 s_start = fill16(kFromLse ? -lse / s2 : 0.f), dp_start = fill16(-D);
   f32x16 acc[L::kCols];
 #pragma unroll
   for (int c = 0; c < L::kCols; ++c) acc[c] = fill16(0.f);
@@ -148,7 +157,7 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        s[i] = fmaf(s[i], s2, BIAS ? bias[i] : -lse);
+        s[i] = fmaf(s[i], s2, kFromLse ? bias[i] : BIAS ? bias[i] - lse : -lse);
       if (k1 + 32 * t + 31 > first_lim) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -157,12 +166,16 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i]) * dp[i];
       if constexpr (HIST) add_to_buckets(my_hist, idw[t], s, a.n_buckets);
-      L::mma_cols(k_tile, t, s, acc, lane);
+      // a row's dS add up to zero, so what its keys have in common cancels, and in heads
+      // of up to 16 that is much of them: there dS goes in as two bf16 pieces (8 heads of
+      // 8, 1,500 rows: dQ's error 1.6 -> 1.07 times that of rounding the result; 35 -> 45 us)
+      L::template mma_cols<DP == 16>(k_tile, t, s, acc, lane);
     }
   }
 #pragma unroll
   for (int c = 0; c < L::kCols; ++c) join_sets<RW, KS>(acc[c], buf, wave, set, lane);
   if (qi < nq && set == 0) {
+    const float by = sign * a.scale;
     T* o = reinterpret_cast<T*>(a.gq) + ((q0 + qi) * a.H + h) * int64_t(a.d);
 #pragma unroll
     for (int c = 0; c < L::kCols; ++c)
@@ -170,8 +183,8 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
       for (int i = 0; i < 4; ++i) {
         const int at = 32 * c + 8 * i + 4 * half;
         if (at < a.d)
-          store4(o + at, acc[c][4 * i] * a.scale, acc[c][4 * i + 1] * a.scale,
-                 acc[c][4 * i + 2] * a.scale, acc[c][4 * i + 3] * a.scale);
+          store4(o + at, acc[c][4 * i] * by, acc[c][4 * i + 1] * by, acc[c][4 * i + 2] * by,
+                 acc[c][4 * i + 3] * by);
       }
   }
   if constexpr (HIST) {
@@ -180,7 +193,9 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
       double sum = 0.;
       for (int w = 0; w < RW * KS; ++w) {
         const double* hw = hist + (w * (a.n_buckets + 1) + b) * 32;
-        for (int i = 0; i < 32; ++i) sum += hw[(i + b) & 31];  // from its own place: no bank twice
+        // from its own place: no bank twice; odd rows with their sign
+        for (int i = 0; i < 32; ++i)
+          sum += kTurn && ((i + b) & 1) ? -hw[(i + b) & 31] : hw[(i + b) & 31];
       }
       a.part_table[(int64_t(h) * a.n_items + it) * a.n_buckets + b] = static_cast<float>(sum);
     }
@@ -242,7 +257,10 @@ k_packed_dkv(BwdArgs a) {
 
   const int64_t sg = int64_t(a.H) * a.d * L::kEs;
   Stage<T, DP, kRows, N> pq(a.sq, a.d, tid), pg(sg, a.d, tid);
-  const float lse_per = -1.f / s2;  // into product units
+  // bf16: the products start from -lse, in their units; in fp32 that would cost them
+  // bits (9 windows of 33 to 1,777, heads of 16: dK's error 7.4e-7 -> 4.4e-7 of its norm)
+  constexpr bool kFromLse = sizeof(T) == 2;
+  const float lse_per = kFromLse ? -1.f / s2 : -1.f;
   float pl = 0.f, pd = 0.f;
   u32x4 idw[2], id_next[2];
   const char* q_tile = qs + 64 * set * L::kRow;
@@ -295,11 +313,12 @@ k_packed_dkv(BwdArgs a) {
       for (int t = 0; t < 2; ++t) {
         f32x16 bias;
         if constexpr (BIAS) bias = look_up(tab, idw[t]);
-        f32x16 s, dp;  // start from -lse, in product units, and -D of the rows
+        f32x16 s, dp;  // start from -lse (bf16) and -D of the rows
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int at = 64 * set + 32 * t + 16 * half + 4 * i;
-          const float4 x = *reinterpret_cast<const float4*>(ls + at);
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+          if constexpr (kFromLse) x = *reinterpret_cast<const float4*>(ls + at);
           const float4 y = *reinterpret_cast<const float4*>(ds + at);
           s[4 * i] = x.x, s[4 * i + 1] = x.y, s[4 * i + 2] = x.z, s[4 * i + 3] = x.w;
           dp[4 * i] = y.x, dp[4 * i + 1] = y.y, dp[4 * i + 2] = y.z, dp[4 * i + 3] = y.w;
@@ -310,8 +329,14 @@ k_packed_dkv(BwdArgs a) {
           dp = L::mma(L::load_a(g_tile, t, c, l32, half), v.w[c], dp);
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          s[i] = BIAS ? fmaf(s[i], s2, bias[i]) : s[i] * s2;
+        for (int i = 0; i < 16; ++i) {
+          if constexpr (kFromLse) {
+            s[i] = BIAS ? fmaf(s[i], s2, bias[i]) : s[i] * s2;
+          } else {
+            const float minus = ls[64 * set + 32 * t + 16 * half + i];
+            s[i] = fmaf(s[i], s2, BIAS ? bias[i] + minus : minus);
+          }
+        }
         if (q1 + 32 * t < last_lim) {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
