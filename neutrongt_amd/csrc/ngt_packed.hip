@@ -1,5 +1,19 @@
 // Attention over packed windows: sequences of different lengths back to back,
 // grouped heads, causal order, a learned bias per pair bucket.  Forward.
+//   s_ij = scale q_i.k_j + table[id_ij, h],  o_i = sum_j e^(s_ij - lse_i) v_j over the
+//   pairs that i sees,  lse_i = log sum_j e^s_ij (kept in log2 units for the backward)
+// in one pass over a window's keys, with the running base and sum of each row in
+// registers (RowSoftmax); no score goes to memory.  Scores, sums and statistics are
+// fp32; in bf16 a weight is rounded to bf16 for its product with v (a half step of
+// each, as the result's own), in fp32 it goes in as three bf16 pieces.
+//
+// What bounds it.  1,024 pairs cost a SIMD 4 DP clocks of the matrix cores for both
+// products and some 9 vector instructions a lane's score, the exponential four times as
+// long as another: 600 to 800 clocks, which set the pace up to d = 64 and weigh about as
+// much as the products at 128 (5 causal windows of 500 to 4,096, 32 heads of 128 over 8:
+// 290 us, 865 TFLOP/s of the pairs seen).  With a bias a pair adds a byte of ids from
+// memory and a table entry from LDS, and the vector instructions are 62 % of the time (3
+// windows of 1,000 to 3,333, 32 heads of 24: 245 us).
 #include "ngt_packed.h"
 
 #include <string.h>
@@ -87,7 +101,8 @@ struct RowSoftmax {
 };
 
 // One block: RW * 32 query rows of one window and head; the window's keys pass
-// through LDS 64 * KS at a time.
+// through LDS 64 * KS at a time (pick_shape says which and why).  The next stage's
+// pieces are on their way while one is used.
 template <typename T, int DP, bool BIAS, int RW, int KS>
 __global__ __launch_bounds__(64 * RW * KS) void k_packed_fwd(FwdArgs a) {
   using L = Tile<T, DP>;
@@ -261,6 +276,9 @@ struct FewArgs {
 // The rows of one window and key head: row r is query r % nq of the group's
 // head r / nq.  One block: the keys of one split, each wave its own tiles of
 // 32 keys straight from memory (nothing is shared between waves but the end).
+// Bound by the cache's bytes: 32 windows of 1,000 to 16,384 keys, 8 key heads of 128,
+// 230 us, 3.8 TB/s of the 4.9 of a copy; short ones by the launches (8 windows of 60 to
+// 1,000: NODES_FIG).
 template <typename T, int DP, bool BIAS>
 __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
   using L = Tile<T, DP>;
