@@ -278,7 +278,7 @@ struct FewArgs {
 // 32 keys straight from memory (nothing is shared between waves but the end).
 // Bound by the cache's bytes: 32 windows of 1,000 to 16,384 keys, 8 key heads of 128,
 // 230 us, 3.8 TB/s of the 4.9 of a copy; short ones by the launches (8 windows of 60 to
-// 1,000: NODES_FIG).
+// 1,000: 7 us one after another in a graph, with the join).
 template <typename T, int DP, bool BIAS>
 __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
   using L = Tile<T, DP>;
@@ -457,21 +457,39 @@ __global__ __launch_bounds__(256) void k_packed_few_join(FewArgs fa) {
   float top = -INFINITY, sum = 0.f, o[4 * kCols];
 #pragma unroll
   for (int i = 0; i < 4 * kCols; ++i) o[i] = 0.f;
-  for (int s = 0; s < fa.splits; ++s)
-    top = fmaxf(top, fa.part_ml[((slot + s) * 32 + jr) * 2]);
-  for (int s = 0; s < fa.splits; ++s) {
-    const float* ml = fa.part_ml + ((slot + s) * 32 + jr) * 2;
-    if (ml[0] == -INFINITY) continue;
-    const float f = __builtin_amdgcn_exp2f(ml[0] - top);
-    sum = fmaf(ml[1], f, sum);
+  const int last = fa.splits - 1;
+  const float* ml = fa.part_ml + (slot * 32 + jr) * 2;
+  const float* acc = fa.part_acc + (slot * 32 + jr) * (32 * kCols) + jd;
+  for (int s = 0; s < fa.splits; s += 8) {
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) {
-      const float4 y = *reinterpret_cast<const float4*>(
-          fa.part_acc + ((slot + s) * 32 + jr) * (32 * kCols) + 32 * c + jd);
-      o[4 * c] = fmaf(y.x, f, o[4 * c]);
-      o[4 * c + 1] = fmaf(y.y, f, o[4 * c + 1]);
-      o[4 * c + 2] = fmaf(y.z, f, o[4 * c + 2]);
-      o[4 * c + 3] = fmaf(y.w, f, o[4 * c + 3]);
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, ml[min(s + i, last) * 64]);
+  }
+  // kAtOnce splits' reads under way together
+  constexpr int kAtOnce = kCols > 2 ? 4 : 8;
+  for (int s = 0; s < fa.splits; s += kAtOnce) {
+    float2 x[kAtOnce];
+    float4 y[kAtOnce][kCols];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int64_t at = min(s + i, last);
+      x[i] = *reinterpret_cast<const float2*>(ml + at * 64);
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+        y[i][c] = *reinterpret_cast<const float4*>(acc + at * (32 * 32 * kCols) + 32 * c);
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      // (a split that saw nothing has written no sums)
+      if (s + i > last || x[i].x == -INFINITY) continue;
+      const float f = __builtin_amdgcn_exp2f(x[i].x - top);
+      sum = fmaf(x[i].y, f, sum);
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) {
+        o[4 * c] = fmaf(y[i][c].x, f, o[4 * c]);
+        o[4 * c + 1] = fmaf(y[i][c].y, f, o[4 * c + 1]);
+        o[4 * c + 2] = fmaf(y[i][c].z, f, o[4 * c + 2]);
+        o[4 * c + 3] = fmaf(y[i][c].w, f, o[4 * c + 3]);
+      }
     }
   }
   const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
@@ -595,9 +613,17 @@ FewPlan few_plan(const ngt_packed_windows& w, int H, int Hkv, int dp) {
   if (!p.use) return p;
   const int64_t blocks = int64_t(w.n_windows) * Hkv;
   const int tiles = (w.max_k + 31) / 32;
-  p.splits = static_cast<int>(std::min<int64_t>((kTargetBlocks + blocks - 1) / blocks,
-                                                std::max(1, tiles / 8)));
-  p.splits = std::max(1, std::min(p.splits, 64));
+  // Two blocks for each compute unit, of two tiles a wave or more; many splits cost the
+  // join (us, 8 heads of 16, one window of 16,000 keys: 62 splits 16.8, 31 12.7, 15 12.1;
+  // 4,000: 15 8.0, 7 8.0, 3 10.5; 1,000: 3 6.9, 1 7.0), and none saves its launch (600 keys:
+  // 2 splits 7.2, 1 5.7).
+  if (tiles < 24) {
+    p.splits = 1;
+  } else {
+    const int most = std::min({64, tiles / 8, std::max(16, tiles / 32)});
+    p.splits = static_cast<int>(
+        std::min<int64_t>((kTargetBlocks + blocks - 1) / blocks, most));
+  }
   if (p.splits > 1) {
     const size_t rows = size_t(blocks) * p.splits * 32;
     p.acc = align256(rows * 8);
