@@ -473,11 +473,17 @@ __global__ __launch_bounds__(256) void k_transpose(const uint16_t* __restrict__ 
                                                    uint16_t* __restrict__ out) {
   __shared__ uint16_t t[64][66];
   const int r0 = wg_x() / tiles_c * 64, c0 = wg_x() % tiles_c * 64;
-  for (int e = tid_x(); e < 4096; e += 256) {
-    const int r = r0 + e / 64, c = c0 + e % 64;
-    if (r < rows && c < cols) t[e / 64][e % 64] = in[int64_t(r) * cols + c];
+  // all reads under way at once: of what is there, not written where it is not
+  uint16_t v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int e = tid_x() + 256 * i;
+    v[i] = in[int64_t(min(r0 + e / 64, rows - 1)) * cols + min(c0 + e % 64, cols - 1)];
   }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) t[(tid_x() + 256 * i) / 64][tid_x() % 64] = v[i];
   __syncthreads();
+#pragma unroll
   for (int e = tid_x(); e < 4096; e += 256) {
     const int c = c0 + e / 64, r = r0 + e % 64;
     if (r < rows && c < cols) out[int64_t(c) * rows + r] = t[e % 64][e / 64];
