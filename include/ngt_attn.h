@@ -458,9 +458,10 @@ int ngt_adj_weights(const int64_t* edge_index, const float* ppr_val, int64_t n_e
  * Table entries may be -infinity (never seen) or the type's lowest value (seen
  * where nothing greater is).
  *
- * out_f32 and lse [H, n_q] (log2 units) are what the backward needs (both
- * nullable in a forward without one): out again in fp32, and each row's
- * softmax statistic.  The backward writes grad_q [n_q, H, d], grad_k and
+ * out_f32 and lse [H, n_q], with a table [2, H, n_q] (log2 units), are what the
+ * backward needs (both nullable in a forward without one): out again in fp32,
+ * and each row's softmax statistic (with a table and rows whose greatest score is
+ * beyond +-256 its two parts).  The backward writes grad_q [n_q, H, d], grad_k and
  * grad_v [n_k, H_kv, d] and, where grad_table is not null, grad_table
  * [n_buckets, H]; grad_out is contiguous.  All sums are fp32 in a fixed order.
  * workspace: ngt_packed_workspace_bytes with the same dtype, windows and heads;

@@ -615,7 +615,7 @@ PackedForward packed_forward(const Tensor& q, const Tensor& k, const Tensor& v, 
   r.out = at::empty({n_q, H, d}, q.options());
   if (want_grad) {
     r.out32 = q.scalar_type() == at::kFloat ? r.out : at::empty({n_q, H, d}, f32);
-    r.lse = at::empty({H, n_q}, f32);
+    r.lse = at::empty({table.defined() ? 2 * H : H, n_q}, f32);
   }
   const int dt = dtype_code(q);
   const auto h = static_cast<int32_t>(H), hkv = static_cast<int32_t>(k.size(1));

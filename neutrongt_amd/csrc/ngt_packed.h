@@ -405,7 +405,14 @@ __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d)
 // entries in log2 units, -inf (not attended) behind the n_buckets there are.
 // Finite entries act as if within +-2^60: a row of the type's lowest values
 // still gives every pair the same weight instead of none.
+//
+// A bias beyond kFar in a row's greatest score leaves no bits in fp32 for the base
+// and the sum in one number, nor for starting a product from it: such rows subtract
+// the base and then log2 of the sum, each by itself, and keep both (lse and, H * n_q
+// further, the logarithm).  They are as rare as masks of large finite values: a wave
+// that has one takes a few instructions a score more.
 constexpr int kTable = 256;
+constexpr float kFar = 256.f;
 template <typename T>
 __device__ __forceinline__ void load_table(float* tab, const T* __restrict__ table, int n_buckets,
                                            int n_heads, int h, int tid, int n_threads) {

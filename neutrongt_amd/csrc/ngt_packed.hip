@@ -43,7 +43,7 @@ struct FwdArgs {
   const uint8_t* ids;
   void* out;
   float* out32;
-  float* lse;  // [H, n_q], log2 units; +inf for a row that attends to nothing
+  float* lse;  // [H, n_q], log2 units; +inf for a row that attends to nothing (and kFar)
   int64_t n_q;
 };
 
@@ -53,16 +53,21 @@ struct FwdArgs {
 // and an exponential.  The base moves only when some row exceeds it by kRebase,
 // so most tiles rescale nothing; weights and sums share the base, so this is
 // exact.
+template <bool BIAS>
 struct RowSoftmax {
   float c2, per, step;  // per: product units per unit of x
   float m = 0.f;
   float thr = -INFINITY;  // -inf before the row's first key
   float l = 0.f;
+  float far = 0.f;  // the base where it is beyond kFar: no product starts from it
   f32x16 start = fill16(0.f);
   __device__ __forceinline__ RowSoftmax(float c2_, float per_) : c2(c2_), per(per_), step(kRebase / c2_) {}
 
   template <int NT, int NC>
   __device__ __forceinline__ void weights(f32x16 (&x)[NT], f32x16 (&acc)[NC]) {
+    if constexpr (BIAS) {
+      if (__any(far != 0.f)) from_far(x, acc);
+    }
     float mx = x[0][0];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -76,7 +81,7 @@ struct RowSoftmax {
       if (mx > -INFINITY) thr = step;
       m += up;
       l *= f;
-      start = fill16(-m * per);
+      restart();
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -96,9 +101,43 @@ struct RowSoftmax {
       }
     l += s;
   }
+  __device__ __forceinline__ void restart() {
+    if constexpr (BIAS) far = fabsf(m) < kFar ? 0.f : m;
+    start = fill16(BIAS && far != 0.f ? 0.f : -m * per);
+  }
+  // Rows whose base is far have scores that are not relative to it yet.
+  template <int NT, int NC>
+  __device__ __forceinline__ void from_far(f32x16 (&x)[NT], f32x16 (&acc)[NC]) {
+    const bool mine = far != 0.f;
+    float mx = x[0][0];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[t][i]);
+    const float to = fmaxf(m, max_halves(mx));
+    const float f = mine ? __builtin_amdgcn_exp2f(m - to) : 1.f, by = mine ? to : 0.f;
+    l *= f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[t][i] -= by;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[c][i] *= f;
+    if (mine) m = to;
+    restart();
+  }
   // the row's base in log2 units, -inf where it has seen no key
   __device__ __forceinline__ float base() const { return thr == -INFINITY ? thr : m * c2; }
 };
+
+__device__ __forceinline__ void store_lse(const FwdArgs& a, int64_t at, float base, float sum) {
+  const float log = __builtin_amdgcn_logf(sum);
+  const bool far = a.table && fabsf(base) >= kFar && sum != 0.f;
+  a.lse[at] = sum == 0.f ? INFINITY : far ? base : base + log;
+  if (a.table) a.lse[int64_t(a.H) * a.n_q + at] = far ? log : 0.f;
+}
 
 // One block: RW * 32 query rows of one window and head; the window's keys pass
 // through LDS 64 * KS at a time (pick_shape says which and why).  The next stage's
@@ -150,7 +189,7 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_fwd(FwdArgs a) {
     ids = a.ids + a.b_start[item.x] + int64_t(item.y) * ld;
   }
   const float s2 = a.scale * kLog2e;
-  RowSoftmax sm(BIAS ? 1.f : s2, BIAS ? 1.f / s2 : 1.f);
+  RowSoftmax<BIAS> sm(BIAS ? 1.f : s2, BIAS ? 1.f / s2 : 1.f);
   f32x16 acc[L::kCols];
 #pragma unroll
   for (int c = 0; c < L::kCols; ++c) acc[c] = fill16(0.f);
@@ -260,8 +299,7 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_fwd(FwdArgs a) {
                    acc[c][4 * g + 3] * r);
         }
       }
-    if (a.lse && half == 0)
-      a.lse[int64_t(h) * a.n_q + q0 + qi] = l == 0.f ? INFINITY : base + __builtin_amdgcn_logf(l);
+    if (a.lse && half == 0) store_lse(a, int64_t(h) * a.n_q + q0 + qi, base, l);
   }
 }
 
@@ -325,7 +363,7 @@ __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
     __syncthreads();
   }
   const float s2 = a.scale * kLog2e;
-  RowSoftmax sm(BIAS ? 1.f : s2, BIAS ? 1.f / s2 : 1.f);
+  RowSoftmax<BIAS> sm(BIAS ? 1.f : s2, BIAS ? 1.f / s2 : 1.f);
   f32x16 acc[L::kCols];
 #pragma unroll
   for (int c = 0; c < L::kCols; ++c) acc[c] = fill16(0.f);
@@ -436,8 +474,7 @@ __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
       fa.part_ml[(slot * 32 + jr) * 2] = top;
       fa.part_ml[(slot * 32 + jr) * 2 + 1] = sum;
     } else if (a.lse) {
-      a.lse[int64_t(jh) * a.n_q + q0 + jq] =
-          sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+      store_lse(a, int64_t(jh) * a.n_q + q0 + jq, top, sum);
     }
   }
 }
@@ -504,8 +541,7 @@ __global__ __launch_bounds__(256) void k_packed_few_join(FewArgs fa) {
       store4(a.out32 + row, o[4 * c] * inv, o[4 * c + 1] * inv, o[4 * c + 2] * inv,
              o[4 * c + 3] * inv);
   }
-  if (a.lse && jd == 0)
-    a.lse[int64_t(jh) * a.n_q + q0 + jq] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+  if (a.lse && jd == 0) store_lse(a, int64_t(jh) * a.n_q + q0 + jq, top, sum);
 }
 
 // The windows' bucket ids as the kernels read them: one byte a pair, rows padded

@@ -87,7 +87,15 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
   }
   D = sum_halves(D);
   // a lane without a row has no weight anywhere
-  const float lse = qi < nq ? a.lse[int64_t(h) * a.n_q + q0 + qi] : INFINITY;
+  float lse = qi < nq ? a.lse[int64_t(h) * a.n_q + q0 + qi] : INFINITY;
+  float far = 0.f, far_log = 0.f;  // of a row beyond kFar, whose lse is then 0 here
+  if constexpr (BIAS) {
+    if (fabsf(lse) >= kFar && lse < INFINITY) {
+      far = lse, lse = 0.f;
+      far_log = a.lse[int64_t(a.H + h) * a.n_q + q0 + qi];
+    }
+  }
+  const bool any_far = BIAS && __any(far != 0.f);
   if (qi < nq && half == 0 && set == 0) a.dsum[int64_t(h) * a.n_q + q0 + qi] = -D;
 
   const int ld = (nk + 63) & ~63;
@@ -170,6 +178,10 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         s[i] = fmaf(s[i], s2, kFromLse ? bias[i] : BIAS ? bias[i] - lse : -lse);
+      if (any_far) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = (s[i] - far) - far_log;
+      }
       if (k1 + 32 * t + 31 > first_lim) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -232,6 +244,7 @@ k_packed_dkv(BwdArgs a) {
   __shared__ __align__(16) char
       buf[2 * kTileBytes > B::kJoinBytes ? 2 * kTileBytes : B::kJoinBytes];
   __shared__ __align__(16) float ls[kRows], ds[kRows];
+  __shared__ float far[BIAS ? kRows : 1][2];  // of rows beyond kFar, whose ls is then 0
   __shared__ float tab[BIAS ? kTable : 1];
   char *const qs = buf, *const gs = buf + kTileBytes;
   const int tid = tid_x(), lane = tid & 63, half = lane >> 5, l32 = lane & 31;
@@ -273,7 +286,7 @@ k_packed_dkv(BwdArgs a) {
   // bits (9 windows of 33 to 1,777, heads of 16: dK's error 7.4e-7 -> 4.4e-7 of its norm)
   constexpr bool kFromLse = sizeof(T) == 2;
   const float lse_per = kFromLse ? -1.f / s2 : -1.f;
-  float pl = 0.f, pd = 0.f;
+  float pl = 0.f, pl_log = 0.f, pd = 0.f;
   u32x4 idw[2], id_next[2];
   const char* q_tile = qs + 64 * set * L::kRow;
   const char* g_tile = gs + 64 * set * L::kRow;
@@ -283,6 +296,8 @@ k_packed_dkv(BwdArgs a) {
                   int64_t(h) * a.d;
     const T* gb = reinterpret_cast<const T*>(a.go) + (q0 * a.H + h) * int64_t(a.d);
     const Buffer lse = make_buffer(a.lse + int64_t(h) * a.n_q + q0, int64_t(nq) * 4);
+    const Buffer lse_log = make_buffer(a.lse + int64_t(a.H + h) * a.n_q + q0,
+                                       BIAS ? int64_t(nq) * 4 : 0);
     const Buffer dsum = make_buffer(a.dsum + int64_t(h) * a.n_q + q0, int64_t(nq) * 4);
     auto fetch = [&](int qt) {
       if constexpr (BIAS) {
@@ -293,6 +308,7 @@ k_packed_dkv(BwdArgs a) {
       // (a row that is not there has no weight)
       pl = read4(lse, 4 * (qt + tid));
       pl = qt + tid < nq ? pl : INFINITY;
+      if constexpr (BIAS) pl_log = read4(lse_log, 4 * (qt + tid));
       pd = read4(dsum, 4 * (qt + tid));
       if constexpr (kAhead) {
         pq.load(qb, a.sq, qt, nq, a.d);
@@ -315,12 +331,18 @@ k_packed_dkv(BwdArgs a) {
         pq.store(qs, tid);
         pg.store(gs, tid);
       }
-      if (tid < kRows) ls[tid] = pl * lse_per, ds[tid] = pd;
+      if (tid < kRows) {
+        const bool is_far = BIAS && fabsf(pl) >= kFar && pl < INFINITY;
+        ls[tid] = is_far ? 0.f : pl * lse_per, ds[tid] = pd;
+        if constexpr (BIAS) far[tid][0] = is_far ? pl : 0.f, far[tid][1] = is_far ? pl_log : 0.f;
+      }
       __syncthreads();
       idw[0] = id_next[0], idw[1] = id_next[1];
       if (qt + kRows < nq) fetch(qt + kRows);
       const int q1 = qt + 64 * set;  // this set's first query
       if (q1 + 64 <= wave_begin || q1 >= nq || item.y + wave * 32 >= nk) continue;
+      bool any_far = false;
+      if constexpr (BIAS) any_far = __any(far[64 * set + lane][0] != 0.f);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         f32x16 bias;
@@ -347,6 +369,15 @@ k_packed_dkv(BwdArgs a) {
           } else {
             const float minus = ls[64 * set + 32 * t + 16 * half + i];
             s[i] = fmaf(s[i], s2, BIAS ? bias[i] + minus : minus);
+          }
+        }
+        if constexpr (BIAS) {
+          if (any_far) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float* by = far[64 * set + 32 * t + 16 * half + i];
+              s[i] = (s[i] - by[0]) - by[1];
+            }
           }
         }
         if (q1 + 32 * t < last_lim) {

@@ -162,7 +162,7 @@ class PackedAttentionFunction(torch.autograd.Function):
             # fp32: out itself
             out32 = (out if q.dtype == torch.float32
                      else torch.empty(n_q, H, d, dtype=torch.float32, device=dev))
-            lse = torch.empty(H, n_q, dtype=torch.float32, device=dev)
+            lse = torch.empty(H if table is None else 2 * H, n_q, dtype=torch.float32, device=dev)
         n_buckets = table.shape[0] if table is not None else 0
         fwd_bytes, _ = windows.workspace_bytes(dt, H, h_kv, d)
         ws = _workspace(fwd_bytes, dev) if fwd_bytes else None

@@ -476,3 +476,63 @@ def test_two_graphs_and_eager_calls_of_one_plan(dev):
         torch.cuda.synchronize()
         for a, w in ((static[0], want[0]), (static[1], want[1]), (eager, want[i % 2])):
             assert all(torch.equal(x, y) for x, y in zip(a, w))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n_q,n_k", [(7, 300), (200, 200)])
+def test_rows_of_large_finite_table_entries(dev, dtype, n_q, n_k):
+    """Masks of finite values: a row of nothing else weighs its greatest alike (scores of
+    32 bits vanish beside them), any other row does not see them, in whichever order
+    they come; and so do the gradients."""
+    H, d = (4, 16) if n_q == 200 else (2, 16)
+    far = [torch.finfo(dtype).min, -1e9, 1e9]
+    q, k, v, go, table, _ = _inputs([n_q], [n_k], H, H, d, dtype, 6, seed=n_q, cut=0.0)
+    for i, x in enumerate(far):
+        table[i] = x
+    g = torch.Generator().manual_seed(5)
+    ids = torch.randint(3, 6, (n_q, n_k), generator=g)  # of ordinary entries
+    half_way = n_k // 2 + 3
+    ids[0] = 0
+    ids[1, :half_way] = 0
+    ids[2] = 1
+    ids[3, :half_way] = 1
+    ids[4, :half_way], ids[4, half_way:] = 0, 1
+    ids[5, half_way:] = 2
+    ids[6, :70] = 1
+    ids[6, 70:] = 255
+    win = PackedWindows([n_q], [n_k], device=dev)
+    got = _run(dev, q, k, v, go, table, ids.flatten(), win)
+
+    u, half = 2.0 ** -24, HALF[dtype] if dtype == BF16 else 0.0
+    Q, K, V, G = (t.double().transpose(0, 1) for t in (q, k, v, go))
+    bias = table.double()[ids.clamp(max=5)].permute(2, 0, 1)
+    s = Q @ K.transpose(1, 2) / math.sqrt(d)
+    x = torch.where(bias.abs() > 1e8, bias, s + bias)
+    x = x.masked_fill(ids == 255, -math.inf)
+    p = torch.softmax(x, -1)
+    small = torch.where(bias.abs() > 1e8, torch.zeros_like(bias), bias.abs())
+    mag = Q.abs() @ K.abs().transpose(1, 2) / math.sqrt(d) + small
+    # as oracle.packed.bounds, and 2^-15 of the weights: an ordinary row's base may be up to
+    # 256 away from its products' start
+    e_s = (((d + 4) * u * torch.where(p > 0, mag, 0.0)).amax(-1, keepdim=True)
+           + (2.0 ** -15 if dtype == BF16 else 0.0))
+    e_p = 2 * e_s + (n_k + 12) * u
+    o = p @ V
+    err_o = (e_p + half + n_k * u) * (p @ V.abs())
+    dp = G @ V.transpose(1, 2)
+    D = (G * o).sum(-1, keepdim=True)
+    err_D = (G.abs() * err_o).sum(-1, keepdim=True) + d * u * (G * o).abs().sum(-1, keepdim=True)
+    ds = p * (dp - D)
+    err = p * (err_D + (d + 2) * u * (G.abs() @ V.abs().transpose(1, 2))) + (e_p + 4 * u) * ds.abs()
+    r = err + half * (ds.abs() + err)
+    sc, n = 1 / math.sqrt(d), max(n_q, n_k)
+    ref = [o, sc * ds @ K, sc * ds.transpose(1, 2) @ Q, p.transpose(1, 2) @ G]
+    bound = [err_o, sc * (r + (n + 2) * u * ds.abs()) @ K.abs(),
+             sc * (r + (n + 2) * u * ds.abs()).transpose(1, 2) @ Q.abs(),
+             ((e_p + half + n * u) * p).transpose(1, 2) @ G.abs()]
+    one = torch.nn.functional.one_hot(ids, 256)[..., :6].double()
+    ref = [t.transpose(0, 1) for t in ref] + [torch.einsum("hij,ijb->bh", ds, one)]
+    bound = [t.transpose(0, 1) for t in bound]
+    bound.append(torch.einsum("hij,ijb->bh", err + 4096 * u * ds.abs(), one))
+    _check(got, ref, [b + HALF[dtype] * (t.abs() + b) for t, b in zip(ref, bound)], "far")
+    assert (p[:, [0, 2]] - 1 / n_k).abs().max() < 1e-12
