@@ -13,7 +13,7 @@
 // much as the products at 128 (5 causal windows of 500 to 4,096, 32 heads of 128 over 8:
 // 290 us, 865 TFLOP/s of the pairs seen).  With a bias a pair adds a byte of ids from
 // memory and a table entry from LDS, and the vector instructions are 62 % of the time (3
-// windows of 1,000 to 3,333, 32 heads of 24: 245 us).
+// windows of 1,000 to 3,333, 32 heads of 24: 250 us).
 #include "ngt_packed.h"
 
 #include <string.h>

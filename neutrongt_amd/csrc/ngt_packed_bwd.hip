@@ -10,7 +10,7 @@
 // windows of 100 to 1,500: dQ 45, dK/dV 41 us); at d = 64 causal the products and the
 // waits of the longest windows (106 and 165 us).  With the bias's gradient dQ is bound
 // by LDS, 63 % of it: a table entry and an addition of a double per pair (3 windows of
-// 1,000 to 3,333, 32 heads of 24: 450 us, dK/dV 335).
+// 1,000 to 3,333, 32 heads of 24: 455 us, dK/dV 345).
 #include "ngt_packed.h"
 
 namespace ngt {
