@@ -479,7 +479,7 @@ def test_two_graphs_and_eager_calls_of_one_plan(dev):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("n_q,n_k", [(7, 300), (200, 200)])
+@pytest.mark.parametrize("n_q,n_k", [(7, 300), (7, 2000), (200, 200)])
 def test_rows_of_large_finite_table_entries(dev, dtype, n_q, n_k):
     """Masks of finite values: a row of nothing else weighs its greatest alike (scores of
     32 bits vanish beside them), any other row does not see them, in whichever order

@@ -2,7 +2,10 @@
 launched (no GPU needed)."""
 import ctypes as C
 
+import pytest
+
 from neutrongt_amd import _lib
+from tests.test_gpu_linear_epilogue import _inputs, _ref
 
 P = 1 << 20  # an address that nothing reads
 
@@ -32,3 +35,24 @@ def test_refusals_touch_no_gpu():
                       (dict(dz=P + 8), 1), (dict(ws=None), 4), (dict(n=95), 4), (dict(ws=P + 8), 4)):
         assert bwd(**bad) == code, bad
         assert b"ngt_linear_bwd" in lib.ngt_last_error()
+
+
+@pytest.mark.parametrize("act", [None, "relu", "gelu"])
+def test_the_formulas_of_the_gradients_against_differences(act):
+    """The float64 reference of the GPU tests: every gradient against central
+    differences of its forward (step 1e-5: truncation 1e-10, rounding 1e-11)."""
+    x, w, b, r, gy = (t.double() for t in _inputs(5, 4, 6, True, True, 2))
+
+    def loss():
+        return (_ref(x, w, b, r, gy, act)[0][0] * gy).sum().item()
+
+    for t, (got, _) in zip((x, w, b), _ref(x, w, b, r, gy, act)[1:]):
+        for i in range(t.numel()):
+            at, h = t.view(-1), 1e-5
+            keep = at[i].item()
+            at[i] = keep + h
+            up = loss()
+            at[i] = keep - h
+            down = loss()
+            at[i] = keep
+            assert abs((up - down) / (2 * h) - got.reshape(-1)[i].item()) < 1e-7
