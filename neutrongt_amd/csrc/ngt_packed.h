@@ -496,7 +496,16 @@ struct BwdArgs {
   void* gk;
   void* gv;
   void* grad_table;
+  int32_t hist_shift;
 };
+// log2 of the columns of a wave's sums per bucket in the dQ pass (doubles).  Fewer let
+// more waves run, but more lanes of an instruction meet: 16, 8 in fp32, whose pairs take
+// longer elsewhere, and for large tables (forward and backward, us, 32 | 16 | 8 columns:
+// 3 windows of 1,000 to 3,333, 32 heads of 24, 64 buckets 1,185 | 1,135 | 1,227; 40 windows of
+// 150 to 300, as many heads, 200 buckets 361 | 238 | 193; 4 windows of 750 to 1,500, 40
+// buckets, fp32 739 | 716 | 656; 3,001 rows, 8 heads of 8, 10 buckets, fp32 279 | 275 | 289).
+inline int hist_shift(bool f32, int n_buckets) { return f32 || n_buckets > 100 ? 3 : 4; }
+
 struct BwdPlan {
   const int2* items_q;
   const int2* items_k;

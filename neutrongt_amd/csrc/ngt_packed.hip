@@ -777,10 +777,10 @@ BwdLayout bwd_layout(int dtype, const ngt_packed_windows& w, int H, int Hkv, int
   static_assert(Tile<bf16_t, 16>::kRow == 32 && Tile<float, 16>::kRow == 96 &&
                     Tile<float, 128>::kRow == 512, "row below");
   const int row = dtype != NGT_F32 ? 2 * dp : dp == 128 ? 4 * dp : 6 * dp;
-  // with a table gradient a wave holds 64 sums per bucket
+  const size_t sums = size_t(8) << hist_shift(dtype == NGT_F32, n_buckets);
   L.dq = pick_shape(w.max_q, (w.max_k + 63) / 64, w.steps_q * H, int64_t(w.n_items_q[2]) * H,
                     size_t(128) * row,
-                    n_buckets ? size_t(n_buckets + 1) * 256 : 0, most_sets(row, false));
+                    n_buckets ? size_t(n_buckets + 1) * sums : 0, most_sets(row, false));
   L.dkv = pick_shape(w.max_k, int64_t((w.max_q + 63) / 64) * (H / Hkv), w.steps_k * H,
                      int64_t(w.n_items_k[2]) * Hkv, size_t(128) * row, 0, most_sets(row, true));
   L.part = align256(size_t(w.n_q) * H * 4);
@@ -1022,6 +1022,7 @@ extern "C" int ngt_packed_bwd(int dtype, const void* q, const void* k, const voi
   a.table = table, a.ids = buckets_q, a.ids_t = buckets_k;
   a.part_table = reinterpret_cast<float*>(ws + L.part);
   a.gq = grad_q, a.gk = grad_k, a.gv = grad_v, a.grad_table = grad_table;
+  a.hist_shift = hist_shift(dtype == NGT_F32, n_buckets);
   BwdPlan p{};
   p.dq = L.dq, p.dkv = L.dkv;
   p.items_q = reinterpret_cast<const int2*>(w->items_q[list_of(L.dq)]);

@@ -9,8 +9,8 @@
 // What bounds them: vector instructions a pair as in the forward (8 heads of 8, 24
 // windows of 100 to 1,500: dQ 45, dK/dV 41 us); at d = 64 causal the products and the
 // waits of the longest windows (106 and 165 us).  With the bias's gradient dQ is bound
-// by LDS, 63 % of it: a table entry and an addition of a double per pair (3 windows of
-// 1,000 to 3,333, 32 heads of 24: 455 us, dK/dV 345).
+// by LDS, a table entry and an addition of a double per pair, which is busy for two
+// thirds of the time (3 windows of 1,000 to 3,333, 32 heads of 24: 415 us, dK/dV 345).
 #include "ngt_packed.h"
 
 namespace ngt {
@@ -18,23 +18,24 @@ namespace packed {
 namespace {
 
 // Adds a lane's 16 values to the wave's running sums of their buckets, in the
-// lane's column: hist[bucket][l % 32], doubles.  LDS adds a double in 9 clocks
+// lane's column: hist[bucket][l mod columns], doubles.  LDS adds a double in 9 clocks
 // a wave instruction where a float takes 193 (3 a lane); reading, adding and
-// writing back takes 10 and seven compares and selects a value.  Only the two
-// halves of one row share a column.
+// writing back takes 10 and seven compares and selects a value.  The lanes of an
+// instruction that meet in one sum are always the same ones, added in lane order.
 __device__ __forceinline__ void add_to_buckets(double* hist, const u32x4& ids, const f32x16& x,
-                                               int n_buckets) {
+                                               int n_buckets, int shift) {
 #pragma unroll
   for (int i = 0; i < 16; ++i)
-    unsafeAtomicAdd(hist + min(bucket_of(ids, i), n_buckets) * 32, static_cast<double>(x[i]));
+    unsafeAtomicAdd(hist + (min(bucket_of(ids, i), n_buckets) << shift),
+                    static_cast<double>(x[i]));
 }
 
 // dQ, D = G . out and the bias's gradient.  One block: RW * 32 query rows of
 // one window and head (lane = query); the window's keys pass through LDS
 // 64 * KS at a time.
 //   S^T = K Q^T, dP^T = V G^T, P = exp2(S - lse), dS = P (dP - D), dQ^T += K^T dS^T
-// HIST: the wave keeps 32 running sums per bucket, one a row, so that every
-// sum has a fixed order; the block adds them up at its end.
+// HIST: the wave keeps 8 or 16 running sums per bucket (hist_shift), each of the same
+// rows' pairs in the same order; the block adds them up at its end.
 template <typename T, int DP, bool BIAS, bool HIST, int RW, int KS>
 __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
   using L = Tile<T, DP>;
@@ -45,7 +46,7 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
   __shared__ __align__(16) char
       buf[2 * kTileBytes > B::kJoinBytes ? 2 * kTileBytes : B::kJoinBytes];
   __shared__ float tab[BIAS ? kTable : 1];
-  extern __shared__ __align__(8) double hist[];  // HIST: [RW * KS][n_buckets + 1][32]
+  extern __shared__ __align__(8) double hist[];  // HIST: [RW * KS][n_buckets + 1][columns]
   char *const ks = buf, *const vs = buf + kTileBytes;
   const int tid = tid_x(), lane = tid & 63, half = lane >> 5, l32 = lane & 31;
   const int wid = wave_id(), wave = wid % RW, set = wid / RW;
@@ -101,13 +102,14 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
   const int ld = (nk + 63) & ~63;
   const uint8_t* ids = nullptr;  // of the block's first query
   double* my_hist = nullptr;
+  const int cols = (1 << a.hist_shift) - 1;
   if constexpr (BIAS) {
     load_table(tab, reinterpret_cast<const T*>(a.table), a.n_buckets, a.H, h, tid, N);
     ids = a.ids + a.b_start[item.x] + int64_t(item.y) * ld;
   }
   if constexpr (HIST) {
-    for (int i = tid; i < RW * KS * (a.n_buckets + 1) * 32; i += N) hist[i] = 0.;
-    my_hist = hist + wid * (a.n_buckets + 1) * 32 + l32;
+    for (int i = tid; i < RW * KS * (a.n_buckets + 1) << a.hist_shift; i += N) hist[i] = 0.;
+    my_hist = hist + (wid * (a.n_buckets + 1) << a.hist_shift) + (l32 & cols);
   }
   const float s2 = a.scale * kLog2e;
   // The bf16 matrix instructions round their sums down, a row's dP - D by some 2^-25 of
@@ -189,7 +191,7 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i]) * dp[i];
-      if constexpr (HIST) add_to_buckets(my_hist, idw[t], s, a.n_buckets);
+      if constexpr (HIST) add_to_buckets(my_hist, idw[t], s, a.n_buckets, a.hist_shift);
       // a row's dS add up to zero, so what its keys have in common cancels, and in heads
       // of up to 16 that is much of them: there dS goes in as two bf16 pieces (8 heads of
       // 8, 1,500 rows: dQ's error 1.6 -> 1.07 times that of rounding the result; 35 -> 45 us)
@@ -216,10 +218,10 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
     for (int b = tid; b < a.n_buckets; b += N) {
       double sum = 0.;
       for (int w = 0; w < RW * KS; ++w) {
-        const double* hw = hist + (w * (a.n_buckets + 1) + b) * 32;
+        const double* hw = hist + (w * (a.n_buckets + 1) + b << a.hist_shift);
         // from its own place: no bank twice; odd rows with their sign
-        for (int i = 0; i < 32; ++i)
-          sum += kTurn && ((i + b) & 1) ? -hw[(i + b) & 31] : hw[(i + b) & 31];
+        for (int i = 0; i <= cols; ++i)
+          sum += kTurn && ((i + b) & 1) ? -hw[(i + b) & cols] : hw[(i + b) & cols];
       }
       a.part_table[(int64_t(h) * a.n_items + it) * a.n_buckets + b] = static_cast<float>(sum);
     }
@@ -474,7 +476,7 @@ int bwd(const BwdPlan& p, const BwdArgs& base, hipStream_t st) {
   if (p.dq_blocks > 0) {
     a.items = p.items_q;
     a.n_items = p.n_items_q;
-    const size_t lds = size_t(p.dq.rw) * p.dq.ks * (a.n_buckets + 1) * 256;
+    const size_t lds = size_t(p.dq.rw) * p.dq.ks * (a.n_buckets + 1) * (size_t(8) << a.hist_shift);
     NGT_CHECK_OK(hist   ? (launch_dq<T, DP, true, true>(a, p, lds, st))
                  : bias ? (launch_dq<T, DP, true, false>(a, p, 0, st))
                         : (launch_dq<T, DP, false, false>(a, p, 0, st)));
