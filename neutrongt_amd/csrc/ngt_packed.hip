@@ -600,6 +600,7 @@ __global__ __launch_bounds__(256) void k_packed_buckets(const I* __restrict__ id
 // ------------------------------------------------------------------ host side
 constexpr int kTargetBlocks = 512;  // two blocks for each of the 256 compute units
 constexpr int kSimds = 1024;
+constexpr int64_t kMostThreads = 0xffffffff;  // of a launch
 constexpr size_t kLds = 160 * 1024;
 constexpr int kMostIds = 1 << 23;      // of a window with a bias
 constexpr int32_t kMostRows = 1 << 28;  // of a window
@@ -741,12 +742,14 @@ int run_fwd(const ngt_packed_windows& w, const FewPlan& fp, FwdArgs a, void* ws,
       pick_shape(w.max_q, (w.max_k + 63) / 64, w.steps_q * a.H, int64_t(w.n_items_q[2]) * a.H,
                  128 * Tile<T, DP>::kRow, 512, kMost);
   const int i = list_of(shape);
-  const unsigned blocks = unsigned(w.n_items_q[i]) * unsigned(a.H);
+  const int64_t blocks = int64_t(w.n_items_q[i]) * a.H;
   if (!blocks) return NGT_OK;
+  if (blocks * 64 * shape.rw * shape.ks > kMostThreads)
+    return set_error(NGT_ERR_UNSUPPORTED, "ngt_packed_fwd: too many rows and heads for one launch");
   a.items = reinterpret_cast<const int2*>(w.items_q[i]);
   KernelTimer timer_("packed_fwd", st);
   return with_shape<kMost>(shape, [&](auto rw, auto ks) {
-    hipLaunchKernelGGL((k_packed_fwd<T, DP, BIAS, rw.value, ks.value>), dim3(blocks),
+    hipLaunchKernelGGL((k_packed_fwd<T, DP, BIAS, rw.value, ks.value>), dim3(unsigned(blocks)),
                        dim3(64 * rw.value * ks.value), 0, st, a);
     NGT_HIP_CHECK(hipGetLastError());
     return int(NGT_OK);
@@ -927,6 +930,8 @@ extern "C" int ngt_packed_buckets(const ngt_packed_windows* w, const void* ids, 
   hipStream_t st = static_cast<hipStream_t>(stream);
   KernelTimer timer_("packed_buckets", st);
   const int n = std::max(w->n_items_q[1], 1), most = 4096 / n;
+  if (int64_t(n) * 256 > kMostThreads)
+    return set_error(NGT_ERR_UNSUPPORTED, "ngt_packed_buckets: too many rows for one launch");
   const int steps = most < 1 ? 1 : most > 64 ? 64 : most;
   auto run = [&](auto kernel, auto* p) {
     hipLaunchKernelGGL(kernel, dim3(unsigned(n), unsigned(steps)), dim3(256), 0, st, p,
@@ -975,7 +980,7 @@ extern "C" int ngt_packed_fwd(int dtype, const void* q, const void* k, const voi
   const FewPlan fp = few_plan(*w, n_heads, n_kv_heads, dp);
   if (fp.total && (!workspace || workspace_bytes < fp.total))
     return set_error(NGT_ERR_WORKSPACE, "%s: workspace %zu < %zu", fn, workspace_bytes, fp.total);
-  if (fp.use && int64_t(w->n_windows) * n_kv_heads * fp.splits > 0x7fffffff)
+  if (fp.use && int64_t(w->n_windows) * n_kv_heads * fp.splits * 256 > kMostThreads)
     return set_error(NGT_ERR_UNSUPPORTED, "%s: too many windows for one launch", fn);
   FwdArgs a{w->q_start, w->k_start, w->b_start, nullptr, n_heads, n_kv_heads, head_dim, w->causal,
             n_buckets, scale, q_stride * es, k_stride * es, v_stride * es, q, k, v, table,
@@ -1030,5 +1035,8 @@ extern "C" int ngt_packed_bwd(int dtype, const void* q, const void* k, const voi
   p.n_items_q = w->n_items_q[list_of(L.dq)];
   p.dq_blocks = int64_t(p.n_items_q) * n_heads;
   p.dkv_blocks = int64_t(w->n_items_k[list_of(L.dkv)]) * n_kv_heads;
+  if (p.dq_blocks * 64 * L.dq.rw * L.dq.ks > kMostThreads ||
+      p.dkv_blocks * 64 * L.dkv.rw * L.dkv.ks > kMostThreads)
+    return set_error(NGT_ERR_UNSUPPORTED, "%s: too many rows and heads for one launch", fn);
   return packed_bwd(dtype, p, a, static_cast<hipStream_t>(stream));
 }

@@ -149,3 +149,24 @@ def test_call_refusals_in_python():
         packed_attention(t, t, t, w)
     with pytest.raises(ValueError, match=r"rows, heads"):
         packed_attention(t[0], t, t, w)
+
+
+def test_more_blocks_than_a_launch_takes_are_refused():
+    """Plans of more rows than any test holds: the counts alone decide."""
+    lib = _lib.load()
+    p = 1 << 20
+    st, _ = _plan([4096], [4096], 0)
+    for i in range(3):
+        st.n_items_q[i] = st.n_items_k[i] = 1 << 22
+    assert lib.ngt_packed_fwd(1, p, p, p, 64, 64, 64, C.byref(st), 4, 4, 16, 1.0, None, 0, None, p,
+                              None, None, None, 0, None) == 2
+    assert b"one launch" in lib.ngt_last_error()
+    wb = C.c_size_t()
+    assert lib.ngt_packed_workspace_bytes(1, C.byref(st), 4, 4, 16, 0, None, C.byref(wb)) == 0
+    assert lib.ngt_packed_bwd(1, p, p, p, 64, 64, 64, p, p, p, C.byref(st), 4, 4, 16, 1.0, None, 0,
+                              None, None, p, p, p, None, p, wb.value, None) == 2
+    assert b"one launch" in lib.ngt_last_error()
+    few, _ = _plan([1], [200], 1)
+    few.n_windows = 1 << 24
+    assert lib.ngt_packed_fwd(1, p, p, p, 16, 16, 16, C.byref(few), 1, 1, 16, 1.0, None, 0, None, p,
+                              None, None, None, 0, None) == 2
