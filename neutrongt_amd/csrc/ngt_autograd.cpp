@@ -32,7 +32,8 @@
 //
 // PackedAttention and LinearEpilogue are PackedAttentionFunction (packed.py) and
 // LinearEpilogueFunction (linear.py).  Their entries return nothing where an
-// argument is not one that they take: Python then checks it and says why.
+// argument is not one that they take (a forward-mode dual tensor among them, whose
+// tangent a call without gradients would drop): Python then checks it and says why.
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
@@ -565,6 +566,10 @@ std::tuple<Tensor, Tensor> add_layernorm(Tensor x, Tensor y, Tensor weight, Tens
 }
 
 // ------------------------------------------------------------ packed windows
+// A forward-mode tangent, which requires_grad does not show.
+bool has_tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
+bool has_tangent(const std::optional<Tensor>& t) { return t.has_value() && has_tangent(*t); }
+
 // Gradients of a backward that cannot itself be differentiated: under
 // create_graph they carry a node that says so.
 tensor_list once(const char* name, tensor_list grads) {
@@ -708,6 +713,8 @@ std::optional<Tensor> packed_attention(const Tensor& q, const Tensor& k, const T
       !std::isfinite(scale) || !q.has_storage() || !k.has_storage() || !v.has_storage())
     return std::nullopt;
   if (table.has_value() != by_query.has_value()) return std::nullopt;
+  if (has_tangent(q) || has_tangent(k) || has_tangent(v) || has_tangent(table))
+    return std::nullopt;
   if (table.has_value() &&
       (table->dim() != 2 || table->size(1) != H || table->size(0) < 1 || table->size(0) > 255 ||
        table->scalar_type() != type || table->device() != q.device()))
@@ -843,6 +850,8 @@ std::optional<Tensor> linear_epilogue(const Tensor& x, const Tensor& weight,
       (!linear_type(*residual, x) || residual->dim() != x.dim() ||
        residual->size(-1) != weight.size(0) ||
        residual->sizes().slice(0, x.dim() - 1) != x.sizes().slice(0, x.dim() - 1)))
+    return std::nullopt;
+  if (has_tangent(x) || has_tangent(weight) || has_tangent(bias) || has_tangent(residual))
     return std::nullopt;
   const at::DeviceGuard guard(x.device());
   if (at::GradMode::is_enabled() &&
