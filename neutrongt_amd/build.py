@@ -41,7 +41,8 @@ HIPCC_FLAGS = [
 # with the IEEE-mode bit off: fmaxf then needs no canonicalising v_max of each
 # MFMA result (9 of the forward's 77 VALU instructions per 32 x 32 score tile).
 # The fp32 ones and the packed windows' take the same flags for the same reason; a
-# NaN input still goes through their arithmetic to the outputs that depend on it.
+# NaN input still goes through their arithmetic to the outputs that depend on it, and
+# where a value that may be one decides something, it is tested by its bits.
 FILE_FLAGS = {
     "ngt_dense_mfma.hip": ["-fno-honor-nans", "-mno-amdgpu-ieee"],
     "ngt_dense_fx.hip": ["-fno-honor-nans", "-mno-amdgpu-ieee"],

@@ -62,6 +62,16 @@ __device__ __forceinline__ f32x16 fill16(float v) {
   return r;
 }
 
+// The bits of a value that may be a NaN.  These files are compiled as if there were none
+// (see build.py), so a comparison of one may come out either way, and what is derived
+// from its bits is not to be concluded from the arithmetic that made it.
+__device__ __forceinline__ uint32_t bits_of(float x) {
+  uint32_t b = __float_as_uint(x);
+  asm("" : "+v"(b));
+  return b;
+}
+__device__ __forceinline__ bool is_nan(float x) { return (bits_of(x) & 0x7fffffffu) > 0x7f800000u; }
+
 // The two wave halves' values of a row, joined: v_permlane32_swap leaves the
 // lower half's value in r[0] and the upper half's in r[1] of both.
 __device__ __forceinline__ float max_halves(float x) {
@@ -413,6 +423,10 @@ __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d)
 // that has one takes a few instructions a score more.
 constexpr int kTable = 256;
 constexpr float kFar = 256.f;
+__device__ __forceinline__ bool is_far(float base) {  // an infinity or a NaN is not
+  const uint32_t from = __float_as_uint(kFar);
+  return (bits_of(base) & 0x7fffffffu) - from < 0x7f800000u - from;
+}
 template <typename T>
 __device__ __forceinline__ void load_table(float* tab, const T* __restrict__ table, int n_buckets,
                                            int n_heads, int h, int tid, int n_threads) {

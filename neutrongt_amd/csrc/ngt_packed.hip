@@ -128,14 +128,24 @@ struct RowSoftmax {
     if (mine) m = to;
     restart();
   }
-  // the row's base in log2 units, -inf where it has seen no key
-  __device__ __forceinline__ float base() const { return thr == -INFINITY ? thr : m * c2; }
+  // The row's base in log2 units, -inf where it has seen no key, and its sum.  Where one
+  // of its scores is NaN, so is the sum, and the base is 0: what joins such rows compares
+  // only numbers.
+  __device__ __forceinline__ void finish(float& base, float& sum) const {
+    sum = sum_halves(l);
+    base = is_nan(sum) ? 0.f : thr == -INFINITY ? thr : m * c2;
+  }
 };
+
+// A row's sum is 0 (it saw no key), positive, or NaN where one of its scores is.
+__device__ __forceinline__ bool saw_nothing(float sum) { return bits_of(sum) == 0u; }
+__device__ __forceinline__ float inverse(float sum) { return saw_nothing(sum) ? 0.f : 1.f / sum; }
 
 __device__ __forceinline__ void store_lse(const FwdArgs& a, int64_t at, float base, float sum) {
   const float log = __builtin_amdgcn_logf(sum);
-  const bool far = a.table && fabsf(base) >= kFar && sum != 0.f;
-  a.lse[at] = sum == 0.f ? INFINITY : far ? base : base + log;
+  const bool none = saw_nothing(sum), nan = is_nan(sum);
+  const bool far = a.table && is_far(base) && !none && !nan;
+  a.lse[at] = none ? INFINITY : far ? base : base + log;
   if (a.table) a.lse[int64_t(a.H) * a.n_q + at] = far ? log : 0.f;
 }
 
@@ -259,7 +269,8 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_fwd(FwdArgs a) {
     for (int t = 0; t < 2; ++t) L::mma_cols(vt_tile, t, x[t], acc, lane);
   }
 
-  float base = sm.base(), l = sum_halves(sm.l);
+  float base, l;
+  sm.finish(base, l);
   if constexpr (KS > 1) {
     ml[set * RW + wave][0][lane] = base;
     ml[set * RW + wave][1][lane] = l;
@@ -283,7 +294,7 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_fwd(FwdArgs a) {
     if (set > 0) return;
   }
   if (qi < nq) {
-    const float r = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+    const float r = inverse(l);
     T* o = reinterpret_cast<T*>(a.out) + ((q0 + qi) * a.H + h) * int64_t(a.d);
     float* o32 = a.out32 ? a.out32 + ((q0 + qi) * a.H + h) * int64_t(a.d) : nullptr;
 #pragma unroll
@@ -420,9 +431,10 @@ __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
   }
 
   // join the four waves, in wave order
-  const float l = sum_halves(sm.l);
+  float base, l;
+  sm.finish(base, l);
   if (half == 0) {
-    ml[wave][l32][0] = sm.base();
+    ml[wave][l32][0] = base;
     ml[wave][l32][1] = l;
   }
   __syncthreads();
@@ -437,7 +449,7 @@ __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
   }
   const int64_t slot = (int64_t(w) * a.Hkv + kvh) * fa.splits + split;
   const int jg = jr / nq, jq = jr - jg * nq, jh = kvh * G + jg;
-  const float inv = fa.splits > 1 ? 1.f : sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+  const float inv = fa.splits > 1 ? 1.f : inverse(sum);
   float* jb = reinterpret_cast<float*>(buf);
 #pragma unroll
   for (int c = 0; c < L::kCols; ++c) {
@@ -529,7 +541,7 @@ __global__ __launch_bounds__(256) void k_packed_few_join(FewArgs fa) {
       }
     }
   }
-  const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+  const float inv = inverse(sum);
 #pragma unroll
   for (int c = 0; c < kCols; ++c) {
     const int at = 32 * c + jd;

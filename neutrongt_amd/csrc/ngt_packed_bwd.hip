@@ -91,7 +91,7 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
   float lse = qi < nq ? a.lse[int64_t(h) * a.n_q + q0 + qi] : INFINITY;
   float far = 0.f, far_log = 0.f;  // of a row beyond kFar, whose lse is then 0 here
   if constexpr (BIAS) {
-    if (fabsf(lse) >= kFar && lse < INFINITY) {
+    if (is_far(lse)) {
       far = lse, lse = 0.f;
       far_log = a.lse[int64_t(a.H + h) * a.n_q + q0 + qi];
     }
@@ -334,9 +334,9 @@ k_packed_dkv(BwdArgs a) {
         pg.store(gs, tid);
       }
       if (tid < kRows) {
-        const bool is_far = BIAS && fabsf(pl) >= kFar && pl < INFINITY;
-        ls[tid] = is_far ? 0.f : pl * lse_per, ds[tid] = pd;
-        if constexpr (BIAS) far[tid][0] = is_far ? pl : 0.f, far[tid][1] = is_far ? pl_log : 0.f;
+        const bool two = BIAS && is_far(pl);
+        ls[tid] = two ? 0.f : pl * lse_per, ds[tid] = pd;
+        if constexpr (BIAS) far[tid][0] = two ? pl : 0.f, far[tid][1] = two ? pl_log : 0.f;
       }
       __syncthreads();
       idw[0] = id_next[0], idw[1] = id_next[1];
