@@ -437,6 +437,7 @@ int ngt_adj_weights(const int64_t* edge_index, const float* ppr_val, int64_t n_e
  * multiple of 8 up to 128, H a multiple of H_kv (query head h reads key head
  * h / (H / H_kv)).  Per window and head, over its own rows:
  *   S = scale q k^T (+ table[bucket(i, j)][h]);  out = softmax_j(S) v
+ * with scale in [2^-100, 2^100].
  * causal: query i sees the keys j <= i + (keys - queries) of its window.
  * A query that sees no key gets a zero row and gives no gradient.  q, k and v
  * may have rows further apart than heads * d: *_stride is in elements, rows

@@ -39,7 +39,6 @@
 
 #include <c10/hip/HIPStream.h>
 
-#include <cmath>
 #include <map>
 #include <string>
 
@@ -709,8 +708,8 @@ std::optional<Tensor> packed_attention(const Tensor& q, const Tensor& k, const T
       H < 1 || hkv < 1 || H % hkv || d < 8 || d > 128 || d % 8 ||
       (type != at::kFloat && type != at::kBFloat16) || k.scalar_type() != type ||
       v.scalar_type() != type || q.device() != win_mem.device() ||
-      k.device() != win_mem.device() || v.device() != win_mem.device() || !(scale > 0.) ||
-      !std::isfinite(scale) || !q.has_storage() || !k.has_storage() || !v.has_storage())
+      k.device() != win_mem.device() || v.device() != win_mem.device() || !(scale >= 0x1p-100) ||
+      !(scale <= 0x1p100) || !q.has_storage() || !k.has_storage() || !v.has_storage())
     return std::nullopt;
   if (table.has_value() != by_query.has_value()) return std::nullopt;
   if (has_tangent(q) || has_tangent(k) || has_tangent(v) || has_tangent(table))

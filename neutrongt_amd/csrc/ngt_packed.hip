@@ -692,8 +692,11 @@ int check_call(const char* fn, int dtype, const ngt_packed_windows* w, int H, in
     return set_error(NGT_ERR_ARG, "%s: %d heads over %d key heads", fn, H, Hkv);
   if (d < 8 || d > 128 || d % 8)
     return set_error(NGT_ERR_UNSUPPORTED, "%s: head_dim=%d (a multiple of 8 up to 128)", fn, d);
-  if (!(scale > 0.f) || !(scale < INFINITY))
-    return set_error(NGT_ERR_ARG, "%s: scale must be finite and > 0", fn);
+  // A base or lse of up to kFar is divided by scale log2(e), and scores are multiplied by
+  // it: inside this range neither leaves fp32 (at 1e-40 a bias gave NaN, at 1e-38 bf16
+  // lost its gradients).
+  if (!(scale >= 0x1p-100f) || !(scale <= 0x1p100f))
+    return set_error(NGT_ERR_ARG, "%s: scale must lie in [2^-100, 2^100]", fn);
   if (w->n_windows < 0 || w->n_q < 0 || w->n_k < 0 || w->max_q < 0 || w->max_k < 0 || w->steps_q < 0 ||
       w->steps_k < 0)
     return set_error(NGT_ERR_ARG, "%s: bad windows", fn);

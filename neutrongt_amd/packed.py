@@ -231,7 +231,7 @@ def packed_attention(q, k, v, windows: PackedWindows, scale: float | None = None
     windows back to back; H a multiple of H_kv (query head h reads key head
     h // (H // H_kv)); d a multiple of 8 up to 128.  ``scale`` (default
     1/sqrt(d); dense_attention's default is the reference's sqrt(d)) multiplies
-    the products.  ``bias_table`` [n_buckets <= 255, H] of q's dtype with
+    the products; it lies in [2^-100, 2^100].  ``bias_table`` [n_buckets <= 255, H] of q's dtype with
     ``buckets`` (windows.pack_buckets): adds table[id, h] to a pair's score, and
     leaves pairs out whose id is not in the table.  A query that sees no key
     gives zeros.  Differentiable once, in q, k, v and bias_table; deterministic."""
@@ -278,8 +278,8 @@ def packed_attention(q, k, v, windows: PackedWindows, scale: float | None = None
                              f"{tuple(bias_table.shape)} {bias_table.dtype} on {bias_table.device}")
         bias_table = bias_table.contiguous()
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"scale must be finite and > 0, got {scale}")
+    if not 2.0 ** -100 <= scale <= 2.0 ** 100:
+        raise ValueError(f"scale must lie in [2^-100, 2^100], got {scale}")
     want_grad = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (q, k, v, bias_table))
     return PackedAttentionFunction.apply(q, k, v, bias_table, windows, buckets, scale, want_grad)
