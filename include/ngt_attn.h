@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define NGT_ABI_VERSION 12
+#define NGT_ABI_VERSION 13
 
 #define NGT_F32 0
 #define NGT_BF16 1
@@ -450,8 +450,8 @@ int ngt_adj_weights(const int64_t* edge_index, const float* ppr_val, int64_t n_e
  * Lengths are host arrays, 0 <= length <= 2^28 (2^23
  * with a bias).  Neither call touches the GPU.
  *
- * The bias.  table [n_buckets, H] has the element type of q, 1 <= n_buckets
- * <= 255.  ngt_packed_buckets lays the pairs' bucket ids out once for all
+ * The bias.  table [n_buckets, H] has the element type of q, or is fp32 where
+ * NGT_TABLE_F32 is or'd into dtype (and grad_table with it), 1 <= n_buckets <= 255.  ngt_packed_buckets lays the pairs' bucket ids out once for all
  * heads, layers and steps: ids holds the windows' [queries, keys] matrices
  * back to back (n_pairs elements of 1 (unsigned), 4 or 8 bytes (signed)),
  * buckets_q and buckets_k take bucket_bytes_q and bucket_bytes_k bytes,
@@ -468,6 +468,7 @@ int ngt_adj_weights(const int64_t* edge_index, const float* ppr_val, int64_t n_e
  * workspace: ngt_packed_workspace_bytes with the same dtype, windows and heads;
  * n_buckets there is the table's for a backward that writes grad_table, else 0.
  */
+#define NGT_TABLE_F32 0x100
 typedef struct ngt_packed_windows {
   int32_t n_windows;
   int32_t causal;

@@ -13,10 +13,11 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libngt_attn.so"
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 NGT_F32 = 0
 NGT_BF16 = 1
+NGT_TABLE_F32 = 0x100  # or'd into the packed attention's dtype: an fp32 table
 
 INFO_ITEMS_Q = 0
 INFO_PARTS_Q = 1

@@ -606,6 +606,12 @@ const ngt_packed_windows* windows_of(const Tensor& bytes) {
   return reinterpret_cast<const ngt_packed_windows*>(bytes.data_ptr());
 }
 
+// the dtype of a call: the rows', and whether the table is fp32
+int packed_type(const Tensor& q, const Tensor& table) {
+  return dtype_code(q) |
+         (table.defined() && table.scalar_type() == at::kFloat ? NGT_TABLE_F32 : 0);
+}
+
 struct PackedForward {
   Tensor out, out32, lse;
 };
@@ -621,7 +627,7 @@ PackedForward packed_forward(const Tensor& q, const Tensor& k, const Tensor& v, 
     r.out32 = q.scalar_type() == at::kFloat ? r.out : at::empty({n_q, H, d}, f32);
     r.lse = at::empty({table.defined() ? 2 * H : H, n_q}, f32);
   }
-  const int dt = dtype_code(q);
+  const int dt = packed_type(q, table);
   const auto h = static_cast<int32_t>(H), hkv = static_cast<int32_t>(k.size(1));
   size_t bytes = 0;
   check(g_packed_ws(dt, windows_of(win), h, hkv, static_cast<int32_t>(d), 0, &bytes, nullptr));
@@ -672,7 +678,7 @@ struct PackedAttention : public torch::autograd::Function<PackedAttention> {
     res[2] = at::empty(v.sizes(), v.options());
     const bool want_table = bias && ctx->needs_input_grad(3);
     if (want_table) res[3] = at::empty_like(table);
-    const int dt = dtype_code(q);
+    const int dt = packed_type(q, table);
     const auto h = static_cast<int32_t>(H), hkv = static_cast<int32_t>(k.size(1)),
                nb = bias ? static_cast<int32_t>(table.size(0)) : 0;
     size_t bytes = 0;
@@ -716,7 +722,8 @@ std::optional<Tensor> packed_attention(const Tensor& q, const Tensor& k, const T
     return std::nullopt;
   if (table.has_value() &&
       (table->dim() != 2 || table->size(1) != H || table->size(0) < 1 || table->size(0) > 255 ||
-       table->scalar_type() != type || table->device() != q.device()))
+       (table->scalar_type() != type && table->scalar_type() != at::kFloat) ||
+       table->device() != q.device()))
     return std::nullopt;
   const at::DeviceGuard guard(q.device());
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() ||

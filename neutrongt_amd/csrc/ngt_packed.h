@@ -428,12 +428,15 @@ __device__ __forceinline__ bool is_far(float base) {  // an infinity or a NaN is
   return (bits_of(base) & 0x7fffffffu) - from < 0x7f800000u - from;
 }
 template <typename T>
-__device__ __forceinline__ void load_table(float* tab, const T* __restrict__ table, int n_buckets,
-                                           int n_heads, int h, int tid, int n_threads) {
+__device__ __forceinline__ void load_table(float* tab, const void* __restrict__ table, int table_f32,
+                                           int n_buckets, int n_heads, int h, int tid,
+                                           int n_threads) {
   for (int b = tid; b < kTable; b += n_threads) {
     float x = -INFINITY;
     if (b < n_buckets) {
-      x = elem<T>::load(table + int64_t(b) * n_heads + h);
+      const int64_t at = int64_t(b) * n_heads + h;
+      x = table_f32 ? static_cast<const float*>(table)[at]
+                    : elem<T>::load(static_cast<const T*>(table) + at);
       const uint32_t mag = __float_as_uint(x) & 0x7fffffffu;
       if (mag < 0x7f800000u) x = fminf(fmaxf(x * kLog2e, -0x1p60f), 0x1p60f);
     }
@@ -491,7 +494,7 @@ struct BwdArgs {
   const int64_t* bt_start;
   const int2* items;
   int n_items;
-  int H, Hkv, d, causal, n_buckets;
+  int H, Hkv, d, causal, n_buckets, table_f32;
   float scale;
   int64_t sq, sk, sv;  // bytes between rows
   int64_t n_q;

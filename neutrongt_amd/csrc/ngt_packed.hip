@@ -33,7 +33,7 @@ struct FwdArgs {
   const int64_t* k_start;
   const int64_t* b_start;
   const int2* items;
-  int H, Hkv, d, causal, n_buckets;
+  int H, Hkv, d, causal, n_buckets, table_f32;
   float scale;
   int64_t sq, sk, sv;  // bytes between rows
   const void* q;
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_fwd(FwdArgs a) {
   const int ld = (nk + 63) & ~63;
   const uint8_t* ids = nullptr;  // of the block's first query
   if constexpr (BIAS) {
-    load_table(tab, reinterpret_cast<const T*>(a.table), a.n_buckets, a.H, h, tid, N);
+    load_table<T>(tab, a.table, a.table_f32, a.n_buckets, a.H, h, tid, N);
     ids = a.ids + a.b_start[item.x] + int64_t(item.y) * ld;
   }
   const float s2 = a.scale * kLog2e;
@@ -367,8 +367,8 @@ __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
   const float* tab = nullptr;
   if constexpr (BIAS) {
     for (int g = 0; g < G; ++g)
-      load_table(tabs + g * kTable, reinterpret_cast<const T*>(a.table), a.n_buckets, a.H,
-                 kvh * G + g, tid, 256);
+      load_table<T>(tabs + g * kTable, a.table, a.table_f32, a.n_buckets, a.H, kvh * G + g, tid,
+                    256);
     ids = a.ids + a.b_start[w];
     tab = tabs + grp * kTable;
     __syncthreads();
@@ -963,6 +963,7 @@ extern "C" int ngt_packed_buckets(const ngt_packed_windows* w, const void* ids, 
 extern "C" int ngt_packed_workspace_bytes(int dtype, const ngt_packed_windows* w, int32_t n_heads,
                                           int32_t n_kv_heads, int32_t head_dim, int32_t n_buckets,
                                           size_t* fwd_bytes, size_t* bwd_bytes) {
+  dtype &= ~NGT_TABLE_F32;
   NGT_CHECK_OK(check_call("ngt_packed_workspace_bytes", dtype, w, n_heads, n_kv_heads, head_dim,
                           1.f, nullptr, 0, nullptr));
   if (n_buckets < 0 || n_buckets > 255)
@@ -980,6 +981,8 @@ extern "C" int ngt_packed_fwd(int dtype, const void* q, const void* k, const voi
                               const uint8_t* buckets_q, void* out, float* out_f32, float* lse,
                               void* workspace, size_t workspace_bytes, void* stream) {
   const char* fn = "ngt_packed_fwd";
+  const int table_f32 = dtype & NGT_TABLE_F32;
+  dtype &= ~NGT_TABLE_F32;
   NGT_CHECK_OK(check_call(fn, dtype, w, n_heads, n_kv_heads, head_dim, scale, table, n_buckets,
                           buckets_q));
   if (w->n_q == 0) return NGT_OK;
@@ -998,7 +1001,7 @@ extern "C" int ngt_packed_fwd(int dtype, const void* q, const void* k, const voi
   if (fp.use && int64_t(w->n_windows) * n_kv_heads * fp.splits * 256 > kMostThreads)
     return set_error(NGT_ERR_UNSUPPORTED, "%s: too many windows for one launch", fn);
   FwdArgs a{w->q_start, w->k_start, w->b_start, nullptr, n_heads, n_kv_heads, head_dim, w->causal,
-            n_buckets, scale, q_stride * es, k_stride * es, v_stride * es, q, k, v, table,
+            n_buckets, table_f32, scale, q_stride * es, k_stride * es, v_stride * es, q, k, v, table,
             buckets_q, out, out_f32, lse, w->n_q};
   hipStream_t st = static_cast<hipStream_t>(stream);
   return dtype == NGT_F32 ? run_fwd_d<float>(dp, *w, fp, a, workspace, st)
@@ -1014,6 +1017,8 @@ extern "C" int ngt_packed_bwd(int dtype, const void* q, const void* k, const voi
                               void* grad_k, void* grad_v, void* grad_table, void* workspace,
                               size_t workspace_bytes, void* stream) {
   const char* fn = "ngt_packed_bwd";
+  const int table_f32 = dtype & NGT_TABLE_F32;
+  dtype &= ~NGT_TABLE_F32;
   NGT_CHECK_OK(check_call(fn, dtype, w, n_heads, n_kv_heads, head_dim, scale, table, n_buckets,
                           buckets_q));
   const int es = dtype == NGT_F32 ? 4 : 2;
@@ -1036,6 +1041,7 @@ extern "C" int ngt_packed_bwd(int dtype, const void* q, const void* k, const voi
   BwdArgs a{};
   a.q_start = w->q_start, a.k_start = w->k_start, a.b_start = w->b_start, a.bt_start = w->bt_start;
   a.H = n_heads, a.Hkv = n_kv_heads, a.d = head_dim, a.causal = w->causal, a.n_buckets = n_buckets;
+  a.table_f32 = table_f32;
   a.scale = scale, a.sq = q_stride * es, a.sk = k_stride * es, a.sv = v_stride * es, a.n_q = w->n_q;
   a.q = q, a.k = k, a.v = v, a.go = grad_out, a.out32 = out_f32, a.lse = lse;
   a.dsum = reinterpret_cast<float*>(ws);

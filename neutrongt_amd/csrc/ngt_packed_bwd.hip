@@ -104,7 +104,7 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
   double* my_hist = nullptr;
   const int cols = (1 << a.hist_shift) - 1;
   if constexpr (BIAS) {
-    load_table(tab, reinterpret_cast<const T*>(a.table), a.n_buckets, a.H, h, tid, N);
+    load_table<T>(tab, a.table, a.table_f32, a.n_buckets, a.H, h, tid, N);
     ids = a.ids + a.b_start[item.x] + int64_t(item.y) * ld;
   }
   if constexpr (HIST) {
@@ -319,7 +319,7 @@ k_packed_dkv(BwdArgs a) {
     };
     if constexpr (BIAS) {
       __syncthreads();  // the last head's rows are done with its table
-      load_table(tab, reinterpret_cast<const T*>(a.table), a.n_buckets, a.H, h, tid, N);
+      load_table<T>(tab, a.table, a.table_f32, a.n_buckets, a.H, h, tid, N);
     }
     fetch(block_begin);
     for (int qt = block_begin; qt < nq; qt += kRows) {
@@ -487,9 +487,14 @@ int bwd(const BwdPlan& p, const BwdArgs& base, hipStream_t st) {
   }
   if (hist) {
     KernelTimer timer_("packed_table_grad", st);
-    hipLaunchKernelGGL(k_packed_table_grad<T>, dim3(unsigned(a.H * ((a.n_buckets + 63) / 64))),
-                       dim3(1024), 0, st, a.part_table, p.dq_blocks > 0 ? p.n_items_q : 0,
-                       a.n_buckets, a.H, static_cast<T*>(a.grad_table));
+    auto run = [&](auto* grad) {
+      hipLaunchKernelGGL(k_packed_table_grad<std::remove_pointer_t<decltype(grad)>>,
+                         dim3(unsigned(a.H * ((a.n_buckets + 63) / 64))),
+                         dim3(1024), 0, st, a.part_table, p.dq_blocks > 0 ? p.n_items_q : 0,
+                         a.n_buckets, a.H, grad);
+    };
+    if (a.table_f32) run(static_cast<float*>(a.grad_table));
+    else run(static_cast<T*>(a.grad_table));
     NGT_HIP_CHECK(hipGetLastError());
   }
   return NGT_OK;

@@ -146,6 +146,12 @@ class PairBuckets:
                 t.record_stream(torch.cuda.current_stream(self.windows.device))
 
 
+def _call_dtype(q: torch.Tensor, table: torch.Tensor | None) -> int:
+    """The C entries' dtype: the rows', and whether the table is fp32."""
+    f32 = table is not None and table.dtype == torch.float32
+    return _dtype_code(q) | (_lib.NGT_TABLE_F32 if f32 else 0)
+
+
 class PackedAttentionFunction(torch.autograd.Function):
     """out [n_q, H, d] of q [n_q, H, d], k/v [n_k, H_kv, d] over a
     PackedWindows (ngt_packed_fwd / ngt_packed_bwd); ``table`` [n_buckets, H]
@@ -155,7 +161,7 @@ class PackedAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, windows, buckets, scale, want_grad):
         n_q, H, d = q.shape
-        h_kv, dev, dt = k.shape[1], q.device, _dtype_code(q)
+        h_kv, dev, dt = k.shape[1], q.device, _call_dtype(q, table)
         out = torch.empty(n_q, H, d, dtype=q.dtype, device=dev)
         out32 = lse = None
         if want_grad:
@@ -185,7 +191,7 @@ class PackedAttentionFunction(torch.autograd.Function):
     def backward(ctx, g_out):
         q, k, v, table, out32, lse = ctx.saved_tensors
         n_q, H, d = q.shape
-        h_kv, dev, dt = k.shape[1], q.device, _dtype_code(q)
+        h_kv, dev, dt = k.shape[1], q.device, _call_dtype(q, table)
         windows, buckets = ctx.windows, ctx.buckets
         g = _prep(g_out.to(q.dtype), "grad_out")
         gq = torch.empty(n_q, H, d, dtype=q.dtype, device=dev)
@@ -231,10 +237,12 @@ def packed_attention(q, k, v, windows: PackedWindows, scale: float | None = None
     windows back to back; H a multiple of H_kv (query head h reads key head
     h // (H // H_kv)); d a multiple of 8 up to 128.  ``scale`` (default
     1/sqrt(d); dense_attention's default is the reference's sqrt(d)) multiplies
-    the products; it lies in [2^-100, 2^100].  ``bias_table`` [n_buckets <= 255, H] of q's dtype with
-    ``buckets`` (windows.pack_buckets): adds table[id, h] to a pair's score, and
-    leaves pairs out whose id is not in the table.  A query that sees no key
-    gives zeros.  Differentiable once, in q, k, v and bias_table; deterministic."""
+    the products and lies in [2^-100, 2^100].  ``bias_table`` [n_buckets <= 255,
+    H] of q's dtype or fp32 (an fp32 parameter beside bf16 rows goes in
+    unrounded, its gradient is fp32) with ``buckets`` (windows.pack_buckets):
+    adds table[id, h] to a pair's score, and leaves pairs out whose id is not in
+    the table.  A query that sees no key gives zeros.  Differentiable once, in
+    q, k, v and bias_table; deterministic."""
     if not isinstance(windows, PackedWindows):
         raise TypeError("windows must be a PackedWindows")
     if buckets is not None and (not isinstance(buckets, PairBuckets)
@@ -272,9 +280,10 @@ def packed_attention(q, k, v, windows: PackedWindows, scale: float | None = None
         raise ValueError("bias_table and buckets go together")
     if bias_table is not None:
         if (bias_table.dim() != 2 or bias_table.shape[1] != H
-                or not 1 <= bias_table.shape[0] <= 255 or bias_table.dtype != q.dtype
+                or not 1 <= bias_table.shape[0] <= 255
+                or bias_table.dtype not in (q.dtype, torch.float32)
                 or bias_table.device != q.device):
-            raise ValueError(f"bias_table must be [1..255, {H}] {q.dtype} on {q.device}, got "
+            raise ValueError(f"bias_table must be [1..255, {H}] {q.dtype} or fp32 on {q.device}, got "
                              f"{tuple(bias_table.shape)} {bias_table.dtype} on {bias_table.device}")
         bias_table = bias_table.contiguous()
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
