@@ -5,7 +5,8 @@
 // sum has one owner and one order; the scores are formed in both (14 d flops a pair
 // instead of 10 d) and the exponential with them, which costs less than sums over blocks
 // through memory would.  In bf16 P and dS are rounded to bf16 for their products, a half
-// step of each term; everything else is fp32.
+// step of each term (dQ, dK and dV are then off by 1.38 to 1.44 times the rounding of the
+// result; what two pieces cost stands in ngt_packed.hip); everything else is fp32.
 // What bounds them: vector instructions a pair as in the forward (8 heads of 8, 24
 // windows of 100 to 1,500: dQ 45, dK/dV 41 us); at d = 64 causal the products and the
 // waits of the longest windows (106 and 165 us).  With the bias's gradient dQ is bound
