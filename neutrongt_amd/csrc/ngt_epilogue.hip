@@ -8,6 +8,11 @@
 // has outputs n in its registers: with the row order of ngt_packed.h a lane
 // ends up with 16 consecutive outputs of one row, so bias, residual and result
 // are 16-byte accesses.
+//
+// Rounded to bf16 besides the results: z, kept for the backward, and dz, the operand of dx,
+// dW and db.  Trained with GELU (4,096 x 768 -> 768) the gradients are off by 2.41e-3 where
+// rounding them alone makes 1.66e-3; nearly all of the rest is dz, which is an operand's type
+// (z in fp32: 2.35e-3 for twice its bytes; act'(z) kept in bf16 instead of z: 3.03e-3).
 #include "ngt_packed.h"
 
 namespace ngt {
