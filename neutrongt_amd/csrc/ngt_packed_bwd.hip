@@ -234,10 +234,13 @@ __global__ __launch_bounds__(64 * RW * KS) void k_packed_dq(BwdArgs a) {
 // time, head after head: dK and dV of shared heads are one sum.
 //   S = Q K^T, dP = G V^T, P = exp2(S - lse), dS = P (dP - D)
 //   dV^T += G^T P, dK^T += Q^T dS
-// With a bias, whose table lookups it waits for, three waves a SIMD where the
-// registers allow it: 32 heads of 24, 8,556 rows, 379 -> 343 us (without, 42 -> 45).
+// With a bias, whose table lookups it waits for, three waves a SIMD in the one shape whose
+// registers allow it, four row waves in bf16 at 32: 32 heads of 24, 8,556 rows, 379 -> 343 us
+// (without a bias 42 -> 45).  Held to three, the other shapes there spill 6 to 50 registers
+// (300 windows of 8 to 32, 8 heads of 24: 20 us, 14 without the bound).
 template <typename T, int DP, bool BIAS, int RW, int KS>
-__global__ __launch_bounds__(64 * RW * KS, BIAS && DP == 32 && sizeof(T) == 2 ? 3 : 1) void
+__global__ __launch_bounds__(64 * RW * KS,
+                             BIAS && DP == 32 && sizeof(T) == 2 && RW == 4 && KS == 1 ? 3 : 1) void
 k_packed_dkv(BwdArgs a) {
   using L = Tile<T, DP>;
   using B = Block<RW, KS>;
