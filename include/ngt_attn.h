@@ -441,14 +441,16 @@ int ngt_adj_weights(const int64_t* edge_index, const float* ppr_val, int64_t n_e
  * causal: query i sees the keys j <= i + (keys - queries) of its window.
  * A query that sees no key gets a zero row and gives no gradient.  q, k and v
  * may have rows further apart than heads * d: *_stride is in elements, rows
- * 16-byte aligned and less than 8 MB apart.  Values of unseen keys enter with weight 0, so they must be
- * finite where any query of their window is not to see a NaN.
+ * 16-byte aligned and less than 8 MB apart.  Values of unseen keys enter with weight 0, so
+ * they must be finite where any query of their window is not to see a NaN.  fp32 heads up to
+ * 64 wide are multiplied as three bf16 pieces: finite values up to 3.39e38, all 24 bits from
+ * 2^-110 on.
  *
  * The plan.  ngt_packed_plan writes the windows' offsets and work lists for
  * ngt_packed_plan_bytes bytes at device, which the caller then copies there
  * from host, and fills *out (host memory; its pointers point into device).
- * Lengths are host arrays, 0 <= length <= 2^28 (2^23
- * with a bias).  Neither call touches the GPU.
+ * Lengths are host arrays, 0 <= length <= 2^28 (2^23 with a bias).  Neither call touches
+ * the GPU.
  *
  * The bias.  table [n_buckets, H] has the element type of q, or is fp32 where
  * NGT_TABLE_F32 is or'd into dtype (and grad_table with it), 1 <= n_buckets <= 255.  ngt_packed_buckets lays the pairs' bucket ids out once for all
@@ -464,7 +466,8 @@ int ngt_adj_weights(const int64_t* edge_index, const float* ppr_val, int64_t n_e
  * and each row's softmax statistic (with a table and rows whose greatest score is
  * beyond +-256 its two parts).  The backward writes grad_q [n_q, H, d], grad_k and
  * grad_v [n_k, H_kv, d] and, where grad_table is not null, grad_table
- * [n_buckets, H]; grad_out is contiguous.  All sums are fp32 in a fixed order.
+ * [n_buckets, H]; grad_out is contiguous.  All sums are fp32 in a fixed order, those of a
+ * block's buckets doubles.
  * workspace: ngt_packed_workspace_bytes with the same dtype, windows and heads;
  * n_buckets there is the table's for a backward that writes grad_table, else 0.
  */

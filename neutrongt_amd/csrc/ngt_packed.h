@@ -89,7 +89,9 @@ __device__ __forceinline__ float sum_halves(float x) {
 // what the ones before it leave.  Six of the nine products of two such operands
 // reach fp32 precision (the three left out are below 2^-24 of the first), and
 // the bf16 matrix instructions are 16 times as fast as the fp32 ones.  What lies
-// below 2^-110 keeps fewer bits (its lower pieces fall below the type).
+// below 2^-110 keeps fewer bits (its lower pieces fall below the type), a value above
+// bf16's largest, 3.39e38, is an infinity, and a sum that an infinity enters may be NaN
+// (infinity times a zero piece).
 struct Pieces2 {
   uint32_t hi, mid, lo;
 };
@@ -521,6 +523,7 @@ struct BwdArgs {
 // 3 windows of 1,000 to 3,333, 32 heads of 24, 64 buckets 1,185 | 1,135 | 1,227; 40 windows of
 // 150 to 300, as many heads, 200 buckets 361 | 238 | 193; 4 windows of 750 to 1,500, 40
 // buckets, fp32 739 | 716 | 656; 3,001 rows, 8 heads of 8, 10 buckets, fp32 279 | 275 | 289).
+// The line at 100 buckets lies between the tables measured, 64 and 200.
 inline int hist_shift(bool f32, int n_buckets) { return f32 || n_buckets > 100 ? 3 : 4; }
 
 struct BwdPlan {

@@ -12,12 +12,13 @@
 // 32 bits passes fp32 rows: there they go in as three pieces.
 //
 // What bounds it.  1,024 pairs cost a SIMD 4 DP clocks of the matrix cores for both
-// products and some 9 vector instructions a lane's score, the exponential four times as
-// long as another: 600 to 800 clocks, which set the pace up to d = 64 and weigh about as
-// much as the products at 128 (5 causal windows of 500 to 4,096, 32 heads of 128 over 8:
-// 290 us, 865 TFLOP/s of the pairs seen).  With a bias a pair adds a byte of ids from
-// memory and a table entry from LDS, and the vector instructions are 62 % of the time (3
-// windows of 1,000 to 3,333, 32 heads of 24: 250 us).
+// products and some 5.5 vector instructions a lane's score, the exponential four times as
+// long as another: about 540 clocks, which set the pace for narrow heads and are as much as
+// the products at 128.  There the two take turns instead of overlapping (matrix cores busy
+// for 43 % of the time, vector units 40 %): 5 causal windows of 500 to 4,096, 32 heads of 128
+// over 8, 268 us, 936 TFLOP/s of the pairs seen.  With a bias a pair adds a byte of ids from
+// memory and a table entry from LDS, and the vector units are busy for 61 % of the time (3
+// windows of 1,000 to 3,333, 32 heads of 24: 248 us).
 #include "ngt_packed.h"
 
 #include <string.h>

@@ -8,10 +8,11 @@
 // step of each term (dQ, dK and dV are then off by 1.38 to 1.44 times the rounding of the
 // result; what two pieces cost stands in ngt_packed.hip); everything else is fp32.
 // What bounds them: vector instructions a pair as in the forward (8 heads of 8, 24
-// windows of 100 to 1,500: dQ 45, dK/dV 41 us); at d = 64 causal the products and the
-// waits of the longest windows (106 and 165 us).  With the bias's gradient dQ is bound
-// by LDS, a table entry and an addition of a double per pair, which is busy for two
-// thirds of the time (3 windows of 1,000 to 3,333, 32 heads of 24: 415 us, dK/dV 345).
+// windows of 100 to 1,500: dQ 41, dK/dV 37 us).  At d = 64 causal no unit is busy for more
+// than 34 % of the time in dQ (101 us) or 30 % in dK/dV (149 us): waits, of dK/dV's four sets
+// before the diagonal for one another and of blocks of 66 KB for a place.  With the bias's
+// gradient dQ is bound by LDS, a table entry and an addition of a double per pair, busy for
+// 69 % of the time (3 windows of 1,000 to 3,333, 32 heads of 24: 408 us, dK/dV 345).
 #include "ngt_packed.h"
 
 namespace ngt {
