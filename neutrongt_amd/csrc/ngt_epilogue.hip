@@ -177,8 +177,8 @@ __device__ __forceinline__ void wait_for_all_but() {
 // block a CU, where nothing else fills the waits (2,048 x 4,096 -> 1,024 41 us,
 // BUFS = 1 64 us).
 // What is left then is the wait for each stage's first fragments and, with GELU, the
-// epilogue: some 100 clocks for a wave's 64 outputs, 6,600 a block, the MFMA time of
-// 800 of the contraction (blocks on the same CU overlap it, a lone one does not).
+// epilogue: some 110 clocks for a wave's 64 outputs, 7,200 a block, the MFMA time of
+// 900 of the contraction (blocks on the same CU overlap it, a lone one does not).
 template <int BM, int BN, int BUFS, bool ALIGNED>
 __global__ __launch_bounds__(256) void k_gemm(GemmArgs a) {
   constexpr int FM = BM / 64, FN = BN / 64;  // 32 x 32 tiles of a wave

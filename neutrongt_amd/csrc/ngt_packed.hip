@@ -334,7 +334,7 @@ struct FewArgs {
 // are what is waited for that costs nothing (the two cases below 231 -> 230 and 11.8 -> 11.7
 // us with the host's part; error 2.31e-3 -> 1.65e-3, the rounding of the result).
 // Bound by the cache's bytes: 32 windows of 1,000 to 16,384 keys, 8 key heads of 128,
-// 230 us, 3.8 TB/s of the 4.9 of a copy; short ones by the launches (8 windows of 60 to
+// 230 us, 3.9 TB/s of the 4.9 of a copy; short ones by the launches (8 windows of 60 to
 // 1,000: 7 us one after another in a graph, with the join).
 template <typename T, int DP, bool BIAS>
 __global__ __launch_bounds__(256) void k_packed_few(FewArgs fa) {
@@ -567,7 +567,8 @@ __global__ __launch_bounds__(256) void k_packed_few_join(FewArgs fa) {
 // The windows' bucket ids as the kernels read them: one byte a pair, rows padded
 // to 64 with 255, by queries and by keys.  One block: 64 queries of a window and
 // every gridDim.y-th 64 of its keys (3 windows of 1,000 to 3,333, 16 M pairs: 21 us,
-// with all of the keys in one block 215).
+// with all of the keys in one block 215; about twice a copy of its bytes, no unit busy for
+// more than 19 % of it: a block waits for a tile's ids before it turns them).
 template <typename I>
 __global__ __launch_bounds__(256) void k_packed_buckets(const I* __restrict__ ids,
                                                         const int64_t* __restrict__ q_start,
