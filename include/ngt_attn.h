@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define NGT_ABI_VERSION 13
+#define NGT_ABI_VERSION 14
 
 #define NGT_F32 0
 #define NGT_BF16 1
@@ -790,6 +790,91 @@ int ngt_wgrad_workspace_bytes(int64_t n_rows, int32_t n_out, int32_t n_in, size_
 int ngt_wgrad_pays(int64_t n_rows, int64_t n_out, int64_t n_in);
 int ngt_wgrad_bf16(const void* x, const void* dy, int64_t n_rows, int32_t n_out, int32_t n_in,
                    float* dw, float* db, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Gated linear layer, bf16: y = act(x Wg^T + bg) * (x Wu^T + bu) from x [n_rows,
+ * n_in] (rows x_stride elements apart), Wg and Wu [n_out, n_in] and biases [n_out]
+ * (nullable), summed in fp32 and rounded once; sizes and alignment as ngt_linear_fwd.
+ * keep, where not null, receives [n_rows, 2 n_out] for the backward: zu act'(zg) in
+ * the first n_out columns, act(zg) behind them.
+ * ngt_gated_bwd: dz [n_rows, 2 n_out] = dy times keep's columns (the gradients of
+ * zg and zu) and, where dx is not null, dx = dzg Wg + dzu Wu.  dW and db of both
+ * layers are ngt_wgrad_bf16 of x and dz (rows 0 .. n_out-1 of its results are Wg's).
+ * dy, keep and dz are contiguous.  NGT_ACT_SILU is z / (1 + e^-z).
+ * A gated form of the encoder's FFN, NeutronGT/models/graphormer_dist_node_level.py:18-30.
+ */
+#define NGT_ACT_SILU 3
+int ngt_gated_fwd(const void* x, int64_t x_stride, const void* w_gate, const void* w_up,
+                  const void* b_gate, const void* b_up, int64_t n_rows, int32_t n_out,
+                  int32_t n_in, int32_t activation, void* y, void* keep, void* stream);
+int ngt_gated_bwd_workspace_bytes(int64_t n_rows, int32_t n_out, int32_t n_in, size_t* bytes);
+int ngt_gated_bwd(const void* dy, const void* keep, const void* w_gate, const void* w_up,
+                  int64_t n_rows, int32_t n_out, int32_t n_in, void* dz, void* dx, void* workspace,
+                  size_t workspace_bytes, void* stream);
+
+/*
+ * Norm and rotation of query and key heads, in one pass over rows x [n_rows, n_heads, d]:
+ *   u = x / sqrt(mean(x^2) + eps) * gain   per row and head (gain null: u = x)
+ *   y = u with its first `dim` components turned in pairs (a, b) by t = position * f:
+ *       y_a = m (u_a cos t - u_b sin t),  y_b = m (u_a sin t + u_b cos t)
+ * where pair i is (i, i + dim/2), or (2i, 2i + 1) where interleaved, and f_i comes in
+ * whole turns per position (fp64).  x and y in dtype (NGT_F32 or NGT_BF16), gains in
+ * either, all arithmetic fp32 from angles reduced in fp64.  d is even, at most 256.
+ * The backward writes dx from dy, and dgain (in the gain's type, nullable) as sums over
+ * rows and heads in a fixed order.  y and dx are contiguous and do not overlap x or dy.
+ * One call takes queries and keys (k may be null); both have n_rows rows.
+ * The reference's attention has neither; the rows are those of its q and k
+ * (NeutronGT/models/graphormer_dist_node_level.py:128-173).
+ */
+typedef struct ngt_head_rows {
+  const void* x;       /* [n_rows, n_heads, d], last dimension contiguous */
+  const void* gain;    /* [d], or null */
+  void* y;             /* forward: the result; backward: dx (nullable) */
+  const void* dy;      /* backward: the result's gradient, last dimension contiguous */
+  void* dgain;         /* backward: [d], or null */
+  int64_t x_row, x_head;   /* elements between rows and heads */
+  int64_t dy_row, dy_head;
+  int32_t n_heads;
+  int32_t gain_dtype;
+} ngt_head_rows;
+
+typedef struct ngt_rotation {
+  const void* positions;  /* device int32 or int64 [n_rows] */
+  const double* turns;    /* device [dim / 2] */
+  int32_t position_bytes; /* 4 or 8 */
+  int32_t dim;            /* even, at most d; 0: no rotation (the pointers are not read) */
+  int32_t interleaved;
+  float magnitude;
+} ngt_rotation;
+
+int ngt_norm_rotary_fwd(int dtype, const ngt_head_rows* q, const ngt_head_rows* k, int64_t n_rows,
+                        int32_t d, const ngt_rotation* rotation, float eps, void* stream);
+int ngt_norm_rotary_bwd_workspace_bytes(int64_t n_rows, int32_t d, size_t* bytes);
+int ngt_norm_rotary_bwd(int dtype, const ngt_head_rows* q, const ngt_head_rows* k, int64_t n_rows,
+                        int32_t d, const ngt_rotation* rotation, float eps, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/*
+ * The 2-norm over many gradients, and the gradients scaled by min(1, max_norm / norm).
+ * tensors: host array of n_tensors; elements are dtype & 0xff (NGT_F32 or NGT_BF16) in
+ * one run of memory each, aligned to their type.  Sums are fp64 in a fixed order; *norm (device)
+ * is the fp32 norm.  A norm that is not finite scales nothing.  A tensor's result goes
+ * to out (in out_dtype) or, where out is null, back to x, whose memory is left alone
+ * where the factor is 1.  max_norm < 0: the norm alone.
+ * No two results may overlap, nor a result another tensor's x.  workspace: 16-byte
+ * aligned, of ngt_clip_workspace_bytes.  The training step of the reference has no
+ * clipping (NeutronGT/core/node_level_pipeline/train_eval.py:255-300).
+ */
+typedef struct ngt_gradient {
+  void* x;
+  void* out;
+  int64_t n;
+  int32_t dtype, out_dtype;
+} ngt_gradient;
+
+int ngt_clip_workspace_bytes(const ngt_gradient* tensors, int32_t n_tensors, size_t* bytes);
+int ngt_clip_gradients(const ngt_gradient* tensors, int32_t n_tensors, double max_norm, float* norm,
+                       void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -10,6 +10,10 @@ dense_attention(...)     functional full-window attention
 packed_attention(...)    attention over a PackedWindows batch (grouped heads, causal, bucket bias)
 PackedWindows            plan of windows of different lengths back to back
 linear_epilogue(...)     act(x W^T + b) + residual as one kernel, differentiable
+gated_linear(...)        act(x Wg^T + bg) * (x Wu^T + bu) as one kernel, differentiable
+norm_rotary(...)         RMS norm and position rotation of query and key heads, differentiable
+Rotary                   the angles of such a rotation
+clip_gradients(...)      gradients scaled to a largest global norm; gradient_norm(...): the norm
 WindowAdjacency          device CSR/transposed CSR/work lists of one window
 """
 from .attention import (CoreAttention, DenseAttentionBiasFunction, DenseAttentionFunction,
@@ -17,8 +21,10 @@ from .attention import (CoreAttention, DenseAttentionBiasFunction, DenseAttentio
                         dense_attention_bias, install, sparse_attention, window_attention)
 from .csr import (AdjacencyCache, WindowAdjacency, chunk_for_heads, default_cache, pack_q_adaptive,
                   small_for_heads)
-from .linear import LinearEpilogueFunction, linear_epilogue
+from .gradients import clip_gradients, gradient_norm
+from .linear import GatedLinearFunction, LinearEpilogueFunction, gated_linear, linear_epilogue
 from .packed import PackedAttentionFunction, PackedWindows, PairBuckets, packed_attention
+from .rotary import NormRotaryFunction, Rotary, norm_rotary
 
 __all__ = [
     "CoreAttention",
@@ -37,6 +43,13 @@ __all__ = [
     "PairBuckets",
     "linear_epilogue",
     "LinearEpilogueFunction",
+    "gated_linear",
+    "GatedLinearFunction",
+    "norm_rotary",
+    "NormRotaryFunction",
+    "Rotary",
+    "clip_gradients",
+    "gradient_norm",
     "WindowAdjacency",
     "AdjacencyCache",
     "chunk_for_heads",

@@ -13,7 +13,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libngt_attn.so"
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 NGT_F32 = 0
 NGT_BF16 = 1
@@ -107,12 +107,58 @@ class PackedWindowsC(C.Structure):
     ]
 
 
+class HeadRowsC(C.Structure):
+    """Mirror of ``ngt_head_rows``."""
+
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("gain", C.c_void_p),
+        ("y", C.c_void_p),
+        ("dy", C.c_void_p),
+        ("dgain", C.c_void_p),
+        ("x_row", C.c_int64),
+        ("x_head", C.c_int64),
+        ("dy_row", C.c_int64),
+        ("dy_head", C.c_int64),
+        ("n_heads", C.c_int32),
+        ("gain_dtype", C.c_int32),
+    ]
+
+
+class RotationC(C.Structure):
+    """Mirror of ``ngt_rotation``."""
+
+    _fields_ = [
+        ("positions", C.c_void_p),
+        ("turns", C.c_void_p),
+        ("position_bytes", C.c_int32),
+        ("dim", C.c_int32),
+        ("interleaved", C.c_int32),
+        ("magnitude", C.c_float),
+    ]
+
+
+class GradientC(C.Structure):
+    """Mirror of ``ngt_gradient``."""
+
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("out", C.c_void_p),
+        ("n", C.c_int64),
+        ("dtype", C.c_int32),
+        ("out_dtype", C.c_int32),
+    ]
+
+
 _i32, _i64, _f32, _vp, _sz = C.c_int32, C.c_int64, C.c_float, C.c_void_p, C.c_size_t
 _u64 = C.c_uint64
 _pi32 = C.POINTER(C.c_int32)
 _psz = C.POINTER(C.c_size_t)
 _pcsr = C.POINTER(WindowCSR)
 _ppw = C.POINTER(PackedWindowsC)
+_phr = C.POINTER(HeadRowsC)
+_prot = C.POINTER(RotationC)
+_pgr = C.POINTER(GradientC)
 
 # name -> argtypes (restype is int unless listed in _RESTYPES)
 SIGNATURES = {
@@ -174,6 +220,14 @@ SIGNATURES = {
     "ngt_linear_fwd": [_vp, _i64, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp],
     "ngt_linear_bwd_workspace_bytes": [_i64, _i32, _i32, _psz],
     "ngt_linear_bwd": [_vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _sz, _vp],
+    "ngt_gated_fwd": [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp],
+    "ngt_gated_bwd_workspace_bytes": [_i64, _i32, _i32, _psz],
+    "ngt_gated_bwd": [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _sz, _vp],
+    "ngt_norm_rotary_fwd": [_i32, _phr, _phr, _i64, _i32, _prot, _f32, _vp],
+    "ngt_norm_rotary_bwd_workspace_bytes": [_i64, _i32, _psz],
+    "ngt_norm_rotary_bwd": [_i32, _phr, _phr, _i64, _i32, _prot, _f32, _vp, _sz, _vp],
+    "ngt_clip_workspace_bytes": [_pgr, _i32, _psz],
+    "ngt_clip_gradients": [_pgr, _i32, C.c_double, _vp, _vp, _sz, _vp],
     "ngt_wgrad_workspace_bytes": [_i64, _i32, _i32, _psz],
     "ngt_wgrad_pays": [_i64, _i64, _i64],
     "ngt_wgrad_bf16": [_vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _sz, _vp],

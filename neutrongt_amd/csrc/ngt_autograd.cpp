@@ -31,7 +31,8 @@
 // 113 -> 91 us (74 -> 60 us on a faster host).
 //
 // PackedAttention and LinearEpilogue are PackedAttentionFunction (packed.py) and
-// LinearEpilogueFunction (linear.py).  Their entries return nothing where an
+// LinearEpilogueFunction (linear.py); GatedLinear and NormRotary GatedLinearFunction
+// (linear.py) and NormRotaryFunction (rotary.py).  Their entries return nothing where an
 // argument is not one that they take (a forward-mode dual tensor among them, whose
 // tangent a call without gradients would drop): Python then checks it and says why.
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -39,6 +40,8 @@
 
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
+#include <cmath>
 #include <map>
 #include <string>
 
@@ -70,6 +73,14 @@ decltype(&ngt_packed_bwd) g_packed_bwd = nullptr;
 decltype(&ngt_linear_fwd) g_linear_fwd = nullptr;
 decltype(&ngt_linear_bwd_workspace_bytes) g_linear_bwd_ws = nullptr;
 decltype(&ngt_linear_bwd) g_linear_bwd = nullptr;
+decltype(&ngt_gated_fwd) g_gated_fwd = nullptr;
+decltype(&ngt_gated_bwd_workspace_bytes) g_gated_bwd_ws = nullptr;
+decltype(&ngt_gated_bwd) g_gated_bwd = nullptr;
+decltype(&ngt_norm_rotary_fwd) g_rotary_fwd = nullptr;
+decltype(&ngt_norm_rotary_bwd_workspace_bytes) g_rotary_bwd_ws = nullptr;
+decltype(&ngt_norm_rotary_bwd) g_rotary_bwd = nullptr;
+decltype(&ngt_clip_workspace_bytes) g_clip_ws = nullptr;
+decltype(&ngt_clip_gradients) g_clip = nullptr;
 
 void check(int rc) {
   if (rc != NGT_OK) {
@@ -867,6 +878,354 @@ std::optional<Tensor> linear_epilogue(const Tensor& x, const Tensor& weight,
   return epilogue_forward(x, weight, bias, residual, act, false).y;
 }
 
+// --------------------------------------------------------------- gated linear
+struct GatedForward {
+  Tensor x2, wg, wu, y, keep;
+};
+
+GatedForward gated_forward(const Tensor& x, const Tensor& w_gate, const Tensor& w_up,
+                           const std::optional<Tensor>& b_gate, const std::optional<Tensor>& b_up,
+                           int64_t act, bool want_grad) {
+  NoAutocast off;
+  const int64_t n_out = w_gate.size(0), n_in = w_gate.size(1);
+  GatedForward r;
+  r.x2 = bf16(x).reshape({-1, n_in});
+  const int64_t m = r.x2.size(0);
+  if ((n_in > 1 && r.x2.stride(1) != 1) || (m > 1 && r.x2.stride(0) < n_in))
+    r.x2 = r.x2.clone(at::MemoryFormat::Contiguous);
+  r.wg = bf16(w_gate).contiguous(), r.wu = bf16(w_up).contiguous();
+  const Tensor bg = b_gate.has_value() ? bf16(*b_gate).contiguous() : Tensor();
+  const Tensor bu = b_up.has_value() ? bf16(*b_up).contiguous() : Tensor();
+  auto shape = x.sizes().vec();
+  shape.back() = n_out;
+  r.y = at::empty(shape, r.x2.options());
+  if (want_grad) r.keep = at::empty({m, 2 * n_out}, r.x2.options());
+  check(g_gated_fwd(r.x2.data_ptr(), m > 1 ? r.x2.stride(0) : n_in, r.wg.data_ptr(),
+                    r.wu.data_ptr(), bg.defined() ? bg.data_ptr() : nullptr,
+                    bu.defined() ? bu.data_ptr() : nullptr, m, static_cast<int32_t>(n_out),
+                    static_cast<int32_t>(n_in), static_cast<int32_t>(act), r.y.data_ptr(),
+                    want_grad ? r.keep.data_ptr() : nullptr, stream_of(x)));
+  return r;
+}
+
+int64_t type_of(const std::optional<Tensor>& t) {
+  return t.has_value() ? static_cast<int64_t>(t->scalar_type()) : -1;
+}
+
+struct GatedLinear : public torch::autograd::Function<GatedLinear> {
+  static Tensor forward(AutogradContext* ctx, Tensor x, Tensor w_gate, Tensor w_up,
+                        std::optional<Tensor> b_gate, std::optional<Tensor> b_up, int64_t act) {
+    const auto r = gated_forward(x, w_gate, w_up, b_gate, b_up, act, true);
+    ctx->save_for_backward({r.x2, r.wg, r.wu, r.keep});
+    ctx->saved_data["types"] = std::vector<int64_t>{
+        type_of(x), type_of(w_gate), type_of(w_up), type_of(b_gate), type_of(b_up)};
+    ctx->saved_data["shape"] = x.sizes().vec();
+    return r.y;
+  }
+
+  static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+    NoAutocast off;
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x2 = saved[0], &wg = saved[1], &wu = saved[2], &keep = saved[3];
+    const at::DeviceGuard guard(x2.device());
+    const int64_t m = x2.size(0), n_in = x2.size(1), n_out = wg.size(0);
+    const auto types = ctx->saved_data["types"].toIntVector();
+    // the node's edges are numbered over the tensors that were given
+    bool want[5];
+    for (int i = 0, edge = 0; i < 5; ++i)
+      want[i] = types[i] >= 0 && ctx->needs_input_grad(static_cast<size_t>(edge++));
+    const auto n = static_cast<int32_t>(n_out), k = static_cast<int32_t>(n_in);
+    const Tensor g = rows16(bf16(grads[0]));
+    const Tensor dz = at::empty({m, 2 * n_out}, g.options());
+    Tensor dx = want[0] ? at::empty({m, n_in}, g.options()) : Tensor();
+    size_t bytes = 0;
+    if (want[0]) check(g_gated_bwd_ws(m, n, k, &bytes));
+    Tensor ws = bytes ? workspace(static_cast<int64_t>(bytes), g) : Tensor();
+    check(g_gated_bwd(g.data_ptr(), keep.data_ptr(), wg.data_ptr(), wu.data_ptr(), m, n, k,
+                      dz.data_ptr(), want[0] ? dx.data_ptr() : nullptr,
+                      bytes ? ws.data_ptr() : nullptr, bytes, stream_of(x2)));
+    tensor_list res(6);
+    auto type = [&](int i) { return static_cast<at::ScalarType>(types[i]); };
+    if (want[0]) res[0] = dx.view(ctx->saved_data["shape"].toIntVector()).to(type(0));
+    Tensor dw, db;
+    if (want[1] || want[2]) {
+      const Tensor xc = x2.contiguous();
+      const auto opt = x2.options().dtype(at::kFloat);
+      dw = at::empty({2 * n_out, n_in}, opt);
+      if (want[3] || want[4]) db = at::empty({2 * n_out}, opt);
+      check(g_wgrad_ws(m, 2 * n, k, &bytes));
+      ws = workspace(static_cast<int64_t>(bytes), x2);
+      check(g_wgrad(xc.data_ptr(), dz.data_ptr(), m, 2 * n, k, dw.data_ptr<float>(),
+                    db.defined() ? db.data_ptr<float>() : nullptr, ws.data_ptr(), bytes,
+                    stream_of(x2)));
+    } else if (want[3] || want[4]) {
+      db = colsum(dz);
+    }
+    for (int i = 1; i < 5; ++i)
+      if (want[i])
+        res[i] = (i < 3 ? dw : db).narrow(0, i % 2 ? 0 : n_out, n_out).to(type(i));
+    return once("gated_linear", res);
+  }
+};
+
+// The checks of linear.py's gated_linear, without their messages: nothing where one
+// of them fails.
+std::optional<Tensor> gated_linear(const Tensor& x, const Tensor& w_gate, const Tensor& w_up,
+                                   const std::optional<Tensor>& b_gate,
+                                   const std::optional<Tensor>& b_up, int64_t act) {
+  if (!x.is_cuda() || !linear_type(x, x) || !linear_type(w_gate, x) || !linear_type(w_up, x) ||
+      w_gate.dim() != 2 || w_up.sizes() != w_gate.sizes() || x.dim() < 1 ||
+      x.size(-1) != w_gate.size(1) || w_gate.numel() == 0)
+    return std::nullopt;
+  bool grad = x.requires_grad() || w_gate.requires_grad() || w_up.requires_grad();
+  for (const auto* b : {&b_gate, &b_up}) {
+    if (!b->has_value()) continue;
+    if (!linear_type(**b, x) || (*b)->dim() != 1 || (*b)->size(0) != w_gate.size(0))
+      return std::nullopt;
+    grad = grad || (*b)->requires_grad();
+  }
+  if (has_tangent(x) || has_tangent(w_gate) || has_tangent(w_up) || has_tangent(b_gate) ||
+      has_tangent(b_up))
+    return std::nullopt;
+  const at::DeviceGuard guard(x.device());
+  if (at::GradMode::is_enabled() && grad)
+    return GatedLinear::apply(x, w_gate, w_up, b_gate, b_up, act);
+  return gated_forward(x, w_gate, w_up, b_gate, b_up, act, false).y;
+}
+
+// -------------------------------------------------------- norm and rotation
+// heads [..., H, d] as rows [n, H, d] that the kernels read where they are
+Tensor head_rows(const Tensor& t) {
+  const Tensor r = t.dim() == 3 ? t : t.reshape({-1, t.size(-2), t.size(-1)});
+  if (r.numel() && r.stride(2) != 1) return r.contiguous();
+  return r;
+}
+
+ngt_head_rows head_struct(const Tensor& x, const Tensor& gain) {
+  ngt_head_rows r{};
+  r.x = x.data_ptr();
+  r.x_row = x.stride(0), r.x_head = x.stride(1);
+  r.n_heads = static_cast<int32_t>(x.size(1));
+  if (gain.defined()) r.gain = gain.data_ptr(), r.gain_dtype = dtype_code(gain);
+  return r;
+}
+
+struct Turns {
+  Tensor positions, turns;
+  bool interleaved;
+  double magnitude;
+  ngt_rotation rotation() const {
+    ngt_rotation r{};
+    if (!turns.defined()) return r;
+    r.positions = positions.data_ptr();
+    r.turns = turns.data_ptr<double>();
+    r.position_bytes = static_cast<int32_t>(positions.element_size());
+    r.dim = static_cast<int32_t>(2 * turns.numel());
+    r.interleaved = interleaved;
+    r.magnitude = static_cast<float>(magnitude);
+    return r;
+  }
+};
+
+tensor_list rotary_forward(const Tensor& q, const Tensor& k, const Tensor& q_gain,
+                           const Tensor& k_gain, const Turns& t, double eps) {
+  auto hq = head_struct(q, q_gain), hk = k.defined() ? head_struct(k, k_gain) : ngt_head_rows{};
+  tensor_list y{at::empty(q.sizes(), q.options()), k.defined() ? at::empty(k.sizes(), k.options()) : Tensor()};
+  hq.y = y[0].data_ptr();
+  if (k.defined()) hk.y = y[1].data_ptr();
+  const auto rot = t.rotation();
+  check(g_rotary_fwd(dtype_code(q), &hq, k.defined() ? &hk : nullptr, q.size(0),
+                     static_cast<int32_t>(q.size(2)), &rot, static_cast<float>(eps),
+                     stream_of(q)));
+  return y;
+}
+
+struct NormRotary : public torch::autograd::Function<NormRotary> {
+  // q [.., H, d], k [.., H_kv, d]; the results have their shapes
+  static tensor_list forward(AutogradContext* ctx, Tensor q, std::optional<Tensor> k,
+                             std::optional<Tensor> q_gain, std::optional<Tensor> k_gain,
+                             std::optional<Tensor> positions_opt, std::optional<Tensor> turns_opt,
+                             bool interleaved, double magnitude, double eps) {
+    const Tensor positions = positions_opt.value_or(Tensor()), turns = turns_opt.value_or(Tensor());
+    const Tensor q3 = head_rows(q), k3 = k.has_value() ? head_rows(*k) : Tensor();
+    const Tensor gq = q_gain.has_value() ? q_gain->contiguous() : Tensor();
+    const Tensor gk = k_gain.has_value() ? k_gain->contiguous() : Tensor();
+    const auto y = rotary_forward(q3, k3, gq, gk, {positions, turns, interleaved, magnitude}, eps);
+    ctx->save_for_backward({q3, k3, gq, gk, positions, turns});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["magnitude"] = magnitude;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["q_shape"] = q.sizes().vec();
+    tensor_list out{y[0].view(q.sizes())};
+    if (k.has_value()) {
+      ctx->saved_data["k_shape"] = k->sizes().vec();
+      out.push_back(y[1].view(k->sizes()));
+    }
+    return out;
+  }
+
+  static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &q_gain = saved[2], &k_gain = saved[3];
+    const at::DeviceGuard guard(q.device());
+    // the node's edges are numbered over the tensors that were given
+    size_t edge = 0;
+    tensor_list res(9);
+    auto wanted = [&](const Tensor& t) {
+      if (!t.defined()) return Tensor();
+      const bool w = ctx->needs_input_grad(edge++);
+      return w ? at::empty(t.sizes(), t.options()) : Tensor();
+    };
+    res[0] = wanted(q), res[1] = wanted(k), res[2] = wanted(q_gain), res[3] = wanted(k_gain);
+    auto hq = head_struct(q, q_gain), hk = k.defined() ? head_struct(k, k_gain) : ngt_head_rows{};
+    const Tensor gq = head_rows(grads[0].to(q.scalar_type()));
+    const Tensor gk = k.defined() ? head_rows(grads[1].to(k.scalar_type())) : Tensor();
+    auto fill = [](ngt_head_rows& h, const Tensor& dy, const Tensor& dx, const Tensor& dgain) {
+      h.dy = dy.data_ptr(), h.dy_row = dy.stride(0), h.dy_head = dy.stride(1);
+      if (dx.defined()) h.y = dx.data_ptr();
+      if (dgain.defined()) h.dgain = dgain.data_ptr();
+    };
+    fill(hq, gq, res[0], res[2]);
+    if (k.defined()) fill(hk, gk, res[1], res[3]);
+    size_t bytes = 0;
+    if (res[2].defined() || res[3].defined())
+      check(g_rotary_bwd_ws(q.size(0), static_cast<int32_t>(q.size(2)), &bytes));
+    const Tensor ws = bytes ? workspace(static_cast<int64_t>(bytes), q) : Tensor();
+    const auto rot = Turns{saved[4], saved[5], ctx->saved_data["interleaved"].toBool(),
+                           ctx->saved_data["magnitude"].toDouble()}
+                         .rotation();
+    check(g_rotary_bwd(dtype_code(q), &hq, k.defined() ? &hk : nullptr, q.size(0),
+                       static_cast<int32_t>(q.size(2)), &rot,
+                       static_cast<float>(ctx->saved_data["eps"].toDouble()),
+                       bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)));
+    if (res[0].defined()) res[0] = res[0].view(ctx->saved_data["q_shape"].toIntVector());
+    if (res[1].defined()) res[1] = res[1].view(ctx->saved_data["k_shape"].toIntVector());
+    return once("norm_rotary", res);
+  }
+};
+
+// The checks of rotary.py's norm_rotary, without their messages: nothing where one of
+// them fails.
+std::optional<tensor_list> norm_rotary(const Tensor& q, const std::optional<Tensor>& k,
+                                       const std::optional<Tensor>& q_gain,
+                                       const std::optional<Tensor>& k_gain,
+                                       const std::optional<Tensor>& positions,
+                                       const std::optional<Tensor>& turns, bool interleaved,
+                                       double magnitude, double eps) {
+  if (!q.is_cuda() || q.dim() < 2 || !q.has_storage()) return std::nullopt;
+  const int64_t d = q.size(-1), lead = q.dim() - 2;
+  const auto type = q.scalar_type();
+  if ((type != at::kFloat && type != at::kBFloat16) || d < 2 || d > 256 || d % 2 ||
+      q.size(-2) < 1 || !(eps >= 0) || !(eps < INFINITY) || turns.has_value() != positions.has_value())
+    return std::nullopt;
+  bool grad = q.requires_grad();
+  if (k.has_value()) {
+    if (k->dim() != q.dim() || k->size(-1) != d || k->size(-2) < 1 || k->scalar_type() != type ||
+        k->device() != q.device() || !k->has_storage() ||
+        k->sizes().slice(0, lead) != q.sizes().slice(0, lead))
+      return std::nullopt;
+    grad = grad || k->requires_grad();
+  } else if (k_gain.has_value()) {
+    return std::nullopt;
+  }
+  for (const auto* g : {&q_gain, &k_gain}) {
+    if (!g->has_value()) continue;
+    const auto gt = (*g)->scalar_type();
+    if ((*g)->dim() != 1 || (*g)->size(0) != d || (*g)->device() != q.device() ||
+        (gt != type && gt != at::kFloat) || !(*g)->has_storage())
+      return std::nullopt;
+    grad = grad || (*g)->requires_grad();
+  }
+  std::optional<Tensor> pos;
+  if (turns.has_value()) {
+    const auto pt = positions->scalar_type();
+    if (turns->device() != q.device() || 2 * turns->numel() > d ||
+        positions->device() != q.device() || (pt != at::kInt && pt != at::kLong) ||
+        positions->sizes() != q.sizes().slice(0, lead) || !positions->has_storage())
+      return std::nullopt;
+    pos = positions->reshape({-1}).contiguous();
+  }
+  if (has_tangent(q) || has_tangent(k) || has_tangent(q_gain) || has_tangent(k_gain))
+    return std::nullopt;
+  const at::DeviceGuard guard(q.device());
+  if (at::GradMode::is_enabled() && grad)
+    return NormRotary::apply(q, k, q_gain, k_gain, pos, turns, interleaved, magnitude, eps);
+  auto y = rotary_forward(head_rows(q), k.has_value() ? head_rows(*k) : Tensor(),
+                          q_gain.has_value() ? q_gain->contiguous() : Tensor(),
+                          k_gain.has_value() ? k_gain->contiguous() : Tensor(),
+                          {pos.value_or(Tensor()), turns.value_or(Tensor()), interleaved, magnitude},
+                          eps);
+  y[0] = y[0].view(q.sizes());
+  if (k.has_value()) y[1] = y[1].view(k->sizes());
+  else y.pop_back();
+  return y;
+}
+
+// ------------------------------------------------------------------ clipping
+bool clip_type(const Tensor& t, const Tensor& like) {
+  return t.layout() == at::kStrided && t.device() == like.device() && t.has_storage() &&
+         (t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16) &&
+         (t.numel() == 0 || t.is_non_overlapping_and_dense());
+}
+
+// gradients.py's call: the norm, or nothing where one of its checks fails.
+std::optional<Tensor> clip_gradients(const std::vector<Tensor>& grads,
+                                     const std::optional<std::vector<Tensor>>& out,
+                                     double max_norm) {
+  if (grads.empty() || !grads[0].is_cuda() || (out.has_value() && out->size() != grads.size()))
+    return std::nullopt;
+  const size_t n = grads.size();
+  std::vector<ngt_gradient> table(n);
+  struct Run {
+    uintptr_t from, to;
+    size_t tensor;
+    bool result;
+  };
+  std::vector<Run> runs;
+  runs.reserve(out.has_value() ? 2 * n : n);
+  auto add = [&](const Tensor& t, size_t i, bool result) {
+    const auto at = reinterpret_cast<uintptr_t>(t.data_ptr());
+    if (t.numel()) runs.push_back({at, at + t.numel() * t.element_size(), i, result});
+  };
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor& g = grads[i];
+    if (!clip_type(g, grads[0])) return std::nullopt;
+    table[i] = {g.data_ptr(), nullptr, g.numel(), dtype_code(g), 0};
+    add(g, i, false);
+    if (!out.has_value()) continue;
+    const Tensor& o = (*out)[i];
+    if (!clip_type(o, grads[0]) || o.sizes() != g.sizes()) return std::nullopt;
+    for (int64_t a = 0; g.numel() && a < g.dim(); ++a)
+      if (g.size(a) != 1 && g.stride(a) != o.stride(a)) return std::nullopt;
+    table[i].out = o.data_ptr(), table[i].out_dtype = dtype_code(o);
+    add(o, i, true);
+  }
+  if (max_norm >= 0) {
+    // a result may lie in its own gradient's memory, nothing else may overlap
+    std::sort(runs.begin(), runs.end(), [](const Run& a, const Run& b) {
+      return a.from != b.from ? a.from < b.from : a.tensor != b.tensor ? a.tensor < b.tensor
+                                                                       : a.result < b.result;
+    });
+    for (size_t i = 1, last = 0; i < runs.size(); ++i) {
+      const Run &a = runs[last], &b = runs[i];
+      if (b.from < a.to && !(a.tensor == b.tensor && a.from == b.from && a.to == b.to))
+        return std::nullopt;
+      if (b.to > a.to) last = i;
+    }
+  }
+  const at::DeviceGuard guard(grads[0].device());
+  size_t bytes = 0;
+  check(g_clip_ws(table.data(), static_cast<int32_t>(n), &bytes));
+  const Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
+  const Tensor ws = workspace(static_cast<int64_t>(bytes), norm);
+  check(g_clip(table.data(), static_cast<int32_t>(n), max_norm, norm.data_ptr<float>(),
+               ws.data_ptr(), bytes, stream_of(norm)));
+  if (max_norm >= 0)
+    for (const Tensor& t : out.has_value() ? *out : grads)
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  return norm;
+}
+
 template <typename F>
 void entry(F*& fn, const std::map<std::string, int64_t>& addr, const char* name) {
   const auto it = addr.find(name);
@@ -895,6 +1254,14 @@ void init(const std::map<std::string, int64_t>& addr) {
   entry(g_linear_fwd, addr, "ngt_linear_fwd");
   entry(g_linear_bwd_ws, addr, "ngt_linear_bwd_workspace_bytes");
   entry(g_linear_bwd, addr, "ngt_linear_bwd");
+  entry(g_gated_fwd, addr, "ngt_gated_fwd");
+  entry(g_gated_bwd_ws, addr, "ngt_gated_bwd_workspace_bytes");
+  entry(g_gated_bwd, addr, "ngt_gated_bwd");
+  entry(g_rotary_fwd, addr, "ngt_norm_rotary_fwd");
+  entry(g_rotary_bwd_ws, addr, "ngt_norm_rotary_bwd_workspace_bytes");
+  entry(g_rotary_bwd, addr, "ngt_norm_rotary_bwd");
+  entry(g_clip_ws, addr, "ngt_clip_workspace_bytes");
+  entry(g_clip, addr, "ngt_clip_gradients");
 }
 
 }  // namespace
@@ -922,4 +1289,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "packed.py's PackedAttentionFunction; windows: the bytes of one ngt_packed_windows");
   m.def("linear_epilogue", &linear_epilogue,
         "(x, weight, bias, residual, activation) -> y or None: linear.py's LinearEpilogueFunction");
+  m.def("gated_linear", &gated_linear,
+        "(x, w_gate, w_up, b_gate, b_up, activation) -> y or None: linear.py's GatedLinearFunction");
+  m.def("norm_rotary", &norm_rotary,
+        "(q, k, q_gain, k_gain, positions, turns, interleaved, magnitude, eps) -> [q', k'] (or [q']) "
+        "or None: rotary.py's NormRotaryFunction");
+  m.def("clip_gradients", &clip_gradients,
+        "(gradients, results or None, max_norm; negative: the norm alone) -> norm or None: "
+        "gradients.py's call");
 }

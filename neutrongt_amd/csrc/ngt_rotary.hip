@@ -1,0 +1,467 @@
+// RMS norm of query and key heads with a gain, and the rotation of their first
+// components by the row's position, in one pass; forward and backward.  What stands
+// between the projections of packed attention and the attention itself.
+//
+//   s = 1 / sqrt(mean(x^2) + eps),  h = x s,  u = h gain        (no gain: u = x)
+//   y_a = m (u_a cos t - u_b sin t),  y_b = m (u_a sin t + u_b cos t),  t = position f
+// and backward, with g = the transposed rotation of dy:
+//   dgain = sum over rows and heads of g h,  w = g gain,  dx = s (w - h mean(w h)).
+// s is formed again from x, which the backward reads anyway.
+//
+// Bound by memory: a head is read once and written once.  A lane holds 2 V of its
+// components, V pairs (16 bytes twice where sizes and alignment allow), a group of
+// lanes a head, so the mean is a few steps within the wave.  Cosines and sines are
+// formed once for all heads of a row, in LDS: the angle in fp64 turns, of which only the
+// part behind the quarter turn enters the fp32 functions, so that a far position
+// costs no precision.
+#include "ngt_common.h"
+
+namespace ngt {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxDim = 256;
+constexpr int64_t kMaxRows = int64_t(1) << 30;
+constexpr int kTableBytes = 16384;  // cosines and sines of a block's rows
+constexpr int kBwdBlocks = 1024;    // most blocks, so most partial sums, of a backward
+
+// One of queries and keys, as the kernels see it.
+struct Rows {
+  const void* x;
+  const void* gain;
+  void* y;
+  const void* dy;
+  float* part;  // [blocks][d] of dgain, or null
+  int64_t x_row, x_head, dy_row, dy_head;
+  int32_t n_heads, gain_f32;
+  int32_t tile_rows;  // rows of a tile
+  int32_t splits;     // blocks that share a tile's heads
+  int32_t tiles;
+  int32_t blocks;
+};
+
+struct Args {
+  Rows r[2];
+  const void* positions;
+  const double* turns;
+  int64_t n_rows;
+  float eps, magnitude;
+  int32_t d, dim, units, group_log;  // 2^group_log lanes a head
+  int32_t pos64;
+};
+
+// cos and sin of 2 pi x, x in turns.
+__device__ __forceinline__ float2 cos_sin(double x) {
+  x -= rint(x);
+  const double q = rint(4.0 * x);
+  // less than an eighth of a turn is left, exact until it is rounded
+  const float f = static_cast<float>(fma(q, -0.25, x));
+  float s, c;
+  sincospif(2.f * f, &s, &c);
+  const int k = static_cast<int>(q) & 3;
+  const float a = k & 1 ? -s : c, b = k & 1 ? c : s;
+  return k & 2 ? make_float2(-a, -b) : make_float2(a, b);
+}
+
+template <typename T, int V>
+struct Chunk {
+  static constexpr int kBytes = V * static_cast<int>(sizeof(T));
+  uint32_t w[kBytes < 4 ? 1 : kBytes / 4];
+  __device__ __forceinline__ void load(const T* __restrict__ p) {
+    if constexpr (kBytes == 16) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else if constexpr (kBytes == 8) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      w[0] = v.x, w[1] = v.y;
+    } else if constexpr (kBytes == 4) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (uint32_t& v : w) v = 0u;
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+    return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+  }
+  __device__ __forceinline__ static void store(T* __restrict__ p, const float* v) {
+    if constexpr (sizeof(T) == 4) {
+      if constexpr (V == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+      else if constexpr (V == 2) *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+      else *p = v[0];
+    } else {
+      if constexpr (V == 8)
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]),
+                                                  pack2_bf16(v[4], v[5]), pack2_bf16(v[6], v[7]));
+      else if constexpr (V == 4)
+        *reinterpret_cast<uint2*>(p) = make_uint2(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]));
+      else if constexpr (V == 2) *reinterpret_cast<uint32_t*>(p) = pack2_bf16(v[0], v[1]);
+      else p->x = static_cast<uint16_t>(pack2_bf16(v[0], 0.f));
+    }
+  }
+};
+
+// Sum over the 2^log adjacent lanes of a head, the same in all of them.
+__device__ __forceinline__ float group_sum(float v, int log) {
+  for (int i = 0; i < log; ++i) v += shfl_xor(v, 1 << i);
+  return v;
+}
+
+// V pairs of components of each of a lane's U units; INTER: pairs are adjacent.
+template <typename T, int V, int U, bool INTER, bool BWD>
+__global__ __launch_bounds__(kThreads) void k_norm_rotary(const Args a) {
+  extern __shared__ float2 table[];  // [tile_rows][dim / 2]
+  __shared__ float sums[BWD ? kThreads / kWave : 1][BWD ? kMaxDim : 1];
+  const int tid = threadIdx.x;
+  const bool second = int(blockIdx.x) >= a.r[0].blocks;  // block-uniform
+  const Rows r = second ? a.r[1] : a.r[0];
+  const int block = blockIdx.x - (second ? a.r[0].blocks : 0);
+  const int pairs = a.dim / 2, lanes = 1 << a.group_log, groups = kThreads >> a.group_log;
+  const int lane = tid & (lanes - 1), group = tid >> a.group_log;
+  const bool norm = r.gain != nullptr;
+  const float by_d = 1.f / static_cast<float>(a.d);
+
+  // where this lane's units lie in a head
+  int at[U][2], turn[U];
+  bool there[U], turned[U];
+  float gain[U][2 * V];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int unit = lane * U + u;
+    there[u] = unit < a.units;
+    turned[u] = 2 * V * unit < a.dim;
+    turn[u] = turned[u] ? unit * V : 0;
+    const bool apart = !INTER && turned[u];
+    at[u][0] = apart ? unit * V : 2 * V * unit;
+    at[u][1] = apart ? pairs + unit * V : 2 * V * unit + V;
+#pragma unroll
+    for (int i = 0; i < 2 * V; ++i) {
+      gain[u][i] = 1.f;
+      if (norm && there[u]) {
+        const int c = at[u][i / V] + i % V;
+        gain[u][i] = r.gain_f32 ? static_cast<const float*>(r.gain)[c]
+                                : bf16_to_f32(static_cast<const bf16_t*>(r.gain)[c].x);
+      }
+    }
+  }
+  float acc[U][2 * V];
+  if constexpr (BWD)
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 2 * V; ++i) acc[u][i] = 0.f;
+
+  const int slot = block % r.splits, per_round = r.blocks / r.splits;
+  for (int tile = block / r.splits; tile < r.tiles; tile += per_round) {
+    const int64_t row0 = int64_t(tile) * r.tile_rows;
+    const int rows = a.n_rows - row0 < r.tile_rows ? int(a.n_rows - row0) : r.tile_rows;
+    __syncthreads();
+    for (int e = tid; e < rows * pairs; e += kThreads) {
+      const int row = e / pairs;
+      const double p = a.pos64 ? static_cast<double>(static_cast<const int64_t*>(a.positions)[row0 + row])
+                               : static_cast<double>(static_cast<const int32_t*>(a.positions)[row0 + row]);
+      const float2 cs = cos_sin(p * a.turns[e - row * pairs]);
+      table[e] = make_float2(cs.x * a.magnitude, cs.y * a.magnitude);
+    }
+    __syncthreads();
+    const int items = rows * r.n_heads, step = groups * r.splits;
+    for (int item = slot * groups + group; item < items; item += step) {
+      const int row = item / r.n_heads, head = item - row * r.n_heads;
+      const T* x = static_cast<const T*>(r.x) + (row0 + row) * r.x_row + head * r.x_head;
+      const int64_t to = ((row0 + row) * r.n_heads + head) * a.d;
+      Chunk<T, V> xr[U][2], gr[U][2];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          xr[u][c].zero();
+          if (there[u]) xr[u][c].load(x + at[u][c]);
+          if constexpr (BWD) {
+            gr[u][c].zero();
+            if (there[u])
+              gr[u][c].load(static_cast<const T*>(r.dy) + (row0 + row) * r.dy_row +
+                            head * r.dy_head + at[u][c]);
+          }
+        }
+      float v[U][2 * V];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 2 * V; ++i) v[u][i] = xr[u][i / V].get(i % V);
+      float scale = 1.f;
+      if (norm) {
+        float s = 0.f;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < 2 * V; ++i) s = fmaf(v[u][i], v[u][i], s);
+        scale = 1.f / sqrtf(fmaf(group_sum(s, a.group_log), by_d, a.eps));
+      }
+      float w[U][2 * V], dot = 0.f;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float2* cs = table + row * pairs + turn[u];
+        float in[2 * V];
+#pragma unroll
+        for (int i = 0; i < 2 * V; ++i)
+          in[i] = BWD ? gr[u][i / V].get(i % V) : norm ? v[u][i] * scale * gain[u][i] : v[u][i];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          constexpr int kA = INTER ? 2 : 1, kB = INTER ? 1 : V;
+          const int ia = kA * j, ib = kA * j + kB;
+          w[u][ia] = in[ia], w[u][ib] = in[ib];
+          if (turned[u]) {
+            const float c = cs[j].x, s = BWD ? -cs[j].y : cs[j].y;
+            w[u][ia] = fmaf(in[ia], c, -(in[ib] * s));
+            w[u][ib] = fmaf(in[ia], s, in[ib] * c);
+          }
+        }
+        if constexpr (BWD)
+          if (norm) {
+#pragma unroll
+            for (int i = 0; i < 2 * V; ++i) {
+              v[u][i] *= scale;
+              acc[u][i] = fmaf(w[u][i], v[u][i], acc[u][i]);
+              w[u][i] *= gain[u][i];
+              dot = fmaf(w[u][i], v[u][i], dot);
+            }
+          }
+      }
+      if constexpr (BWD) {
+        if (norm) {
+          dot = group_sum(dot, a.group_log) * by_d;
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < 2 * V; ++i) w[u][i] = scale * fmaf(-v[u][i], dot, w[u][i]);
+        }
+        if (!r.y) continue;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (there[u]) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            Chunk<T, V>::store(static_cast<T*>(r.y) + to + at[u][c], &w[u][c * V]);
+        }
+    }
+  }
+  if constexpr (BWD) {
+    if (!r.part) return;  // block-uniform
+    // the groups of a wave, then the waves in their order
+    const int wave = tid / kWave;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 2 * V; ++i) {
+        for (int off = lanes; off < kWave; off <<= 1) acc[u][i] += shfl_xor(acc[u][i], off);
+        if (tid % kWave < lanes && there[u]) sums[wave][at[u][i / V] + i % V] = acc[u][i];
+      }
+    __syncthreads();
+    if (tid < a.d) {
+      float s = 0.f;
+#pragma unroll
+      for (int q = 0; q < kThreads / kWave; ++q) s += sums[q][tid];
+      r.part[int64_t(block) * a.d + tid] = s;
+    }
+  }
+}
+
+// dgain: the blocks' sums added, 32 columns a block, 32 lanes a column that take
+// every 32nd block; in fp64.
+struct Join {
+  const float* part[2];
+  void* out[2];
+  int32_t blocks[2], f32[2];
+  int32_t d;
+};
+__global__ __launch_bounds__(1024) void k_join_gain(const Join j) {
+  __shared__ double red[32][33];
+  const int which = blockIdx.y, col = blockIdx.x * 32 + threadIdx.x % 32, lane = threadIdx.x / 32;
+  if (!j.out[which]) return;
+  double s = 0.0;
+  if (col < j.d) {
+#pragma unroll 4
+    for (int b = lane; b < j.blocks[which]; b += 32)
+      s += static_cast<double>(j.part[which][int64_t(b) * j.d + col]);
+  }
+  red[lane][threadIdx.x % 32] = s;
+  __syncthreads();
+  if (lane != 0 || col >= j.d) return;
+  for (int l = 1; l < 32; ++l) s += red[l][threadIdx.x];
+  if (j.f32[which]) static_cast<float*>(j.out[which])[col] = static_cast<float>(s);
+  else static_cast<bf16_t*>(j.out[which])[col].x = f32_to_bf16(static_cast<float>(s));
+}
+
+bool multiple(const void* p, int64_t a, int64_t b, int v, int es) {
+  return reinterpret_cast<uintptr_t>(p) % (v * es) == 0 && a % v == 0 && b % v == 0;
+}
+
+int check(const char* fn, int dtype, const ngt_head_rows* q, const ngt_head_rows* k,
+          int64_t n_rows, int32_t d, const ngt_rotation* rot, float eps, bool bwd) {
+  if (dtype != NGT_F32 && dtype != NGT_BF16) return set_error(NGT_ERR_ARG, "%s: dtype %d", fn, dtype);
+  if (n_rows < 0 || n_rows > kMaxRows)
+    return set_error(NGT_ERR_ARG, "%s: n_rows=%lld", fn, static_cast<long long>(n_rows));
+  if (d < 2 || d % 2 || d > kMaxDim)
+    return set_error(NGT_ERR_UNSUPPORTED, "%s: head_dim %d is not even or not within 2 .. %d", fn, d,
+                     kMaxDim);
+  if (!q) return set_error(NGT_ERR_ARG, "%s: null q", fn);
+  if (!(eps >= 0.f)) return set_error(NGT_ERR_ARG, "%s: eps=%g", fn, double(eps));
+  if (rot && (rot->dim < 0 || rot->dim % 2 || rot->dim > d))
+    return set_error(NGT_ERR_ARG, "%s: %d rotated components of %d", fn, rot->dim, d);
+  if (rot && rot->dim > 0 && rot->position_bytes != 4 && rot->position_bytes != 8)
+    return set_error(NGT_ERR_ARG, "%s: positions of %d bytes", fn, rot->position_bytes);
+  if (n_rows > 0 && rot && rot->dim > 0 && (!rot->positions || !rot->turns))
+    return set_error(NGT_ERR_ARG, "%s: null positions or turns", fn);
+  for (const ngt_head_rows* h : {q, k}) {
+    if (!h) continue;
+    if (h->n_heads < 1 || h->n_heads > (1 << 16))
+      return set_error(NGT_ERR_ARG, "%s: %d heads", fn, h->n_heads);
+    if (h->gain && h->gain_dtype != NGT_F32 && h->gain_dtype != NGT_BF16)
+      return set_error(NGT_ERR_ARG, "%s: gain dtype %d", fn, h->gain_dtype);
+    if (n_rows > 0 && (!h->x || (bwd ? !h->dy : !h->y)))
+      return set_error(NGT_ERR_ARG, "%s: null %s", fn, bwd ? "x or dy" : "x or y");
+    if (h->dgain && !h->gain) return set_error(NGT_ERR_ARG, "%s: dgain without a gain", fn);
+    if (h->x_row < 0 || h->x_head < 0 || h->dy_row < 0 || h->dy_head < 0)
+      return set_error(NGT_ERR_ARG, "%s: negative stride", fn);
+  }
+  return NGT_OK;
+}
+
+template <typename T, int V, int U, bool BWD>
+void launch(const Args& a, bool inter, int blocks, size_t lds, hipStream_t st) {
+  auto kernel = inter ? &k_norm_rotary<T, V, U, true, BWD> : &k_norm_rotary<T, V, U, false, BWD>;
+  hipLaunchKernelGGL(kernel, dim3(unsigned(blocks)), dim3(kThreads), lds, st, a);
+}
+
+template <bool BWD>
+int run(const char* fn, int dtype, const ngt_head_rows* q, const ngt_head_rows* k, int64_t n_rows,
+        int32_t d, const ngt_rotation* rot, float eps, void* workspace, hipStream_t st) {
+  const int es = dtype == NGT_F32 ? 4 : 2;
+  Args a{};
+  a.n_rows = n_rows, a.eps = eps, a.d = d;
+  a.dim = rot ? rot->dim : 0;
+  if (a.dim) {
+    a.positions = rot->positions, a.turns = rot->turns, a.magnitude = rot->magnitude;
+    a.pos64 = rot->position_bytes == 8;
+  }
+  // the widest pieces that sizes and alignment allow
+  const ngt_head_rows* in[2] = {q, k};
+  int v = 16 / es;
+  auto fits = [&](int n) {
+    if (d % (2 * n) || a.dim % (2 * n)) return false;
+    for (const ngt_head_rows* h : in) {
+      if (!h) continue;
+      if (!multiple(h->x, h->x_row, h->x_head, n, es) || !multiple(h->y, d, d, n, es)) return false;
+      if (BWD && !multiple(h->dy, h->dy_row, h->dy_head, n, es)) return false;
+    }
+    return true;
+  };
+  while (v > 1 && !fits(v)) v /= 2;
+  a.units = d / (2 * v);
+  const int per_lane = v == 1 ? 2 : 1;
+  while ((per_lane << a.group_log) < a.units) ++a.group_log;
+  const int groups = kThreads >> a.group_log;
+  int blocks = 0;
+  Join join{};
+  join.d = d;
+  float* part = static_cast<float*>(workspace);
+  for (int i = 0; i < 2; ++i) {
+    Rows& r = a.r[i];
+    const ngt_head_rows* h = in[i];
+    if (!h || (BWD && !h->y && !h->dgain)) continue;
+    r.x = h->x, r.gain = h->gain, r.y = h->y, r.dy = h->dy;
+    r.x_row = h->x_row, r.x_head = h->x_head, r.dy_row = h->dy_row, r.dy_head = h->dy_head;
+    r.n_heads = h->n_heads, r.gain_f32 = h->gain_dtype == NGT_F32;
+    // 8 heads for each group, so that a row's cosines serve many
+    int rows = 8 * groups / h->n_heads;
+    const int most = a.dim ? kTableBytes / (a.dim * 4) : 1024;
+    rows = rows < 1 ? 1 : rows > most ? most : rows;
+    // .. unless that leaves CUs without a block
+    while (rows > 1 && (n_rows + rows - 1) / rows < 512) rows /= 2;
+    r.tile_rows = rows;
+    const int64_t tiles = (n_rows + rows - 1) / rows;
+    r.tiles = static_cast<int32_t>(tiles);
+    r.splits = 1;
+    const int rounds = (rows * h->n_heads + groups - 1) / groups;
+    while (r.splits < rounds && tiles * r.splits < 512) ++r.splits;
+    int64_t n = tiles * r.splits;
+    const int64_t most_blocks = BWD ? kBwdBlocks / 2 : 1 << 20;
+    if (n > most_blocks) n = most_blocks / r.splits * r.splits;
+    r.blocks = static_cast<int32_t>(n);
+    blocks += r.blocks;
+    if (BWD && h->dgain) {
+      r.part = part;
+      part += int64_t(r.blocks) * d;
+      join.part[i] = r.part, join.out[i] = h->dgain, join.blocks[i] = r.blocks;
+      join.f32[i] = r.gain_f32;
+    }
+  }
+  if (blocks > 0) {
+    KernelTimer timer_(BWD ? "norm_rotary_bwd" : "norm_rotary_fwd", st);
+    const int tile = a.r[0].tile_rows > a.r[1].tile_rows ? a.r[0].tile_rows : a.r[1].tile_rows;
+    const size_t lds = size_t(tile) * (a.dim / 2) * sizeof(float2);
+    const bool inter = rot && rot->interleaved;
+    if (dtype == NGT_F32) {
+      if (v == 4) launch<float, 4, 1, BWD>(a, inter, blocks, lds, st);
+      else if (v == 2) launch<float, 2, 1, BWD>(a, inter, blocks, lds, st);
+      else launch<float, 1, 2, BWD>(a, inter, blocks, lds, st);
+    } else {
+      if (v == 8) launch<bf16_t, 8, 1, BWD>(a, inter, blocks, lds, st);
+      else if (v == 4) launch<bf16_t, 4, 1, BWD>(a, inter, blocks, lds, st);
+      else if (v == 2) launch<bf16_t, 2, 1, BWD>(a, inter, blocks, lds, st);
+      else launch<bf16_t, 1, 2, BWD>(a, inter, blocks, lds, st);
+    }
+    NGT_HIP_CHECK(hipGetLastError());
+  }
+  if (BWD && (join.out[0] || join.out[1])) {
+    KernelTimer timer_("norm_rotary_gain", st);
+    hipLaunchKernelGGL(k_join_gain, dim3((d + 31) / 32, 2), dim3(1024), 0, st, join);
+    NGT_HIP_CHECK(hipGetLastError());
+  }
+  return NGT_OK;
+}
+
+}  // namespace
+}  // namespace ngt
+
+using namespace ngt;
+
+extern "C" int ngt_norm_rotary_fwd(int dtype, const ngt_head_rows* q, const ngt_head_rows* k,
+                                   int64_t n_rows, int32_t d, const ngt_rotation* rotation,
+                                   float eps, void* stream) {
+  const char* fn = "ngt_norm_rotary_fwd";
+  NGT_CHECK_OK(check(fn, dtype, q, k, n_rows, d, rotation, eps, false));
+  if (n_rows == 0) return NGT_OK;
+  return run<false>(fn, dtype, q, k, n_rows, d, rotation, eps, nullptr,
+                    static_cast<hipStream_t>(stream));
+}
+
+extern "C" int ngt_norm_rotary_bwd_workspace_bytes(int64_t n_rows, int32_t d, size_t* bytes) {
+  const char* fn = "ngt_norm_rotary_bwd_workspace_bytes";
+  if (n_rows < 0 || n_rows > kMaxRows || d < 2 || d > kMaxDim || !bytes)
+    return set_error(NGT_ERR_ARG, "%s: n_rows=%lld head_dim=%d", fn,
+                     static_cast<long long>(n_rows), d);
+  *bytes = size_t(kBwdBlocks) * d * sizeof(float);
+  return NGT_OK;
+}
+
+extern "C" int ngt_norm_rotary_bwd(int dtype, const ngt_head_rows* q, const ngt_head_rows* k,
+                                   int64_t n_rows, int32_t d, const ngt_rotation* rotation,
+                                   float eps, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  const char* fn = "ngt_norm_rotary_bwd";
+  NGT_CHECK_OK(check(fn, dtype, q, k, n_rows, d, rotation, eps, true));
+  const bool sums = q->dgain || (k && k->dgain);
+  if (sums && n_rows > 0 &&
+      (!workspace || workspace_bytes < size_t(kBwdBlocks) * d * sizeof(float) ||
+       reinterpret_cast<uintptr_t>(workspace) % 16))
+    return set_error(NGT_ERR_WORKSPACE, "%s: workspace %zu < %zu or not 16-byte aligned", fn,
+                     workspace_bytes, size_t(kBwdBlocks) * d * sizeof(float));
+  return run<true>(fn, dtype, q, k, n_rows, d, rotation, eps, workspace,
+                   static_cast<hipStream_t>(stream));
+}

@@ -42,6 +42,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .attention import CoreAttention
+from .gradients import clip_gradients
 from .layernorm import FusedLayerNorm, add_dropout_layernorm
 from .linear import WgradLinear, groupable, project
 
@@ -304,11 +305,13 @@ class WindowGT(_WindowModel):
 
 
 def window_step(model: nn.Module, optimizer, x, edge_index, labels, train_mask,
-                kv_cache=None, autocast_dtype=None):
+                kv_cache=None, autocast_dtype=None, max_grad_norm=None):
     """One window iteration of train_eval.py:255-300 on one GPU: forward, NLL
     over the window's training nodes, backward, optimizer step.  Returns
     (loss tensor, last layer's node scores).  ``autocast_dtype`` (e.g.
-    torch.bfloat16) runs the forward under torch.autocast.
+    torch.bfloat16) runs the forward under torch.autocast; ``max_grad_norm``
+    clips the model's gradients by their global norm before the optimizer step
+    (the reference does not).
 
     Nothing here synchronises with the host, so the whole step can be captured
     in a HIP graph (with a capturable optimizer): the masked mean is a
@@ -324,5 +327,7 @@ def window_step(model: nn.Module, optimizer, x, edge_index, labels, train_mask,
     loss = (F.nll_loss(out, labels, reduction="none") * w).sum() / w.sum()
     optimizer.zero_grad(set_to_none=True)
     loss.backward()
+    if max_grad_norm is not None:
+        clip_gradients(model.parameters(), max_grad_norm)
     optimizer.step()
     return loss.detach(), scores[-1]

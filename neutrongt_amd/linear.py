@@ -404,3 +404,100 @@ def linear_epilogue(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | 
     want_grad = torch.is_grad_enabled() and any(t.requires_grad for t in ts)
     return LinearEpilogueFunction.apply(x2, weight, bias, r2, ACTIVATIONS[activation],
                                         want_grad).view(shape)
+
+
+GATES = {None: 0, "relu": 1, "gelu": 2, "silu": 3}
+
+
+class GatedLinearFunction(torch.autograd.Function):
+    """act(x2 Wg^T + bg) * (x2 Wu^T + bu) of bf16 rows x2 [M, n_in] (ngt_gated_fwd /
+    ngt_gated_bwd / ngt_wgrad_bf16); the gradients of weights and biases come in
+    their own type, from fp32 sums."""
+
+    @staticmethod
+    def forward(ctx, x2, w_gate, w_up, b_gate, b_up, act, want_grad):
+        m, n_in = x2.shape
+        n_out, dev = w_gate.shape[0], x2.device
+        wg, wu = (w.to(torch.bfloat16).contiguous() for w in (w_gate, w_up))
+        bg, bu = (b.to(torch.bfloat16).contiguous() if b is not None else None
+                  for b in (b_gate, b_up))
+        y = torch.empty(m, n_out, dtype=torch.bfloat16, device=dev)
+        keep = torch.empty(m, 2 * n_out, dtype=torch.bfloat16, device=dev) if want_grad else None
+        with torch.cuda.device(dev):
+            _lib.check(_lib.load().ngt_gated_fwd(
+                x2.data_ptr(), x2.stride(0) if m > 1 else n_in, wg.data_ptr(), wu.data_ptr(),
+                bg.data_ptr() if bg is not None else None,
+                bu.data_ptr() if bu is not None else None, m, n_out, n_in, act, y.data_ptr(),
+                keep.data_ptr() if keep is not None else None, _lib.stream_ptr(dev)))
+        if want_grad:
+            ctx.save_for_backward(x2, wg, wu, keep)
+            ctx.dtypes = [t.dtype if t is not None else None for t in (w_gate, w_up, b_gate, b_up)]
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        x2, wg, wu, keep = ctx.saved_tensors
+        (m, n_in), n_out, dev = x2.shape, wg.shape[0], x2.device
+        want_x, *want = ctx.needs_input_grad[:5]
+        g = gy.to(torch.bfloat16).contiguous()
+        dz = torch.empty(m, 2 * n_out, dtype=torch.bfloat16, device=dev)
+        dx = torch.empty(m, n_in, dtype=torch.bfloat16, device=dev) if want_x else None
+        nb = C.c_size_t()
+        _lib.check(_lib.load().ngt_gated_bwd_workspace_bytes(m, n_out, n_in, C.byref(nb)))
+        ws = torch.empty(nb.value if want_x else 0, dtype=torch.uint8, device=dev)
+        with torch.cuda.device(dev):
+            _lib.check(_lib.load().ngt_gated_bwd(
+                g.data_ptr(), keep.data_ptr(), wg.data_ptr(), wu.data_ptr(), m, n_out, n_in,
+                dz.data_ptr(), dx.data_ptr() if want_x else None,
+                ws.data_ptr() if want_x else None, ws.numel(), _lib.stream_ptr(dev)))
+            grads = [None] * 4
+            if want[0] or want[1]:
+                dw, db = linear_grads(x2, dz, want[2] or want[3])
+                grads[0], grads[1] = dw[:n_out], dw[n_out:]
+            elif want[2] or want[3]:
+                db = colsum_bf16(dz)
+            if want[2] or want[3]:
+                grads[2], grads[3] = db[:n_out], db[n_out:]
+        return (dx, *(t.to(d) if w else None for t, d, w in zip(grads, ctx.dtypes, want)), None,
+                None)
+
+
+def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
+                 b_gate: torch.Tensor | None = None, b_up: torch.Tensor | None = None,
+                 activation: str | None = "silu"):
+    """act(x Wg^T + bg) * (x Wu^T + bu) as one kernel in bf16, the first half of a
+    gated feed-forward block (linear_epilogue is the second): x [..., n_in], weights
+    [n_out, n_in] and biases [n_out] as two nn.Linear hold them, or the halves of a
+    joint one; activation "silu" (z / (1 + e^-z)), "gelu" (the erf form), "relu" or None.
+    fp32 inputs are rounded to bf16 as autocast does; the sums, the activation and the
+    product are fp32 and the result is rounded once.  The gradients have the inputs'
+    types; those of weights and biases are fp32 sums in a fixed order.
+    Differentiable once."""
+    if activation not in GATES:
+        raise ValueError(f"activation must be one of {list(GATES)}, got {activation!r}")
+    ext = _lib.node_ext()
+    y = ext and ext.gated_linear(x, w_gate, w_up, b_gate, b_up, GATES[activation])
+    if y is not None:
+        return y
+    ts = [t for t in (x, w_gate, w_up, b_gate, b_up) if t is not None]
+    if any(not t.is_cuda for t in ts):
+        raise ValueError("gated_linear takes GPU tensors (there is no CPU path)")
+    if any(t.device != x.device for t in ts):
+        raise ValueError("x, weights and biases must be on one device")
+    if any(t.dtype not in (torch.bfloat16, torch.float32) for t in ts):
+        raise TypeError("gated_linear takes bfloat16 or float32 tensors")
+    if (w_gate.dim() != 2 or x.dim() < 1 or x.shape[-1] != w_gate.shape[1] or 0 in w_gate.shape
+            or w_up.shape != w_gate.shape):
+        raise ValueError(f"x {tuple(x.shape)} and weights {tuple(w_gate.shape)}, "
+                         f"{tuple(w_up.shape)} do not match")
+    n_out, n_in = w_gate.shape
+    for name, b in (("b_gate", b_gate), ("b_up", b_up)):
+        if b is not None and tuple(b.shape) != (n_out,):
+            raise ValueError(f"{name} must be [{n_out}], got {tuple(b.shape)}")
+    x2 = x.to(torch.bfloat16).reshape(-1, n_in)
+    if (n_in > 1 and x2.stride(1) != 1) or (x2.shape[0] > 1 and x2.stride(0) < n_in):
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    want_grad = torch.is_grad_enabled() and any(t.requires_grad for t in ts)
+    return GatedLinearFunction.apply(x2, w_gate, w_up, b_gate, b_up, GATES[activation],
+                                     want_grad).view(*x.shape[:-1], n_out)

@@ -100,6 +100,15 @@ class PackedWindows:
                                                           n_buckets, C.byref(f), C.byref(b)))
         return f.value, b.value
 
+    def positions(self) -> torch.Tensor:
+        """int32 [n_q], each query row's position in its window, counted from its first
+        key as the causal order does: i + (k_length - q_length).  For norm_rotary; made
+        on the host and copied, so make it once for all layers and steps."""
+        rows = [torch.arange(b - a, b, dtype=torch.int32)
+                for a, b in zip(self.q_lengths, self.k_lengths)]
+        rows = torch.cat(rows) if rows else torch.empty(0, dtype=torch.int32)
+        return rows.to(self.device)
+
     def pack_buckets(self, ids) -> "PairBuckets":
         """The pairs' bucket ids in the kernels' layouts (by queries and by
         keys).  ``ids``: a 1-D integer tensor, the windows' [queries, keys]
