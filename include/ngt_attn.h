@@ -797,20 +797,30 @@ int ngt_wgrad_bf16(const void* x, const void* dy, int64_t n_rows, int32_t n_out,
  * (nullable), summed in fp32 and rounded once; sizes and alignment as ngt_linear_fwd.
  * keep, where not null, receives [n_rows, 2 n_out] for the backward: zu act'(zg) in
  * the first n_out columns, act(zg) behind them.
- * ngt_gated_bwd: dz [n_rows, 2 n_out] = dy times keep's columns (the gradients of
- * zg and zu) and, where dx is not null, dx = dzg Wg + dzu Wu.  dW and db of both
- * layers are ngt_wgrad_bf16 of x and dz (rows 0 .. n_out-1 of its results are Wg's).
- * dy, keep and dz are contiguous.  NGT_ACT_SILU is z / (1 + e^-z).
+ * ngt_gated_bwd: from dy, what was kept and x (all contiguous) the gradients that are not
+ * null: dx [n_rows, n_in] bf16, and those of weights and biases in their own types, from
+ * fp32 sums in a fixed order.  All matrices and the workspace are 16-byte aligned.
+ * NGT_ACT_SILU is z / (1 + e^-z).
  * A gated form of the encoder's FFN, NeutronGT/models/graphormer_dist_node_level.py:18-30.
  */
 #define NGT_ACT_SILU 3
+typedef struct ngt_gated_grads {
+  void* dx;
+  void* dw_gate; /* [n_out, n_in] */
+  void* dw_up;
+  void* db_gate; /* [n_out] */
+  void* db_up;
+  int32_t dw_gate_dtype, dw_up_dtype, db_gate_dtype, db_up_dtype;
+} ngt_gated_grads;
+
 int ngt_gated_fwd(const void* x, int64_t x_stride, const void* w_gate, const void* w_up,
                   const void* b_gate, const void* b_up, int64_t n_rows, int32_t n_out,
                   int32_t n_in, int32_t activation, void* y, void* keep, void* stream);
 int ngt_gated_bwd_workspace_bytes(int64_t n_rows, int32_t n_out, int32_t n_in, size_t* bytes);
-int ngt_gated_bwd(const void* dy, const void* keep, const void* w_gate, const void* w_up,
-                  int64_t n_rows, int32_t n_out, int32_t n_in, void* dz, void* dx, void* workspace,
-                  size_t workspace_bytes, void* stream);
+int ngt_gated_bwd(const void* dy, const void* keep, const void* x, const void* w_gate,
+                  const void* w_up, int64_t n_rows, int32_t n_out, int32_t n_in,
+                  const ngt_gated_grads* grads, void* workspace, size_t workspace_bytes,
+                  void* stream);
 
 /*
  * Norm and rotation of query and key heads, in one pass over rows x [n_rows, n_heads, d]:

@@ -138,6 +138,22 @@ class RotationC(C.Structure):
     ]
 
 
+class GatedGradsC(C.Structure):
+    """Mirror of ``ngt_gated_grads``."""
+
+    _fields_ = [
+        ("dx", C.c_void_p),
+        ("dw_gate", C.c_void_p),
+        ("dw_up", C.c_void_p),
+        ("db_gate", C.c_void_p),
+        ("db_up", C.c_void_p),
+        ("dw_gate_dtype", C.c_int32),
+        ("dw_up_dtype", C.c_int32),
+        ("db_gate_dtype", C.c_int32),
+        ("db_up_dtype", C.c_int32),
+    ]
+
+
 class GradientC(C.Structure):
     """Mirror of ``ngt_gradient``."""
 
@@ -158,6 +174,7 @@ _pcsr = C.POINTER(WindowCSR)
 _ppw = C.POINTER(PackedWindowsC)
 _phr = C.POINTER(HeadRowsC)
 _prot = C.POINTER(RotationC)
+_pgg = C.POINTER(GatedGradsC)
 _pgr = C.POINTER(GradientC)
 
 # name -> argtypes (restype is int unless listed in _RESTYPES)
@@ -222,7 +239,7 @@ SIGNATURES = {
     "ngt_linear_bwd": [_vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _sz, _vp],
     "ngt_gated_fwd": [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp],
     "ngt_gated_bwd_workspace_bytes": [_i64, _i32, _i32, _psz],
-    "ngt_gated_bwd": [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _sz, _vp],
+    "ngt_gated_bwd": [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _pgg, _vp, _sz, _vp],
     "ngt_norm_rotary_fwd": [_i32, _phr, _phr, _i64, _i32, _prot, _f32, _vp],
     "ngt_norm_rotary_bwd_workspace_bytes": [_i64, _i32, _psz],
     "ngt_norm_rotary_bwd": [_i32, _phr, _phr, _i64, _i32, _prot, _f32, _vp, _sz, _vp],

@@ -50,6 +50,12 @@ FILE_FLAGS = {
     "ngt_packed_bwd.hip": ["-fno-honor-nans", "-mno-amdgpu-ieee"],
 }
 
+# Flags of HIPCC_FLAGS that a source goes without.  The gated layer's backward products hold
+# 192 or 256 accumulators a lane: in AGPRs, beside as many VGPRs of operands.
+FILE_DROPS = {
+    "ngt_gated_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+}
+
 
 def _hipcc() -> str:
     for cand in (os.environ.get("HIPCC"), shutil.which("hipcc"), "/opt/rocm/bin/hipcc"):
@@ -59,7 +65,8 @@ def _hipcc() -> str:
 
 
 def _compile(src: Path, obj: Path, verbose: bool, extra: list[str]) -> None:
-    cmd = [_hipcc(), *HIPCC_FLAGS, *FILE_FLAGS.get(src.name, []), *extra, "-c", str(src), "-o",
+    common = [f for f in HIPCC_FLAGS if f not in FILE_DROPS.get(src.name, [])]
+    cmd = [_hipcc(), *common, *FILE_FLAGS.get(src.name, []), *extra, "-c", str(src), "-o",
            str(obj)]
     if verbose:
         print(" ".join(cmd), flush=True)

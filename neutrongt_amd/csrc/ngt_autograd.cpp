@@ -926,8 +926,9 @@ struct GatedLinear : public torch::autograd::Function<GatedLinear> {
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
     NoAutocast off;
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x2 = saved[0], &wg = saved[1], &wu = saved[2], &keep = saved[3];
+    const Tensor &x2 = saved[0], &keep = saved[3];
     const at::DeviceGuard guard(x2.device());
+    const Tensor wg = rows16(saved[1]), wu = rows16(saved[2]);
     const int64_t m = x2.size(0), n_in = x2.size(1), n_out = wg.size(0);
     const auto types = ctx->saved_data["types"].toIntVector();
     // the node's edges are numbered over the tensors that were given
@@ -935,35 +936,27 @@ struct GatedLinear : public torch::autograd::Function<GatedLinear> {
     for (int i = 0, edge = 0; i < 5; ++i)
       want[i] = types[i] >= 0 && ctx->needs_input_grad(static_cast<size_t>(edge++));
     const auto n = static_cast<int32_t>(n_out), k = static_cast<int32_t>(n_in);
-    const Tensor g = rows16(bf16(grads[0]));
-    const Tensor dz = at::empty({m, 2 * n_out}, g.options());
-    Tensor dx = want[0] ? at::empty({m, n_in}, g.options()) : Tensor();
-    size_t bytes = 0;
-    if (want[0]) check(g_gated_bwd_ws(m, n, k, &bytes));
-    Tensor ws = bytes ? workspace(static_cast<int64_t>(bytes), g) : Tensor();
-    check(g_gated_bwd(g.data_ptr(), keep.data_ptr(), wg.data_ptr(), wu.data_ptr(), m, n, k,
-                      dz.data_ptr(), want[0] ? dx.data_ptr() : nullptr,
-                      bytes ? ws.data_ptr() : nullptr, bytes, stream_of(x2)));
-    tensor_list res(6);
+    const Tensor g = rows16(bf16(grads[0])), xc = rows16(x2);
     auto type = [&](int i) { return static_cast<at::ScalarType>(types[i]); };
-    if (want[0]) res[0] = dx.view(ctx->saved_data["shape"].toIntVector()).to(type(0));
-    Tensor dw, db;
-    if (want[1] || want[2]) {
-      const Tensor xc = x2.contiguous();
-      const auto opt = x2.options().dtype(at::kFloat);
-      dw = at::empty({2 * n_out, n_in}, opt);
-      if (want[3] || want[4]) db = at::empty({2 * n_out}, opt);
-      check(g_wgrad_ws(m, 2 * n, k, &bytes));
-      ws = workspace(static_cast<int64_t>(bytes), x2);
-      check(g_wgrad(xc.data_ptr(), dz.data_ptr(), m, 2 * n, k, dw.data_ptr<float>(),
-                    db.defined() ? db.data_ptr<float>() : nullptr, ws.data_ptr(), bytes,
-                    stream_of(x2)));
-    } else if (want[3] || want[4]) {
-      db = colsum(dz);
-    }
+    tensor_list res(6);
+    ngt_gated_grads out{};
+    if (want[0]) res[0] = at::empty({m, n_in}, g.options());
     for (int i = 1; i < 5; ++i)
       if (want[i])
-        res[i] = (i < 3 ? dw : db).narrow(0, i % 2 ? 0 : n_out, n_out).to(type(i));
+        res[i] = i < 3 ? at::empty({n_out, n_in}, g.options().dtype(type(i)))
+                       : at::empty({n_out}, g.options().dtype(type(i)));
+    auto at_of = [&](int i) { return want[i] ? res[i].data_ptr() : nullptr; };
+    auto code = [&](int i) { return want[i] ? dtype_code(res[i]) : NGT_F32; };
+    out.dx = at_of(0), out.dw_gate = at_of(1), out.dw_up = at_of(2);
+    out.db_gate = at_of(3), out.db_up = at_of(4);
+    out.dw_gate_dtype = code(1), out.dw_up_dtype = code(2);
+    out.db_gate_dtype = code(3), out.db_up_dtype = code(4);
+    size_t bytes = 0;
+    check(g_gated_bwd_ws(m, n, k, &bytes));
+    const Tensor ws = workspace(static_cast<int64_t>(bytes), g);
+    check(g_gated_bwd(g.data_ptr(), keep.data_ptr(), xc.data_ptr(), wg.data_ptr(), wu.data_ptr(), m,
+                      n, k, &out, ws.data_ptr(), bytes, stream_of(x2)));
+    if (want[0]) res[0] = res[0].view(ctx->saved_data["shape"].toIntVector()).to(type(0));
     return once("gated_linear", res);
   }
 };

@@ -103,17 +103,6 @@ __device__ __forceinline__ void finish8(const GemmArgs& a, int m, int n, const f
   }
 }
 
-// 64 pieces of a wave from memory to LDS, one after another from `at`.
-__device__ __forceinline__ void to_lds(packed::Buffer b, int offset, char* at) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(
-      b, (__attribute__((address_space(3))) void*)at, 16, offset, 0, 0, 0);
-}
-// Until at most N of this wave's reads from memory are under way.
-template <int N>
-__device__ __forceinline__ void wait_for_all_but() {
-  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);
-}
-
 // One block: BM rows by BN outputs, 2 x 2 waves of (BM / 2) x (BN / 2), stages of 64
 // of the contraction in LDS.  A 128 x 128 block's stage takes 512 clocks of the CU's
 // MFMA, 512 of its reads from LDS, 256 of the writes there and 512 of its path from L2

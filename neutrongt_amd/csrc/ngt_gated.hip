@@ -3,18 +3,12 @@
 //   keep = [zu act'(zg) | act(zg)],  dz = [dzg | dzu] = dy * keep,  dx = dzg Wg + dzu Wu.
 // The forward keeps the two factors of dy instead of zg and zu, so that the backward
 // forms no activation; either way two roundings to bf16 stand between dy and dz.
-#include "ngt_linear.h"
+#include "ngt_gated.h"
+
+#include <utility>
 
 namespace ngt {
 namespace {
-
-using packed::f32x16;
-using packed::fill16;
-using packed::tid_x;
-using packed::wg_x;
-
-constexpr int kStage = 64;  // contraction per LDS stage: rows of 128 bytes
-using L = packed::Tile<bf16_t, kStage>;
 
 struct GatedArgs {
   const uint16_t* x;   // [M, K], rows x_stride apart
@@ -33,17 +27,52 @@ struct GatedArgs {
 struct Gate {
   float value, slope;
 };
-__device__ __forceinline__ Gate gate_of(int act, float z) {
-  if (act == NGT_ACT_SILU) {
+template <int ACT>
+__device__ __forceinline__ Gate gate_of(float z) {
+  if constexpr (ACT == NGT_ACT_SILU) {
     const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
     return {z * s, s * fmaf(z, 1.f - s, 1.f)};
   }
-  if (act == NGT_ACT_GELU) {
+  if constexpr (ACT == NGT_ACT_GELU) {
     const Normal n = normal(z);
     return {z * n.cdf, fmaf(z * 0.39894228040143268f, n.pdf, n.cdf)};
   }
-  if (act == NGT_ACT_RELU) return {z > 0.f ? z : (z != z ? z : 0.f), z > 0.f ? 1.f : 0.f};
+  if constexpr (ACT == NGT_ACT_RELU)
+    return {z > 0.f ? z : (z != z ? z : 0.f), z > 0.f ? 1.f : 0.f};
   return {z, 1.f};
+}
+
+// f with the activation as a constant.
+template <typename F>
+__device__ __forceinline__ void with_act(int act, F f) {
+  if (act == NGT_ACT_SILU) f(std::integral_constant<int, NGT_ACT_SILU>{});
+  else if (act == NGT_ACT_GELU) f(std::integral_constant<int, NGT_ACT_GELU>{});
+  else if (act == NGT_ACT_RELU) f(std::integral_constant<int, NGT_ACT_RELU>{});
+  else f(std::integral_constant<int, NGT_ACT_NONE>{});
+}
+
+// Pieces of 8 results and, for the backward, of what it keeps, from their sums.
+struct Results {
+  u32x4 y, kg, ku;
+};
+template <int ACT>
+__device__ __forceinline__ Results results8(const float (&sg)[8], const float (&su)[8],
+                                            const u32x4& bg, const u32x4& bu) {
+  Results r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float v[2], g[2], u[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const float zu = su[2 * i + t] + half_of(bu, 2 * i + t);
+      const Gate q = gate_of<ACT>(sg[2 * i + t] + half_of(bg, 2 * i + t));
+      v[t] = q.value * zu, g[t] = zu * q.slope, u[t] = q.value;
+    }
+    r.y[i] = pack2_bf16(v[0], v[1]);
+    r.kg[i] = pack2_bf16(g[0], g[1]);
+    r.ku[i] = pack2_bf16(u[0], u[1]);
+  }
+  return r;
 }
 
 __device__ __forceinline__ void store8(uint16_t* row, int c, int n, const u32x4& v) {
@@ -60,27 +89,16 @@ __device__ __forceinline__ void store8(uint16_t* row, int c, int n, const u32x4&
 __device__ __forceinline__ void finish8(const GatedArgs& a, int m, int n, const float (&sg)[8],
                                         const float (&su)[8]) {
   if (m >= a.M || n >= a.N) return;
-  u32x4 bg = {0u, 0u, 0u, 0u}, bu = {0u, 0u, 0u, 0u}, y, kg, ku;
+  u32x4 bg = {0u, 0u, 0u, 0u}, bu = {0u, 0u, 0u, 0u};
   if (a.bg) bg = load8<false>(a.bg, n, a.N);
   if (a.bu) bu = load8<false>(a.bu, n, a.N);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float v[2], g[2], u[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const float zu = su[2 * i + t] + half_of(bu, 2 * i + t);
-      const Gate q = gate_of(a.act, sg[2 * i + t] + half_of(bg, 2 * i + t));
-      v[t] = q.value * zu, g[t] = zu * q.slope, u[t] = q.value;
-    }
-    y[i] = pack2_bf16(v[0], v[1]);
-    kg[i] = pack2_bf16(g[0], g[1]);
-    ku[i] = pack2_bf16(u[0], u[1]);
-  }
-  store8(a.y + int64_t(m) * a.N, n, a.N, y);
+  Results r;
+  with_act(a.act, [&](auto act) { r = results8<act.value>(sg, su, bg, bu); });
+  store8(a.y + int64_t(m) * a.N, n, a.N, r.y);
   if (a.keep) {
     uint16_t* row = a.keep + int64_t(m) * 2 * a.N;
-    store8(row, n, a.N, kg);
-    store8(row + a.N, n, a.N, ku);
+    store8(row, n, a.N, r.kg);
+    store8(row + a.N, n, a.N, r.ku);
   }
 }
 
@@ -135,27 +153,141 @@ __global__ __launch_bounds__(256) void k_gated_any(GatedArgs a) {
   }
 }
 
-// dz = [dy keep_g | dy keep_u], 8 columns a thread.
+// dz = [dy keep_g | dy keep_u], and the biases' gradients: part_b[chunk][2 N], sums of the
+// unrounded products.  A block: 256 columns of kDzRows rows, 8 columns a thread.  BLOCKS: whole
+// pieces, and dz in DzBlocks, else [M, 2 N].
+constexpr int kDzRows = 128;
+template <bool BLOCKS>
 __global__ __launch_bounds__(256) void k_gated_dz(const uint16_t* __restrict__ dy,
                                                   const uint16_t* __restrict__ keep, int64_t rows,
-                                                  int32_t n, uint16_t* __restrict__ dz) {
-  const int64_t per_row = (n + 7) / 8, total = rows * per_row;
-  const int64_t step = int64_t(__builtin_amdgcn_grid_size_x());
-  for (int64_t i = int64_t(wg_x()) * 256 + tid_x(); i < total; i += step) {
-    const int64_t row = i / per_row;
-    const int c = static_cast<int>(i - row * per_row) * 8;
-    const u32x4 g = load8<false>(dy + row * n, c, n);
+                                                  int32_t n, int32_t tiles_n,
+                                                  uint16_t* __restrict__ dz,
+                                                  float* __restrict__ part_b) {
+  __shared__ float red[2][8][256];
+  const int64_t chunk = wg_x() / tiles_n;
+  const int cg = tid_x() & 31, lane = tid_x() >> 5;
+  const int c = (wg_x() - static_cast<int>(chunk) * tiles_n) * 256 + 8 * cg;
+  const DzBlocks blocks(rows, n);
+  const int64_t end = BLOCKS ? blocks.row_blocks * 32 : rows;  // of what is written
+  const int64_t r0 = chunk * kDzRows, r1 = r0 + kDzRows < end ? r0 + kDzRows : end;
+  float sum[2][8];
 #pragma unroll
-    for (int part = 0; part < 2; ++part) {
-      const u32x4 v = load8<false>(keep + (2 * row + part) * n, c, n);
-      u32x4 o;
+  for (int p = 0; p < 2; ++p)
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-        o[t] = pack2_bf16(half_of(g, 2 * t) * half_of(v, 2 * t),
-                          half_of(g, 2 * t + 1) * half_of(v, 2 * t + 1));
-      store8(dz + (2 * row + part) * n, c, n, o);
+    for (int t = 0; t < 8; ++t) sum[p][t] = 0.f;
+  if (c < (BLOCKS ? 64 * blocks.per_layer : n)) {
+#pragma unroll 2
+    for (int64_t row = r0 + lane; row < r1; row += 8) {
+      u32x4 g = {0u, 0u, 0u, 0u}, v[2] = {g, g};
+      if (!BLOCKS || (row < rows && c < n)) {
+        g = load8<BLOCKS>(dy + row * n, c, n);
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const uint16_t* from = keep + (2 * row + p) * n;
+          // the last time that it is read
+          if constexpr (BLOCKS)
+            v[p] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(from + c));
+          else
+            v[p] = load8<false>(from, c, n);
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        u32x4 o;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const float lo = half_of(g, 2 * t) * half_of(v[p], 2 * t);
+          const float hi = half_of(g, 2 * t + 1) * half_of(v[p], 2 * t + 1);
+          sum[p][2 * t] += lo, sum[p][2 * t + 1] += hi;
+          o[t] = pack2_bf16(lo, hi);
+        }
+        if constexpr (BLOCKS)
+          *reinterpret_cast<u32x4*>(dz + (row / 32 * blocks.across() + p * blocks.per_layer + c / 64) * 2048 +
+                                    row % 32 * 64 + c % 64) = o;
+        else
+          store8(dz + (2 * row + p) * n, c, n, o);
+      }
     }
   }
+  if (!part_b) return;
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+#pragma unroll
+    for (int t = 0; t < 8; ++t) red[p][lane][8 * cg + t] = sum[p][t];
+  __syncthreads();
+  const int col = c - 8 * cg + tid_x();
+  if (col >= n) return;
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    float s = 0.f;
+#pragma unroll
+    for (int l = 0; l < 8; ++l) s += red[p][l][tid_x()];
+    part_b[(2 * chunk + p) * n + col] = s;
+  }
+}
+
+// The parameters' gradients in their types: of each weight the splits' sums added in their
+// order, 4 elements a thread; of the biases the chunks', 8 lanes a column that take every
+// 8th, added in their order.
+struct JoinArgs {
+  const float* part;    // [splits][2 N][K]
+  const float* part_b;  // [chunks][2 N]
+  void* dw[2];
+  void* db[2];
+  int64_t nk;           // N K
+  int32_t n, splits, chunks, blocks_w;
+  int32_t dw_f32[2], db_f32[2];
+};
+__device__ __forceinline__ void put(void* to, int64_t i, bool f32, float v) {
+  if (f32) static_cast<float*>(to)[i] = v;
+  else static_cast<uint16_t*>(to)[i] = f32_to_bf16(v);
+}
+__global__ __launch_bounds__(256) void k_gated_join(JoinArgs a) {
+  __shared__ float red[8][32];
+  if (wg_x() < a.blocks_w) {
+    const int64_t i = (int64_t(wg_x()) * 256 + tid_x()) * 4, all = 2 * a.nk;
+    if (i >= all) return;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool whole = all % 4 == 0;
+#pragma unroll 4
+    for (int c = 0; c < a.splits; ++c) {
+      const float* p = a.part + c * all + i;
+      if (whole) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
+      } else {
+        for (int t = 0; t < 4; ++t)
+          if (i + t < all) s[t] += p[t];
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      if (!a.dw[w]) continue;
+      const int64_t o = i - w * a.nk;
+      const bool f32 = a.dw_f32[w];
+      if (o >= 0 && o + 4 <= a.nk && a.nk % 4 == 0) {
+        if (f32) *reinterpret_cast<float4*>(static_cast<float*>(a.dw[w]) + o) = make_float4(s[0], s[1], s[2], s[3]);
+        else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.dw[w]) + o) = make_uint2(pack2_bf16(s[0], s[1]), pack2_bf16(s[2], s[3]));
+      } else {
+        for (int t = 0; t < 4; ++t)
+          if (o + t >= 0 && o + t < a.nk) put(a.dw[w], o + t, f32, s[t]);
+      }
+    }
+    return;
+  }
+  const int col = (wg_x() - a.blocks_w) * 32 + tid_x() % 32, lane = tid_x() / 32;
+  float s = 0.f;
+  if (col < 2 * a.n)
+#pragma unroll 8
+    for (int c = lane; c < a.chunks; c += 8) s += a.part_b[int64_t(c) * 2 * a.n + col];
+  red[lane][tid_x() % 32] = s;
+  __syncthreads();
+  if (lane != 0 || col >= 2 * a.n) return;
+  s = 0.f;
+#pragma unroll
+  for (int l = 0; l < 8; ++l) s += red[l][tid_x()];
+  const int w = col >= a.n;
+  if (a.db[w]) put(a.db[w], col - w * a.n, a.db_f32[w], s);
 }
 
 struct DxArgs {
@@ -218,6 +350,147 @@ __global__ __launch_bounds__(256) void k_gated_dx_any(DxArgs a) {
   }
 }
 
+// Aligned sizes.  One block: 64 FM rows by 64 outputs of both layers, 2 x 2 waves, each FM tiles
+// of 32 x 32 of the gate and the same of the other layer.  A wave takes a stage's
+// operands into registers before it multiplies, so the one buffer is free for the next
+// stage while it does, and two blocks on a CU fill each other's reads and epilogues.
+template <int FM>
+__global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
+  constexpr int BM = 64 * FM, kRowsBytes = BM * 128;
+  __shared__ __align__(16) char lds[kRowsBytes + 128 * 128];
+  const int lane = tid_x() & 63, wave = packed::wave_id(), half = lane >> 5;
+  const TileAt at = tile_at(a.tiles_m, a.tiles_n, 1);
+  if (!at.there) return;  // block-uniform
+  const int m0 = at.m * BM, n0 = at.n * 64;
+  const int wm = (wave >> 1) * FM, wn = wave & 1;  // in 32s
+  f32x16 g[FM], u[FM];
+#pragma unroll
+  for (int i = 0; i < FM; ++i) g[i] = u[i] = fill16(0.f);
+  RowsOperand x, w;
+  x.init(a.x_stride), w.init(a.K);
+  const uint32_t mine = lds_at(lds) + 1024 * wave;
+  // 32 rows of Wg, the same of Wu, the next of Wg, of Wu: a wave of a block's two columns of
+  // waves has its own beside one another
+  auto fetch = [&](int k) {
+    const u32x4 fx = RowsOperand::source(a.x + m0 * a.x_stride, a.M - m0, BM, a.x_stride, k, a.K);
+#pragma unroll
+    for (int i = 0; i < 2 * FM; ++i) x.load(fx, i, k, a.K, mine + 4096 * i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = n0 + 32 * (i >> 1);
+      const u32x4 fw = RowsOperand::source((i & 1 ? a.wu : a.wg) + int64_t(n) * a.K, a.N - n, 32, a.K,
+                                           k, a.K);
+      w.load(fw, 0, k, a.K, mine + kRowsBytes + 4096 * i);
+    }
+  };
+  fetch(0);
+  for (int k = 0; k < a.K; k += kStage) {
+    all_there();
+    meet();
+    L::Op fx[L::kChunks][FM], fw[L::kChunks][2];
+#pragma unroll
+    for (int c = 0; c < L::kChunks; ++c) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) fw[c][j] = RowsOperand::frag(lds + kRowsBytes, 2 * wn + j, c, lane);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) fx[c][i] = RowsOperand::frag(lds, wm + i, c, lane);
+    }
+    all_read();
+    meet();
+    fetch(k + kStage);  // (behind the last stage: zeros)
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int c = 0; c < L::kChunks; ++c)
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        g[i] = L::mma(fw[c][0], fx[c][i], g[i]);
+        u[i] = L::mma(fw[c][1], fx[c][i], u[i]);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  all_there();  // nothing is on its way to LDS any more, of any wave
+  meet();
+  // A lane has 16 consecutive outputs of row a_row(lane) of each tile.  They go through LDS,
+  // 32 rows at a time, so that a store's lanes fill 64 bytes of a row.
+  const int n = n0 + 32 * wn + 16 * half, back = lane / 4, n_back = n0 + 32 * wn + 8 * (lane % 4);
+  u32x4 bg[2], bu[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    bg[e] = bu[e] = u32x4{0u, 0u, 0u, 0u};
+    if (a.bg) bg[e] = load8<true>(a.bg, n + 8 * e, a.N);
+    if (a.bu) bu[e] = load8<true>(a.bu, n + 8 * e, a.N);
+  }
+  char* stage = lds + 6144 * wave;
+  auto slot = [&](int kind, int row, int piece) {
+    return reinterpret_cast<u32x4*>(stage + 2048 * kind + 64 * row + 16 * (piece ^ (row >> 4 & 1)));
+  };
+  with_act(a.act, [&](auto act) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float sg[8], su[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) sg[t] = g[i][8 * e + t], su[t] = u[i][8 * e + t];
+        const Results r = results8<act.value>(sg, su, bg[e], bu[e]);
+        const int row = L::a_row(lane & 31);
+        *slot(0, row, 2 * half + e) = r.y;
+        if (a.keep) *slot(1, row, 2 * half + e) = r.kg, *slot(2, row, 2 * half + e) = r.ku;
+      }
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int row = back + 16 * q, m = m0 + 32 * (wm + i) + row;
+        const u32x4 y = *slot(0, row, lane % 4);
+        u32x4 kg, ku;
+        if (a.keep) kg = *slot(1, row, lane % 4), ku = *slot(2, row, lane % 4);
+        if (m >= a.M || n_back >= a.N) continue;
+        *reinterpret_cast<u32x4*>(a.y + int64_t(m) * a.N + n_back) = y;
+        if (a.keep) {
+          // not read again before the backward
+          uint16_t* to = a.keep + int64_t(m) * 2 * a.N + n_back;
+          __builtin_nontemporal_store(kg, reinterpret_cast<u32x4*>(to));
+          __builtin_nontemporal_store(ku, reinterpret_cast<u32x4*>(to + a.N));
+        }
+      }
+    }
+  });
+}
+
+// How a backward is cut, and where its workspace holds what.
+struct BwdPlan {
+  bool tiled;
+  int32_t fn;          // columns of x a tile has, in 64s
+  int32_t splits;      // of the rows, for the weights' gradients
+  int64_t split_rows;
+  int64_t chunks;      // of kDzRows rows
+  size_t dz, part, part_b, wgrad, bytes;
+};
+constexpr int64_t kDwRows = 512;  // fewer rows: ngt_wgrad_bf16
+int plan_bwd(int64_t M, int32_t N, int32_t K, BwdPlan* p) {
+  p->tiled = tiled(N, K) && M >= kDwRows;
+  p->chunks = (M + kDzRows - 1) / kDzRows;
+  auto align = [](size_t b) { return (b + 255) & ~size_t(255); };
+  const size_t w = size_t(2) * N * K * sizeof(float);
+  p->dz = 0;
+  p->part = align(p->tiled ? DzBlocks(M, N).bytes() : size_t(M) * 2 * N * 2);
+  p->splits = 1, p->split_rows = M;
+  size_t ws = 0;
+  if (p->tiled) {
+    const GatedDwShape shape = gated_dw_shape(M, N, K);
+    p->fn = shape.fn;
+    const int64_t splits = shape.splits;
+    const int64_t stages = (M + kStage - 1) / kStage, per = (stages + splits - 1) / splits;
+    p->split_rows = per * kStage;
+    p->splits = static_cast<int32_t>((stages + per - 1) / per);
+  } else {
+    NGT_CHECK_OK(ngt_wgrad_workspace_bytes(M, 2 * N, K, &ws));
+  }
+  p->part_b = p->part + align(p->splits * w);
+  p->wgrad = p->part_b + align(size_t(p->chunks) * 2 * N * sizeof(float));
+  p->bytes = p->wgrad + ws;
+  return NGT_OK;
+}
+
 int check_sizes(const char* fn, int64_t M, int32_t N, int32_t K) {
   if (M < 0 || N < 1 || K < 1)
     return set_error(NGT_ERR_ARG, "%s: bad sizes rows=%lld n_out=%d n_in=%d", fn,
@@ -225,7 +498,8 @@ int check_sizes(const char* fn, int64_t M, int32_t N, int32_t K) {
   // 32-bit rows, and fewer than 2^24 blocks for each of the tile grids
   auto blocks = [](int64_t r, int64_t c, int t) { return (r + t - 1) / t * ((c + t - 1) / t); };
   constexpr int64_t kMost = (1 << 24) - 8;
-  if (M > (1 << 30) || N > (1 << 29) || blocks(M, N, 64) > kMost || blocks(M, K, 64) > kMost)
+  if (M > (1 << 30) || N > (1 << 29) || blocks(M, N, 64) > kMost || blocks(M, K, 64) > kMost ||
+      blocks(N, K, 32) > kMost)
     return set_error(NGT_ERR_UNSUPPORTED, "%s: rows=%lld n_out=%d n_in=%d exceed the grid", fn,
                      static_cast<long long>(M), N, K);
   return NGT_OK;
@@ -253,6 +527,14 @@ extern "C" int ngt_gated_fwd(const void* x, int64_t x_stride, const void* w_gate
               activation, 0, 0};
   hipStream_t st = static_cast<hipStream_t>(stream);
   KernelTimer timer_("gated_fwd", st);
+  if (tiled(n_out, n_in) && x_stride < kFar && x_stride % 8 == 0 && n_rows > 64 &&
+      all_aligned16({x, w_gate, w_up, b_gate, b_up, y, keep})) {
+    a.tiles_m = (a.M + 255) / 256, a.tiles_n = (a.N + 63) / 64;
+    const int64_t blocks = (int64_t(a.tiles_m) * a.tiles_n + 7) / 8 * 8;
+    hipLaunchKernelGGL(k_gated<4>, dim3(unsigned(blocks)), dim3(256), 0, st, a);
+    NGT_HIP_CHECK(hipGetLastError());
+    return NGT_OK;
+  }
   a.tiles_m = (a.M + 63) / 64, a.tiles_n = (a.N + 63) / 64;
   hipLaunchKernelGGL(k_gated_any, dim3(unsigned(int64_t(a.tiles_m) * a.tiles_n)), dim3(256), 0, st,
                      a);
@@ -262,37 +544,92 @@ extern "C" int ngt_gated_fwd(const void* x, int64_t x_stride, const void* w_gate
 
 extern "C" int ngt_gated_bwd_workspace_bytes(int64_t n_rows, int32_t n_out, int32_t n_in,
                                              size_t* bytes) {
-  NGT_CHECK_OK(check_sizes("ngt_gated_bwd_workspace_bytes", n_rows, n_out, n_in));
-  if (!bytes) return set_error(NGT_ERR_ARG, "ngt_gated_bwd_workspace_bytes: null bytes");
-  *bytes = 0;
+  const char* fn = "ngt_gated_bwd_workspace_bytes";
+  NGT_CHECK_OK(check_sizes(fn, n_rows, n_out, n_in));
+  if (!bytes) return set_error(NGT_ERR_ARG, "%s: null bytes", fn);
+  BwdPlan p;
+  NGT_CHECK_OK(plan_bwd(n_rows, n_out, n_in, &p));
+  *bytes = p.bytes;
   return NGT_OK;
 }
 
-extern "C" int ngt_gated_bwd(const void* dy, const void* keep, const void* w_gate,
+extern "C" int ngt_gated_bwd(const void* dy, const void* keep, const void* x, const void* w_gate,
                              const void* w_up, int64_t n_rows, int32_t n_out, int32_t n_in,
-                             void* dz, void* dx, void* workspace, size_t workspace_bytes,
+                             const ngt_gated_grads* grads, void* workspace, size_t workspace_bytes,
                              void* stream) {
   const char* fn = "ngt_gated_bwd";
   NGT_CHECK_OK(check_sizes(fn, n_rows, n_out, n_in));
-  if (n_rows == 0) return NGT_OK;
-  if (!dy || !keep || !dz) return set_error(NGT_ERR_ARG, "%s: null dy, keep or dz", fn);
-  if (dx && (!w_gate || !w_up)) return set_error(NGT_ERR_ARG, "%s: null w", fn);
+  if (!grads) return set_error(NGT_ERR_ARG, "%s: null grads", fn);
+  const ngt_gated_grads& g = *grads;
+  const bool want_w = g.dw_gate || g.dw_up, want_b = g.db_gate || g.db_up;
+  if (n_rows > 0 && (!dy || !keep)) return set_error(NGT_ERR_ARG, "%s: null dy or keep", fn);
+  if (n_rows > 0 && g.dx && (!w_gate || !w_up)) return set_error(NGT_ERR_ARG, "%s: null w", fn);
+  if (n_rows > 0 && want_w && !x) return set_error(NGT_ERR_ARG, "%s: null x", fn);
+  for (const auto& t : {std::pair<const void*, int32_t>(g.dw_gate, g.dw_gate_dtype),
+                        {g.dw_up, g.dw_up_dtype}, {g.db_gate, g.db_gate_dtype},
+                        {g.db_up, g.db_up_dtype}})
+    if (t.first && t.second != NGT_F32 && t.second != NGT_BF16)
+      return set_error(NGT_ERR_ARG, "%s: gradient dtype %d", fn, t.second);
+  if (!all_aligned16({dy, keep, x, w_gate, w_up, g.dx, g.dw_gate, g.dw_up}))
+    return set_error(NGT_ERR_ARG, "%s: matrices must be 16-byte aligned", fn);
+  BwdPlan p;
+  NGT_CHECK_OK(plan_bwd(n_rows, n_out, n_in, &p));
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes || !aligned16(workspace)))
+    return set_error(NGT_ERR_WORKSPACE, "%s: workspace %zu < %zu or not 16-byte aligned", fn,
+                     workspace_bytes, p.bytes);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  {
+  char* ws = static_cast<char*>(workspace);
+  auto* dz = reinterpret_cast<uint16_t*>(ws + p.dz);
+  auto* part = reinterpret_cast<float*>(ws + p.part);
+  auto* part_b = reinterpret_cast<float*>(ws + p.part_b);
+  const auto *wg = static_cast<const uint16_t*>(w_gate), *wu = static_cast<const uint16_t*>(w_up);
+  const auto M = static_cast<int32_t>(n_rows);
+  const GatedBwd products{dz, static_cast<const uint16_t*>(x), wg, wu, static_cast<uint16_t*>(g.dx),
+                          part, n_rows, p.split_rows, n_out, n_in, p.splits};
+  if (n_rows > 0) {
     KernelTimer timer_("gated_dz", st);
-    const int64_t blocks = (n_rows * ((n_out + 7) / 8) + 255) / 256;
-    hipLaunchKernelGGL(k_gated_dz, dim3(unsigned(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st,
+    const int32_t tiles_n = (n_out + 255) / 256;
+    hipLaunchKernelGGL(p.tiled ? &k_gated_dz<true> : &k_gated_dz<false>,
+                       dim3(unsigned(p.chunks * tiles_n)), dim3(256), 0, st,
                        static_cast<const uint16_t*>(dy), static_cast<const uint16_t*>(keep), n_rows,
-                       n_out, static_cast<uint16_t*>(dz));
+                       n_out, tiles_n, dz, want_b ? part_b : nullptr);
     NGT_HIP_CHECK(hipGetLastError());
   }
-  if (!dx) return NGT_OK;
-  KernelTimer timer_("gated_dx", st);
-  DxArgs a{static_cast<const uint16_t*>(dz), static_cast<const uint16_t*>(w_gate),
-           static_cast<const uint16_t*>(w_up), static_cast<uint16_t*>(dx),
-           static_cast<int32_t>(n_rows), n_out, n_in, (n_in + 63) / 64};
-  hipLaunchKernelGGL(k_gated_dx_any, dim3(unsigned((n_rows + 63) / 64 * a.tiles_k)), dim3(256), 0,
-                     st, a);
-  NGT_HIP_CHECK(hipGetLastError());
+  if (n_rows > 0 && g.dx) {
+    KernelTimer timer_("gated_dx", st);
+    if (p.tiled) {
+      NGT_CHECK_OK(launch_gated_dx(products, st));
+    } else {
+      DxArgs a{dz, wg, wu, static_cast<uint16_t*>(g.dx), M, n_out, n_in, (n_in + 63) / 64};
+      hipLaunchKernelGGL(k_gated_dx_any, dim3(unsigned((n_rows + 63) / 64 * a.tiles_k)), dim3(256),
+                         0, st, a);
+      NGT_HIP_CHECK(hipGetLastError());
+    }
+  }
+  int32_t splits = p.splits;
+  if (want_w && n_rows > 0) {
+    if (p.tiled) {
+      KernelTimer timer_("gated_dw", st);
+      NGT_CHECK_OK(launch_gated_dw(products, p.fn, st));
+    } else {
+      NGT_CHECK_OK(ngt_wgrad_bf16(x, dz, n_rows, 2 * n_out, n_in, part, nullptr, ws + p.wgrad,
+                                  p.bytes - p.wgrad, stream));
+    }
+  }
+  if (n_rows == 0) splits = 0;
+  if (want_w || want_b) {
+    KernelTimer timer_("gated_join", st);
+    JoinArgs j{};
+    j.part = part, j.part_b = part_b;
+    j.dw[0] = g.dw_gate, j.dw[1] = g.dw_up, j.db[0] = g.db_gate, j.db[1] = g.db_up;
+    j.dw_f32[0] = g.dw_gate_dtype == NGT_F32, j.dw_f32[1] = g.dw_up_dtype == NGT_F32;
+    j.db_f32[0] = g.db_gate_dtype == NGT_F32, j.db_f32[1] = g.db_up_dtype == NGT_F32;
+    j.nk = int64_t(n_out) * n_in, j.n = n_out, j.splits = splits;
+    j.chunks = static_cast<int32_t>(p.chunks);
+    j.blocks_w = want_w ? static_cast<int32_t>((2 * j.nk + 1023) / 1024) : 0;
+    const int blocks_b = want_b ? (2 * n_out + 31) / 32 : 0;
+    hipLaunchKernelGGL(k_gated_join, dim3(unsigned(j.blocks_w + blocks_b)), dim3(256), 0, st, j);
+    NGT_HIP_CHECK(hipGetLastError());
+  }
   return NGT_OK;
 }

@@ -60,6 +60,17 @@ __device__ __forceinline__ float half_of(const u32x4& v, int i) {
   return __uint_as_float((i & 1) ? (w & 0xffff0000u) : (w << 16));
 }
 
+// 64 pieces of a wave from memory to LDS, one after another from `at`.
+__device__ __forceinline__ void to_lds(packed::Buffer b, int offset, char* at) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      b, (__attribute__((address_space(3))) void*)at, 16, offset, 0, 0, 0);
+}
+// Until at most N of this wave's reads from memory are under way.
+template <int N>
+__device__ __forceinline__ void wait_for_all_but() {
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);
+}
+
 inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 }  // namespace

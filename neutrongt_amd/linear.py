@@ -411,7 +411,7 @@ GATES = {None: 0, "relu": 1, "gelu": 2, "silu": 3}
 
 class GatedLinearFunction(torch.autograd.Function):
     """act(x2 Wg^T + bg) * (x2 Wu^T + bu) of bf16 rows x2 [M, n_in] (ngt_gated_fwd /
-    ngt_gated_bwd / ngt_wgrad_bf16); the gradients of weights and biases come in
+    ngt_gated_bwd); the gradients of weights and biases come in
     their own type, from fp32 sums."""
 
     @staticmethod
@@ -440,27 +440,25 @@ class GatedLinearFunction(torch.autograd.Function):
         x2, wg, wu, keep = ctx.saved_tensors
         (m, n_in), n_out, dev = x2.shape, wg.shape[0], x2.device
         want_x, *want = ctx.needs_input_grad[:5]
-        g = gy.to(torch.bfloat16).contiguous()
-        dz = torch.empty(m, 2 * n_out, dtype=torch.bfloat16, device=dev)
+        g, xc, wg, wu = (t.contiguous() if t.data_ptr() % 16 == 0 else
+                         t.clone(memory_format=torch.contiguous_format)
+                         for t in (gy.to(torch.bfloat16), x2, wg, wu))
+        shapes = ((n_out, n_in),) * 2 + ((n_out,),) * 2
         dx = torch.empty(m, n_in, dtype=torch.bfloat16, device=dev) if want_x else None
+        grads = [torch.empty(s, dtype=d, device=dev) if w else None
+                 for s, d, w in zip(shapes, ctx.dtypes, want)]
+        out = _lib.GatedGradsC(dx.data_ptr() if want_x else None,
+                               *(t.data_ptr() if t is not None else None for t in grads),
+                               *(_lib.NGT_F32 if d == torch.float32 else _lib.NGT_BF16
+                                 for d in ctx.dtypes))
         nb = C.c_size_t()
         _lib.check(_lib.load().ngt_gated_bwd_workspace_bytes(m, n_out, n_in, C.byref(nb)))
-        ws = torch.empty(nb.value if want_x else 0, dtype=torch.uint8, device=dev)
+        ws = torch.empty(nb.value, dtype=torch.uint8, device=dev)
         with torch.cuda.device(dev):
             _lib.check(_lib.load().ngt_gated_bwd(
-                g.data_ptr(), keep.data_ptr(), wg.data_ptr(), wu.data_ptr(), m, n_out, n_in,
-                dz.data_ptr(), dx.data_ptr() if want_x else None,
-                ws.data_ptr() if want_x else None, ws.numel(), _lib.stream_ptr(dev)))
-            grads = [None] * 4
-            if want[0] or want[1]:
-                dw, db = linear_grads(x2, dz, want[2] or want[3])
-                grads[0], grads[1] = dw[:n_out], dw[n_out:]
-            elif want[2] or want[3]:
-                db = colsum_bf16(dz)
-            if want[2] or want[3]:
-                grads[2], grads[3] = db[:n_out], db[n_out:]
-        return (dx, *(t.to(d) if w else None for t, d, w in zip(grads, ctx.dtypes, want)), None,
-                None)
+                g.data_ptr(), keep.data_ptr(), xc.data_ptr(), wg.data_ptr(), wu.data_ptr(), m,
+                n_out, n_in, C.byref(out), ws.data_ptr(), nb.value, _lib.stream_ptr(dev)))
+        return (dx, *grads, None, None)
 
 
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,

@@ -79,11 +79,19 @@ def test_gated_refusals_touch_no_gpu():
     nb = C.c_size_t()
     assert lib.ngt_gated_bwd_workspace_bytes(4, 6, 8, C.byref(nb)) == 0
 
-    def bwd(dy=P, keep=P, wg=P, wu=P, dz=P, dx=P):
-        return lib.ngt_gated_bwd(dy, keep, wg, wu, 4, 6, 8, dz, dx, P, nb.value, None)
+    def bwd(dy=P, keep=P, x=P, wg=P, wu=P, ws=P, n=nb.value, grads=True, **kw):
+        g = _lib.GatedGradsC(P, P, P, P, P, 0, 1, 0, 1)
+        for name, v in kw.items():
+            setattr(g, name, v)
+        return lib.ngt_gated_bwd(dy, keep, x, wg, wu, 4, 6, 8, C.byref(g) if grads else None, ws, n,
+                                 None)
 
-    for bad in ("dy", "keep", "wg", "wu", "dz"):
-        assert bwd(**{bad: None}) == 1, bad
+    for bad, code in ((dict(dy=None), 1), (dict(keep=None), 1), (dict(x=None), 1), (dict(wg=None), 1),
+                      (dict(wu=None), 1), (dict(grads=False), 1), (dict(dw_gate_dtype=4), 1),
+                      (dict(db_up_dtype=-1), 1), (dict(dw_up=P + 8), 1), (dict(x=P + 2), 1),
+                      (dict(wu=P + 8), 1), (dict(dy=P + 2), 1), (dict(dx=P + 4), 1), (dict(ws=None), 4),
+                      (dict(n=nb.value - 1), 4), (dict(ws=P + 8), 4)):
+        assert bwd(**bad) == code, bad
         assert b"ngt_gated_bwd" in lib.ngt_last_error()
 
 

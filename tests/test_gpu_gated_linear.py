@@ -116,6 +116,12 @@ def test_tiles(dev, M, N, K, act, bias):
     _case(dev, M, N, K, act, bias, seed=N)
 
 
+@pytest.mark.parametrize("M,N,K", [(512, 72, 136), (513, 264, 520), (600, 8, 8), (5000, 136, 264),
+                                   (511, 264, 520), (70000, 40, 24), (777, 1000, 1288)])
+def test_gradients_of_whole_pieces_with_edges(dev, M, N, K):
+    _case(dev, M, N, K, "silu", seed=M)
+
+
 # a stage of the contraction, a part of one, several
 @pytest.mark.parametrize("K", [8, 56, 64, 72, 128, 192, 200, 256, 320, 456, 512])
 def test_lengths_of_the_contraction(dev, K):
@@ -147,6 +153,17 @@ def test_shapes_strides_and_alignment(dev):
     for v, a, b in ((wide[:, 8:72], joint[:48], joint[48:]), (odd, wg, wu),
                     (x.t().contiguous().t(), wg.t().contiguous().t(), wu)):
         assert (gated_linear(v, a, b, bg, bu).float() - want.float()).abs().max() <= tol
+    # the backward of weights and rows that are not aligned, in the tiled form too
+    for m in (60, 600):
+        x, wg, wu, _, _, gy = _inputs(m, 72, 64, False, m)
+        odd = [torch.empty(t.numel() + 1, dtype=BF16, device=dev)[1:].view(t.shape) for t in (x, wg, wu, gy)]
+        for o, t in zip(odd, (x, wg, wu, gy)):
+            o.copy_(t)
+        leaves = [t.requires_grad_() for t in odd[:3]]
+        y = gated_linear(*leaves)
+        _check([y.detach(), *torch.autograd.grad(y, leaves, odd[3])],
+               _ref(x, wg, wu, None, None, gy, "silu"), "odd")
+    x, wg, wu, bg, bu, _ = (t.to(dev) for t in _inputs(60, 48, 64, True, 4))
     same = gated_linear(x[:1].expand(60, 64), wg, wu, bg, bu)
     assert (same[3].float() - want[0].float()).abs().max() <= tol
 
