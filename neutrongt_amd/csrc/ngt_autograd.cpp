@@ -44,6 +44,7 @@
 #include <cmath>
 #include <map>
 #include <string>
+#include <unordered_set>
 
 #include "ngt_attn.h"
 
@@ -1162,9 +1163,14 @@ bool clip_type(const Tensor& t, const Tensor& like) {
 }
 
 // gradients.py's call: the norm, or nothing where one of its checks fails.
-std::optional<Tensor> clip_gradients(const std::vector<Tensor>& grads,
+std::optional<Tensor> clip_gradients(const std::vector<Tensor>& parameters,
                                      const std::optional<std::vector<Tensor>>& out,
                                      double max_norm) {
+  std::vector<Tensor> grads;
+  grads.reserve(parameters.size());
+  std::unordered_set<const void*> seen;
+  for (const Tensor& p : parameters)
+    if (p.grad().defined() && seen.insert(p.unsafeGetTensorImpl()).second) grads.push_back(p.grad());
   if (grads.empty() || !grads[0].is_cuda() || (out.has_value() && out->size() != grads.size()))
     return std::nullopt;
   const size_t n = grads.size();
@@ -1288,6 +1294,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "(q, k, q_gain, k_gain, positions, turns, interleaved, magnitude, eps) -> [q', k'] (or [q']) "
         "or None: rotary.py's NormRotaryFunction");
   m.def("clip_gradients", &clip_gradients,
-        "(gradients, results or None, max_norm; negative: the norm alone) -> norm or None: "
+        "(parameters, results or None, max_norm; negative: the norm alone) -> norm or None: "
         "gradients.py's call");
 }

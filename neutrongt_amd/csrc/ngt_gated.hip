@@ -153,6 +153,100 @@ __global__ __launch_bounds__(256) void k_gated_any(GatedArgs a) {
   }
 }
 
+// Few rows, aligned: a block is 16 NT outputs of both layers for up to 16 MT rows, its waves
+// every WAVES-th 64 of the contraction each, weights and rows straight from memory to
+// registers; their sums meet in LDS and are added in wave order.  Bound by the weights'
+// bytes, or, where those are few, by one wait for memory and the join.
+template <int MT, int NT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void k_gated_few(GatedArgs a) {
+  typedef float f32x4 __attribute__((ext_vector_type(4)));
+  constexpr int kTiles = 2 * NT * MT;
+  __shared__ __align__(16) float red[WAVES][kTiles][16][20];  // [x row][output], padded
+  const int lane = tid_x() & 63, wave = packed::wave_id(), quad = lane >> 4, l16 = lane & 15;
+  const int n0 = wg_x() * 16 * NT;
+  f32x4 acc[2][NT][MT];
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[p][j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // a row that is not there is the last one again: nobody reads what comes of it
+  const uint16_t *x[MT], *w[2][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) x[i] = a.x + min(16 * i + l16, a.M - 1) * a.x_stride;
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int64_t at = int64_t(min(n0 + 16 * j + l16, a.N - 1)) * a.K;
+    w[0][j] = a.wg + at, w[1][j] = a.wu + at;
+  }
+  struct Step {
+    u32x4 x[2][MT], w[2][2][NT];
+  };
+  auto fetch = [&](int k) {
+    Step s;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = k + 32 * h + 8 * quad;
+      const bool there = c < a.K;
+      auto read = [&](const uint16_t* row) {
+        return there ? *reinterpret_cast<const u32x4*>(row + c) : u32x4{0u, 0u, 0u, 0u};
+      };
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) s.w[h][p][j] = read(w[p][j]);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) s.x[h][i] = read(x[i]);
+    }
+    return s;
+  };
+  auto multiply = [&](const Step& s) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+            acc[p][j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                __builtin_bit_cast(packed::bf16x8, s.w[h][p][j]),
+                __builtin_bit_cast(packed::bf16x8, s.x[h][i]), acc[p][j][i], 0, 0, 0);
+  };
+  constexpr int kApart = 64 * WAVES;
+  Step now = fetch(64 * wave);
+  for (int k = 64 * wave; k < a.K; k += kApart) {
+    const Step next = fetch(k + kApart);
+    multiply(now);
+    now = next;
+  }
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        *reinterpret_cast<f32x4*>(&red[wave][(p * NT + j) * MT + i][l16][4 * quad]) = acc[p][j][i];
+  __syncthreads();
+  for (int e = tid_x(); e < 16 * MT * NT * 2; e += 64 * WAVES) {
+    const int m = e / (2 * NT), j = e % (2 * NT) / 2, half = e % 2;
+    if (m >= a.M) break;
+    float s[2][8];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) s[p][t] = 0.f;
+#pragma unroll
+      for (int v = 0; v < WAVES; ++v)
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+          s[p][t] += red[v][(p * NT + j) * MT + m / 16][m % 16][8 * half + t];
+    }
+    finish8(a, m, n0 + 16 * j + 8 * half, s[0], s[1]);
+  }
+}
+
 // dz = [dy keep_g | dy keep_u], and the biases' gradients: part_b[chunk][2 N], sums of the
 // unrounded products.  A block: 256 columns of kDzRows rows, 8 columns a thread.  BLOCKS: whole
 // pieces, and dz in DzBlocks, else [M, 2 N].
@@ -527,11 +621,35 @@ extern "C" int ngt_gated_fwd(const void* x, int64_t x_stride, const void* w_gate
               activation, 0, 0};
   hipStream_t st = static_cast<hipStream_t>(stream);
   KernelTimer timer_("gated_fwd", st);
-  if (tiled(n_out, n_in) && x_stride < kFar && x_stride % 8 == 0 && n_rows > 64 &&
+  if (n_in % 8 == 0 && x_stride % 8 == 0 && n_rows <= 64 && all_aligned16({x, w_gate, w_up})) {
+    auto run = [&](auto mt) {
+      constexpr int MT = decltype(mt)::value;
+      const int blocks = (n_out + 15) / 16;
+      if (blocks >= 512)
+        hipLaunchKernelGGL((k_gated_few<MT, 2, MT < 3 ? 8 : 4>), dim3(unsigned((n_out + 31) / 32)),
+                           dim3(MT < 3 ? 512 : 256), 0, st, a);
+      else
+        hipLaunchKernelGGL((k_gated_few<MT, 1, 8>), dim3(unsigned(blocks)), dim3(512), 0, st, a);
+    };
+    if (n_rows <= 16) run(std::integral_constant<int, 1>{});
+    else if (n_rows <= 32) run(std::integral_constant<int, 2>{});
+    else if (n_rows <= 48) run(std::integral_constant<int, 3>{});
+    else run(std::integral_constant<int, 4>{});
+    NGT_HIP_CHECK(hipGetLastError());
+    return NGT_OK;
+  }
+  if (tiled(n_out, n_in) && x_stride < kFar && x_stride % 8 == 0 &&
       all_aligned16({x, w_gate, w_up, b_gate, b_up, y, keep})) {
-    a.tiles_m = (a.M + 255) / 256, a.tiles_n = (a.N + 63) / 64;
-    const int64_t blocks = (int64_t(a.tiles_m) * a.tiles_n + 7) / 8 * 8;
-    hipLaunchKernelGGL(k_gated<4>, dim3(unsigned(blocks)), dim3(256), 0, st, a);
+    auto run = [&](auto fm) {
+      constexpr int FM = decltype(fm)::value;
+      a.tiles_m = (a.M + 64 * FM - 1) / (64 * FM), a.tiles_n = (a.N + 63) / 64;
+      const int64_t blocks = (int64_t(a.tiles_m) * a.tiles_n + 7) / 8 * 8;
+      hipLaunchKernelGGL(k_gated<FM>, dim3(unsigned(blocks)), dim3(256), 0, st, a);
+    };
+    const int64_t across = (n_out + 63) / 64;
+    if ((n_rows + 255) / 256 * across >= 384) run(std::integral_constant<int, 4>{});
+    else if ((n_rows + 127) / 128 * across >= 384) run(std::integral_constant<int, 2>{});
+    else run(std::integral_constant<int, 1>{});
     NGT_HIP_CHECK(hipGetLastError());
     return NGT_OK;
   }

@@ -170,7 +170,9 @@ int launch(const GatedBwd& g, hipStream_t st) {
   return NGT_OK;
 }
 
-// Blocks of 64 fn columns take fn units of time each; the rounds that 256 CUs need for them.
+// The rounds that 256 CUs need for so many blocks.  A stage of a block with 64 fn columns takes
+// about fn + 2 units of time (32,768 rows, 4,096 x 768: dx 1.31, 1.6, 1.76 us at fn = 2, 3, 4,
+// dw 1.12, 1.55, 1.85).
 int64_t rounds(int64_t blocks) { return (blocks + 255) / 256; }
 
 }  // namespace
@@ -179,7 +181,7 @@ int launch_gated_dx(const GatedBwd& g, hipStream_t st) {
   int best = 4;
   int64_t cost = INT64_MAX;
   for (int fn = 4; fn >= 2; --fn) {
-    const int64_t c = fn * rounds((g.M + 255) / 256 * ((g.K + 64 * fn - 1) / (64 * fn)));
+    const int64_t c = (fn + 2) * rounds((g.M + 255) / 256 * ((g.K + 64 * fn - 1) / (64 * fn)));
     if (c < cost) cost = c, best = fn;
   }
   return best == 4 ? launch<4, kDx>(g, st) : best == 3 ? launch<3, kDx>(g, st) : launch<2, kDx>(g, st);
@@ -195,7 +197,7 @@ GatedDwShape gated_dw_shape(int64_t M, int32_t N, int32_t K) {
     int64_t splits = 256 / tiles;
     if (splits > stages / 4) splits = stages / 4;
     if (splits < 1) splits = 1;
-    const int64_t c = fn * rounds(tiles * splits) * ((stages + splits - 1) / splits);
+    const int64_t c = (fn + 2) * rounds(tiles * splits) * ((stages + splits - 1) / splits);
     if (c < cost) cost = c, best = {fn, static_cast<int>(splits)};
   }
   return best;

@@ -50,19 +50,17 @@ def _check(t: torch.Tensor, name: str, dev) -> None:
 
 def _run(parameters, max_norm: float, out):
     params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    with_grad = [p for p in dict.fromkeys(params) if p.grad is not None]
-    grads = [p.grad for p in with_grad]
-    if out is not None:
-        out = list(out)
-        if len(out) != len(grads):
-            raise ValueError(f"{len(out)} results for {len(grads)} gradients")
+    out = list(out) if out is not None else None
+    ext = _lib.autograd_ext()
+    norm = ext and ext.clip_gradients(params, out, max_norm)
+    if norm is not None:
+        return norm
+    grads = [p.grad for p in dict.fromkeys(params) if p.grad is not None]
+    if out is not None and len(out) != len(grads):
+        raise ValueError(f"{len(out)} results for {len(grads)} gradients")
     if not grads:
         dev = params[0].device if params else torch.device("cuda", torch.cuda.current_device())
         return torch.zeros((), dtype=torch.float32, device=dev)
-    ext = _lib.autograd_ext()
-    norm = ext and ext.clip_gradients(grads, out, max_norm)
-    if norm is not None:
-        return norm
     dev = grads[0].device
     for i, g in enumerate(grads):
         _check(g, f"gradient {i}", dev)
