@@ -23,7 +23,10 @@ constexpr int kThreads = 256;
 constexpr int kMaxDim = 256;
 constexpr int64_t kMaxRows = int64_t(1) << 30;
 constexpr int kTableBytes = 16384;  // cosines and sines of a block's rows
-constexpr int kBwdBlocks = 1024;    // most blocks, so most partial sums, of a backward
+// About the most blocks, so partial sums, of a backward: five a CU is what its registers allow
+// (32,768 rows of 32 + 32 heads of 24, bf16: 1,024 blocks 82 us, 1,280 76, 2,048 84).
+constexpr int kBwdBlocks = 1280;
+inline size_t sums_bytes(int32_t d) { return size_t(kBwdBlocks + 2) * d * sizeof(float); }
 
 // One of queries and keys, as the kernels see it.
 struct Rows {
@@ -105,10 +108,28 @@ struct Chunk {
   }
 };
 
-// Sum over the 2^log adjacent lanes of a head, the same in all of them.
+// Sum over the 2^log adjacent lanes of a head, the same in all of them: within 16 lanes by
+// lane permutations of the addition itself (neighbours, pairs, halves of 8 and of 16 mirrored).
+template <int CTRL>
+__device__ __forceinline__ float add_lanes(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
 __device__ __forceinline__ float group_sum(float v, int log) {
-  for (int i = 0; i < log; ++i) v += shfl_xor(v, 1 << i);
+  if (log > 0) v = add_lanes<0xb1>(v);   // quad_perm 1 0 3 2
+  if (log > 1) v = add_lanes<0x4e>(v);   // quad_perm 2 3 0 1
+  if (log > 2) v = add_lanes<0x141>(v);  // row_half_mirror
+  if (log > 3) v = add_lanes<0x140>(v);  // row_mirror
+  if (log > 4) v += shfl_xor(v, 16);
+  if (log > 5) v += shfl_xor(v, 32);
   return v;
+}
+
+// 1 / sqrt(x): the instruction's result and a Newton step, within 1.5 half steps of fp32.
+__device__ __forceinline__ float inverse_root(float x) {
+  const float r = __builtin_amdgcn_rsqf(x);
+  const float e = fmaf(-x * r, r, 1.f);
+  // (0, infinities and NaN as they come: a step would make NaN of them)
+  return x > 1e-30f && x < 1e30f ? fmaf(0.5f * r, e, r) : 1.f / sqrtf(x);
 }
 
 // V pairs of components of each of a lane's U units; INTER: pairs are adjacent.
@@ -123,7 +144,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_rotary(const Args a) {
   const int pairs = a.dim / 2, lanes = 1 << a.group_log, groups = kThreads >> a.group_log;
   const int lane = tid & (lanes - 1), group = tid >> a.group_log;
   const bool norm = r.gain != nullptr;
-  const float by_d = 1.f / static_cast<float>(a.d);
+  const float by_d = 1.f / static_cast<float>(a.d), by_heads = 1.f / static_cast<float>(r.n_heads);
 
   // where this lane's units lie in a head
   int at[U][2], turn[U];
@@ -169,29 +190,42 @@ __global__ __launch_bounds__(kThreads) void k_norm_rotary(const Args a) {
     }
     __syncthreads();
     const int items = rows * r.n_heads, step = groups * r.splits;
-    for (int item = slot * groups + group; item < items; item += step) {
-      const int row = item / r.n_heads, head = item - row * r.n_heads;
+    // (below 2^17, so the quotient, half an item off the next whole number, is exact)
+    auto row_of = [&](int item) { return static_cast<int>((item + 0.5f) * by_heads); };
+    struct Head {
+      Chunk<T, V> x[U][2], g[U][2];
+    };
+    auto fetch = [&](int item) {
+      Head h;
+      const int row = row_of(item), head = item - row * r.n_heads;
       const T* x = static_cast<const T*>(r.x) + (row0 + row) * r.x_row + head * r.x_head;
-      const int64_t to = ((row0 + row) * r.n_heads + head) * a.d;
-      Chunk<T, V> xr[U][2], gr[U][2];
+      const T* g = static_cast<const T*>(r.dy) + (row0 + row) * r.dy_row + head * r.dy_head;
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          xr[u][c].zero();
-          if (there[u]) xr[u][c].load(x + at[u][c]);
-          if constexpr (BWD) {
-            gr[u][c].zero();
-            if (there[u])
-              gr[u][c].load(static_cast<const T*>(r.dy) + (row0 + row) * r.dy_row +
-                            head * r.dy_head + at[u][c]);
+          h.x[u][c].zero();
+          if (BWD) h.g[u][c].zero();
+          if (there[u] && item < items) {
+            h.x[u][c].load(x + at[u][c]);
+            if constexpr (BWD) h.g[u][c].load(g + at[u][c]);
           }
         }
+      return h;
+    };
+    // the next head is on its way while one is computed
+    int item = slot * groups + group;
+    Head next = fetch(item);
+    for (; item < items; item += step) {
+      const Head now = next;
+      next = fetch(item + step);
+      const int row = row_of(item), head = item - row * r.n_heads;
+      const int64_t to = ((row0 + row) * r.n_heads + head) * a.d;
       float v[U][2 * V];
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int i = 0; i < 2 * V; ++i) v[u][i] = xr[u][i / V].get(i % V);
+        for (int i = 0; i < 2 * V; ++i) v[u][i] = now.x[u][i / V].get(i % V);
       float scale = 1.f;
       if (norm) {
         float s = 0.f;
@@ -199,7 +233,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_rotary(const Args a) {
         for (int u = 0; u < U; ++u)
 #pragma unroll
           for (int i = 0; i < 2 * V; ++i) s = fmaf(v[u][i], v[u][i], s);
-        scale = 1.f / sqrtf(fmaf(group_sum(s, a.group_log), by_d, a.eps));
+        scale = inverse_root(fmaf(group_sum(s, a.group_log), by_d, a.eps));
       }
       float w[U][2 * V], dot = 0.f;
 #pragma unroll
@@ -208,7 +242,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_rotary(const Args a) {
         float in[2 * V];
 #pragma unroll
         for (int i = 0; i < 2 * V; ++i)
-          in[i] = BWD ? gr[u][i / V].get(i % V) : norm ? v[u][i] * scale * gain[u][i] : v[u][i];
+          in[i] = BWD ? now.g[u][i / V].get(i % V) : norm ? v[u][i] * scale * gain[u][i] : v[u][i];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           constexpr int kA = INTER ? 2 : 1, kB = INTER ? 1 : V;
@@ -386,11 +420,14 @@ int run(const char* fn, int dtype, const ngt_head_rows* q, const ngt_head_rows* 
     r.tile_rows = rows;
     const int64_t tiles = (n_rows + rows - 1) / rows;
     r.tiles = static_cast<int32_t>(tiles);
-    r.splits = 1;
+    // a backward's blocks by the tensors' work
+    const int all = h->n_heads + (in[1 - i] ? in[1 - i]->n_heads : 0);
+    int64_t most_blocks = BWD ? int64_t(kBwdBlocks) * h->n_heads / all : 1 << 20;
+    if (most_blocks < 1) most_blocks = 1;
     const int rounds = (rows * h->n_heads + groups - 1) / groups;
-    while (r.splits < rounds && tiles * r.splits < 512) ++r.splits;
+    r.splits = 1;
+    while (r.splits < rounds && r.splits < most_blocks && tiles * r.splits < 512) ++r.splits;
     int64_t n = tiles * r.splits;
-    const int64_t most_blocks = BWD ? kBwdBlocks / 2 : 1 << 20;
     if (n > most_blocks) n = most_blocks / r.splits * r.splits;
     r.blocks = static_cast<int32_t>(n);
     blocks += r.blocks;
@@ -446,7 +483,7 @@ extern "C" int ngt_norm_rotary_bwd_workspace_bytes(int64_t n_rows, int32_t d, si
   if (n_rows < 0 || n_rows > kMaxRows || d < 2 || d > kMaxDim || !bytes)
     return set_error(NGT_ERR_ARG, "%s: n_rows=%lld head_dim=%d", fn,
                      static_cast<long long>(n_rows), d);
-  *bytes = size_t(kBwdBlocks) * d * sizeof(float);
+  *bytes = sums_bytes(d);
   return NGT_OK;
 }
 
@@ -458,10 +495,10 @@ extern "C" int ngt_norm_rotary_bwd(int dtype, const ngt_head_rows* q, const ngt_
   NGT_CHECK_OK(check(fn, dtype, q, k, n_rows, d, rotation, eps, true));
   const bool sums = q->dgain || (k && k->dgain);
   if (sums && n_rows > 0 &&
-      (!workspace || workspace_bytes < size_t(kBwdBlocks) * d * sizeof(float) ||
+      (!workspace || workspace_bytes < sums_bytes(d) ||
        reinterpret_cast<uintptr_t>(workspace) % 16))
     return set_error(NGT_ERR_WORKSPACE, "%s: workspace %zu < %zu or not 16-byte aligned", fn,
-                     workspace_bytes, size_t(kBwdBlocks) * d * sizeof(float));
+                     workspace_bytes, sums_bytes(d));
   return run<true>(fn, dtype, q, k, n_rows, d, rotation, eps, workspace,
                    static_cast<hipStream_t>(stream));
 }

@@ -74,6 +74,12 @@ def test_rows(dev, n, dtype):
     _case(dev, n, 8, 2, 32, 32, "half", dtype, far=100, seed=n)
 
 
+@pytest.mark.parametrize("H,Hk", [(700, 1), (1, 700), (300, 300)])
+def test_many_heads(dev, H, Hk):
+    _case(dev, 3, H, Hk, 6, 2, "half", F32, far=9, seed=H)
+    _case(dev, 900, H, Hk, 8, 8, "half", BF16, far=9, seed=H)
+
+
 @pytest.mark.parametrize("n", [9000, 20011])
 def test_more_tiles_than_blocks_of_the_backward(dev, n):
     _case(dev, n, 4, 1, 16, 8, "interleaved", BF16, far=n, seed=n)
