@@ -83,10 +83,6 @@ struct Chunk {
       w[0] = *reinterpret_cast<const uint16_t*>(p);
     }
   }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (uint32_t& v : w) v = 0u;
-  }
   __device__ __forceinline__ float get(int i) const {
     if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
     return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
@@ -155,10 +151,11 @@ __global__ __launch_bounds__(kThreads) void k_norm_rotary(const Args a) {
     const int unit = lane * U + u;
     there[u] = unit < a.units;
     turned[u] = 2 * V * unit < a.dim;
-    turn[u] = turned[u] ? unit * V : 0;
+    turn[u] = turned[u] ? unit * V : 0;  // (its first pair)
     const bool apart = !INTER && turned[u];
-    at[u][0] = apart ? unit * V : 2 * V * unit;
-    at[u][1] = apart ? pairs + unit * V : 2 * V * unit + V;
+    // (a lane without a unit reads the first one again)
+    at[u][0] = !there[u] ? 0 : apart ? unit * V : 2 * V * unit;
+    at[u][1] = !there[u] ? V : apart ? pairs + unit * V : 2 * V * unit + V;
 #pragma unroll
     for (int i = 0; i < 2 * V; ++i) {
       gain[u][i] = 1.f;
@@ -197,6 +194,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_rotary(const Args a) {
     };
     auto fetch = [&](int item) {
       Head h;
+      item = min(item, items - 1);  // behind the last: that one again
       const int row = row_of(item), head = item - row * r.n_heads;
       const T* x = static_cast<const T*>(r.x) + (row0 + row) * r.x_row + head * r.x_head;
       const T* g = static_cast<const T*>(r.dy) + (row0 + row) * r.dy_row + head * r.dy_head;
@@ -204,12 +202,8 @@ __global__ __launch_bounds__(kThreads) void k_norm_rotary(const Args a) {
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          h.x[u][c].zero();
-          if (BWD) h.g[u][c].zero();
-          if (there[u] && item < items) {
-            h.x[u][c].load(x + at[u][c]);
-            if constexpr (BWD) h.g[u][c].load(g + at[u][c]);
-          }
+          h.x[u][c].load(x + at[u][c]);
+          if constexpr (BWD) h.g[u][c].load(g + at[u][c]);
         }
       return h;
     };
@@ -230,9 +224,12 @@ __global__ __launch_bounds__(kThreads) void k_norm_rotary(const Args a) {
       if (norm) {
         float s = 0.f;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) {
+          float q = 0.f;
 #pragma unroll
-          for (int i = 0; i < 2 * V; ++i) s = fmaf(v[u][i], v[u][i], s);
+          for (int i = 0; i < 2 * V; ++i) q = fmaf(v[u][i], v[u][i], q);
+          s += there[u] ? q : 0.f;
+        }
         scale = inverse_root(fmaf(group_sum(s, a.group_log), by_d, a.eps));
       }
       float w[U][2 * V], dot = 0.f;
@@ -244,11 +241,12 @@ __global__ __launch_bounds__(kThreads) void k_norm_rotary(const Args a) {
         for (int i = 0; i < 2 * V; ++i)
           in[i] = BWD ? now.g[u][i / V].get(i % V) : norm ? v[u][i] * scale * gain[u][i] : v[u][i];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          constexpr int kA = INTER ? 2 : 1, kB = INTER ? 1 : V;
-          const int ia = kA * j, ib = kA * j + kB;
-          w[u][ia] = in[ia], w[u][ib] = in[ib];
-          if (turned[u]) {
+        for (int i = 0; i < 2 * V; ++i) w[u][i] = in[i];
+        if (turned[u]) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            constexpr int kA = INTER ? 2 : 1, kB = INTER ? 1 : V;
+            const int ia = kA * j, ib = kA * j + kB;
             const float c = cs[j].x, s = BWD ? -cs[j].y : cs[j].y;
             w[u][ia] = fmaf(in[ia], c, -(in[ib] * s));
             w[u][ib] = fmaf(in[ia], s, in[ib] * c);
@@ -256,13 +254,15 @@ __global__ __launch_bounds__(kThreads) void k_norm_rotary(const Args a) {
         }
         if constexpr (BWD)
           if (norm) {
+            float q = 0.f;
 #pragma unroll
             for (int i = 0; i < 2 * V; ++i) {
               v[u][i] *= scale;
               acc[u][i] = fmaf(w[u][i], v[u][i], acc[u][i]);
               w[u][i] *= gain[u][i];
-              dot = fmaf(w[u][i], v[u][i], dot);
+              q = fmaf(w[u][i], v[u][i], q);
             }
+            dot += there[u] ? q : 0.f;
           }
       }
       if constexpr (BWD) {
