@@ -74,6 +74,7 @@ decltype(&ngt_packed_bwd) g_packed_bwd = nullptr;
 decltype(&ngt_linear_fwd) g_linear_fwd = nullptr;
 decltype(&ngt_linear_bwd_workspace_bytes) g_linear_bwd_ws = nullptr;
 decltype(&ngt_linear_bwd) g_linear_bwd = nullptr;
+decltype(&ngt_gated_keep_bytes) g_gated_keep = nullptr;
 decltype(&ngt_gated_fwd) g_gated_fwd = nullptr;
 decltype(&ngt_gated_bwd_workspace_bytes) g_gated_bwd_ws = nullptr;
 decltype(&ngt_gated_bwd) g_gated_bwd = nullptr;
@@ -900,7 +901,11 @@ GatedForward gated_forward(const Tensor& x, const Tensor& w_gate, const Tensor& 
   auto shape = x.sizes().vec();
   shape.back() = n_out;
   r.y = at::empty(shape, r.x2.options());
-  if (want_grad) r.keep = at::empty({m, 2 * n_out}, r.x2.options());
+  if (want_grad) {
+    size_t bytes = 0;
+    check(g_gated_keep(m, static_cast<int32_t>(n_out), &bytes));
+    r.keep = workspace(static_cast<int64_t>(bytes), r.x2);
+  }
   check(g_gated_fwd(r.x2.data_ptr(), m > 1 ? r.x2.stride(0) : n_in, r.wg.data_ptr(),
                     r.wu.data_ptr(), bg.defined() ? bg.data_ptr() : nullptr,
                     bu.defined() ? bu.data_ptr() : nullptr, m, static_cast<int32_t>(n_out),
@@ -1253,6 +1258,7 @@ void init(const std::map<std::string, int64_t>& addr) {
   entry(g_linear_fwd, addr, "ngt_linear_fwd");
   entry(g_linear_bwd_ws, addr, "ngt_linear_bwd_workspace_bytes");
   entry(g_linear_bwd, addr, "ngt_linear_bwd");
+  entry(g_gated_keep, addr, "ngt_gated_keep_bytes");
   entry(g_gated_fwd, addr, "ngt_gated_fwd");
   entry(g_gated_bwd_ws, addr, "ngt_gated_bwd_workspace_bytes");
   entry(g_gated_bwd, addr, "ngt_gated_bwd");

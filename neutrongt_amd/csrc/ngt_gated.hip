@@ -1,8 +1,8 @@
 // Gated linear layer, bf16: y = act(x Wg^T + bg) * (x Wu^T + bu), fp32 inside, and its
-// backward up to the weights' gradients (ngt_wgrad.hip):
-//   keep = [zu act'(zg) | act(zg)],  dz = [dzg | dzu] = dy * keep,  dx = dzg Wg + dzu Wu.
-// The forward keeps the two factors of dy instead of zg and zu, so that the backward
-// forms no activation; either way two roundings to bf16 stand between dy and dz.
+// backward:
+//   dzg = dy zu act'(zg), dzu = dy act(zg);  dx = dzg Wg + dzu Wu,  dW = dz^T x,  db = sums of dz.
+// The forward keeps the two factors of dy instead of zg and zu (Keep, ngt_gated.h), so
+// that the backward forms no activation.
 #include "ngt_gated.h"
 
 #include <utility>
@@ -17,7 +17,7 @@ struct GatedArgs {
   const uint16_t* bg;  // [N] or null
   const uint16_t* bu;
   uint16_t* y;         // [M, N]
-  uint16_t* keep;      // [M, 2 N] or null
+  void* keep;          // Keep, or null
   int64_t x_stride;
   int32_t M, N, K, act;
   int32_t tiles_m, tiles_n;
@@ -42,23 +42,37 @@ __device__ __forceinline__ Gate gate_of(float z) {
   return {z, 1.f};
 }
 
-// f with the activation as a constant.
+// f with the activation, and whether the backward's factors are wanted, as constants.
 template <typename F>
-__device__ __forceinline__ void with_act(int act, F f) {
-  if (act == NGT_ACT_SILU) f(std::integral_constant<int, NGT_ACT_SILU>{});
-  else if (act == NGT_ACT_GELU) f(std::integral_constant<int, NGT_ACT_GELU>{});
-  else if (act == NGT_ACT_RELU) f(std::integral_constant<int, NGT_ACT_RELU>{});
-  else f(std::integral_constant<int, NGT_ACT_NONE>{});
+__device__ __forceinline__ void with_act(int act, bool keep, F f) {
+  auto go = [&](auto a) {
+    if (keep) f(a, std::true_type{});
+    else f(a, std::false_type{});
+  };
+  if (act == NGT_ACT_SILU) go(std::integral_constant<int, NGT_ACT_SILU>{});
+  else if (act == NGT_ACT_GELU) go(std::integral_constant<int, NGT_ACT_GELU>{});
+  else if (act == NGT_ACT_RELU) go(std::integral_constant<int, NGT_ACT_RELU>{});
+  else go(std::integral_constant<int, NGT_ACT_NONE>{});
 }
 
 // Pieces of 8 results and, for the backward, of what it keeps, from their sums.
 struct Results {
   u32x4 y, kg, ku;
+  uint32_t lg, lu;
 };
-template <int ACT>
+// Two fp32 to 20 bits each, rounded to the nearest: the upper halves together, the 4 bits
+// behind them at bits `at` and `at` + 4 of low.  (A NaN stays one: no sum of bf16 products has
+// all its lower bits set.)
+__device__ __forceinline__ uint32_t keep2(float a, float b, int at, uint32_t& low) {
+  const uint32_t u = __float_as_uint(a) + 0x800u, v = __float_as_uint(b) + 0x800u;
+  low |= (u >> 12 & 15u) << at | (v >> 12 & 15u) << (at + 4);
+  return __builtin_amdgcn_perm(v, u, 0x07060302u);
+}
+template <int ACT, bool KEEP>
 __device__ __forceinline__ Results results8(const float (&sg)[8], const float (&su)[8],
                                             const u32x4& bg, const u32x4& bu) {
   Results r;
+  r.lg = r.lu = 0u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float v[2], g[2], u[2];
@@ -69,8 +83,10 @@ __device__ __forceinline__ Results results8(const float (&sg)[8], const float (&
       v[t] = q.value * zu, g[t] = zu * q.slope, u[t] = q.value;
     }
     r.y[i] = pack2_bf16(v[0], v[1]);
-    r.kg[i] = pack2_bf16(g[0], g[1]);
-    r.ku[i] = pack2_bf16(u[0], u[1]);
+    if constexpr (KEEP) {
+      r.kg[i] = keep2(g[0], g[1], 8 * i, r.lg);
+      r.ku[i] = keep2(u[0], u[1], 8 * i, r.lu);
+    }
   }
   return r;
 }
@@ -85,7 +101,7 @@ __device__ __forceinline__ void store8(uint16_t* row, int c, int n, const u32x4&
   }
 }
 
-// 8 outputs n .. n+7 of row m from their sums.
+// 8 outputs n .. n+7 (n a multiple of 8) of row m from their sums.
 __device__ __forceinline__ void finish8(const GatedArgs& a, int m, int n, const float (&sg)[8],
                                         const float (&su)[8]) {
   if (m >= a.M || n >= a.N) return;
@@ -93,12 +109,16 @@ __device__ __forceinline__ void finish8(const GatedArgs& a, int m, int n, const 
   if (a.bg) bg = load8<false>(a.bg, n, a.N);
   if (a.bu) bu = load8<false>(a.bu, n, a.N);
   Results r;
-  with_act(a.act, [&](auto act) { r = results8<act.value>(sg, su, bg, bu); });
+  with_act(a.act, a.keep != nullptr, [&](auto act, auto keep) {
+    r = results8<act.value, keep.value>(sg, su, bg, bu);
+  });
   store8(a.y + int64_t(m) * a.N, n, a.N, r.y);
   if (a.keep) {
-    uint16_t* row = a.keep + int64_t(m) * 2 * a.N;
-    store8(row, n, a.N, r.kg);
-    store8(row + a.N, n, a.N, r.ku);
+    const Keep k(a.M, a.N);
+    store8(k.high(a.keep, m, 0), n, a.N, r.kg);
+    store8(k.high(a.keep, m, 1), n, a.N, r.ku);
+    *k.low(a.keep, m, 0, n) = r.lg;
+    *k.low(a.keep, m, 1, n) = r.lu;
   }
 }
 
@@ -247,13 +267,13 @@ __global__ __launch_bounds__(64 * WAVES) void k_gated_few(GatedArgs a) {
   }
 }
 
-// dz = [dy keep_g | dy keep_u], and the biases' gradients: part_b[chunk][2 N], sums of the
+// dz = [dzg | dzu], and the biases' gradients: part_b[chunk][2 N], sums of the
 // unrounded products.  A block: 256 columns of kDzRows rows, 8 columns a thread.  BLOCKS: whole
 // pieces, and dz in DzBlocks, else [M, 2 N].
 constexpr int kDzRows = 128;
 template <bool BLOCKS>
 __global__ __launch_bounds__(256) void k_gated_dz(const uint16_t* __restrict__ dy,
-                                                  const uint16_t* __restrict__ keep, int64_t rows,
+                                                  void* keep, int64_t rows,
                                                   int32_t n, int32_t tiles_n,
                                                   uint16_t* __restrict__ dz,
                                                   float* __restrict__ part_b) {
@@ -262,6 +282,7 @@ __global__ __launch_bounds__(256) void k_gated_dz(const uint16_t* __restrict__ d
   const int cg = tid_x() & 31, lane = tid_x() >> 5;
   const int c = (wg_x() - static_cast<int>(chunk) * tiles_n) * 256 + 8 * cg;
   const DzBlocks blocks(rows, n);
+  const Keep kept(rows, n);
   const int64_t end = BLOCKS ? blocks.row_blocks * 32 : rows;  // of what is written
   const int64_t r0 = chunk * kDzRows, r1 = r0 + kDzRows < end ? r0 + kDzRows : end;
   float sum[2][8];
@@ -273,16 +294,18 @@ __global__ __launch_bounds__(256) void k_gated_dz(const uint16_t* __restrict__ d
 #pragma unroll 2
     for (int64_t row = r0 + lane; row < r1; row += 8) {
       u32x4 g = {0u, 0u, 0u, 0u}, v[2] = {g, g};
+      uint32_t low[2] = {0u, 0u};
       if (!BLOCKS || (row < rows && c < n)) {
         g = load8<BLOCKS>(dy + row * n, c, n);
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          const uint16_t* from = keep + (2 * row + p) * n;
+          const uint16_t* from = kept.high(keep, row, p);
           // the last time that it is read
           if constexpr (BLOCKS)
             v[p] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(from + c));
           else
             v[p] = load8<false>(from, c, n);
+          low[p] = *kept.low(keep, row, p, c);
         }
       }
 #pragma unroll
@@ -290,8 +313,9 @@ __global__ __launch_bounds__(256) void k_gated_dz(const uint16_t* __restrict__ d
         u32x4 o;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const float lo = half_of(g, 2 * t) * half_of(v[p], 2 * t);
-          const float hi = half_of(g, 2 * t + 1) * half_of(v[p], 2 * t + 1);
+          const float k0 = __uint_as_float(v[p][t] << 16 | (low[p] >> (8 * t) & 15u) << 12);
+          const float k1 = __uint_as_float((v[p][t] & 0xffff0000u) | (low[p] >> (8 * t + 4) & 15u) << 12);
+          const float lo = half_of(g, 2 * t) * k0, hi = half_of(g, 2 * t + 1) * k1;
           sum[p][2 * t] += lo, sum[p][2 * t + 1] += hi;
           o[t] = pack2_bf16(lo, hi);
         }
@@ -451,7 +475,7 @@ __global__ __launch_bounds__(256) void k_gated_dx_any(DxArgs a) {
 template <int FM>
 __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
   constexpr int BM = 64 * FM, kRowsBytes = BM * 128;
-  __shared__ __align__(16) char lds[kRowsBytes + 128 * 128];
+  __shared__ __align__(16) char lds[kRowsBytes + 128 * 128];  // (6 KB a wave for the results)
   const int lane = tid_x() & 63, wave = packed::wave_id(), half = lane >> 5;
   const TileAt at = tile_at(a.tiles_m, a.tiles_n, 1);
   if (!at.there) return;  // block-uniform
@@ -518,32 +542,42 @@ __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
   auto slot = [&](int kind, int row, int piece) {
     return reinterpret_cast<u32x4*>(stage + 2048 * kind + 64 * row + 16 * (piece ^ (row >> 4 & 1)));
   };
-  with_act(a.act, [&](auto act) {
+  const Keep kept(a.M, a.N);
+  with_act(a.act, a.keep != nullptr, [&](auto act, auto keep) {
+    constexpr bool KEEP = decltype(keep)::value;
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
+      const int row = L::a_row(lane & 31), m = m0 + 32 * (wm + i) + row;
+      uint2 lg, lu;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float sg[8], su[8];
 #pragma unroll
         for (int t = 0; t < 8; ++t) sg[t] = g[i][8 * e + t], su[t] = u[i][8 * e + t];
-        const Results r = results8<act.value>(sg, su, bg[e], bu[e]);
-        const int row = L::a_row(lane & 31);
+        const Results r = results8<act.value, KEEP>(sg, su, bg[e], bu[e]);
         *slot(0, row, 2 * half + e) = r.y;
-        if (a.keep) *slot(1, row, 2 * half + e) = r.kg, *slot(2, row, 2 * half + e) = r.ku;
+        if constexpr (KEEP) {
+          *slot(1, row, 2 * half + e) = r.kg, *slot(2, row, 2 * half + e) = r.ku;
+          (e ? lg.y : lg.x) = r.lg, (e ? lu.y : lu.x) = r.lu;
+        }
       }
+      if constexpr (KEEP)
+        if (m < a.M && n < a.N) {  // (both words are there, whatever N)
+          *reinterpret_cast<uint2*>(kept.low(a.keep, m, 0, n)) = lg;
+          *reinterpret_cast<uint2*>(kept.low(a.keep, m, 1, n)) = lu;
+        }
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const int row = back + 16 * q, m = m0 + 32 * (wm + i) + row;
-        const u32x4 y = *slot(0, row, lane % 4);
+        const int r_back = back + 16 * q, m_back = m0 + 32 * (wm + i) + r_back;
+        const u32x4 y = *slot(0, r_back, lane % 4);
         u32x4 kg, ku;
-        if (a.keep) kg = *slot(1, row, lane % 4), ku = *slot(2, row, lane % 4);
-        if (m >= a.M || n_back >= a.N) continue;
-        *reinterpret_cast<u32x4*>(a.y + int64_t(m) * a.N + n_back) = y;
-        if (a.keep) {
+        if constexpr (KEEP) kg = *slot(1, r_back, lane % 4), ku = *slot(2, r_back, lane % 4);
+        if (m_back >= a.M || n_back >= a.N) continue;
+        *reinterpret_cast<u32x4*>(a.y + int64_t(m_back) * a.N + n_back) = y;
+        if constexpr (KEEP) {
           // not read again before the backward
-          uint16_t* to = a.keep + int64_t(m) * 2 * a.N + n_back;
-          __builtin_nontemporal_store(kg, reinterpret_cast<u32x4*>(to));
-          __builtin_nontemporal_store(ku, reinterpret_cast<u32x4*>(to + a.N));
+          __builtin_nontemporal_store(kg, reinterpret_cast<u32x4*>(kept.high(a.keep, m_back, 0) + n_back));
+          __builtin_nontemporal_store(ku, reinterpret_cast<u32x4*>(kept.high(a.keep, m_back, 1) + n_back));
         }
       }
     }
@@ -604,6 +638,13 @@ int check_sizes(const char* fn, int64_t M, int32_t N, int32_t K) {
 
 using namespace ngt;
 
+extern "C" int ngt_gated_keep_bytes(int64_t n_rows, int32_t n_out, size_t* bytes) {
+  NGT_CHECK_OK(check_sizes("ngt_gated_keep_bytes", n_rows, n_out, 1));
+  if (!bytes) return set_error(NGT_ERR_ARG, "ngt_gated_keep_bytes: null bytes");
+  *bytes = static_cast<size_t>(Keep(n_rows, n_out).bytes());
+  return NGT_OK;
+}
+
 extern "C" int ngt_gated_fwd(const void* x, int64_t x_stride, const void* w_gate, const void* w_up,
                              const void* b_gate, const void* b_up, int64_t n_rows, int32_t n_out,
                              int32_t n_in, int32_t activation, void* y, void* keep, void* stream) {
@@ -614,11 +655,11 @@ extern "C" int ngt_gated_fwd(const void* x, int64_t x_stride, const void* w_gate
   if (n_rows == 0) return NGT_OK;
   if (!x || !w_gate || !w_up || !y) return set_error(NGT_ERR_ARG, "%s: null x, w or y", fn);
   if (x_stride < n_in) return set_error(NGT_ERR_ARG, "%s: x rows overlap", fn);
+  if (!aligned16(keep)) return set_error(NGT_ERR_ARG, "%s: keep must be 16-byte aligned", fn);
   GatedArgs a{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(w_gate),
               static_cast<const uint16_t*>(w_up), static_cast<const uint16_t*>(b_gate),
               static_cast<const uint16_t*>(b_up), static_cast<uint16_t*>(y),
-              static_cast<uint16_t*>(keep), x_stride, static_cast<int32_t>(n_rows), n_out, n_in,
-              activation, 0, 0};
+              keep, x_stride, static_cast<int32_t>(n_rows), n_out, n_in, activation, 0, 0};
   hipStream_t st = static_cast<hipStream_t>(stream);
   KernelTimer timer_("gated_fwd", st);
   if (n_in % 8 == 0 && x_stride % 8 == 0 && n_rows <= 64 && all_aligned16({x, w_gate, w_up})) {
@@ -709,8 +750,8 @@ extern "C" int ngt_gated_bwd(const void* dy, const void* keep, const void* x, co
     const int32_t tiles_n = (n_out + 255) / 256;
     hipLaunchKernelGGL(p.tiled ? &k_gated_dz<true> : &k_gated_dz<false>,
                        dim3(unsigned(p.chunks * tiles_n)), dim3(256), 0, st,
-                       static_cast<const uint16_t*>(dy), static_cast<const uint16_t*>(keep), n_rows,
-                       n_out, tiles_n, dz, want_b ? part_b : nullptr);
+                       static_cast<const uint16_t*>(dy), const_cast<void*>(keep), n_rows, n_out,
+                       tiles_n, dz, want_b ? part_b : nullptr);
     NGT_HIP_CHECK(hipGetLastError());
   }
   if (n_rows > 0 && g.dx) {

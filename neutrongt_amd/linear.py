@@ -422,7 +422,11 @@ class GatedLinearFunction(torch.autograd.Function):
         bg, bu = (b.to(torch.bfloat16).contiguous() if b is not None else None
                   for b in (b_gate, b_up))
         y = torch.empty(m, n_out, dtype=torch.bfloat16, device=dev)
-        keep = torch.empty(m, 2 * n_out, dtype=torch.bfloat16, device=dev) if want_grad else None
+        keep = None
+        if want_grad:
+            nb = C.c_size_t()
+            _lib.check(_lib.load().ngt_gated_keep_bytes(m, n_out, C.byref(nb)))
+            keep = torch.empty(nb.value, dtype=torch.uint8, device=dev)
         with torch.cuda.device(dev):
             _lib.check(_lib.load().ngt_gated_fwd(
                 x2.data_ptr(), x2.stride(0) if m > 1 else n_in, wg.data_ptr(), wu.data_ptr(),

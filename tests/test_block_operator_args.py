@@ -66,17 +66,20 @@ def test_norm_rotary_refusals_touch_no_gpu():
 def test_gated_refusals_touch_no_gpu():
     lib = _lib.load()
 
-    def fwd(x=P, xs=8, wg=P, wu=P, rows=4, n_out=6, n_in=8, act=3, y=P):
-        return lib.ngt_gated_fwd(x, xs, wg, wu, None, None, rows, n_out, n_in, act, y, None, None)
+    def fwd(x=P, xs=8, wg=P, wu=P, rows=4, n_out=6, n_in=8, act=3, y=P, keep=None):
+        return lib.ngt_gated_fwd(x, xs, wg, wu, None, None, rows, n_out, n_in, act, y, keep, None)
 
     for bad, code in ((dict(rows=-1), 1), (dict(n_out=0), 1), (dict(n_in=0), 1), (dict(act=4), 1),
                       (dict(act=-1), 1), (dict(x=None), 1), (dict(wg=None), 1), (dict(wu=None), 1),
-                      (dict(y=None), 1), (dict(xs=7), 1), (dict(rows=(1 << 30) + 1), 2),
-                      (dict(rows=1 << 30, n_out=1 << 12), 2), (dict(n_out=(1 << 29) + 1), 2)):
+                      (dict(y=None), 1), (dict(xs=7), 1), (dict(keep=P + 8), 1),
+                      (dict(rows=(1 << 30) + 1), 2), (dict(rows=1 << 30, n_out=1 << 12), 2),
+                      (dict(n_out=(1 << 29) + 1), 2)):
         assert fwd(**bad) == code, bad
         assert b"ngt_gated_fwd" in lib.ngt_last_error()
     assert fwd(rows=0, x=None, y=None) == 0
     nb = C.c_size_t()
+    assert lib.ngt_gated_keep_bytes(4, 6, C.byref(nb)) == 0 and nb.value >= 4 * 6 * 2 * 2
+    assert lib.ngt_gated_keep_bytes(-1, 6, C.byref(nb)) == 1
     assert lib.ngt_gated_bwd_workspace_bytes(4, 6, 8, C.byref(nb)) == 0
 
     def bwd(dy=P, keep=P, x=P, wg=P, wu=P, ws=P, n=nb.value, grads=True, **kw):

@@ -8,7 +8,8 @@ bf16's), a sum of n of them is off by at most n u of their absolute values.
   slope: act'(zg): 0.8 e_g (no second derivative is larger) + 16 u (1 + |zg|); relu's may
          differ where |zg| <= e_g
   y:     |zu| e_a + (|a| + e_a) e_u + 2 u |y|, then h |y|
-  kept:  zu slope and a, the same way, each rounded to bf16; dz = dy times them, rounded
+  kept:  zu slope and a, the same way, each rounded to 12 bits of mantissa, off by at
+         most k = 2^-12 of itself; dz = dy times them, rounded to bf16
   dx, dw, db: sums of dz's error and n u of the terms, then h (bf16) or nothing"""
 import math
 
@@ -19,7 +20,7 @@ from neutrongt_amd import _lib, gated_linear
 from neutrongt_amd.linear import GATES
 
 pytestmark = pytest.mark.gpu
-U, HB = 2.0 ** -24, 2.0 ** -8
+U, HB, HK = 2.0 ** -24, 2.0 ** -8, 2.0 ** -12
 BF16, F32 = torch.bfloat16, torch.float32
 
 
@@ -48,13 +49,13 @@ def _ref(x, wg, wu, bg, bu, gy, act, w_type=BF16):
     ea = 1.13 * eg + 8 * U * (zg.abs() + a.abs())
     es = ((zg.abs() <= eg).double() if act == "relu" else
           0.8 * eg + 16 * U * (1 + zg.abs()) if act else torch.zeros_like(zg))
-    up = lambda v, e: e + HB * (v.abs() + e)
+    up = lambda v, e, half=HB: e + half * (v.abs() + e)
     y = a * zu
     ey = zu.abs() * ea + (a.abs() + ea) * eu + 2 * U * y.abs()
     out = [(y, up(y, ey))]
     kg = zu * s
-    ekg = up(kg, zu.abs() * es + (s.abs() + es) * eu + 2 * U * kg.abs())
-    dzs = [(gy * v, up(gy * v, gy.abs() * e)) for v, e in ((kg, ekg), (a, up(a, ea)))]
+    ekg = up(kg, zu.abs() * es + (s.abs() + es) * eu + 2 * U * kg.abs(), HK)
+    dzs = [(gy * v, up(gy * v, gy.abs() * e)) for v, e in ((kg, ekg), (a, up(a, ea, HK)))]
     dx = dzs[0][0] @ wg + dzs[1][0] @ wu
     e = sum(ez @ w.abs() + (2 * N + 2) * U * (z.abs() @ w.abs())
             for (z, ez), w in zip(dzs, (wg, wu)))
