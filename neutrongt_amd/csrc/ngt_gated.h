@@ -33,8 +33,7 @@ struct Keep {
 // dz as the tiled products read it: blocks of 32 rows by 64 columns, 4 KB each, one after
 // another along the columns of dzg and then of dzu, each layer's columns filled up with zeros
 // to whole blocks and the rows to whole stages.  What a product brings to LDS at a time
-// lies together in memory whether it takes dz by rows or by columns (rows of 2 N elements:
-// dx 221 us instead of 203 for 32,768 x 4,096 x 768).
+// lies together in memory, whole and without masks, whether it takes dz by rows or by columns.
 struct DzBlocks {
   int64_t row_blocks;
   int32_t per_layer;  // blocks along a layer's columns
@@ -43,25 +42,28 @@ struct DzBlocks {
   __host__ __device__ int64_t bytes() const { return row_blocks * across() * 4096; }
 };
 
-// Backward products, aligned sizes (ngt_gated_bwd.hip): dx = dzg Wg + dzu Wu, and
-// part[split][2 N][K] = dz^T x over the split's rows.
+// Backward products, aligned sizes (ngt_gated_bwd.hip): dx = dzg Wg + dzu Wu, or, with the
+// contraction split, parts of it, and dW = dz^T x, or parts of it over splits of the rows.
 struct GatedBwd {
   const uint16_t* dz;  // DzBlocks
   const uint16_t* x;   // [M, K]
   const uint16_t* wg;  // [N, K]
   const uint16_t* wu;
   uint16_t* dx;        // [M, K]
-  float* part;
-  int64_t M, split_rows;
-  int32_t N, K, splits;
+  void* dw[2];         // [N, K], where there is one split
+  float* part;         // [splits][M][K] of dx, [splits][2 N][K] of dW
+  int64_t M;
+  int32_t N, K;
+  int32_t dw_f32[2];
 };
-// The columns of an x tile, in 64s (2 to 4), and the splits of the rows.
-struct GatedDwShape {
-  int fn, splits;
+// A product's blocks: 64 fn columns each, and so many splits of `per_split` stages.
+struct GatedShape {
+  int32_t fn, splits, per_split;
 };
-GatedDwShape gated_dw_shape(int64_t M, int32_t N, int32_t K);
-int launch_gated_dx(const GatedBwd& g, hipStream_t st);
-int launch_gated_dw(const GatedBwd& g, int fn, hipStream_t st);
+GatedShape gated_dx_shape(int64_t M, int32_t N, int32_t K);
+GatedShape gated_dw_shape(int64_t M, int32_t N, int32_t K);
+int launch_gated_dx(const GatedBwd& g, const GatedShape& s, hipStream_t st);
+int launch_gated_dw(const GatedBwd& g, const GatedShape& s, hipStream_t st);
 
 namespace {
 

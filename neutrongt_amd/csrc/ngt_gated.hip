@@ -268,13 +268,12 @@ __global__ __launch_bounds__(64 * WAVES) void k_gated_few(GatedArgs a) {
 }
 
 // dz = [dzg | dzu], and the biases' gradients: part_b[chunk][2 N], sums of the
-// unrounded products.  A block: 256 columns of kDzRows rows, 8 columns a thread.  BLOCKS: whole
+// unrounded products.  A block: 256 columns of chunk_rows rows, 8 columns a thread.  BLOCKS: whole
 // pieces, and dz in DzBlocks, else [M, 2 N].
-constexpr int kDzRows = 128;
 template <bool BLOCKS>
 __global__ __launch_bounds__(256) void k_gated_dz(const uint16_t* __restrict__ dy,
                                                   void* keep, int64_t rows,
-                                                  int32_t n, int32_t tiles_n,
+                                                  int32_t n, int32_t tiles_n, int32_t chunk_rows,
                                                   uint16_t* __restrict__ dz,
                                                   float* __restrict__ part_b) {
   __shared__ float red[2][8][256];
@@ -284,7 +283,7 @@ __global__ __launch_bounds__(256) void k_gated_dz(const uint16_t* __restrict__ d
   const DzBlocks blocks(rows, n);
   const Keep kept(rows, n);
   const int64_t end = BLOCKS ? blocks.row_blocks * 32 : rows;  // of what is written
-  const int64_t r0 = chunk * kDzRows, r1 = r0 + kDzRows < end ? r0 + kDzRows : end;
+  const int64_t r0 = chunk * chunk_rows, r1 = r0 + chunk_rows < end ? r0 + chunk_rows : end;
   float sum[2][8];
 #pragma unroll
   for (int p = 0; p < 2; ++p)
@@ -413,58 +412,95 @@ struct DxArgs {
   const uint16_t* wg;  // [N, K]
   const uint16_t* wu;
   uint16_t* dx;        // [M, K]
+  float* part;         // [splits][M][K] where the contraction is split, else null
   int32_t M, N, K;
-  int32_t tiles_k;
+  int32_t tiles_k, tiles, per_split;  // stages of a split
 };
 
 // dx = dzg Wg + dzu Wu at any sizes and alignment: the same blocks, 64 rows by 64 of K,
-// contracted over the outputs of one layer and then of the other; W's stages are
-// turned on their way to LDS.
+// contracted over the outputs of one layer and then of the other (a stage holds one
+// layer's); W's stages are turned on their way to LDS.
 __global__ __launch_bounds__(256) void k_gated_dx_any(DxArgs a) {
   constexpr int NP = 64 * 8 / 256;
   __shared__ __align__(16) char lz[64 * 128];
   __shared__ __align__(16) char lw[64 * 128];
   const int tid = tid_x(), lane = tid & 63, wave = tid >> 6, half = lane >> 5, l32 = lane & 31;
-  const int m0 = wg_x() / a.tiles_k * 64, k0 = wg_x() % a.tiles_k * 64;
+  const int split = wg_x() / a.tiles, tile = wg_x() - split * a.tiles;
+  const int m0 = tile / a.tiles_k * 64, k0 = tile % a.tiles_k * 64;
   const int wm = (wave >> 1) * 32, wk = (wave & 1) * 32;
+  const int layer = (a.N + kStage - 1) / kStage;
+  const int first = split * a.per_split, end = min(first + a.per_split, 2 * layer);
   f32x16 acc = fill16(0.f);
-  for (int part = 0; part < 2; ++part) {
+  u32x4 z[NP], v[NP];
+  auto fetch = [&](int s) {
+    const int part = s >= layer, n0 = (s - part * layer) * kStage;
     const uint16_t* w = part ? a.wu : a.wg;
-    for (int n0 = 0; n0 < a.N; n0 += kStage) {
-      u32x4 z[NP], v[NP];
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const int e = tid + i * 256, m = m0 + e / 8, n = n0 + e / 8;
-        z[i] = v[i] = u32x4{0u, 0u, 0u, 0u};
-        if (m < a.M) z[i] = load8<false>(a.dz + (int64_t(m) * 2 + part) * a.N, n0 + 8 * (e % 8), a.N);
-        if (n < a.N) v[i] = load8<false>(w + int64_t(n) * a.K, k0 + 8 * (e % 8), a.K);
-      }
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const int e = tid + i * 256, r = e / 8, c = e % 8;
-        *reinterpret_cast<u32x4*>(lz + L::offset(r, c)) = z[i];
-#pragma unroll
-        for (int t = 0; t < 8; ++t)
-          *reinterpret_cast<uint16_t*>(lw + L::offset(8 * c + t, r / 8) + 2 * (r % 8)) =
-              static_cast<uint16_t>(v[i][t / 2] >> (16 * (t & 1)));
-      }
-      __syncthreads();
-#pragma unroll
-      for (int c = 0; c < L::kChunks; ++c)
-        acc = L::mma(L::load_a(lw + wk * 128, 0, c, l32, half),
-                     L::load_a(lz + wm * 128, 0, c, l32, half), acc);
+    for (int i = 0; i < NP; ++i) {
+      const int e = tid + i * 256, m = m0 + e / 8, n = n0 + e / 8;
+      z[i] = v[i] = u32x4{0u, 0u, 0u, 0u};
+      if (m < a.M) z[i] = load8<false>(a.dz + (int64_t(m) * 2 + part) * a.N, n0 + 8 * (e % 8), a.N);
+      if (n < a.N) v[i] = load8<false>(w + int64_t(n) * a.K, k0 + 8 * (e % 8), a.K);
     }
+  };
+  fetch(first);
+  for (int s = first; s < end; ++s) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int e = tid + i * 256, r = e / 8, c = e % 8;
+      *reinterpret_cast<u32x4*>(lz + L::offset(r, c)) = z[i];
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+        *reinterpret_cast<uint16_t*>(lw + L::offset(8 * c + t, r / 8) + 2 * (r % 8)) =
+            static_cast<uint16_t>(v[i][t / 2] >> (16 * (t & 1)));
+    }
+    __syncthreads();
+    if (s + 1 < end) fetch(s + 1);
+#pragma unroll
+    for (int c = 0; c < L::kChunks; ++c)
+      acc = L::mma(L::load_a(lw + wk * 128, 0, c, l32, half),
+                   L::load_a(lz + wm * 128, 0, c, l32, half), acc);
   }
   const int m = m0 + wm + L::a_row(l32);
   if (m >= a.M) return;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    u32x4 o;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) o[t] = pack2_bf16(acc[8 * e + 2 * t], acc[8 * e + 2 * t + 1]);
     const int k = k0 + wk + 16 * half + 8 * e;
-    if (k < a.K) store8(a.dx + int64_t(m) * a.K, k, a.K, o);
+    if (k >= a.K) continue;
+    if (a.part) {
+      float* to = a.part + (int64_t(split) * a.M + m) * a.K + k;
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+        if (k + t < a.K) to[t] = acc[8 * e + t];
+    } else {
+      u32x4 o;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) o[t] = pack2_bf16(acc[8 * e + 2 * t], acc[8 * e + 2 * t + 1]);
+      store8(a.dx + int64_t(m) * a.K, k, a.K, o);
+    }
+  }
+}
+
+// dx from the splits' sums, added in their order, 4 elements a thread.
+__global__ __launch_bounds__(256) void k_gated_join_dx(const float* __restrict__ part, int32_t splits,
+                                                       int64_t n, uint16_t* __restrict__ dx) {
+  const int64_t step = int64_t(__builtin_amdgcn_grid_size_x()) * 4;
+  for (int64_t i = (int64_t(wg_x()) * 256 + tid_x()) * 4; i < n; i += step) {
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (n % 4 == 0) {
+#pragma unroll 8
+      for (int c = 0; c < splits; ++c) {
+        const float4 v = *reinterpret_cast<const float4*>(part + c * n + i);
+        s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
+      }
+      *reinterpret_cast<uint2*>(dx + i) = make_uint2(pack2_bf16(s[0], s[1]), pack2_bf16(s[2], s[3]));
+    } else {
+      for (int t = 0; t < 4 && i + t < n; ++t) {
+        for (int c = 0; c < splits; ++c) s[t] += part[c * n + i + t];
+        dx[i + t] = f32_to_bf16(s[t]);
+      }
+    }
   }
 }
 
@@ -587,33 +623,39 @@ __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
 // How a backward is cut, and where its workspace holds what.
 struct BwdPlan {
   bool tiled;
-  int32_t fn;          // columns of x a tile has, in 64s
-  int32_t splits;      // of the rows, for the weights' gradients
-  int64_t split_rows;
-  int64_t chunks;      // of kDzRows rows
-  size_t dz, part, part_b, wgrad, bytes;
+  GatedShape dx, dw;   // (not tiled: dx's splits alone)
+  int32_t chunk_rows;  // of a block of k_gated_dz
+  int64_t chunks;
+  size_t dz, part, part_b, wgrad, bytes;  // part: dx's sums, then the weights'
 };
-constexpr int64_t kDwRows = 512;  // fewer rows: ngt_wgrad_bf16
 int plan_bwd(int64_t M, int32_t N, int32_t K, BwdPlan* p) {
-  p->tiled = tiled(N, K) && M >= kDwRows;
-  p->chunks = (M + kDzRows - 1) / kDzRows;
+  p->tiled = tiled(N, K);
+  // 1,024 blocks where there are rows enough: a block takes 8 at a time
+  p->chunk_rows = 128;
+  while (p->chunk_rows > 8 && (M + p->chunk_rows - 1) / p->chunk_rows * ((N + 255) / 256) < 1024)
+    p->chunk_rows /= 2;
+  // (M filled up to whole blocks of dz)
+  p->chunks = M == 0 ? 0 : ((M + 63) / 64 * 64 + p->chunk_rows - 1) / p->chunk_rows;
   auto align = [](size_t b) { return (b + 255) & ~size_t(255); };
-  const size_t w = size_t(2) * N * K * sizeof(float);
-  p->dz = 0;
-  p->part = align(p->tiled ? DzBlocks(M, N).bytes() : size_t(M) * 2 * N * 2);
-  p->splits = 1, p->split_rows = M;
-  size_t ws = 0;
+  size_t part = size_t(2) * N * K * sizeof(float), ws = 0;
+  p->dw = {4, 1, 0};
   if (p->tiled) {
-    const GatedDwShape shape = gated_dw_shape(M, N, K);
-    p->fn = shape.fn;
-    const int64_t splits = shape.splits;
-    const int64_t stages = (M + kStage - 1) / kStage, per = (stages + splits - 1) / splits;
-    p->split_rows = per * kStage;
-    p->splits = static_cast<int32_t>((stages + per - 1) / per);
+    p->dx = gated_dx_shape(M, N, K), p->dw = gated_dw_shape(M, N, K);
+    part = p->dw.splits > 1 ? part * p->dw.splits : 0;
   } else {
+    // 512 blocks of the 64 x 64 tiles, 4 stages at least each
+    const int64_t stages = (int64_t(N) + 63) / 64 * 2, tiles = (M + 63) / 64 * ((K + 63) / 64);
+    int64_t splits = tiles > 0 ? 512 / tiles : 1;
+    if (splits > stages / 4) splits = stages / 4;
+    if (splits < 1) splits = 1;
+    const int64_t per = (stages + splits - 1) / splits;
+    p->dx = {1, static_cast<int32_t>((stages + per - 1) / per), static_cast<int32_t>(per)};
     NGT_CHECK_OK(ngt_wgrad_workspace_bytes(M, 2 * N, K, &ws));
   }
-  p->part_b = p->part + align(p->splits * w);
+  const size_t part_dx = p->dx.splits > 1 ? size_t(p->dx.splits) * M * K * sizeof(float) : 0;
+  p->dz = 0;
+  p->part = align(p->tiled ? DzBlocks(M, N).bytes() : size_t(M) * 2 * N * 2);
+  p->part_b = p->part + align(part > part_dx ? part : part_dx);
   p->wgrad = p->part_b + align(size_t(p->chunks) * 2 * N * sizeof(float));
   p->bytes = p->wgrad + ws;
   return NGT_OK;
@@ -744,39 +786,49 @@ extern "C" int ngt_gated_bwd(const void* dy, const void* keep, const void* x, co
   const auto *wg = static_cast<const uint16_t*>(w_gate), *wu = static_cast<const uint16_t*>(w_up);
   const auto M = static_cast<int32_t>(n_rows);
   const GatedBwd products{dz, static_cast<const uint16_t*>(x), wg, wu, static_cast<uint16_t*>(g.dx),
-                          part, n_rows, p.split_rows, n_out, n_in, p.splits};
+                          {g.dw_gate, g.dw_up}, part, n_rows, n_out, n_in,
+                          {g.dw_gate_dtype == NGT_F32, g.dw_up_dtype == NGT_F32}};
   if (n_rows > 0) {
     KernelTimer timer_("gated_dz", st);
     const int32_t tiles_n = (n_out + 255) / 256;
     hipLaunchKernelGGL(p.tiled ? &k_gated_dz<true> : &k_gated_dz<false>,
                        dim3(unsigned(p.chunks * tiles_n)), dim3(256), 0, st,
                        static_cast<const uint16_t*>(dy), const_cast<void*>(keep), n_rows, n_out,
-                       tiles_n, dz, want_b ? part_b : nullptr);
+                       tiles_n, p.chunk_rows, dz, want_b ? part_b : nullptr);
     NGT_HIP_CHECK(hipGetLastError());
   }
   if (n_rows > 0 && g.dx) {
     KernelTimer timer_("gated_dx", st);
     if (p.tiled) {
-      NGT_CHECK_OK(launch_gated_dx(products, st));
+      NGT_CHECK_OK(launch_gated_dx(products, p.dx, st));
     } else {
-      DxArgs a{dz, wg, wu, static_cast<uint16_t*>(g.dx), M, n_out, n_in, (n_in + 63) / 64};
-      hipLaunchKernelGGL(k_gated_dx_any, dim3(unsigned((n_rows + 63) / 64 * a.tiles_k)), dim3(256),
-                         0, st, a);
+      const int32_t tiles_k = (n_in + 63) / 64;
+      const int64_t tiles = (n_rows + 63) / 64 * tiles_k;
+      DxArgs a{dz, wg, wu, static_cast<uint16_t*>(g.dx), p.dx.splits > 1 ? part : nullptr, M, n_out,
+               n_in, tiles_k, static_cast<int32_t>(tiles), p.dx.per_split};
+      hipLaunchKernelGGL(k_gated_dx_any, dim3(unsigned(tiles * p.dx.splits)), dim3(256), 0, st, a);
+      NGT_HIP_CHECK(hipGetLastError());
+    }
+    if (p.dx.splits > 1) {
+      const int64_t n = n_rows * n_in, blocks = (n + 1023) / 1024;
+      hipLaunchKernelGGL(k_gated_join_dx, dim3(unsigned(blocks < 4096 ? blocks : 4096)), dim3(256), 0,
+                         st, part, p.dx.splits, n, static_cast<uint16_t*>(g.dx));
       NGT_HIP_CHECK(hipGetLastError());
     }
   }
-  int32_t splits = p.splits;
+  int32_t splits = p.dw.splits;
   if (want_w && n_rows > 0) {
     if (p.tiled) {
       KernelTimer timer_("gated_dw", st);
-      NGT_CHECK_OK(launch_gated_dw(products, p.fn, st));
+      NGT_CHECK_OK(launch_gated_dw(products, p.dw, st));
     } else {
       NGT_CHECK_OK(ngt_wgrad_bf16(x, dz, n_rows, 2 * n_out, n_in, part, nullptr, ws + p.wgrad,
                                   p.bytes - p.wgrad, stream));
     }
   }
   if (n_rows == 0) splits = 0;
-  if (want_w || want_b) {
+  const bool join_w = want_w && !(p.tiled && p.dw.splits == 1 && n_rows > 0);
+  if (join_w || want_b) {
     KernelTimer timer_("gated_join", st);
     JoinArgs j{};
     j.part = part, j.part_b = part_b;
@@ -785,7 +837,7 @@ extern "C" int ngt_gated_bwd(const void* dy, const void* keep, const void* x, co
     j.db_f32[0] = g.db_gate_dtype == NGT_F32, j.db_f32[1] = g.db_up_dtype == NGT_F32;
     j.nk = int64_t(n_out) * n_in, j.n = n_out, j.splits = splits;
     j.chunks = static_cast<int32_t>(p.chunks);
-    j.blocks_w = want_w ? static_cast<int32_t>((2 * j.nk + 1023) / 1024) : 0;
+    j.blocks_w = join_w ? static_cast<int32_t>((2 * j.nk + 1023) / 1024) : 0;
     const int blocks_b = want_b ? (2 * n_out + 31) / 32 : 0;
     hipLaunchKernelGGL(k_gated_join, dim3(unsigned(j.blocks_w + blocks_b)), dim3(256), 0, st, j);
     NGT_HIP_CHECK(hipGetLastError());

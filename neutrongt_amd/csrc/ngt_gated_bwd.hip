@@ -2,9 +2,14 @@
 // shape: 256 by 64 FN outputs, 4 waves of 4 x FN tiles of 32 x 32 (accumulators in
 // AGPRs), one block on a CU, contracted in stages of 64.
 //   dx = dzg Wg + dzu Wu         rows of dz by columns of Wg, then of Wu
-//   part[split] = dz^T x         columns of dz by columns of x, over the split's rows
-// Two stages fit in LDS: one is multiplied while the next comes in.
+//   dW = dz^T x                  columns of dz by columns of x
+// Two stages fit in LDS: one is multiplied while the next comes in.  Where there are fewer
+// blocks than CUs the contraction is split over several, whose fp32 sums are added in order
+// (512 rows of 2,048 -> 8,192: dx 69 us, 220 without).
 #include "ngt_gated.h"
+
+#include <algorithm>
+#include <cmath>
 
 namespace ngt {
 namespace {
@@ -13,6 +18,7 @@ enum Mode { kDx, kDw };
 
 struct BwdArgs {
   GatedBwd g;
+  GatedShape shape;
   int32_t tiles_m, tiles_n;
 };
 
@@ -26,7 +32,7 @@ __global__ __launch_bounds__(256, 1) void k_gated_bwd(BwdArgs args) {
   __shared__ __align__(16) char s1[kStageBytes];
   const GatedBwd& g = args.g;
   const int lane = tid_x() & 63, wave = packed::wave_id(), half = lane >> 5;
-  const TileAt at = tile_at(args.tiles_m, args.tiles_n, MODE == kDw ? g.splits : 1);
+  const TileAt at = tile_at(args.tiles_m, args.tiles_n, args.shape.splits);
   if (!at.there) return;  // block-uniform
   const int m0 = at.m * BM, n0 = at.n * BN;
   const int wm = (wave >> 1) * FM, wn = (wave & 1) * FN;  // in 32s
@@ -41,29 +47,31 @@ __global__ __launch_bounds__(256, 1) void k_gated_bwd(BwdArgs args) {
   BlockOperand oa;
   B ob;
   oa.init(), ob.init(g.K);
-  // the contraction: twice N (a stage holds one layer's), or the split's rows
-  const int half_stages = blocks.per_layer;
-  const int64_t row0 = MODE == kDw ? at.split * g.split_rows : 0;
-  const int64_t rows = g.M - row0 < g.split_rows ? g.M - row0 : g.split_rows;
-  const int stages = MODE == kDx ? 2 * half_stages : static_cast<int>((rows + kStage - 1) / kStage);
+  // the contraction: twice N (a stage holds one layer's), or the rows; this split's part of it
+  const int layer_stages = blocks.per_layer;
+  const int all = MODE == kDx ? 2 * layer_stages : static_cast<int>((g.M + kStage - 1) / kStage);
+  const int first = at.split * args.shape.per_split;
+  const int end = min(first + args.shape.per_split, all), stages = end - first;
   const int cols_b = g.K - n0;
   struct Source {
     u32x4 a, b;
   };
-  // of stage s; behind the last one all is zero
-  auto source = [&](int s) {
+  // of the split's stage i; behind its last one all is zero
+  auto source = [&](int i) {
     Source f;
+    const int s = first + i;
+    const bool there = s < end;
     const char* dz = reinterpret_cast<const char*>(g.dz);
     if constexpr (MODE == kDx) {
-      const int up = s >= half_stages, k = (s - (up ? half_stages : 0)) * kStage;
+      const int up = s >= layer_stages, k = (s - (up ? layer_stages : 0)) * kStage;
       const int64_t from = m0 / 32 * across + int64_t(s) * 4096;
-      f.a = descriptor(dz + from, s < stages ? blocks.bytes() - from : 0);
-      f.b = ColsOperand::source((up ? g.wu : g.wg) + int64_t(k) * g.K + n0, g.N - k, g.K, cols_b);
+      f.a = descriptor(dz + from, there ? blocks.bytes() - from : 0);
+      f.b = ColsOperand::source((up ? g.wu : g.wg) + int64_t(k) * g.K + n0, there ? g.N - k : 0, g.K,
+                                cols_b);
     } else {
-      const int64_t r = row0 + int64_t(s) * kStage, left = rows - int64_t(s) * kStage;
-      const int64_t from = r / 32 * across + m0 / 64 * 4096;
-      f.a = descriptor(dz + from, left > 0 ? blocks.bytes() - from : 0);
-      f.b = ColsOperand::source(g.x + r * g.K + n0, left, g.K, cols_b);
+      const int64_t r = int64_t(s) * kStage, from = r / 32 * across + m0 / 64 * 4096;
+      f.a = descriptor(dz + from, there ? blocks.bytes() - from : 0);
+      f.b = ColsOperand::source(g.x + r * g.K + n0, there ? g.M - r : 0, g.K, cols_b);
     }
     return f;
   };
@@ -132,79 +140,101 @@ __global__ __launch_bounds__(256, 1) void k_gated_bwd(BwdArgs args) {
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
       const int n = n0 + 32 * (wn + j) + 16 * half;
-      if constexpr (MODE == kDx) {
+      // 16 columns of row `row` of a matrix: of fp32 sums or of results in bf16
+      auto put = [&](void* to, int64_t row, bool f32) {
+        if (f32) {
+          float* p = static_cast<float*>(to) + row * g.K + n;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          u32x4 y;
+          for (int e = 0; e < 4; ++e)
+            if (n + 4 * e < g.K)
+              *reinterpret_cast<float4*>(p + 4 * e) =
+                  make_float4(acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2],
+                              acc[i][j][4 * e + 3]);
+        } else {
+          uint16_t* p = static_cast<uint16_t*>(to) + row * g.K + n;
 #pragma unroll
-          for (int t = 0; t < 4; ++t)
-            y[t] = pack2_bf16(acc[i][j][8 * e + 2 * t], acc[i][j][8 * e + 2 * t + 1]);
-          if (m < g.M && n + 8 * e < g.K) *reinterpret_cast<u32x4*>(g.dx + m * g.K + n + 8 * e) = y;
+          for (int e = 0; e < 2; ++e) {
+            u32x4 y;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+              y[t] = pack2_bf16(acc[i][j][8 * e + 2 * t], acc[i][j][8 * e + 2 * t + 1]);
+            if (n + 8 * e < g.K) *reinterpret_cast<u32x4*>(p + 8 * e) = y;
+          }
         }
+      };
+      const bool parts = args.shape.splits > 1;
+      if constexpr (MODE == kDx) {
+        if (m < g.M) put(parts ? static_cast<void*>(g.part) : g.dx, parts ? at.split * g.M + m : m, parts);
       } else {
         // m counts dz's columns with what fills up each layer's
         const int layer = m >= 64 * blocks.per_layer;
         const int64_t o = m - layer * 64 * blocks.per_layer;
-        float* to = g.part + ((2 * int64_t(at.split) + layer) * g.N + o) * g.K + n;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (layer * 64 * blocks.per_layer + o < blocks.across() * 64 && o < g.N && n + 4 * e < g.K)
-            *reinterpret_cast<float4*>(to + 4 * e) =
-                make_float4(acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2],
-                            acc[i][j][4 * e + 3]);
+        if (m < 64 * blocks.across() && o < g.N) {
+          if (parts) put(g.part, (2 * int64_t(at.split) + layer) * g.N + o, true);
+          else if (g.dw[layer]) put(g.dw[layer], o, g.dw_f32[layer]);
+        }
       }
     }
   }
 }
 
 template <int FN, Mode MODE>
-int launch(const GatedBwd& g, hipStream_t st) {
-  BwdArgs a{g, 0, 0};
+int launch_one(const GatedBwd& g, const GatedShape& shape, hipStream_t st) {
+  BwdArgs a{g, shape, 0, 0};
   const int64_t m = MODE == kDx ? g.M : 64 * DzBlocks(g.M, g.N).across();
   a.tiles_m = static_cast<int32_t>((m + 255) / 256);
   a.tiles_n = (g.K + 64 * FN - 1) / (64 * FN);
-  const int64_t blocks = int64_t(a.tiles_m) * a.tiles_n * (MODE == kDw ? g.splits : 1);
-  hipLaunchKernelGGL((k_gated_bwd<FN, MODE>), dim3(unsigned((blocks + 7) / 8 * 8)), dim3(256), 0, st,
-                     a);
+  const int64_t blocks = (int64_t(a.tiles_m) * a.tiles_n * shape.splits + 7) / 8 * 8;
+  hipLaunchKernelGGL((k_gated_bwd<FN, MODE>), dim3(unsigned(blocks)), dim3(256), 0, st, a);
   NGT_HIP_CHECK(hipGetLastError());
   return NGT_OK;
 }
-
-// The rounds that 256 CUs need for so many blocks.  A stage of a block with 64 fn columns takes
-// about fn + 2 units of time (32,768 rows, 4,096 x 768: dx 1.31, 1.6, 1.76 us at fn = 2, 3, 4,
-// dw 1.12, 1.55, 1.85).
-int64_t rounds(int64_t blocks) { return (blocks + 255) / 256; }
-
-}  // namespace
-
-int launch_gated_dx(const GatedBwd& g, hipStream_t st) {
-  int best = 4;
-  int64_t cost = INT64_MAX;
-  for (int fn = 4; fn >= 2; --fn) {
-    const int64_t c = (fn + 2) * rounds((g.M + 255) / 256 * ((g.K + 64 * fn - 1) / (64 * fn)));
-    if (c < cost) cost = c, best = fn;
-  }
-  return best == 4 ? launch<4, kDx>(g, st) : best == 3 ? launch<3, kDx>(g, st) : launch<2, kDx>(g, st);
+template <Mode MODE>
+int launch(const GatedBwd& g, const GatedShape& shape, hipStream_t st) {
+  return shape.fn == 4   ? launch_one<4, MODE>(g, shape, st)
+         : shape.fn == 3 ? launch_one<3, MODE>(g, shape, st)
+                         : launch_one<2, MODE>(g, shape, st);
 }
 
-GatedDwShape gated_dw_shape(int64_t M, int32_t N, int32_t K) {
-  const int64_t stages = (M + kStage - 1) / kStage;
-  GatedDwShape best{4, 1};
-  int64_t cost = INT64_MAX;
+// The cheapest blocks for m by K outputs over `stages` of contraction.  A stage of a block with
+// 64 fn columns takes about fn + 2 units of time, some 0.3 us each (32,768 rows, 4,096 x 768:
+// dx 1.31, 1.6, 1.76 us at fn = 2, 3, 4, dw 1.12, 1.55, 1.85), a block beside its stages about
+// as much as 4 of them, and each round of 256 blocks comes after the one before.  Each of
+// several splits costs its sums, `bytes` written and read again at some 4 TB/s: per + 4 stages
+// and those sums are least where the splits are the square root of their quotient.
+GatedShape shape_of(int64_t m, int32_t K, int64_t stages, int64_t bytes) {
+  GatedShape best{4, 1, static_cast<int32_t>(stages)};
+  if (m == 0 || stages == 0) return best;  // nothing is launched
+  double cost = 1e300;
   for (int fn = 4; fn >= 2; --fn) {
-    const int64_t tiles = (DzBlocks(M, N).across() + 3) / 4 * ((K + 64 * fn - 1) / (64 * fn));
-    // a split has 4 stages at least
-    int64_t splits = 256 / tiles;
-    if (splits > stages / 4) splits = stages / 4;
-    if (splits < 1) splits = 1;
-    const int64_t c = (fn + 2) * rounds(tiles * splits) * ((stages + splits - 1) / splits);
-    if (c < cost) cost = c, best = {fn, static_cast<int>(splits)};
+    const int64_t tiles = (m + 255) / 256 * ((K + 64 * fn - 1) / (64 * fn));
+    const double stage = 0.3 * (fn + 2), sums = 5e-7 * double(bytes);
+    const double alone = double((tiles + 255) / 256) * stage * double(stages + 4);
+    if (alone < cost) cost = alone, best = {fn, 1, static_cast<int32_t>(stages)};
+    const double want = std::sqrt(stage * double(stages) / sums);
+    const int64_t most = std::min<int64_t>(256 / tiles, stages / 4);
+    const int64_t splits = want < double(most) ? std::llround(want) : most;
+    if (splits < 2) continue;
+    const int64_t per = (stages + splits - 1) / splits, used = (stages + per - 1) / per;
+    const double c = stage * double(per + 4) + 3.0 + sums * double(used);
+    if (c < cost) cost = c, best = {fn, static_cast<int32_t>(used), static_cast<int32_t>(per)};
   }
   return best;
 }
 
-int launch_gated_dw(const GatedBwd& g, int fn, hipStream_t st) {
-  return fn == 4 ? launch<4, kDw>(g, st) : fn == 3 ? launch<3, kDw>(g, st) : launch<2, kDw>(g, st);
+}  // namespace
+
+GatedShape gated_dx_shape(int64_t M, int32_t N, int32_t K) {
+  return shape_of(M, K, DzBlocks(M, N).across(), 4 * M * K);
+}
+GatedShape gated_dw_shape(int64_t M, int32_t N, int32_t K) {
+  return shape_of(64 * DzBlocks(M, N).across(), K, (M + kStage - 1) / kStage, int64_t(8) * N * K);
+}
+int launch_gated_dx(const GatedBwd& g, const GatedShape& s, hipStream_t st) {
+  return launch<kDx>(g, s, st);
+}
+int launch_gated_dw(const GatedBwd& g, const GatedShape& s, hipStream_t st) {
+  return launch<kDw>(g, s, st);
 }
 
 }  // namespace ngt

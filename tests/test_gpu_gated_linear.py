@@ -123,6 +123,15 @@ def test_gradients_of_whole_pieces_with_edges(dev, M, N, K):
     _case(dev, M, N, K, "silu", seed=M)
 
 
+# a contraction over many outputs for few blocks, cut into several and not
+@pytest.mark.parametrize("M,N,K", [(1, 1024, 520), (33, 2048, 512), (64, 4096, 8), (65, 1000, 1288),
+                                   (200, 256, 264), (300, 1288, 72), (71, 1001, 33), (130, 2050, 65),
+                                   (450, 520, 2048)])
+@pytest.mark.parametrize("w_type", [BF16, F32])
+def test_gradients_of_few_rows_and_many_outputs(dev, M, N, K, w_type):
+    _case(dev, M, N, K, "silu", bias=True, w_type=w_type, seed=N)
+
+
 # a stage of the contraction, a part of one, several
 @pytest.mark.parametrize("K", [8, 56, 64, 72, 128, 192, 200, 256, 320, 456, 512])
 def test_lengths_of_the_contraction(dev, K):
