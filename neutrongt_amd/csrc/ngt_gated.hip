@@ -5,6 +5,8 @@
 // that the backward forms no activation.
 #include "ngt_gated.h"
 
+#include <algorithm>
+#include <cmath>
 #include <utility>
 
 namespace ngt {
@@ -412,10 +414,11 @@ struct DxArgs {
   const uint16_t* wg;  // [N, K]
   const uint16_t* wu;
   uint16_t* dx;        // [M, K]
-  float* part;         // [splits][M][K] where the contraction is split, else null
+  float* part;         // [splits][M][K filled up to 8s] where the contraction is split, else null
   int32_t M, N, K;
   int32_t tiles_k, tiles, per_split;  // stages of a split
 };
+__host__ __device__ constexpr int32_t up8(int32_t n) { return (n + 7) / 8 * 8; }
 
 // dx = dzg Wg + dzu Wu at any sizes and alignment: the same blocks, 64 rows by 64 of K,
 // contracted over the outputs of one layer and then of the other (a stage holds one
@@ -469,10 +472,11 @@ __global__ __launch_bounds__(256) void k_gated_dx_any(DxArgs a) {
     const int k = k0 + wk + 16 * half + 8 * e;
     if (k >= a.K) continue;
     if (a.part) {
-      float* to = a.part + (int64_t(split) * a.M + m) * a.K + k;
+      float* to = a.part + (int64_t(split) * a.M + m) * up8(a.K) + k;
 #pragma unroll
-      for (int t = 0; t < 8; ++t)
-        if (k + t < a.K) to[t] = acc[8 * e + t];
+      for (int t = 0; t < 8; t += 4)
+        *reinterpret_cast<float4*>(to + t) = make_float4(acc[8 * e + t], acc[8 * e + t + 1],
+                                                         acc[8 * e + t + 2], acc[8 * e + t + 3]);
     } else {
       u32x4 o;
 #pragma unroll
@@ -482,26 +486,25 @@ __global__ __launch_bounds__(256) void k_gated_dx_any(DxArgs a) {
   }
 }
 
-// dx from the splits' sums, added in their order, 4 elements a thread.
+// dx from the splits' sums, added in their order, 8 elements a thread.
 __global__ __launch_bounds__(256) void k_gated_join_dx(const float* __restrict__ part, int32_t splits,
-                                                       int64_t n, uint16_t* __restrict__ dx) {
-  const int64_t step = int64_t(__builtin_amdgcn_grid_size_x()) * 4;
-  for (int64_t i = (int64_t(wg_x()) * 256 + tid_x()) * 4; i < n; i += step) {
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-    if (n % 4 == 0) {
+                                                       int32_t M, int32_t K,
+                                                       uint16_t* __restrict__ dx) {
+  const int across = up8(K) / 8, i = wg_x() * 256 + tid_x();
+  if (i >= M * across) return;
+  float s[8] = {};
 #pragma unroll 8
-      for (int c = 0; c < splits; ++c) {
-        const float4 v = *reinterpret_cast<const float4*>(part + c * n + i);
-        s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
-      }
-      *reinterpret_cast<uint2*>(dx + i) = make_uint2(pack2_bf16(s[0], s[1]), pack2_bf16(s[2], s[3]));
-    } else {
-      for (int t = 0; t < 4 && i + t < n; ++t) {
-        for (int c = 0; c < splits; ++c) s[t] += part[c * n + i + t];
-        dx[i + t] = f32_to_bf16(s[t]);
-      }
-    }
+  for (int c = 0; c < splits; ++c) {
+    const float* p = part + (int64_t(c) * M * across + i) * 8;
+    const float4 v = *reinterpret_cast<const float4*>(p), w = *reinterpret_cast<const float4*>(p + 4);
+    s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
+    s[4] += w.x, s[5] += w.y, s[6] += w.z, s[7] += w.w;
   }
+  u32x4 o;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) o[t] = pack2_bf16(s[2 * t], s[2 * t + 1]);
+  const int m = i / across;
+  store8(dx + int64_t(m) * K, (i - m * across) * 8, K, o);
 }
 
 // Aligned sizes.  One block: 64 FM rows by 64 outputs of both layers, 2 x 2 waves, each FM tiles
@@ -630,7 +633,8 @@ struct BwdPlan {
 };
 int plan_bwd(int64_t M, int32_t N, int32_t K, BwdPlan* p) {
   p->tiled = tiled(N, K);
-  // 1,024 blocks where there are rows enough: a block takes 8 at a time
+  // 1,024 blocks where there are rows enough, of 8 rows a pass (2,048 -> 8,192 us at 64 rows: 6, at
+  // 128 rows a block 12; 768 -> 2,048 at 511: 8 and 20)
   p->chunk_rows = 128;
   while (p->chunk_rows > 8 && (M + p->chunk_rows - 1) / p->chunk_rows * ((N + 255) / 256) < 1024)
     p->chunk_rows /= 2;
@@ -643,16 +647,19 @@ int plan_bwd(int64_t M, int32_t N, int32_t K, BwdPlan* p) {
     p->dx = gated_dx_shape(M, N, K), p->dw = gated_dw_shape(M, N, K);
     part = p->dw.splits > 1 ? part * p->dw.splits : 0;
   } else {
-    // 512 blocks of the 64 x 64 tiles, 4 stages at least each
+    // Splits of 4 stages at least, in no more blocks than the CUs hold at a time (6 each).  A
+    // stage takes 1.3 us and its share of a CU; a split's sums 1 us a MB, written and read again:
+    // best is the square root of their quotient.  33 rows, 2,049 -> 8,193: 37 us, 402 in one
+    // split; 1,025 of them 416 and 546; 1,025 rows, 769 -> 769: 28 and 38.  (M K stays below 2^22.)
     const int64_t stages = (int64_t(N) + 63) / 64 * 2, tiles = (M + 63) / 64 * ((K + 63) / 64);
-    int64_t splits = tiles > 0 ? 512 / tiles : 1;
-    if (splits > stages / 4) splits = stages / 4;
-    if (splits < 1) splits = 1;
+    const int64_t most = tiles > 0 ? std::min<int64_t>(6 * 256 / tiles, stages / 4) : 1;
+    const double want = std::sqrt(1.3 * double(stages) / (1e-6 * 4 * double(M) * K));
+    const int64_t splits = std::max<int64_t>(1, want < double(most) ? std::llround(want) : most);
     const int64_t per = (stages + splits - 1) / splits;
     p->dx = {1, static_cast<int32_t>((stages + per - 1) / per), static_cast<int32_t>(per)};
     NGT_CHECK_OK(ngt_wgrad_workspace_bytes(M, 2 * N, K, &ws));
   }
-  const size_t part_dx = p->dx.splits > 1 ? size_t(p->dx.splits) * M * K * sizeof(float) : 0;
+  const size_t part_dx = p->dx.splits > 1 ? size_t(p->dx.splits) * M * up8(K) * sizeof(float) : 0;
   p->dz = 0;
   p->part = align(p->tiled ? DzBlocks(M, N).bytes() : size_t(M) * 2 * N * 2);
   p->part_b = p->part + align(part > part_dx ? part : part_dx);
@@ -704,9 +711,13 @@ extern "C" int ngt_gated_fwd(const void* x, int64_t x_stride, const void* w_gate
               keep, x_stride, static_cast<int32_t>(n_rows), n_out, n_in, activation, 0, 0};
   hipStream_t st = static_cast<hipStream_t>(stream);
   KernelTimer timer_("gated_fwd", st);
+  // 1 and 64 rows, us, here and in the tiles of 64 rows: 768 -> 2,048 7, 9 and 14, 14; 2,048 -> 8,192
+  // 17, 24 and 31, 31; 4,096 -> 1,024 14, 27 and 44, 43.
   if (n_in % 8 == 0 && x_stride % 8 == 0 && n_rows <= 64 && all_aligned16({x, w_gate, w_up})) {
     auto run = [&](auto mt) {
       constexpr int MT = decltype(mt)::value;
+      // 32 outputs a block where that leaves 256 blocks (64 rows of 2,048 -> 8,192 25 us, 16 outputs
+      // 32; of 768 -> 2,048 12 and 9)
       const int blocks = (n_out + 15) / 16;
       if (blocks >= 512)
         hipLaunchKernelGGL((k_gated_few<MT, 2, MT < 3 ? 8 : 4>), dim3(unsigned((n_out + 31) / 32)),
@@ -729,6 +740,9 @@ extern "C" int ngt_gated_fwd(const void* x, int64_t x_stride, const void* w_gate
       const int64_t blocks = (int64_t(a.tiles_m) * a.tiles_n + 7) / 8 * 8;
       hipLaunchKernelGGL(k_gated<FM>, dim3(unsigned(blocks)), dim3(256), 0, st, a);
     };
+    // The tallest tile that leaves 384 blocks, three quarters of what the CUs hold (us with 256, 128
+    // and 64 rows: 2,048 -> 8,192 at 512 rows 46, 41, 49, at 1,024 66, 79, 93; 768 -> 2,048 at 65
+    // 18, 14, 13, at 2,048 22, 19, 23, at 32,768 240, 261, 292).
     const int64_t across = (n_out + 63) / 64;
     if ((n_rows + 255) / 256 * across >= 384) run(std::integral_constant<int, 4>{});
     else if ((n_rows + 127) / 128 * across >= 384) run(std::integral_constant<int, 2>{});
@@ -810,9 +824,9 @@ extern "C" int ngt_gated_bwd(const void* dy, const void* keep, const void* x, co
       NGT_HIP_CHECK(hipGetLastError());
     }
     if (p.dx.splits > 1) {
-      const int64_t n = n_rows * n_in, blocks = (n + 1023) / 1024;
-      hipLaunchKernelGGL(k_gated_join_dx, dim3(unsigned(blocks < 4096 ? blocks : 4096)), dim3(256), 0,
-                         st, part, p.dx.splits, n, static_cast<uint16_t*>(g.dx));
+      const int64_t blocks = (n_rows * (up8(n_in) / 8) + 255) / 256;
+      hipLaunchKernelGGL(k_gated_join_dx, dim3(unsigned(blocks)), dim3(256), 0, st, part, p.dx.splits,
+                         M, n_in, static_cast<uint16_t*>(g.dx));
       NGT_HIP_CHECK(hipGetLastError());
     }
   }
