@@ -11,7 +11,8 @@ namespace ngt {
 
 // What the forward keeps for the backward: zu act'(zg) and act(zg), the factors of dy, with 12
 // bits of mantissa: the upper 16 bits of the fp32 as rows [M, 2 N], and the 4 bits behind
-// them as one word for each 8 columns, in blocks of 32 rows by 64 columns.  Rounded to bf16
+// them as one word for each 8 columns, in blocks of 32 rows by 32 columns (what a wave of the
+// forward writes at a time).  Rounded to bf16
 // there the gradients were off by 2.9e-3, of which rounding dz and the results makes 2.4e-3,
 // which these leave; the bits cost an eighth of the bytes.
 struct Keep {
@@ -26,7 +27,12 @@ struct Keep {
   // of column c, a multiple of 8
   __host__ __device__ uint32_t* low(void* keep, int64_t row, int part, int c) const {
     return reinterpret_cast<uint32_t*>(static_cast<char*>(keep) + high_bytes) +
-           ((row / 32 * across + c / 64) * 2 + part) * 256 + row % 32 * 8 + c % 64 / 8;
+           ((row / 32 * across + c / 64) * 4 + 2 * part + c % 64 / 32) * 128 + row % 32 * 4 + c % 32 / 8;
+  }
+  // bits 12 to 15 of the word's i-th column
+  __device__ static uint32_t low_of(uint32_t w, int i) {
+    const int at = 8 * (i & 3) + (i < 4 ? 4 : 0);
+    return (at < 12 ? w << (12 - at) : w >> (at - 12)) & 0xf000u;
   }
 };
 

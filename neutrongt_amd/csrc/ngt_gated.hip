@@ -62,34 +62,38 @@ struct Results {
   u32x4 y, kg, ku;
   uint32_t lg, lu;
 };
-// Two fp32 to 20 bits each, rounded to the nearest: the upper halves together, the 4 bits
-// behind them at bits `at` and `at` + 4 of low.  (A NaN stays one: no sum of bf16 products has
-// all its lower bits set.)
-__device__ __forceinline__ uint32_t keep2(float a, float b, int at, uint32_t& low) {
-  const uint32_t u = __float_as_uint(a) + 0x800u, v = __float_as_uint(b) + 0x800u;
-  low |= (u >> 12 & 15u) << at | (v >> 12 & 15u) << (at + 4);
-  return __builtin_amdgcn_perm(v, u, 0x07060302u);
+// 8 fp32 to 20 bits each, rounded to the nearest: their upper halves, and the 4 bits behind
+// them, of the first four in the upper halves of the word's bytes, of the others in the lower.
+// (A NaN stays one: no sum of bf16 products has all its lower bits set.)
+__device__ __forceinline__ void keep8(const float (&v)[8], u32x4& high, uint32_t& low) {
+  uint32_t u[8], b[2];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(v[i]) + 0x800u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) high[i] = __builtin_amdgcn_perm(u[2 * i + 1], u[2 * i], 0x07060302u);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)  // bits 8 to 15 of four
+    b[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(u[4 * i + 3], u[4 * i + 2], 0x0c0c0501u),
+                                 __builtin_amdgcn_perm(u[4 * i + 1], u[4 * i], 0x0c0c0501u), 0x05040100u);
+  low = (b[0] & 0xf0f0f0f0u) | (b[1] >> 4 & 0x0f0f0f0fu);
 }
 template <int ACT, bool KEEP>
-__device__ __forceinline__ Results results8(const float (&sg)[8], const float (&su)[8],
-                                            const u32x4& bg, const u32x4& bu) {
+__device__ __forceinline__ Results results8(const float (&zg)[8], const float (&zu)[8]) {
   Results r;
   r.lg = r.lu = 0u;
+  float g[8], u[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float v[2], g[2], u[2];
+    float v[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const float zu = su[2 * i + t] + half_of(bu, 2 * i + t);
-      const Gate q = gate_of<ACT>(sg[2 * i + t] + half_of(bg, 2 * i + t));
-      v[t] = q.value * zu, g[t] = zu * q.slope, u[t] = q.value;
+      const int c = 2 * i + t;
+      const Gate q = gate_of<ACT>(zg[c]);
+      v[t] = q.value * zu[c], g[c] = zu[c] * q.slope, u[c] = q.value;
     }
     r.y[i] = pack2_bf16(v[0], v[1]);
-    if constexpr (KEEP) {
-      r.kg[i] = keep2(g[0], g[1], 8 * i, r.lg);
-      r.ku[i] = keep2(u[0], u[1], 8 * i, r.lu);
-    }
   }
+  if constexpr (KEEP) keep8(g, r.kg, r.lg), keep8(u, r.ku, r.lu);
   return r;
 }
 
@@ -110,9 +114,12 @@ __device__ __forceinline__ void finish8(const GatedArgs& a, int m, int n, const 
   u32x4 bg = {0u, 0u, 0u, 0u}, bu = {0u, 0u, 0u, 0u};
   if (a.bg) bg = load8<false>(a.bg, n, a.N);
   if (a.bu) bu = load8<false>(a.bu, n, a.N);
+  float zg[8], zu[8];
+#pragma unroll
+  for (int t = 0; t < 8; ++t) zg[t] = sg[t] + half_of(bg, t), zu[t] = su[t] + half_of(bu, t);
   Results r;
   with_act(a.act, a.keep != nullptr, [&](auto act, auto keep) {
-    r = results8<act.value, keep.value>(sg, su, bg, bu);
+    r = results8<act.value, keep.value>(zg, zu);
   });
   store8(a.y + int64_t(m) * a.N, n, a.N, r.y);
   if (a.keep) {
@@ -126,7 +133,7 @@ __device__ __forceinline__ void finish8(const GatedArgs& a, int m, int n, const 
 
 // Any sizes and 2-byte alignment.  One block: 64 rows by 64 outputs of both products,
 // 2 x 2 waves of 32 x 32, stages of 64 of the contraction read into registers while the
-// stage before is multiplied.
+// stage before is multiplied.  32,768 rows, 768 -> 2,048 in it: 350 us (k_gated 231).
 __global__ __launch_bounds__(256) void k_gated_any(GatedArgs a) {
   constexpr int NP = 64 * 8 / 256;  // 16-byte pieces per thread and operand
   __shared__ __align__(16) char lds[3][64 * 128];
@@ -178,7 +185,8 @@ __global__ __launch_bounds__(256) void k_gated_any(GatedArgs a) {
 // Few rows, aligned: a block is 16 NT outputs of both layers for up to 16 MT rows, its waves
 // every WAVES-th 64 of the contraction each, weights and rows straight from memory to
 // registers; their sums meet in LDS and are added in wave order.  Bound by the weights'
-// bytes, or, where those are few, by one wait for memory and the join.
+// bytes (33 rows, 2,048 -> 8,192: 18 us, 3.7 TB/s; a library product of that size 19), or,
+// where those are few, by one wait for memory and the join (5 rows, 768 -> 768: 5 us).
 template <int MT, int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_gated_few(GatedArgs a) {
   typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -271,7 +279,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_gated_few(GatedArgs a) {
 
 // dz = [dzg | dzu], and the biases' gradients: part_b[chunk][2 N], sums of the
 // unrounded products.  A block: 256 columns of chunk_rows rows, 8 columns a thread.  BLOCKS: whole
-// pieces, and dz in DzBlocks, else [M, 2 N].
+// pieces, and dz in DzBlocks, else [M, 2 N].  Bound by memory: 32,768 by 2,048 moves 738 MB in
+// 142 to 147 us, 5.1 TB/s, as a copy does.
 template <bool BLOCKS>
 __global__ __launch_bounds__(256) void k_gated_dz(const uint16_t* __restrict__ dy,
                                                   void* keep, int64_t rows,
@@ -314,8 +323,8 @@ __global__ __launch_bounds__(256) void k_gated_dz(const uint16_t* __restrict__ d
         u32x4 o;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const float k0 = __uint_as_float(v[p][t] << 16 | (low[p] >> (8 * t) & 15u) << 12);
-          const float k1 = __uint_as_float((v[p][t] & 0xffff0000u) | (low[p] >> (8 * t + 4) & 15u) << 12);
+          const float k0 = __uint_as_float(v[p][t] << 16 | Keep::low_of(low[p], 2 * t));
+          const float k1 = __uint_as_float((v[p][t] & 0xffff0000u) | Keep::low_of(low[p], 2 * t + 1));
           const float lo = half_of(g, 2 * t) * k0, hi = half_of(g, 2 * t + 1) * k1;
           sum[p][2 * t] += lo, sum[p][2 * t + 1] += hi;
           o[t] = pack2_bf16(lo, hi);
@@ -347,7 +356,7 @@ __global__ __launch_bounds__(256) void k_gated_dz(const uint16_t* __restrict__ d
 
 // The parameters' gradients in their types: of each weight the splits' sums added in their
 // order, 4 elements a thread; of the biases the chunks', 8 lanes a column that take every
-// 8th, added in their order.
+// 8th, added in their order.  Bound by the sums' bytes: 2 x 2,048 x 768 in two splits 12 us.
 struct JoinArgs {
   const float* part;    // [splits][2 N][K]
   const float* part_b;  // [chunks][2 N]
@@ -510,7 +519,12 @@ __global__ __launch_bounds__(256) void k_gated_join_dx(const float* __restrict__
 // Aligned sizes.  One block: 64 FM rows by 64 outputs of both layers, 2 x 2 waves, each FM tiles
 // of 32 x 32 of the gate and the same of the other layer.  A wave takes a stage's
 // operands into registers before it multiplies, so the one buffer is free for the next
-// stage while it does, and two blocks on a CU fill each other's reads and epilogues.
+// stage while it does, and two blocks on a CU fill each other's reads.
+// 10,007 rows, 1,024 -> 4,096 without keep: 160 us, 1,050 TFLOP/s (a library product of the
+// same size and nothing else 143); 32,768 rows, 768 -> 2,048 with keep: 261, of which the loop is
+// 185 (its products and LDS reads alone 146, its loads alone 111), the rest arithmetic and 470 MB
+// of stores, which the loops of other blocks do not hide.  Measured at the first size: 256 rows
+// by 128 outputs in 8 waves with two buffers 175 us, 192 by 64 in two blocks with two buffers 168.
 template <int FM>
 __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
   constexpr int BM = 64 * FM, kRowsBytes = BM * 128;
@@ -520,9 +534,25 @@ __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
   if (!at.there) return;  // block-uniform
   const int m0 = at.m * BM, n0 = at.n * 64;
   const int wm = (wave >> 1) * FM, wn = wave & 1;  // in 32s
+  // A lane has outputs n .. n+15 of row a_row(lane) of each tile; its sums begin with their biases.
+  const int n = n0 + 32 * wn + 16 * half;
   f32x16 g[FM], u[FM];
+  g[0] = u[0] = fill16(0.f);
 #pragma unroll
-  for (int i = 0; i < FM; ++i) g[i] = u[i] = fill16(0.f);
+  for (int e = 0; e < 2; ++e) {
+    if (a.bg) {
+      const u32x4 b = load8<true>(a.bg, n + 8 * e, a.N);
+#pragma unroll
+      for (int t = 0; t < 8; ++t) g[0][8 * e + t] = half_of(b, t);
+    }
+    if (a.bu) {
+      const u32x4 b = load8<true>(a.bu, n + 8 * e, a.N);
+#pragma unroll
+      for (int t = 0; t < 8; ++t) u[0][8 * e + t] = half_of(b, t);
+    }
+  }
+#pragma unroll
+  for (int i = 1; i < FM; ++i) g[i] = g[0], u[i] = u[0];
   RowsOperand x, w;
   x.init(a.x_stride), w.init(a.K);
   const uint32_t mine = lds_at(lds) + 1024 * wave;
@@ -567,16 +597,10 @@ __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
   }
   all_there();  // nothing is on its way to LDS any more, of any wave
   meet();
-  // A lane has 16 consecutive outputs of row a_row(lane) of each tile.  They go through LDS,
-  // 32 rows at a time, so that a store's lanes fill 64 bytes of a row.
-  const int n = n0 + 32 * wn + 16 * half, back = lane / 4, n_back = n0 + 32 * wn + 8 * (lane % 4);
-  u32x4 bg[2], bu[2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    bg[e] = bu[e] = u32x4{0u, 0u, 0u, 0u};
-    if (a.bg) bg[e] = load8<true>(a.bg, n + 8 * e, a.N);
-    if (a.bu) bu[e] = load8<true>(a.bu, n + 8 * e, a.N);
-  }
+  // The results go through LDS, 32 rows at a time, so that a store's lanes, four neighbours a
+  // row, fill 64 bytes of it (exchanged between lanes without LDS, and with the next 32 rows
+  // computed meanwhile, the kernel was no faster).
+  const int back = lane / 4, n_back = n0 + 32 * wn + 8 * (lane % 4);
   char* stage = lds + 6144 * wave;
   auto slot = [&](int kind, int row, int piece) {
     return reinterpret_cast<u32x4*>(stage + 2048 * kind + 64 * row + 16 * (piece ^ (row >> 4 & 1)));
@@ -593,7 +617,7 @@ __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
         float sg[8], su[8];
 #pragma unroll
         for (int t = 0; t < 8; ++t) sg[t] = g[i][8 * e + t], su[t] = u[i][8 * e + t];
-        const Results r = results8<act.value, KEEP>(sg, su, bg[e], bu[e]);
+        const Results r = results8<act.value, KEEP>(sg, su);
         *slot(0, row, 2 * half + e) = r.y;
         if constexpr (KEEP) {
           *slot(1, row, 2 * half + e) = r.kg, *slot(2, row, 2 * half + e) = r.ku;
