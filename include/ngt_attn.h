@@ -838,7 +838,8 @@ int ngt_gated_bwd(const void* dy, const void* keep, const void* x, const void* w
  * (NeutronGT/models/graphormer_dist_node_level.py:128-173).
  */
 typedef struct ngt_head_rows {
-  const void* x;       /* [n_rows, n_heads, d], last dimension contiguous */
+  const void* x;       /* [n_rows, n_heads, d], last dimension contiguous; backward without
+                          a gain: not read */
   const void* gain;    /* [d], or null */
   void* y;             /* forward: the result; backward: dx (nullable) */
   const void* dy;      /* backward: the result's gradient, last dimension contiguous */

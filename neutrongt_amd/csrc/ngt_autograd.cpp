@@ -1050,7 +1050,9 @@ struct NormRotary : public torch::autograd::Function<NormRotary> {
     const Tensor gq = q_gain.has_value() ? q_gain->contiguous() : Tensor();
     const Tensor gk = k_gain.has_value() ? k_gain->contiguous() : Tensor();
     const auto y = rotary_forward(q3, k3, gq, gk, {positions, turns, interleaved, magnitude}, eps);
-    ctx->save_for_backward({q3, k3, gq, gk, positions, turns});
+    // (without a gain the backward does not need the input)
+    ctx->save_for_backward({gq.defined() ? q3 : Tensor(), gk.defined() ? k3 : Tensor(), gq, gk,
+                            positions, turns});
     ctx->saved_data["interleaved"] = interleaved;
     ctx->saved_data["magnitude"] = magnitude;
     ctx->saved_data["eps"] = eps;
@@ -1065,40 +1067,44 @@ struct NormRotary : public torch::autograd::Function<NormRotary> {
 
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &q = saved[0], &k = saved[1], &q_gain = saved[2], &k_gain = saved[3];
-    const at::DeviceGuard guard(q.device());
+    const Tensor &q_gain = saved[2], &k_gain = saved[3];
+    const at::DeviceGuard guard(grads[0].device());
+    const bool has_k = ctx->saved_data.count("k_shape") > 0;
     // the node's edges are numbered over the tensors that were given
     size_t edge = 0;
     tensor_list res(9);
-    auto wanted = [&](const Tensor& t) {
-      if (!t.defined()) return Tensor();
-      const bool w = ctx->needs_input_grad(edge++);
-      return w ? at::empty(t.sizes(), t.options()) : Tensor();
+    auto heads = [&](int i, const char* shape) {
+      const auto s = ctx->saved_data[shape].toIntVector();
+      if (ctx->needs_input_grad(edge++)) res[i] = at::empty(s, grads[i].options());
     };
-    res[0] = wanted(q), res[1] = wanted(k), res[2] = wanted(q_gain), res[3] = wanted(k_gain);
-    auto hq = head_struct(q, q_gain), hk = k.defined() ? head_struct(k, k_gain) : ngt_head_rows{};
-    const Tensor gq = head_rows(grads[0].to(q.scalar_type()));
-    const Tensor gk = k.defined() ? head_rows(grads[1].to(k.scalar_type())) : Tensor();
-    auto fill = [](ngt_head_rows& h, const Tensor& dy, const Tensor& dx, const Tensor& dgain) {
+    heads(0, "q_shape");
+    if (has_k) heads(1, "k_shape");
+    for (int i = 2; i < 4; ++i)
+      if (saved[i].defined() && ctx->needs_input_grad(edge++))
+        res[i] = at::empty(saved[i].sizes(), saved[i].options());
+    const Tensor gq = head_rows(grads[0]), gk = has_k ? head_rows(grads[1]) : Tensor();
+    auto fill = [](const Tensor& dy, const Tensor& x, const Tensor& gain, const Tensor& dx,
+                   const Tensor& dgain) {
+      auto h = gain.defined() ? head_struct(x, gain) : ngt_head_rows{};
+      h.n_heads = static_cast<int32_t>(dy.size(1));
       h.dy = dy.data_ptr(), h.dy_row = dy.stride(0), h.dy_head = dy.stride(1);
       if (dx.defined()) h.y = dx.data_ptr();
       if (dgain.defined()) h.dgain = dgain.data_ptr();
+      return h;
     };
-    fill(hq, gq, res[0], res[2]);
-    if (k.defined()) fill(hk, gk, res[1], res[3]);
+    const auto hq = fill(gq, saved[0], q_gain, res[0], res[2]);
+    const auto hk = has_k ? fill(gk, saved[1], k_gain, res[1], res[3]) : ngt_head_rows{};
+    const int64_t n = gq.size(0);
+    const auto d = static_cast<int32_t>(gq.size(2));
     size_t bytes = 0;
-    if (res[2].defined() || res[3].defined())
-      check(g_rotary_bwd_ws(q.size(0), static_cast<int32_t>(q.size(2)), &bytes));
-    const Tensor ws = bytes ? workspace(static_cast<int64_t>(bytes), q) : Tensor();
+    if (res[2].defined() || res[3].defined()) check(g_rotary_bwd_ws(n, d, &bytes));
+    const Tensor ws = bytes ? workspace(static_cast<int64_t>(bytes), gq) : Tensor();
     const auto rot = Turns{saved[4], saved[5], ctx->saved_data["interleaved"].toBool(),
                            ctx->saved_data["magnitude"].toDouble()}
                          .rotation();
-    check(g_rotary_bwd(dtype_code(q), &hq, k.defined() ? &hk : nullptr, q.size(0),
-                       static_cast<int32_t>(q.size(2)), &rot,
+    check(g_rotary_bwd(dtype_code(gq), &hq, has_k ? &hk : nullptr, n, d, &rot,
                        static_cast<float>(ctx->saved_data["eps"].toDouble()),
-                       bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)));
-    if (res[0].defined()) res[0] = res[0].view(ctx->saved_data["q_shape"].toIntVector());
-    if (res[1].defined()) res[1] = res[1].view(ctx->saved_data["k_shape"].toIntVector());
+                       bytes ? ws.data_ptr() : nullptr, bytes, stream_of(gq)));
     return once("norm_rotary", res);
   }
 };

@@ -14,7 +14,12 @@
 // formed once for all heads of a row, in LDS: the angle in fp64 turns, of which only the
 // part behind the quarter turn enters the fp32 functions, so that a far position
 // costs no precision.
+// bf16: 12,289 rows of 32 + 8 heads of 128 48 us, 5.3 TB/s; 32,768 rows of 32 + 32 heads of 24
+// 40 forward, 5.0 TB/s, and 69 backward, 4.4 TB/s (its sums take the registers of three
+// of the eight waves that the forward has on a SIMD).
 #include "ngt_common.h"
+
+#include <type_traits>
 
 namespace ngt {
 namespace {
@@ -48,7 +53,7 @@ struct Args {
   const void* positions;
   const double* turns;
   int64_t n_rows;
-  float eps, magnitude;
+  float eps, by_cos, by_sin;  // the rotation's magnitude; by_sin negative: turned back
   int32_t d, dim, units, group_log;  // 2^group_log lanes a head
   int32_t pos64;
 };
@@ -183,7 +188,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_rotary(const Args a) {
       const double p = a.pos64 ? static_cast<double>(static_cast<const int64_t*>(a.positions)[row0 + row])
                                : static_cast<double>(static_cast<const int32_t*>(a.positions)[row0 + row]);
       const float2 cs = cos_sin(p * a.turns[e - row * pairs]);
-      table[e] = make_float2(cs.x * a.magnitude, cs.y * a.magnitude);
+      table[e] = make_float2(cs.x * a.by_cos, cs.y * a.by_sin);
     }
     __syncthreads();
     const int items = rows * r.n_heads, step = groups * r.splits;
@@ -247,7 +252,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_rotary(const Args a) {
           for (int j = 0; j < V; ++j) {
             constexpr int kA = INTER ? 2 : 1, kB = INTER ? 1 : V;
             const int ia = kA * j, ib = kA * j + kB;
-            const float c = cs[j].x, s = BWD ? -cs[j].y : cs[j].y;
+            const float c = cs[j].x, s = cs[j].y;
             w[u][ia] = fmaf(in[ia], c, -(in[ib] * s));
             w[u][ib] = fmaf(in[ia], s, in[ib] * c);
           }
@@ -357,7 +362,7 @@ int check(const char* fn, int dtype, const ngt_head_rows* q, const ngt_head_rows
       return set_error(NGT_ERR_ARG, "%s: %d heads", fn, h->n_heads);
     if (h->gain && h->gain_dtype != NGT_F32 && h->gain_dtype != NGT_BF16)
       return set_error(NGT_ERR_ARG, "%s: gain dtype %d", fn, h->gain_dtype);
-    if (n_rows > 0 && (!h->x || (bwd ? !h->dy : !h->y)))
+    if (n_rows > 0 && ((!h->x && !(bwd && !h->gain)) || (bwd ? !h->dy : !h->y)))
       return set_error(NGT_ERR_ARG, "%s: null %s", fn, bwd ? "x or dy" : "x or y");
     if (h->dgain && !h->gain) return set_error(NGT_ERR_ARG, "%s: dgain without a gain", fn);
     if (h->x_row < 0 || h->x_head < 0 || h->dy_row < 0 || h->dy_head < 0)
@@ -380,11 +385,24 @@ int run(const char* fn, int dtype, const ngt_head_rows* q, const ngt_head_rows* 
   a.n_rows = n_rows, a.eps = eps, a.d = d;
   a.dim = rot ? rot->dim : 0;
   if (a.dim) {
-    a.positions = rot->positions, a.turns = rot->turns, a.magnitude = rot->magnitude;
+    a.positions = rot->positions, a.turns = rot->turns;
+    a.by_cos = rot->magnitude, a.by_sin = BWD ? -rot->magnitude : rot->magnitude;
     a.pos64 = rot->position_bytes == 8;
   }
+  // A gradient without a norm is its dy turned back: x is not read, and where neither has a norm
+  // the forward's kernel does it (fp32, 10,007 rows of 16 + 4 heads of 64: 20 us instead of 28).
+  ngt_head_rows own[2];
+  const ngt_head_rows* in[2] = {};
+  bool sums = false;
+  for (int i = 0; i < 2; ++i) {
+    const ngt_head_rows* h = i ? k : q;
+    if (!h) continue;
+    own[i] = *h, in[i] = &own[i];
+    if (!BWD) continue;
+    if (h->gain) sums = true;
+    else own[i].x = h->dy, own[i].x_row = h->dy_row, own[i].x_head = h->dy_head;
+  }
   // the widest pieces that sizes and alignment allow
-  const ngt_head_rows* in[2] = {q, k};
   int v = 16 / es;
   auto fits = [&](int n) {
     if (d % (2 * n) || a.dim % (2 * n)) return false;
@@ -411,18 +429,20 @@ int run(const char* fn, int dtype, const ngt_head_rows* q, const ngt_head_rows* 
     r.x = h->x, r.gain = h->gain, r.y = h->y, r.dy = h->dy;
     r.x_row = h->x_row, r.x_head = h->x_head, r.dy_row = h->dy_row, r.dy_head = h->dy_head;
     r.n_heads = h->n_heads, r.gain_f32 = h->gain_dtype == NGT_F32;
-    // 8 heads for each group, so that a row's cosines serve many
+    // 8 heads for each group, so that a row's cosines serve many (32,768 rows of 32 + 32 heads of 24,
+    // forward and backward: 4 heads 126 us, 8 116, 16 118)
     int rows = 8 * groups / h->n_heads;
     const int most = a.dim ? kTableBytes / (a.dim * 4) : 1024;
     rows = rows < 1 ? 1 : rows > most ? most : rows;
-    // .. unless that leaves CUs without a block
+    // .. unless that leaves CUs without a block (12,289 rows of 32 + 8 heads of 128: 512 blocks of
+    // keys 48.6 us, 256 50.4, 1,024 48.4)
     while (rows > 1 && (n_rows + rows - 1) / rows < 512) rows /= 2;
     r.tile_rows = rows;
     const int64_t tiles = (n_rows + rows - 1) / rows;
     r.tiles = static_cast<int32_t>(tiles);
     // a backward's blocks by the tensors' work
     const int all = h->n_heads + (in[1 - i] ? in[1 - i]->n_heads : 0);
-    int64_t most_blocks = BWD ? int64_t(kBwdBlocks) * h->n_heads / all : 1 << 20;
+    int64_t most_blocks = sums ? int64_t(kBwdBlocks) * h->n_heads / all : 1 << 20;
     if (most_blocks < 1) most_blocks = 1;
     const int rounds = (rows * h->n_heads + groups - 1) / groups;
     r.splits = 1;
@@ -443,16 +463,21 @@ int run(const char* fn, int dtype, const ngt_head_rows* q, const ngt_head_rows* 
     const int tile = a.r[0].tile_rows > a.r[1].tile_rows ? a.r[0].tile_rows : a.r[1].tile_rows;
     const size_t lds = size_t(tile) * (a.dim / 2) * sizeof(float2);
     const bool inter = rot && rot->interleaved;
-    if (dtype == NGT_F32) {
-      if (v == 4) launch<float, 4, 1, BWD>(a, inter, blocks, lds, st);
-      else if (v == 2) launch<float, 2, 1, BWD>(a, inter, blocks, lds, st);
-      else launch<float, 1, 2, BWD>(a, inter, blocks, lds, st);
-    } else {
-      if (v == 8) launch<bf16_t, 8, 1, BWD>(a, inter, blocks, lds, st);
-      else if (v == 4) launch<bf16_t, 4, 1, BWD>(a, inter, blocks, lds, st);
-      else if (v == 2) launch<bf16_t, 2, 1, BWD>(a, inter, blocks, lds, st);
-      else launch<bf16_t, 1, 2, BWD>(a, inter, blocks, lds, st);
-    }
+    auto go = [&](auto bwd) {
+      constexpr bool B = decltype(bwd)::value;
+      if (dtype == NGT_F32) {
+        if (v == 4) launch<float, 4, 1, B>(a, inter, blocks, lds, st);
+        else if (v == 2) launch<float, 2, 1, B>(a, inter, blocks, lds, st);
+        else launch<float, 1, 2, B>(a, inter, blocks, lds, st);
+      } else {
+        if (v == 8) launch<bf16_t, 8, 1, B>(a, inter, blocks, lds, st);
+        else if (v == 4) launch<bf16_t, 4, 1, B>(a, inter, blocks, lds, st);
+        else if (v == 2) launch<bf16_t, 2, 1, B>(a, inter, blocks, lds, st);
+        else launch<bf16_t, 1, 2, B>(a, inter, blocks, lds, st);
+      }
+    };
+    if (sums) go(std::true_type{});
+    else go(std::false_type{});
     NGT_HIP_CHECK(hipGetLastError());
   }
   if (BWD && (join.out[0] || join.out[1])) {

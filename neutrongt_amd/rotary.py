@@ -97,9 +97,12 @@ class Rotary:
 
 
 def _head_rows(x, gain, y=None, dy=None, dgain=None):
-    """The ngt_head_rows of x [n, heads, d] and, backward, its result's gradient."""
+    """The ngt_head_rows of x [n, heads, d] (backward: None without a gain) and, backward, its
+    result's gradient."""
     r = _lib.HeadRowsC()
-    r.x, r.x_row, r.x_head, r.n_heads = x.data_ptr(), x.stride(0), x.stride(1), x.shape[1]
+    if x is not None:
+        r.x, r.x_row, r.x_head = x.data_ptr(), x.stride(0), x.stride(1)
+    r.n_heads = (x if x is not None else dy).shape[1]
     if gain is not None:
         r.gain, r.gain_dtype = gain.data_ptr(), _dtype_code(gain)
     if y is not None:
@@ -131,8 +134,8 @@ def _rows(t):
 
 class NormRotaryFunction(torch.autograd.Function):
     """(q', k') of q [n, H, d] and k [n, H_kv, d] or None (ngt_norm_rotary_fwd /
-    ngt_norm_rotary_bwd); the backward reads the inputs again and keeps nothing
-    else."""
+    ngt_norm_rotary_bwd); the backward reads the normed inputs again and keeps
+    nothing else."""
 
     @staticmethod
     def forward(ctx, q, k, q_gain, k_gain, positions, rotary, eps):
@@ -144,7 +147,9 @@ class NormRotaryFunction(torch.autograd.Function):
                 _dtype_code(q), _by(_head_rows(q, q_gain, yq)),
                 _by(_head_rows(k, k_gain, yk) if k is not None else None), q.shape[0], q.shape[2],
                 _by(_rotation(rotary, positions)), eps, _stream(dev)))
-        ctx.save_for_backward(q, k, q_gain, k_gain, positions)
+        # (without a gain the backward does not need the input)
+        ctx.save_for_backward(q if q_gain is not None else None, k if k_gain is not None else None,
+                              q_gain, k_gain, positions)
         ctx.rotary, ctx.eps = rotary, eps
         return (yq, yk) if k is not None else yq
 
@@ -152,21 +157,21 @@ class NormRotaryFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gq, gk=None):
         q, k, q_gain, k_gain, positions = ctx.saved_tensors
-        dev, want = q.device, ctx.needs_input_grad
+        dev, want = gq.device, ctx.needs_input_grad
         new = lambda t, wanted: torch.empty(t.shape, dtype=t.dtype, device=dev) if (
             t is not None and wanted) else None
-        dq, dk, dgq, dgk = (new(t, w) for t, w in zip((q, k, q_gain, k_gain), want))
-        gq = _rows(gq.to(q.dtype))
-        gk = _rows(gk.to(k.dtype)) if k is not None else None
+        dq, dk, dgq, dgk = (new(t, w) for t, w in zip((gq, gk, q_gain, k_gain), want))
+        gq = _rows(gq)
+        gk = _rows(gk) if gk is not None else None
+        n, _, d = gq.shape
         nb = C.c_size_t()
-        _lib.check(_lib.load().ngt_norm_rotary_bwd_workspace_bytes(q.shape[0], q.shape[2],
-                                                                   C.byref(nb)))
+        _lib.check(_lib.load().ngt_norm_rotary_bwd_workspace_bytes(n, d, C.byref(nb)))
         ws = _workspace(nb.value, dev) if dgq is not None or dgk is not None else None
         with torch.cuda.device(dev):
             _lib.check(_lib.load().ngt_norm_rotary_bwd(
-                _dtype_code(q), _by(_head_rows(q, q_gain, dq, gq, dgq)),
-                _by(_head_rows(k, k_gain, dk, gk, dgk) if k is not None else None), q.shape[0],
-                q.shape[2], _by(_rotation(ctx.rotary, positions)), ctx.eps,
+                _dtype_code(gq), _by(_head_rows(q, q_gain, dq, gq, dgq)),
+                _by(_head_rows(k, k_gain, dk, gk, dgk) if gk is not None else None), n, d,
+                _by(_rotation(ctx.rotary, positions)), ctx.eps,
                 ws.data_ptr() if ws is not None else None, nb.value if ws is not None else 0,
                 _stream(dev)))
         return dq, dk, dgq, dgk, None, None, None

@@ -55,6 +55,7 @@ def test_norm_rotary_refusals_touch_no_gpu():
     assert lib.ngt_norm_rotary_bwd_workspace_bytes(4, 16, C.byref(nb)) == 0 and nb.value > 0
     gain = dict(gain=P, dgain=P)
     for bad, code in ((dict(q=_heads(dy=None)), 1), (dict(q=_heads(dgain=P)), 1),
+                      (dict(q=_heads(x=None, gain=P)), 1),
                       (dict(q=_heads(**gain), ws=None), 4), (dict(q=_heads(**gain), nb=nb.value - 1), 4),
                       (dict(q=_heads(**gain), ws=P + 8), 4)):
         assert bwd(**bad) == code, bad

@@ -218,6 +218,31 @@ def test_only_some_gradients(dev):
     assert torch.equal(dq, full[0]) and not dk.any() and torch.equal(dgq, full[2]) and not dgk.any()
 
 
+@pytest.mark.parametrize("node", [True, False])
+def test_without_a_norm_the_input_is_not_kept(dev, node, monkeypatch):
+    """What has no gain may change or go before the backward; what has one may not change."""
+    if not node:
+        monkeypatch.setattr(_lib, "node_ext", lambda: None)
+    g = torch.Generator().manual_seed(4)
+    q, k = (torch.randn(50, h, 16, generator=g).to(dev).requires_grad_() for h in (4, 2))
+    gain, gq, gk = _gain(16, g, F32).to(dev), torch.randn_like(q), torch.randn_like(k)
+    pos, rot = torch.arange(50, device=dev), Rotary(12, device=dev)
+    for gains in ((None, None), (None, gain), (gain, None)):
+        want = torch.autograd.grad(norm_rotary(q, k, pos, rot, *gains), (q, k), (gq, gk))
+        ys = norm_rotary(q, k, pos, rot, *gains)
+        with torch.no_grad():
+            for t, gt in zip((q, k), gains):
+                if gt is None:
+                    t.add_(1)
+        assert all(torch.equal(a, b) for a, b in
+                   zip(torch.autograd.grad(ys, (q, k), (gq, gk)), want))
+    ys = norm_rotary(q, k, pos, rot, gain)
+    with torch.no_grad():
+        q.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(ys, (q, k), (gq, gk))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("rotate", [False, True])
 def test_the_cpp_node_and_the_python_class_give_the_same_bits(dev, dtype, rotate, monkeypatch):
