@@ -521,14 +521,14 @@ __global__ __launch_bounds__(256) void k_gated_join_dx(const float* __restrict__
 // operands into registers before it multiplies, so the one buffer is free for the next
 // stage while it does, and two blocks on a CU fill each other's reads.
 // 10,007 rows, 1,024 -> 4,096 without keep: 160 us, 1,050 TFLOP/s (a library product of the
-// same size and nothing else 143); 32,768 rows, 768 -> 2,048 with keep: 261, of which the loop is
+// same size and nothing else 143); 32,768 rows, 768 -> 2,048 with keep: 258, of which the loop is
 // 185 (its products and LDS reads alone 146, its loads alone 111), the rest arithmetic and 470 MB
 // of stores, which the loops of other blocks do not hide.  Measured at the first size: 256 rows
 // by 128 outputs in 8 waves with two buffers 175 us, 192 by 64 in two blocks with two buffers 168.
 template <int FM>
 __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
   constexpr int BM = 64 * FM, kRowsBytes = BM * 128;
-  __shared__ __align__(16) char lds[kRowsBytes + 128 * 128];  // (6 KB a wave for the results)
+  __shared__ __align__(16) char lds[FM > 1 ? 49152 : kRowsBytes + 128 * 128];
   const int lane = tid_x() & 63, wave = packed::wave_id(), half = lane >> 5;
   const TileAt at = tile_at(a.tiles_m, a.tiles_n, 1);
   if (!at.there) return;  // block-uniform
@@ -597,20 +597,20 @@ __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
   }
   all_there();  // nothing is on its way to LDS any more, of any wave
   meet();
-  // The results go through LDS, 32 rows at a time, so that a store's lanes, four neighbours a
-  // row, fill 64 bytes of it (exchanged between lanes without LDS, and with the next 32 rows
-  // computed meanwhile, the kernel was no faster).
-  const int back = lane / 4, n_back = n0 + 32 * wn + 8 * (lane % 4);
-  char* stage = lds + 6144 * wave;
-  auto slot = [&](int kind, int row, int piece) {
-    return reinterpret_cast<u32x4*>(stage + 2048 * kind + 64 * row + 16 * (piece ^ (row >> 4 & 1)));
+  // The results go through LDS, 64 rows at a time in two buffers, so that a store's lanes fill
+  // the 128 bytes of each of 8 rows (64 bytes of 16: 265 us instead of 258 in the second size
+  // above, and 12 % more bytes written).  f: 16 neighbouring lanes meet all 64 banks.
+  const int back = 16 * wave + lane / 8, n_back = n0 + 8 * (lane % 8);
+  auto slot = [&](int i, int kind, int row, int piece) {
+    const int f = (row >> 1 & 3) | (row >> 2 & 4);
+    return reinterpret_cast<u32x4*>(lds + 24576 * (i & 1) + 8192 * kind + 128 * row + 16 * (piece ^ f));
   };
   const Keep kept(a.M, a.N);
   with_act(a.act, a.keep != nullptr, [&](auto act, auto keep) {
     constexpr bool KEEP = decltype(keep)::value;
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-      const int row = L::a_row(lane & 31), m = m0 + 32 * (wm + i) + row;
+      const int row = L::a_row(lane & 31), m = m0 + 32 * (wm + i) + row, at = 32 * (wave >> 1) + row;
       uint2 lg, lu;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -618,9 +618,9 @@ __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
 #pragma unroll
         for (int t = 0; t < 8; ++t) sg[t] = g[i][8 * e + t], su[t] = u[i][8 * e + t];
         const Results r = results8<act.value, KEEP>(sg, su);
-        *slot(0, row, 2 * half + e) = r.y;
+        *slot(i, 0, at, 4 * wn + 2 * half + e) = r.y;
         if constexpr (KEEP) {
-          *slot(1, row, 2 * half + e) = r.kg, *slot(2, row, 2 * half + e) = r.ku;
+          *slot(i, 1, at, 4 * wn + 2 * half + e) = r.kg, *slot(i, 2, at, 4 * wn + 2 * half + e) = r.ku;
           (e ? lg.y : lg.x) = r.lg, (e ? lu.y : lu.x) = r.lu;
         }
       }
@@ -629,16 +629,17 @@ __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
           *reinterpret_cast<uint2*>(kept.low(a.keep, m, 0, n)) = lg;
           *reinterpret_cast<uint2*>(kept.low(a.keep, m, 1, n)) = lu;
         }
+      all_read();
+      meet();
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const int r_back = back + 16 * q, m_back = m0 + 32 * (wm + i) + r_back;
-        const u32x4 y = *slot(0, r_back, lane % 4);
+        const int r = back + 8 * q, m_back = m0 + 32 * ((r >> 5) * FM + i) + (r & 31);
+        const u32x4 y = *slot(i, 0, r, lane % 8);
         u32x4 kg, ku;
-        if constexpr (KEEP) kg = *slot(1, r_back, lane % 4), ku = *slot(2, r_back, lane % 4);
+        if constexpr (KEEP) kg = *slot(i, 1, r, lane % 8), ku = *slot(i, 2, r, lane % 8);
         if (m_back >= a.M || n_back >= a.N) continue;
         *reinterpret_cast<u32x4*>(a.y + int64_t(m_back) * a.N + n_back) = y;
         if constexpr (KEEP) {
-          // not read again before the backward
           __builtin_nontemporal_store(kg, reinterpret_cast<u32x4*>(kept.high(a.keep, m_back, 0) + n_back));
           __builtin_nontemporal_store(ku, reinterpret_cast<u32x4*>(kept.high(a.keep, m_back, 1) + n_back));
         }
