@@ -15,7 +15,7 @@
 // part behind the quarter turn enters the fp32 functions, so that a far position
 // costs no precision.
 // bf16: 12,289 rows of 32 + 8 heads of 128 48 us, 5.3 TB/s; 32,768 rows of 32 + 32 heads of 24
-// 40 forward, 5.0 TB/s, and 69 backward, 4.4 TB/s (its sums take the registers of three
+// 40 forward, 5.0 TB/s, and 67 backward, 4.5 TB/s (its sums take the registers of two
 // of the eight waves that the forward has on a SIMD).
 #include "ngt_common.h"
 
@@ -28,9 +28,11 @@ constexpr int kThreads = 256;
 constexpr int kMaxDim = 256;
 constexpr int64_t kMaxRows = int64_t(1) << 30;
 constexpr int kTableBytes = 16384;  // cosines and sines of a block's rows
-// About the most blocks, so partial sums, of a backward: five a CU is what its registers allow
-// (32,768 rows of 32 + 32 heads of 24, bf16: 1,024 blocks 82 us, 1,280 76, 2,048 84).
-constexpr int kBwdBlocks = 1280;
+// Blocks of a backward that a CU holds, by the registers of its sums, for pieces of `bytes`; a
+// launch has about as many, each with a partial sum (bf16, 32,768 rows of 32 + 32 heads of 24:
+// 1,024 blocks 76 us, 1,280 71, 1,536 67; 12,289 of 32 + 8 of 128: 768 86 us, 1,024 85, 1,280 90).
+constexpr int bwd_blocks(int bytes, int es) { return bytes <= 8 ? 6 : es == 2 ? 4 : 5; }
+constexpr int kBwdBlocks = 6 * 256;
 inline size_t sums_bytes(int32_t d) { return size_t(kBwdBlocks + 2) * d * sizeof(float); }
 
 // One of queries and keys, as the kernels see it.
@@ -135,7 +137,7 @@ __device__ __forceinline__ float inverse_root(float x) {
 
 // V pairs of components of each of a lane's U units; INTER: pairs are adjacent.
 template <typename T, int V, int U, bool INTER, bool BWD>
-__global__ __launch_bounds__(kThreads) void k_norm_rotary(const Args a) {
+__global__ __launch_bounds__(kThreads, BWD ? bwd_blocks(V * sizeof(T), sizeof(T)) : 1) void k_norm_rotary(const Args a) {
   extern __shared__ float2 table[];  // [tile_rows][dim / 2]
   __shared__ float sums[BWD ? kThreads / kWave : 1][BWD ? kMaxDim : 1];
   const int tid = threadIdx.x;
@@ -442,7 +444,7 @@ int run(const char* fn, int dtype, const ngt_head_rows* q, const ngt_head_rows* 
     r.tiles = static_cast<int32_t>(tiles);
     // a backward's blocks by the tensors' work
     const int all = h->n_heads + (in[1 - i] ? in[1 - i]->n_heads : 0);
-    int64_t most_blocks = sums ? int64_t(kBwdBlocks) * h->n_heads / all : 1 << 20;
+    int64_t most_blocks = sums ? int64_t(256 * bwd_blocks(v * es, es)) * h->n_heads / all : 1 << 20;
     if (most_blocks < 1) most_blocks = 1;
     const int rounds = (rows * h->n_heads + groups - 1) / groups;
     r.splits = 1;

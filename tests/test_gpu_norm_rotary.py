@@ -85,6 +85,10 @@ def test_more_tiles_than_blocks_of_the_backward(dev, n):
     _case(dev, n, 4, 1, 16, 8, "interleaved", BF16, far=n, seed=n)
 
 
+def test_more_rounds_of_many_heads(dev):
+    _case(dev, 11003, 64, 64, 16, 16, "half", F32, far=11003, seed=8)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("norm", [(True, False), (False, True), (False, False)])
 def test_norms_of_one_of_them_or_none(dev, norm, dtype):
