@@ -796,7 +796,8 @@ int ngt_wgrad_bf16(const void* x, const void* dy, int64_t n_rows, int32_t n_out,
  * n_in] (rows x_stride elements apart), Wg and Wu [n_out, n_in] and biases [n_out]
  * (nullable), summed in fp32 and rounded once; sizes and alignment as ngt_linear_fwd.
  * keep, where not null, receives what the backward needs (zu act'(zg) and act(zg), each to
- * 12 bits of mantissa): ngt_gated_keep_bytes, 16-byte aligned.
+ * 12 bits of mantissa): ngt_gated_keep_bytes, 16-byte aligned.  workspace: 16-byte aligned,
+ * ngt_gated_fwd_workspace_bytes (0: none).
  * ngt_gated_bwd: from dy, what was kept and x (dy and x contiguous) the gradients that are not
  * null: dx [n_rows, n_in] bf16, and those of weights and biases in their own types, from
  * fp32 sums in a fixed order.  All matrices and the workspace are 16-byte aligned.
@@ -814,9 +815,11 @@ typedef struct ngt_gated_grads {
 } ngt_gated_grads;
 
 int ngt_gated_keep_bytes(int64_t n_rows, int32_t n_out, size_t* bytes);
+int ngt_gated_fwd_workspace_bytes(int64_t n_rows, int32_t n_out, int32_t n_in, size_t* bytes);
 int ngt_gated_fwd(const void* x, int64_t x_stride, const void* w_gate, const void* w_up,
-                  const void* b_gate, const void* b_up, int64_t n_rows, int32_t n_out,
-                  int32_t n_in, int32_t activation, void* y, void* keep, void* stream);
+                  const void* b_gate, const void* b_up, int64_t n_rows, int32_t n_out, int32_t n_in,
+                  int32_t activation, void* y, void* keep, void* workspace, size_t workspace_bytes,
+                  void* stream);
 int ngt_gated_bwd_workspace_bytes(int64_t n_rows, int32_t n_out, int32_t n_in, size_t* bytes);
 int ngt_gated_bwd(const void* dy, const void* keep, const void* x, const void* w_gate,
                   const void* w_up, int64_t n_rows, int32_t n_out, int32_t n_in,

@@ -238,7 +238,8 @@ SIGNATURES = {
     "ngt_linear_bwd_workspace_bytes": [_i64, _i32, _i32, _psz],
     "ngt_linear_bwd": [_vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _sz, _vp],
     "ngt_gated_keep_bytes": [_i64, _i32, _psz],
-    "ngt_gated_fwd": [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp],
+    "ngt_gated_fwd_workspace_bytes": [_i64, _i32, _i32, _psz],
+    "ngt_gated_fwd": [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _sz, _vp],
     "ngt_gated_bwd_workspace_bytes": [_i64, _i32, _i32, _psz],
     "ngt_gated_bwd": [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _pgg, _vp, _sz, _vp],
     "ngt_norm_rotary_fwd": [_i32, _phr, _phr, _i64, _i32, _prot, _f32, _vp],

@@ -75,6 +75,7 @@ decltype(&ngt_linear_fwd) g_linear_fwd = nullptr;
 decltype(&ngt_linear_bwd_workspace_bytes) g_linear_bwd_ws = nullptr;
 decltype(&ngt_linear_bwd) g_linear_bwd = nullptr;
 decltype(&ngt_gated_keep_bytes) g_gated_keep = nullptr;
+decltype(&ngt_gated_fwd_workspace_bytes) g_gated_fwd_ws = nullptr;
 decltype(&ngt_gated_fwd) g_gated_fwd = nullptr;
 decltype(&ngt_gated_bwd_workspace_bytes) g_gated_bwd_ws = nullptr;
 decltype(&ngt_gated_bwd) g_gated_bwd = nullptr;
@@ -906,11 +907,16 @@ GatedForward gated_forward(const Tensor& x, const Tensor& w_gate, const Tensor& 
     check(g_gated_keep(m, static_cast<int32_t>(n_out), &bytes));
     r.keep = workspace(static_cast<int64_t>(bytes), r.x2);
   }
+  const auto n = static_cast<int32_t>(n_out), k = static_cast<int32_t>(n_in);
+  size_t bytes = 0;
+  check(g_gated_fwd_ws(m, n, k, &bytes));
+  const Tensor ws = bytes ? workspace(static_cast<int64_t>(bytes), r.x2) : Tensor();
   check(g_gated_fwd(r.x2.data_ptr(), m > 1 ? r.x2.stride(0) : n_in, r.wg.data_ptr(),
                     r.wu.data_ptr(), bg.defined() ? bg.data_ptr() : nullptr,
-                    bu.defined() ? bu.data_ptr() : nullptr, m, static_cast<int32_t>(n_out),
-                    static_cast<int32_t>(n_in), static_cast<int32_t>(act), r.y.data_ptr(),
-                    want_grad ? r.keep.data_ptr() : nullptr, stream_of(x)));
+                    bu.defined() ? bu.data_ptr() : nullptr, m, n, k,
+                    static_cast<int32_t>(act), r.y.data_ptr(),
+                    want_grad ? r.keep.data_ptr() : nullptr, bytes ? ws.data_ptr() : nullptr, bytes,
+                    stream_of(x)));
   return r;
 }
 
@@ -1265,6 +1271,7 @@ void init(const std::map<std::string, int64_t>& addr) {
   entry(g_linear_bwd_ws, addr, "ngt_linear_bwd_workspace_bytes");
   entry(g_linear_bwd, addr, "ngt_linear_bwd");
   entry(g_gated_keep, addr, "ngt_gated_keep_bytes");
+  entry(g_gated_fwd_ws, addr, "ngt_gated_fwd_workspace_bytes");
   entry(g_gated_fwd, addr, "ngt_gated_fwd");
   entry(g_gated_bwd_ws, addr, "ngt_gated_bwd_workspace_bytes");
   entry(g_gated_bwd, addr, "ngt_gated_bwd");

@@ -23,7 +23,11 @@ struct GatedArgs {
   int64_t x_stride;
   int32_t M, N, K, act;
   int32_t tiles_m, tiles_n;
+  // where the contraction is split: [splits][2][M][N filled up to 8s], and a split's elements of it
+  float* part;
+  int32_t splits, per_split;
 };
+__host__ __device__ constexpr int32_t up8(int32_t n) { return (n + 7) / 8 * 8; }
 
 // act(z) and act'(z).
 struct Gate {
@@ -131,6 +135,39 @@ __device__ __forceinline__ void finish8(const GatedArgs& a, int m, int n, const 
   }
 }
 
+// The same outputs' sums over a split of the contraction.
+__device__ __forceinline__ void part8(const GatedArgs& a, int split, int m, int n,
+                                      const float (&sg)[8], const float (&su)[8]) {
+  if (m >= a.M || n >= a.N) return;
+  float* to = a.part + (int64_t(2 * split) * a.M + m) * up8(a.N) + n;
+#pragma unroll
+  for (int t = 0; t < 8; t += 4) {
+    *reinterpret_cast<float4*>(to + t) = make_float4(sg[t], sg[t + 1], sg[t + 2], sg[t + 3]);
+    *reinterpret_cast<float4*>(to + int64_t(a.M) * up8(a.N) + t) =
+        make_float4(su[t], su[t + 1], su[t + 2], su[t + 3]);
+  }
+}
+// The splits' sums added in their order, and what becomes of them; 8 outputs a thread.
+__global__ __launch_bounds__(256) void k_gated_join_fwd(GatedArgs a) {
+  const int across = up8(a.N) / 8, i = wg_x() * 256 + tid_x();
+  if (i >= a.M * across) return;
+  const int64_t layer = int64_t(a.M) * across * 8;
+  float s[2][8] = {};
+#pragma unroll 4
+  for (int c = 0; c < a.splits; ++c)
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const float* from = a.part + (2 * c + p) * layer + int64_t(i) * 8;
+#pragma unroll
+      for (int t = 0; t < 8; t += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(from + t);
+        s[p][t] += v.x, s[p][t + 1] += v.y, s[p][t + 2] += v.z, s[p][t + 3] += v.w;
+      }
+    }
+  const int m = i / across;
+  finish8(a, m, (i - m * across) * 8, s[0], s[1]);
+}
+
 // Any sizes and 2-byte alignment.  One block: 64 rows by 64 outputs of both products,
 // 2 x 2 waves of 32 x 32, stages of 64 of the contraction read into registers while the
 // stage before is multiplied.  32,768 rows, 768 -> 2,048 in it: 350 us (k_gated 231).
@@ -138,7 +175,9 @@ __global__ __launch_bounds__(256) void k_gated_any(GatedArgs a) {
   constexpr int NP = 64 * 8 / 256;  // 16-byte pieces per thread and operand
   __shared__ __align__(16) char lds[3][64 * 128];
   const int tid = tid_x(), lane = tid & 63, wave = tid >> 6, half = lane >> 5, l32 = lane & 31;
-  const int m0 = wg_x() / a.tiles_n * 64, n0 = wg_x() % a.tiles_n * 64;
+  const int tiles = a.tiles_m * a.tiles_n, split = wg_x() / tiles, tile = wg_x() - split * tiles;
+  const int m0 = tile / a.tiles_n * 64, n0 = tile % a.tiles_n * 64;
+  const int first = split * a.per_split, end = min(first + a.per_split, a.K);
   const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
   f32x16 g = fill16(0.f), u = fill16(0.f);
   u32x4 p[3][NP];
@@ -154,8 +193,8 @@ __global__ __launch_bounds__(256) void k_gated_any(GatedArgs a) {
       }
     }
   };
-  fetch(0);
-  for (int k = 0; k < a.K; k += kStage) {
+  fetch(first);
+  for (int k = first; k < end; k += kStage) {
     __syncthreads();
 #pragma unroll
     for (int o = 0; o < 3; ++o)
@@ -165,7 +204,7 @@ __global__ __launch_bounds__(256) void k_gated_any(GatedArgs a) {
         *reinterpret_cast<u32x4*>(lds[o] + L::offset(e / 8, e % 8)) = p[o][i];
       }
     __syncthreads();
-    fetch(k + kStage);  // (behind the last stage: zeros)
+    fetch(k + kStage);  // (behind the contraction: zeros)
 #pragma unroll
     for (int c = 0; c < L::kChunks; ++c) {
       const L::Op x = L::load_a(lds[0] + wm * 128, 0, c, l32, half);
@@ -178,7 +217,9 @@ __global__ __launch_bounds__(256) void k_gated_any(GatedArgs a) {
     float sg[8], su[8];
 #pragma unroll
     for (int t = 0; t < 8; ++t) sg[t] = g[8 * e + t], su[t] = u[8 * e + t];
-    finish8(a, m0 + wm + L::a_row(l32), n0 + wn + 16 * half + 8 * e, sg, su);
+    const int m = m0 + wm + L::a_row(l32), n = n0 + wn + 16 * half + 8 * e;
+    if (a.splits > 1) part8(a, split, m, n, sg, su);
+    else finish8(a, m, n, sg, su);
   }
 }
 
@@ -193,7 +234,9 @@ __global__ __launch_bounds__(64 * WAVES) void k_gated_few(GatedArgs a) {
   constexpr int kTiles = 2 * NT * MT;
   __shared__ __align__(16) float red[WAVES][kTiles][16][20];  // [x row][output], padded
   const int lane = tid_x() & 63, wave = packed::wave_id(), quad = lane >> 4, l16 = lane & 15;
-  const int n0 = wg_x() * 16 * NT;
+  const int blocks = (a.N + 16 * NT - 1) / (16 * NT), split = wg_x() / blocks;
+  const int n0 = (wg_x() - split * blocks) * 16 * NT;
+  const int first = split * a.per_split, end = min(first + a.per_split, a.K);
   f32x4 acc[2][NT][MT];
 #pragma unroll
   for (int p = 0; p < 2; ++p)
@@ -245,8 +288,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_gated_few(GatedArgs a) {
                 __builtin_bit_cast(packed::bf16x8, s.x[h][i]), acc[p][j][i], 0, 0, 0);
   };
   constexpr int kApart = 64 * WAVES;
-  Step now = fetch(64 * wave);
-  for (int k = 64 * wave; k < a.K; k += kApart) {
+  Step now = fetch(first + 64 * wave);
+  for (int k = first + 64 * wave; k < end; k += kApart) {
     const Step next = fetch(k + kApart);
     multiply(now);
     now = next;
@@ -273,7 +316,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_gated_few(GatedArgs a) {
         for (int t = 0; t < 8; ++t)
           s[p][t] += red[v][(p * NT + j) * MT + m / 16][m % 16][8 * half + t];
     }
-    finish8(a, m, n0 + 16 * j + 8 * half, s[0], s[1]);
+    if (a.splits > 1) part8(a, split, m, n0 + 16 * j + 8 * half, s[0], s[1]);
+    else finish8(a, m, n0 + 16 * j + 8 * half, s[0], s[1]);
   }
 }
 
@@ -427,7 +471,6 @@ struct DxArgs {
   int32_t M, N, K;
   int32_t tiles_k, tiles, per_split;  // stages of a split
 };
-__host__ __device__ constexpr int32_t up8(int32_t n) { return (n + 7) / 8 * 8; }
 
 // dx = dzg Wg + dzu Wu at any sizes and alignment: the same blocks, 64 rows by 64 of K,
 // contracted over the outputs of one layer and then of the other (a stage holds one
@@ -530,9 +573,13 @@ __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
   constexpr int BM = 64 * FM, kRowsBytes = BM * 128;
   __shared__ __align__(16) char lds[FM > 1 ? 49152 : kRowsBytes + 128 * 128];
   const int lane = tid_x() & 63, wave = packed::wave_id(), half = lane >> 5;
-  const TileAt at = tile_at(a.tiles_m, a.tiles_n, 1);
+  constexpr bool kSplit = FM == 1;  // (taller tiles are for many blocks)
+  const TileAt at = tile_at(a.tiles_m, a.tiles_n, kSplit ? a.splits : 1);
   if (!at.there) return;  // block-uniform
   const int m0 = at.m * BM, n0 = at.n * 64;
+  const int first = kSplit ? at.split * a.per_split : 0;
+  const int end = kSplit ? min(first + a.per_split, a.K) : a.K;
+  const bool parts = kSplit && a.splits > 1;
   const int wm = (wave >> 1) * FM, wn = wave & 1;  // in 32s
   // A lane has outputs n .. n+15 of row a_row(lane) of each tile; its sums begin with their biases.
   const int n = n0 + 32 * wn + 16 * half;
@@ -540,12 +587,12 @@ __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
   g[0] = u[0] = fill16(0.f);
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    if (a.bg) {
+    if (a.bg && !parts) {
       const u32x4 b = load8<true>(a.bg, n + 8 * e, a.N);
 #pragma unroll
       for (int t = 0; t < 8; ++t) g[0][8 * e + t] = half_of(b, t);
     }
-    if (a.bu) {
+    if (a.bu && !parts) {
       const u32x4 b = load8<true>(a.bu, n + 8 * e, a.N);
 #pragma unroll
       for (int t = 0; t < 8; ++t) u[0][8 * e + t] = half_of(b, t);
@@ -570,8 +617,8 @@ __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
       w.load(fw, 0, k, a.K, mine + kRowsBytes + 4096 * i);
     }
   };
-  fetch(0);
-  for (int k = 0; k < a.K; k += kStage) {
+  fetch(first);
+  for (int k = first; k < end; k += kStage) {
     all_there();
     meet();
     L::Op fx[L::kChunks][FM], fw[L::kChunks][2];
@@ -584,7 +631,7 @@ __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
     }
     all_read();
     meet();
-    fetch(k + kStage);  // (behind the last stage: zeros)
+    fetch(k + kStage);  // (behind the contraction: zeros)
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int c = 0; c < L::kChunks; ++c)
@@ -596,6 +643,16 @@ __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
     __builtin_amdgcn_sched_barrier(0);
   }
   all_there();  // nothing is on its way to LDS any more, of any wave
+  if (parts) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float sg[8], su[8];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) sg[t] = g[0][8 * e + t], su[t] = u[0][8 * e + t];
+      part8(a, at.split, m0 + 32 * wm + L::a_row(lane & 31), n + 8 * e, sg, su);
+    }
+    return;
+  }
   meet();
   // The results go through LDS, 64 rows at a time in two buffers, so that a store's lanes fill
   // the 128 bytes of each of 8 rows (64 bytes of 16: 265 us instead of 258 in the second size
@@ -693,6 +750,42 @@ int plan_bwd(int64_t M, int32_t N, int32_t K, BwdPlan* p) {
   return NGT_OK;
 }
 
+// How a forward's contraction is split, in elements, where there are few blocks: each split's sums
+// are written and read again (about 4 TB/s), so the best number is a square root, as in the
+// backward; none below 4 stages of 64 each, nor where it saves less than the second launch and a
+// block's start and end again, 8 us.  us, one split / several: 1,024 outputs of 4,096 at 64 rows 27 /
+// 22, at 65 43 / 19, at 1,200 48 / 43; 64 of 8,192 at 1 row 21 / 13, at 300 78 / 19; 255 of 8,191 at 65
+// 118 / 26.
+struct Split {
+  int32_t splits, per_split;
+};
+Split split_of(int64_t M, int32_t N, int32_t K, double stage, int64_t stages, int32_t elements,
+               int64_t most) {
+  const double sums = 2e-6 / 4 * 8 * double(M) * N;
+  const double want = std::sqrt(stage * double(stages) / sums);
+  int64_t splits = want < double(most) ? std::llround(want) : most;
+  if (splits < 2 || stage * double(stages) * (1.0 - 1.0 / double(splits)) < 8.0 + sums * double(splits))
+    return {1, K};
+  const int64_t per = (stages + splits - 1) / splits;
+  return {static_cast<int32_t>((stages + per - 1) / per), static_cast<int32_t>(per * elements)};
+}
+constexpr int kFewRows = 64;
+Split few_split(int64_t M, int32_t N, int32_t K) {
+  // a step of the 8 waves takes 512 elements, and 1.2 us and the rows' share
+  const int64_t stages = (int64_t(K) + 511) / 512;
+  return split_of(M, N, K, 1.2 + 0.03 * double(M), stages, 512, std::min<int64_t>(512 / ((N + 15) / 16), stages));
+}
+Split tile_split(int64_t M, int32_t N, int32_t K) {
+  const int64_t stages = (int64_t(K) + 63) / 64, tiles = (M + 63) / 64 * ((N + 63) / 64);
+  return split_of(M, N, K, 0.65, stages, 64, std::min<int64_t>(768 / std::max<int64_t>(tiles, 1), stages / 4));
+}
+size_t fwd_bytes(int64_t M, int32_t N, int32_t K) {
+  if (M == 0) return 0;
+  int32_t splits = tile_split(M, N, K).splits;
+  if (M <= kFewRows) splits = std::max(splits, few_split(M, N, K).splits);
+  return splits > 1 ? size_t(splits) * 2 * M * up8(N) * sizeof(float) : 0;
+}
+
 int check_sizes(const char* fn, int64_t M, int32_t N, int32_t K) {
   if (M < 0 || N < 1 || K < 1)
     return set_error(NGT_ERR_ARG, "%s: bad sizes rows=%lld n_out=%d n_in=%d", fn,
@@ -719,9 +812,19 @@ extern "C" int ngt_gated_keep_bytes(int64_t n_rows, int32_t n_out, size_t* bytes
   return NGT_OK;
 }
 
+extern "C" int ngt_gated_fwd_workspace_bytes(int64_t n_rows, int32_t n_out, int32_t n_in,
+                                             size_t* bytes) {
+  const char* fn = "ngt_gated_fwd_workspace_bytes";
+  NGT_CHECK_OK(check_sizes(fn, n_rows, n_out, n_in));
+  if (!bytes) return set_error(NGT_ERR_ARG, "%s: null bytes", fn);
+  *bytes = fwd_bytes(n_rows, n_out, n_in);
+  return NGT_OK;
+}
+
 extern "C" int ngt_gated_fwd(const void* x, int64_t x_stride, const void* w_gate, const void* w_up,
                              const void* b_gate, const void* b_up, int64_t n_rows, int32_t n_out,
-                             int32_t n_in, int32_t activation, void* y, void* keep, void* stream) {
+                             int32_t n_in, int32_t activation, void* y, void* keep, void* workspace,
+                             size_t workspace_bytes, void* stream) {
   const char* fn = "ngt_gated_fwd";
   NGT_CHECK_OK(check_sizes(fn, n_rows, n_out, n_in));
   if (activation < NGT_ACT_NONE || activation > NGT_ACT_SILU)
@@ -730,55 +833,69 @@ extern "C" int ngt_gated_fwd(const void* x, int64_t x_stride, const void* w_gate
   if (!x || !w_gate || !w_up || !y) return set_error(NGT_ERR_ARG, "%s: null x, w or y", fn);
   if (x_stride < n_in) return set_error(NGT_ERR_ARG, "%s: x rows overlap", fn);
   if (!aligned16(keep)) return set_error(NGT_ERR_ARG, "%s: keep must be 16-byte aligned", fn);
-  GatedArgs a{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(w_gate),
-              static_cast<const uint16_t*>(w_up), static_cast<const uint16_t*>(b_gate),
-              static_cast<const uint16_t*>(b_up), static_cast<uint16_t*>(y),
-              keep, x_stride, static_cast<int32_t>(n_rows), n_out, n_in, activation, 0, 0};
+  const size_t need = fwd_bytes(n_rows, n_out, n_in);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return set_error(NGT_ERR_WORKSPACE, "%s: workspace %zu < %zu or not 16-byte aligned", fn,
+                     workspace_bytes, need);
+  GatedArgs a{};
+  a.x = static_cast<const uint16_t*>(x), a.x_stride = x_stride;
+  a.wg = static_cast<const uint16_t*>(w_gate), a.wu = static_cast<const uint16_t*>(w_up);
+  a.bg = static_cast<const uint16_t*>(b_gate), a.bu = static_cast<const uint16_t*>(b_up);
+  a.y = static_cast<uint16_t*>(y), a.keep = keep, a.part = static_cast<float*>(workspace);
+  a.M = static_cast<int32_t>(n_rows), a.N = n_out, a.K = n_in, a.act = activation;
+  a.tiles_m = (a.M + 63) / 64, a.tiles_n = (a.N + 63) / 64;
   hipStream_t st = static_cast<hipStream_t>(stream);
   KernelTimer timer_("gated_fwd", st);
+  const bool aligned = n_in % 8 == 0 && x_stride % 8 == 0 && all_aligned16({x, w_gate, w_up});
   // 1 and 64 rows, us, here and in the tiles of 64 rows: 768 -> 2,048 7, 9 and 14, 14; 2,048 -> 8,192
-  // 17, 24 and 31, 31; 4,096 -> 1,024 14, 27 and 44, 43.
-  if (n_in % 8 == 0 && x_stride % 8 == 0 && n_rows <= 64 && all_aligned16({x, w_gate, w_up})) {
+  // 17, 24 and 31, 31.
+  if (aligned && n_rows <= kFewRows) {
+    const Split s = few_split(n_rows, n_out, n_in);
+    a.splits = s.splits, a.per_split = s.per_split;
     auto run = [&](auto mt) {
       constexpr int MT = decltype(mt)::value;
       // 32 outputs a block where that leaves 256 blocks (64 rows of 2,048 -> 8,192 25 us, 16 outputs
       // 32; of 768 -> 2,048 12 and 9)
       const int blocks = (n_out + 15) / 16;
       if (blocks >= 512)
-        hipLaunchKernelGGL((k_gated_few<MT, 2, MT < 3 ? 8 : 4>), dim3(unsigned((n_out + 31) / 32)),
-                           dim3(MT < 3 ? 512 : 256), 0, st, a);
+        hipLaunchKernelGGL((k_gated_few<MT, 2, MT < 3 ? 8 : 4>),
+                           dim3(unsigned((n_out + 31) / 32) * a.splits), dim3(MT < 3 ? 512 : 256), 0,
+                           st, a);
       else
-        hipLaunchKernelGGL((k_gated_few<MT, 1, 8>), dim3(unsigned(blocks)), dim3(512), 0, st, a);
+        hipLaunchKernelGGL((k_gated_few<MT, 1, 8>), dim3(unsigned(blocks) * a.splits), dim3(512), 0, st,
+                           a);
     };
     if (n_rows <= 16) run(std::integral_constant<int, 1>{});
     else if (n_rows <= 32) run(std::integral_constant<int, 2>{});
     else if (n_rows <= 48) run(std::integral_constant<int, 3>{});
     else run(std::integral_constant<int, 4>{});
-    NGT_HIP_CHECK(hipGetLastError());
-    return NGT_OK;
+  } else {
+    const Split s = tile_split(n_rows, n_out, n_in);
+    a.splits = s.splits, a.per_split = s.per_split;
+    if (aligned && tiled(n_out, n_in) && x_stride < kFar && all_aligned16({b_gate, b_up, y, keep})) {
+      auto run = [&](auto fm) {
+        constexpr int FM = decltype(fm)::value;
+        a.tiles_m = (a.M + 64 * FM - 1) / (64 * FM);
+        const int64_t blocks = (int64_t(a.tiles_m) * a.tiles_n * (FM == 1 ? a.splits : 1) + 7) / 8 * 8;
+        hipLaunchKernelGGL(k_gated<FM>, dim3(unsigned(blocks)), dim3(256), 0, st, a);
+      };
+      // The tallest tile that leaves 384 blocks, three quarters of what the CUs hold (us with 256,
+      // 128 and 64 rows: 2,048 -> 8,192 at 512 rows 46, 41, 49, at 1,024 66, 79, 93; 768 -> 2,048 at
+      // 65 18, 14, 13, at 2,048 22, 19, 23, at 32,768 240, 261, 292).
+      if (a.splits == 1 && (n_rows + 255) / 256 * a.tiles_n >= 384) run(std::integral_constant<int, 4>{});
+      else if (a.splits == 1 && (n_rows + 127) / 128 * a.tiles_n >= 384) run(std::integral_constant<int, 2>{});
+      else run(std::integral_constant<int, 1>{});
+    } else {
+      hipLaunchKernelGGL(k_gated_any, dim3(unsigned(int64_t(a.tiles_m) * a.tiles_n * a.splits)), dim3(256),
+                         0, st, a);
+    }
   }
-  if (tiled(n_out, n_in) && x_stride < kFar && x_stride % 8 == 0 &&
-      all_aligned16({x, w_gate, w_up, b_gate, b_up, y, keep})) {
-    auto run = [&](auto fm) {
-      constexpr int FM = decltype(fm)::value;
-      a.tiles_m = (a.M + 64 * FM - 1) / (64 * FM), a.tiles_n = (a.N + 63) / 64;
-      const int64_t blocks = (int64_t(a.tiles_m) * a.tiles_n + 7) / 8 * 8;
-      hipLaunchKernelGGL(k_gated<FM>, dim3(unsigned(blocks)), dim3(256), 0, st, a);
-    };
-    // The tallest tile that leaves 384 blocks, three quarters of what the CUs hold (us with 256, 128
-    // and 64 rows: 2,048 -> 8,192 at 512 rows 46, 41, 49, at 1,024 66, 79, 93; 768 -> 2,048 at 65
-    // 18, 14, 13, at 2,048 22, 19, 23, at 32,768 240, 261, 292).
-    const int64_t across = (n_out + 63) / 64;
-    if ((n_rows + 255) / 256 * across >= 384) run(std::integral_constant<int, 4>{});
-    else if ((n_rows + 127) / 128 * across >= 384) run(std::integral_constant<int, 2>{});
-    else run(std::integral_constant<int, 1>{});
-    NGT_HIP_CHECK(hipGetLastError());
-    return NGT_OK;
-  }
-  a.tiles_m = (a.M + 63) / 64, a.tiles_n = (a.N + 63) / 64;
-  hipLaunchKernelGGL(k_gated_any, dim3(unsigned(int64_t(a.tiles_m) * a.tiles_n)), dim3(256), 0, st,
-                     a);
   NGT_HIP_CHECK(hipGetLastError());
+  if (a.splits > 1) {
+    const int64_t pieces = n_rows * (up8(n_out) / 8);
+    hipLaunchKernelGGL(k_gated_join_fwd, dim3(unsigned((pieces + 255) / 256)), dim3(256), 0, st, a);
+    NGT_HIP_CHECK(hipGetLastError());
+  }
   return NGT_OK;
 }
 

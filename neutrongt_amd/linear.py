@@ -427,12 +427,17 @@ class GatedLinearFunction(torch.autograd.Function):
             nb = C.c_size_t()
             _lib.check(_lib.load().ngt_gated_keep_bytes(m, n_out, C.byref(nb)))
             keep = torch.empty(nb.value, dtype=torch.uint8, device=dev)
+        ws, nb = None, C.c_size_t()
+        _lib.check(_lib.load().ngt_gated_fwd_workspace_bytes(m, n_out, n_in, C.byref(nb)))
+        if nb.value:
+            ws = torch.empty(nb.value, dtype=torch.uint8, device=dev)
         with torch.cuda.device(dev):
             _lib.check(_lib.load().ngt_gated_fwd(
                 x2.data_ptr(), x2.stride(0) if m > 1 else n_in, wg.data_ptr(), wu.data_ptr(),
                 bg.data_ptr() if bg is not None else None,
                 bu.data_ptr() if bu is not None else None, m, n_out, n_in, act, y.data_ptr(),
-                keep.data_ptr() if keep is not None else None, _lib.stream_ptr(dev)))
+                keep.data_ptr() if keep is not None else None,
+                ws.data_ptr() if ws is not None else None, nb.value, _lib.stream_ptr(dev)))
         if want_grad:
             ctx.save_for_backward(x2, wg, wu, keep)
             ctx.dtypes = [t.dtype if t is not None else None for t in (w_gate, w_up, b_gate, b_up)]

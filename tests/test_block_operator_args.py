@@ -67,8 +67,9 @@ def test_norm_rotary_refusals_touch_no_gpu():
 def test_gated_refusals_touch_no_gpu():
     lib = _lib.load()
 
-    def fwd(x=P, xs=8, wg=P, wu=P, rows=4, n_out=6, n_in=8, act=3, y=P, keep=None):
-        return lib.ngt_gated_fwd(x, xs, wg, wu, None, None, rows, n_out, n_in, act, y, keep, None)
+    def fwd(x=P, xs=8, wg=P, wu=P, rows=4, n_out=6, n_in=8, act=3, y=P, keep=None, ws=None, nb=0):
+        return lib.ngt_gated_fwd(x, xs, wg, wu, None, None, rows, n_out, n_in, act, y, keep, ws, nb,
+                                 None)
 
     for bad, code in ((dict(rows=-1), 1), (dict(n_out=0), 1), (dict(n_in=0), 1), (dict(act=4), 1),
                       (dict(act=-1), 1), (dict(x=None), 1), (dict(wg=None), 1), (dict(wu=None), 1),
@@ -79,6 +80,14 @@ def test_gated_refusals_touch_no_gpu():
         assert b"ngt_gated_fwd" in lib.ngt_last_error()
     assert fwd(rows=0, x=None, y=None) == 0
     nb = C.c_size_t()
+    for size in ((4, 6, 8), (0, 64, 8192), (100000, 64, 8192)):
+        assert lib.ngt_gated_fwd_workspace_bytes(*size, C.byref(nb)) == 0 and nb.value == 0
+    assert lib.ngt_gated_fwd_workspace_bytes(4, 0, 8, C.byref(nb)) == 1
+    for rows in (1, 100):
+        assert lib.ngt_gated_fwd_workspace_bytes(rows, 64, 8192, C.byref(nb)) == 0 and nb.value > 0
+        long = dict(xs=8192, rows=rows, n_out=64, n_in=8192)
+        for bad in (dict(nb=nb.value), dict(ws=P, nb=nb.value - 1), dict(ws=P + 8, nb=nb.value)):
+            assert fwd(**long, **bad) == 4, bad
     assert lib.ngt_gated_keep_bytes(4, 6, C.byref(nb)) == 0 and nb.value >= 4 * 6 * 2 * 2
     assert lib.ngt_gated_keep_bytes(-1, 6, C.byref(nb)) == 1
     assert lib.ngt_gated_bwd_workspace_bytes(4, 6, 8, C.byref(nb)) == 0

@@ -123,6 +123,15 @@ def test_gradients_of_whole_pieces_with_edges(dev, M, N, K):
     _case(dev, M, N, K, "silu", seed=M)
 
 
+# a long contraction of the forward for few blocks, cut into several and not
+@pytest.mark.parametrize("M,N,K", [(1, 64, 8192), (16, 16, 4096), (33, 256, 4104), (64, 40, 5000),
+                                   (5, 33, 8191), (65, 64, 8192), (200, 256, 4096), (300, 136, 2056),
+                                   (70, 61, 4097), (130, 257, 3001), (64, 1024, 2048), (449, 520, 1992)])
+@pytest.mark.parametrize("act,bias", [("silu", False), ("gelu", True)])
+def test_few_blocks_and_long_contractions(dev, M, N, K, act, bias):
+    _case(dev, M, N, K, act, bias, seed=K)
+
+
 # a contraction over many outputs for few blocks, cut into several and not
 @pytest.mark.parametrize("M,N,K", [(1, 1024, 520), (33, 2048, 512), (64, 4096, 8), (65, 1000, 1288),
                                    (200, 256, 264), (300, 1288, 72), (71, 1001, 33), (130, 2050, 65),
