@@ -794,7 +794,7 @@ int ngt_wgrad_bf16(const void* x, const void* dy, int64_t n_rows, int32_t n_out,
 /*
  * Gated linear layer, bf16: y = act(x Wg^T + bg) * (x Wu^T + bu) from x [n_rows,
  * n_in] (rows x_stride elements apart), Wg and Wu [n_out, n_in] and biases [n_out]
- * (nullable), summed in fp32 and rounded once; sizes and alignment as ngt_linear_fwd.
+ * (nullable), summed in fp32 and rounded once; any alignment, n_out below 2^20, n_in 2^21.
  * keep, where not null, receives what the backward needs (zu act'(zg) and act(zg), each to
  * 12 bits of mantissa): ngt_gated_keep_bytes, 16-byte aligned.  workspace: 16-byte aligned,
  * ngt_gated_fwd_workspace_bytes (0: none).

@@ -48,8 +48,8 @@ struct DzBlocks {
   __host__ __device__ int64_t bytes() const { return row_blocks * across() * 4096; }
 };
 
-// Backward products, aligned sizes (ngt_gated_bwd.hip): dx = dzg Wg + dzu Wu, or, with the
-// contraction split, parts of it, and dW = dz^T x, or parts of it over splits of the rows.
+// Backward products (ngt_gated_bwd.hip): dx = dzg Wg + dzu Wu, or, with the contraction split,
+// parts of it, and dW = dz^T x, or parts of it over splits of the rows.  K is a multiple of 8.
 struct GatedBwd {
   const uint16_t* dz;  // DzBlocks
   const uint16_t* x;   // [M, K]
@@ -61,6 +61,7 @@ struct GatedBwd {
   int64_t M;
   int32_t N, K;
   int32_t dw_f32[2];
+  int32_t parts;       // so also where there is one split
 };
 // A product's blocks: 64 fn columns each, and so many splits of `per_split` stages.
 struct GatedShape {
@@ -81,12 +82,8 @@ using packed::wg_x;
 constexpr int kStage = 64;  // contraction per LDS stage: rows of 128 bytes
 using L = packed::Tile<bf16_t, kStage>;
 
-// Whether the tiled products take these widths: 16-byte pieces, and 32-bit offsets within
-// 256 rows.
+// Rows that the tiled products take are below kFar: 32-bit offsets within 256 of them.
 constexpr int64_t kFar = 1 << 21;
-inline bool tiled(int64_t n_out, int64_t n_in) {
-  return n_in < kFar && 2 * n_out < kFar && n_in % 8 == 0 && n_out % 8 == 0;
-}
 inline bool all_aligned16(std::initializer_list<const void*> ps) {
   for (const void* p : ps)
     if (!aligned16(p)) return false;

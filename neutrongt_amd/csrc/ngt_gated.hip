@@ -168,9 +168,48 @@ __global__ __launch_bounds__(256) void k_gated_join_fwd(GatedArgs a) {
   finish8(a, m, (i - m * across) * 8, s[0], s[1]);
 }
 
+// x, Wg and Wu with their rows filled up to 8s with zeros, one after another (of widths that are
+// no multiple of 8: 2 x 8,193 rows of 2,049 25 us, 5 TB/s).
+struct PackArgs {
+  const uint16_t* from[3];
+  int64_t rows[3];  // of the three, 0 where not wanted
+  int64_t x_stride;
+  uint16_t* to;
+  int32_t k;
+};
+__global__ __launch_bounds__(256) void k_gated_pack(PackArgs a) {
+  const int across = up8(a.k) / 8, together = across < 256 ? 256 / across : 1;
+  const int r = tid_x() / across;
+  int64_t row = int64_t(wg_x()) * together + (across < 256 ? r : 0);
+  if (across < 256 && r >= together) return;
+  uint16_t* to = a.to + row * across * 8;
+  int which = 0;
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    if (which == i && row >= a.rows[i]) row -= a.rows[i], ++which;
+  if (which > 2) return;
+  const uint16_t* from = (which == 0 ? a.from[0] : which == 1 ? a.from[1] : a.from[2]) + row * (which == 0 ? a.x_stride : a.k);
+  for (int c = across < 256 ? tid_x() - r * across : tid_x(); c < across; c += 256)
+    *reinterpret_cast<u32x4*>(to + 8 * c) = load8<false>(from, 8 * c, a.k);
+}
+// What of it in its workspace is what.
+struct Packed {
+  const uint16_t *x, *wg, *wu;
+};
+int launch_pack(const PackArgs& a, hipStream_t st, Packed* to) {
+  const int across = up8(a.k) / 8, together = across < 256 ? 256 / across : 1;
+  const int64_t rows = a.rows[0] + a.rows[1] + a.rows[2];
+  hipLaunchKernelGGL(k_gated_pack, dim3(unsigned((rows + together - 1) / together)), dim3(256), 0, st, a);
+  NGT_HIP_CHECK(hipGetLastError());
+  to->x = a.to, to->wg = a.to + a.rows[0] * up8(a.k), to->wu = to->wg + a.rows[1] * up8(a.k);
+  return NGT_OK;
+}
+
 // Any sizes and 2-byte alignment.  One block: 64 rows by 64 outputs of both products,
 // 2 x 2 waves of 32 x 32, stages of 64 of the contraction read into registers while the
-// stage before is multiplied.  32,768 rows, 768 -> 2,048 in it: 350 us (k_gated 231).
+// stage before is multiplied.  For rows that are not whole 16-byte pieces where filling them up
+// does not pay (plan_fwd), and for other alignments.  32,768 rows, 768 -> 2,048 in it: 350 us
+// (k_gated 215).
 __global__ __launch_bounds__(256) void k_gated_any(GatedArgs a) {
   constexpr int NP = 64 * 8 / 256;  // 16-byte pieces per thread and operand
   __shared__ __align__(16) char lds[3][64 * 128];
@@ -322,10 +361,10 @@ __global__ __launch_bounds__(64 * WAVES) void k_gated_few(GatedArgs a) {
 }
 
 // dz = [dzg | dzu], and the biases' gradients: part_b[chunk][2 N], sums of the
-// unrounded products.  A block: 256 columns of chunk_rows rows, 8 columns a thread.  BLOCKS: whole
-// pieces, and dz in DzBlocks, else [M, 2 N].  Bound by memory: 32,768 by 2,048 moves 738 MB in
+// unrounded products.  A block: 256 columns of chunk_rows rows, 8 columns a thread.  WHOLE: whole
+// pieces, else any width and 2-byte alignment.  Bound by memory: 32,768 by 2,048 moves 738 MB in
 // 142 to 147 us, 5.1 TB/s, as a copy does.
-template <bool BLOCKS>
+template <bool WHOLE>
 __global__ __launch_bounds__(256) void k_gated_dz(const uint16_t* __restrict__ dy,
                                                   void* keep, int64_t rows,
                                                   int32_t n, int32_t tiles_n, int32_t chunk_rows,
@@ -337,25 +376,25 @@ __global__ __launch_bounds__(256) void k_gated_dz(const uint16_t* __restrict__ d
   const int c = (wg_x() - static_cast<int>(chunk) * tiles_n) * 256 + 8 * cg;
   const DzBlocks blocks(rows, n);
   const Keep kept(rows, n);
-  const int64_t end = BLOCKS ? blocks.row_blocks * 32 : rows;  // of what is written
+  const int64_t end = blocks.row_blocks * 32;  // of what is written
   const int64_t r0 = chunk * chunk_rows, r1 = r0 + chunk_rows < end ? r0 + chunk_rows : end;
   float sum[2][8];
 #pragma unroll
   for (int p = 0; p < 2; ++p)
 #pragma unroll
     for (int t = 0; t < 8; ++t) sum[p][t] = 0.f;
-  if (c < (BLOCKS ? 64 * blocks.per_layer : n)) {
+  if (c < 64 * blocks.per_layer) {
 #pragma unroll 2
     for (int64_t row = r0 + lane; row < r1; row += 8) {
       u32x4 g = {0u, 0u, 0u, 0u}, v[2] = {g, g};
       uint32_t low[2] = {0u, 0u};
-      if (!BLOCKS || (row < rows && c < n)) {
-        g = load8<BLOCKS>(dy + row * n, c, n);
+      if (row < rows && c < n) {
+        g = load8<WHOLE>(dy + row * n, c, n);
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           const uint16_t* from = kept.high(keep, row, p);
           // the last time that it is read
-          if constexpr (BLOCKS)
+          if constexpr (WHOLE)
             v[p] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(from + c));
           else
             v[p] = load8<false>(from, c, n);
@@ -373,11 +412,8 @@ __global__ __launch_bounds__(256) void k_gated_dz(const uint16_t* __restrict__ d
           sum[p][2 * t] += lo, sum[p][2 * t + 1] += hi;
           o[t] = pack2_bf16(lo, hi);
         }
-        if constexpr (BLOCKS)
-          *reinterpret_cast<u32x4*>(dz + (row / 32 * blocks.across() + p * blocks.per_layer + c / 64) * 2048 +
-                                    row % 32 * 64 + c % 64) = o;
-        else
-          store8(dz + (2 * row + p) * n, c, n, o);
+        *reinterpret_cast<u32x4*>(dz + (row / 32 * blocks.across() + p * blocks.per_layer + c / 64) * 2048 +
+                                  row % 32 * 64 + c % 64) = o;
       }
     }
   }
@@ -402,12 +438,12 @@ __global__ __launch_bounds__(256) void k_gated_dz(const uint16_t* __restrict__ d
 // order, 4 elements a thread; of the biases the chunks', 8 lanes a column that take every
 // 8th, added in their order.  Bound by the sums' bytes: 2 x 2,048 x 768 in two splits 12 us.
 struct JoinArgs {
-  const float* part;    // [splits][2 N][K]
+  const float* part;    // [splits][2 N][K filled up to 8s]
   const float* part_b;  // [chunks][2 N]
   void* dw[2];
   void* db[2];
   int64_t nk;           // N K
-  int32_t n, splits, chunks, blocks_w;
+  int32_t n, k, splits, chunks, blocks_w;
   int32_t dw_f32[2], db_f32[2];
 };
 __device__ __forceinline__ void put(void* to, int64_t i, bool f32, float v) {
@@ -417,31 +453,33 @@ __device__ __forceinline__ void put(void* to, int64_t i, bool f32, float v) {
 __global__ __launch_bounds__(256) void k_gated_join(JoinArgs a) {
   __shared__ float red[8][32];
   if (wg_x() < a.blocks_w) {
-    const int64_t i = (int64_t(wg_x()) * 256 + tid_x()) * 4, all = 2 * a.nk;
-    if (i >= all) return;
+    const int pitch = up8(a.k);
+    const int64_t at = (int64_t(wg_x()) * 256 + tid_x()) * 4, all = 2 * int64_t(a.n) * pitch;
+    if (at >= all) return;
     float s[4] = {0.f, 0.f, 0.f, 0.f};
-    const bool whole = all % 4 == 0;
 #pragma unroll 4
     for (int c = 0; c < a.splits; ++c) {
-      const float* p = a.part + c * all + i;
-      if (whole) {
-        const float4 v = *reinterpret_cast<const float4*>(p);
-        s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
-      } else {
-        for (int t = 0; t < 4; ++t)
-          if (i + t < all) s[t] += p[t];
-      }
+      const float4 v = *reinterpret_cast<const float4*>(a.part + c * all + at);
+      s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
+    }
+    // the element of the weights, and how many of the four there are
+    int64_t i = at;
+    int there = 4;
+    if (pitch != a.k) {
+      const int64_t row = at / pitch;
+      const int c = static_cast<int>(at - row * pitch);
+      i = row * a.k + c, there = min(a.k - c, 4);
     }
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       if (!a.dw[w]) continue;
       const int64_t o = i - w * a.nk;
       const bool f32 = a.dw_f32[w];
-      if (o >= 0 && o + 4 <= a.nk && a.nk % 4 == 0) {
+      if (pitch == a.k && o >= 0 && o + 4 <= a.nk) {
         if (f32) *reinterpret_cast<float4*>(static_cast<float*>(a.dw[w]) + o) = make_float4(s[0], s[1], s[2], s[3]);
         else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.dw[w]) + o) = make_uint2(pack2_bf16(s[0], s[1]), pack2_bf16(s[2], s[3]));
       } else {
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < there; ++t)
           if (o + t >= 0 && o + t < a.nk) put(a.dw[w], o + t, f32, s[t]);
       }
     }
@@ -462,92 +500,17 @@ __global__ __launch_bounds__(256) void k_gated_join(JoinArgs a) {
   if (a.db[w]) put(a.db[w], col - w * a.n, a.db_f32[w], s);
 }
 
-struct DxArgs {
-  const uint16_t* dz;  // [M, 2 N]
-  const uint16_t* wg;  // [N, K]
-  const uint16_t* wu;
-  uint16_t* dx;        // [M, K]
-  float* part;         // [splits][M][K filled up to 8s] where the contraction is split, else null
-  int32_t M, N, K;
-  int32_t tiles_k, tiles, per_split;  // stages of a split
-};
-
-// dx = dzg Wg + dzu Wu at any sizes and alignment: the same blocks, 64 rows by 64 of K,
-// contracted over the outputs of one layer and then of the other (a stage holds one
-// layer's); W's stages are turned on their way to LDS.
-__global__ __launch_bounds__(256) void k_gated_dx_any(DxArgs a) {
-  constexpr int NP = 64 * 8 / 256;
-  __shared__ __align__(16) char lz[64 * 128];
-  __shared__ __align__(16) char lw[64 * 128];
-  const int tid = tid_x(), lane = tid & 63, wave = tid >> 6, half = lane >> 5, l32 = lane & 31;
-  const int split = wg_x() / a.tiles, tile = wg_x() - split * a.tiles;
-  const int m0 = tile / a.tiles_k * 64, k0 = tile % a.tiles_k * 64;
-  const int wm = (wave >> 1) * 32, wk = (wave & 1) * 32;
-  const int layer = (a.N + kStage - 1) / kStage;
-  const int first = split * a.per_split, end = min(first + a.per_split, 2 * layer);
-  f32x16 acc = fill16(0.f);
-  u32x4 z[NP], v[NP];
-  auto fetch = [&](int s) {
-    const int part = s >= layer, n0 = (s - part * layer) * kStage;
-    const uint16_t* w = part ? a.wu : a.wg;
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int e = tid + i * 256, m = m0 + e / 8, n = n0 + e / 8;
-      z[i] = v[i] = u32x4{0u, 0u, 0u, 0u};
-      if (m < a.M) z[i] = load8<false>(a.dz + (int64_t(m) * 2 + part) * a.N, n0 + 8 * (e % 8), a.N);
-      if (n < a.N) v[i] = load8<false>(w + int64_t(n) * a.K, k0 + 8 * (e % 8), a.K);
-    }
-  };
-  fetch(first);
-  for (int s = first; s < end; ++s) {
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int e = tid + i * 256, r = e / 8, c = e % 8;
-      *reinterpret_cast<u32x4*>(lz + L::offset(r, c)) = z[i];
-#pragma unroll
-      for (int t = 0; t < 8; ++t)
-        *reinterpret_cast<uint16_t*>(lw + L::offset(8 * c + t, r / 8) + 2 * (r % 8)) =
-            static_cast<uint16_t>(v[i][t / 2] >> (16 * (t & 1)));
-    }
-    __syncthreads();
-    if (s + 1 < end) fetch(s + 1);
-#pragma unroll
-    for (int c = 0; c < L::kChunks; ++c)
-      acc = L::mma(L::load_a(lw + wk * 128, 0, c, l32, half),
-                   L::load_a(lz + wm * 128, 0, c, l32, half), acc);
-  }
-  const int m = m0 + wm + L::a_row(l32);
-  if (m >= a.M) return;
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int k = k0 + wk + 16 * half + 8 * e;
-    if (k >= a.K) continue;
-    if (a.part) {
-      float* to = a.part + (int64_t(split) * a.M + m) * up8(a.K) + k;
-#pragma unroll
-      for (int t = 0; t < 8; t += 4)
-        *reinterpret_cast<float4*>(to + t) = make_float4(acc[8 * e + t], acc[8 * e + t + 1],
-                                                         acc[8 * e + t + 2], acc[8 * e + t + 3]);
-    } else {
-      u32x4 o;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) o[t] = pack2_bf16(acc[8 * e + 2 * t], acc[8 * e + 2 * t + 1]);
-      store8(a.dx + int64_t(m) * a.K, k, a.K, o);
-    }
-  }
-}
-
 // dx from the splits' sums, added in their order, 8 elements a thread.
 __global__ __launch_bounds__(256) void k_gated_join_dx(const float* __restrict__ part, int32_t splits,
-                                                       int32_t M, int32_t K,
+                                                       int64_t M, int32_t K,
                                                        uint16_t* __restrict__ dx) {
-  const int across = up8(K) / 8, i = wg_x() * 256 + tid_x();
+  const int across = up8(K) / 8;
+  const int64_t i = int64_t(wg_x()) * 256 + tid_x();
   if (i >= M * across) return;
   float s[8] = {};
 #pragma unroll 8
   for (int c = 0; c < splits; ++c) {
-    const float* p = part + (int64_t(c) * M * across + i) * 8;
+    const float* p = part + (c * M * across + i) * 8;
     const float4 v = *reinterpret_cast<const float4*>(p), w = *reinterpret_cast<const float4*>(p + 4);
     s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
     s[4] += w.x, s[5] += w.y, s[6] += w.z, s[7] += w.w;
@@ -555,20 +518,21 @@ __global__ __launch_bounds__(256) void k_gated_join_dx(const float* __restrict__
   u32x4 o;
 #pragma unroll
   for (int t = 0; t < 4; ++t) o[t] = pack2_bf16(s[2 * t], s[2 * t + 1]);
-  const int m = i / across;
-  store8(dx + int64_t(m) * K, (i - m * across) * 8, K, o);
+  const int64_t m = i / across;
+  store8(dx + m * K, static_cast<int>(i - m * across) * 8, K, o);
 }
 
-// Aligned sizes.  One block: 64 FM rows by 64 outputs of both layers, 2 x 2 waves, each FM tiles
-// of 32 x 32 of the gate and the same of the other layer.  A wave takes a stage's
-// operands into registers before it multiplies, so the one buffer is free for the next
-// stage while it does, and two blocks on a CU fill each other's reads.
+// Rows of x and W of whole 16-byte pieces, of y too where WHOLE.  One block: 64 FM rows by 64
+// outputs of both layers, 2 x 2 waves, each FM tiles of 32 x 32 of the gate and the same of the
+// other layer.  A wave takes a stage's operands into registers before it multiplies, so the
+// one buffer is free for the next stage while it does, and two blocks on a CU fill each
+// other's reads.
 // 10,007 rows, 1,024 -> 4,096 without keep: 160 us, 1,050 TFLOP/s (a library product of the
 // same size and nothing else 143); 32,768 rows, 768 -> 2,048 with keep: 258, of which the loop is
 // 185 (its products and LDS reads alone 146, its loads alone 111), the rest arithmetic and 470 MB
 // of stores, which the loops of other blocks do not hide.  Measured at the first size: 256 rows
 // by 128 outputs in 8 waves with two buffers 175 us, 192 by 64 in two blocks with two buffers 168.
-template <int FM>
+template <int FM, bool WHOLE>
 __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
   constexpr int BM = 64 * FM, kRowsBytes = BM * 128;
   __shared__ __align__(16) char lds[FM > 1 ? 49152 : kRowsBytes + 128 * 128];
@@ -588,12 +552,12 @@ __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     if (a.bg && !parts) {
-      const u32x4 b = load8<true>(a.bg, n + 8 * e, a.N);
+      const u32x4 b = load8<false>(a.bg, n + 8 * e, a.N);
 #pragma unroll
       for (int t = 0; t < 8; ++t) g[0][8 * e + t] = half_of(b, t);
     }
     if (a.bu && !parts) {
-      const u32x4 b = load8<true>(a.bu, n + 8 * e, a.N);
+      const u32x4 b = load8<false>(a.bu, n + 8 * e, a.N);
 #pragma unroll
       for (int t = 0; t < 8; ++t) u[0][8 * e + t] = half_of(b, t);
     }
@@ -695,6 +659,14 @@ __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
         u32x4 kg, ku;
         if constexpr (KEEP) kg = *slot(i, 1, r, lane % 8), ku = *slot(i, 2, r, lane % 8);
         if (m_back >= a.M || n_back >= a.N) continue;
+        if constexpr (!WHOLE) {
+          store8(a.y + int64_t(m_back) * a.N, n_back, a.N, y);
+          if constexpr (KEEP) {
+            store8(kept.high(a.keep, m_back, 0), n_back, a.N, kg);
+            store8(kept.high(a.keep, m_back, 1), n_back, a.N, ku);
+          }
+          continue;
+        }
         *reinterpret_cast<u32x4*>(a.y + int64_t(m_back) * a.N + n_back) = y;
         if constexpr (KEEP) {
           __builtin_nontemporal_store(kg, reinterpret_cast<u32x4*>(kept.high(a.keep, m_back, 0) + n_back));
@@ -707,47 +679,34 @@ __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
 
 // How a backward is cut, and where its workspace holds what.
 struct BwdPlan {
-  bool tiled;
-  GatedShape dx, dw;   // (not tiled: dx's splits alone)
+  GatedShape dx, dw;
+  bool packed;         // widths that are no multiple of 8: x and W filled up, results by way of sums
   int32_t chunk_rows;  // of a block of k_gated_dz
   int64_t chunks;
-  size_t dz, part, part_b, wgrad, bytes;  // part: dx's sums, then the weights'
+  size_t dz, part, part_b, pack, bytes;  // part: dx's sums, then the weights'
 };
-int plan_bwd(int64_t M, int32_t N, int32_t K, BwdPlan* p) {
-  p->tiled = tiled(N, K);
+BwdPlan plan_bwd(int64_t M, int32_t N, int32_t K) {
+  BwdPlan p;
+  const int32_t pitch = up8(K);
+  p.dx = gated_dx_shape(M, N, pitch), p.dw = gated_dw_shape(M, N, pitch);
+  p.packed = pitch != K;
   // 1,024 blocks where there are rows enough, of 8 rows a pass (2,048 -> 8,192 us at 64 rows: 6, at
   // 128 rows a block 12; 768 -> 2,048 at 511: 8 and 20)
-  p->chunk_rows = 128;
-  while (p->chunk_rows > 8 && (M + p->chunk_rows - 1) / p->chunk_rows * ((N + 255) / 256) < 1024)
-    p->chunk_rows /= 2;
+  p.chunk_rows = 128;
+  while (p.chunk_rows > 8 && (M + p.chunk_rows - 1) / p.chunk_rows * ((N + 255) / 256) < 1024)
+    p.chunk_rows /= 2;
   // (M filled up to whole blocks of dz)
-  p->chunks = M == 0 ? 0 : ((M + 63) / 64 * 64 + p->chunk_rows - 1) / p->chunk_rows;
+  p.chunks = M == 0 ? 0 : ((M + 63) / 64 * 64 + p.chunk_rows - 1) / p.chunk_rows;
   auto align = [](size_t b) { return (b + 255) & ~size_t(255); };
-  size_t part = size_t(2) * N * K * sizeof(float), ws = 0;
-  p->dw = {4, 1, 0};
-  if (p->tiled) {
-    p->dx = gated_dx_shape(M, N, K), p->dw = gated_dw_shape(M, N, K);
-    part = p->dw.splits > 1 ? part * p->dw.splits : 0;
-  } else {
-    // Splits of 4 stages at least, in no more blocks than the CUs hold at a time (6 each).  A
-    // stage takes 1.3 us and its share of a CU; a split's sums 1 us a MB, written and read again:
-    // best is the square root of their quotient.  33 rows, 2,049 -> 8,193: 37 us, 402 in one
-    // split; 1,025 of them 416 and 546; 1,025 rows, 769 -> 769: 28 and 38.  (M K stays below 2^22.)
-    const int64_t stages = (int64_t(N) + 63) / 64 * 2, tiles = (M + 63) / 64 * ((K + 63) / 64);
-    const int64_t most = tiles > 0 ? std::min<int64_t>(6 * 256 / tiles, stages / 4) : 1;
-    const double want = std::sqrt(1.3 * double(stages) / (1e-6 * 4 * double(M) * K));
-    const int64_t splits = std::max<int64_t>(1, want < double(most) ? std::llround(want) : most);
-    const int64_t per = (stages + splits - 1) / splits;
-    p->dx = {1, static_cast<int32_t>((stages + per - 1) / per), static_cast<int32_t>(per)};
-    NGT_CHECK_OK(ngt_wgrad_workspace_bytes(M, 2 * N, K, &ws));
-  }
-  const size_t part_dx = p->dx.splits > 1 ? size_t(p->dx.splits) * M * up8(K) * sizeof(float) : 0;
-  p->dz = 0;
-  p->part = align(p->tiled ? DzBlocks(M, N).bytes() : size_t(M) * 2 * N * 2);
-  p->part_b = p->part + align(part > part_dx ? part : part_dx);
-  p->wgrad = p->part_b + align(size_t(p->chunks) * 2 * N * sizeof(float));
-  p->bytes = p->wgrad + ws;
-  return NGT_OK;
+  auto sums = [&](const GatedShape& s, int64_t rows) {
+    return s.splits > 1 || p.packed ? size_t(s.splits) * rows * pitch * sizeof(float) : 0;
+  };
+  p.dz = 0;
+  p.part = align(DzBlocks(M, N).bytes());
+  p.part_b = p.part + align(std::max(sums(p.dx, M), sums(p.dw, 2 * int64_t(N))));
+  p.pack = p.part_b + align(size_t(p.chunks) * 2 * N * sizeof(float));
+  p.bytes = p.pack + (p.packed ? (size_t(M) + 2 * N) * pitch * 2 : 0);
+  return p;
 }
 
 // How a forward's contraction is split, in elements, where there are few blocks: each split's sums
@@ -779,11 +738,25 @@ Split tile_split(int64_t M, int32_t N, int32_t K) {
   const int64_t stages = (int64_t(K) + 63) / 64, tiles = (M + 63) / 64 * ((N + 63) / 64);
   return split_of(M, N, K, 0.65, stages, 64, std::min<int64_t>(768 / std::max<int64_t>(tiles, 1), stages / 4));
 }
-size_t fwd_bytes(int64_t M, int32_t N, int32_t K) {
-  if (M == 0) return 0;
+// Whether a forward fills up the rows of x and W first: its reading and writing (4 bytes an
+// element at 5 TB/s) against what k_gated_any takes longer (us, it / filled up: 769 -> 2,049 at 1
+// row 18 / 12, at 8,193 223 / 107; 2,049 -> 8,193 at 600 rows 162 / 97, at 129 57 and, were it filled up,
+// 56).
+bool fills_up(int64_t M, int32_t N, int32_t K) {
+  return K % 8 != 0 && 3.0 + 0.8e-6 * double(M + 2 * int64_t(N)) * K < 6.0 + 3.6e-9 * double(M) * N * K;
+}
+struct FwdPlan {
+  bool packed;
+  size_t pack, bytes;
+};
+FwdPlan plan_fwd(int64_t M, int32_t N, int32_t K) {
+  if (M == 0) return {false, 0, 0};
+  FwdPlan p{fills_up(M, N, K), 0, 0};
   int32_t splits = tile_split(M, N, K).splits;
   if (M <= kFewRows) splits = std::max(splits, few_split(M, N, K).splits);
-  return splits > 1 ? size_t(splits) * 2 * M * up8(N) * sizeof(float) : 0;
+  p.pack = splits > 1 ? size_t(splits) * 2 * M * up8(N) * sizeof(float) : 0;
+  p.bytes = p.pack + (p.packed ? (size_t(M) + 2 * N) * up8(K) * 2 : 0);
+  return p;
 }
 
 int check_sizes(const char* fn, int64_t M, int32_t N, int32_t K) {
@@ -793,7 +766,7 @@ int check_sizes(const char* fn, int64_t M, int32_t N, int32_t K) {
   // 32-bit rows, and fewer than 2^24 blocks for each of the tile grids
   auto blocks = [](int64_t r, int64_t c, int t) { return (r + t - 1) / t * ((c + t - 1) / t); };
   constexpr int64_t kMost = (1 << 24) - 8;
-  if (M > (1 << 30) || N > (1 << 29) || blocks(M, N, 64) > kMost || blocks(M, K, 64) > kMost ||
+  if (M > (1 << 30) || 2 * int64_t(N) >= kFar || K >= kFar || blocks(M, N, 64) > kMost || blocks(M, K, 64) > kMost ||
       blocks(N, K, 32) > kMost)
     return set_error(NGT_ERR_UNSUPPORTED, "%s: rows=%lld n_out=%d n_in=%d exceed the grid", fn,
                      static_cast<long long>(M), N, K);
@@ -817,7 +790,7 @@ extern "C" int ngt_gated_fwd_workspace_bytes(int64_t n_rows, int32_t n_out, int3
   const char* fn = "ngt_gated_fwd_workspace_bytes";
   NGT_CHECK_OK(check_sizes(fn, n_rows, n_out, n_in));
   if (!bytes) return set_error(NGT_ERR_ARG, "%s: null bytes", fn);
-  *bytes = fwd_bytes(n_rows, n_out, n_in);
+  *bytes = plan_fwd(n_rows, n_out, n_in).bytes;
   return NGT_OK;
 }
 
@@ -833,10 +806,10 @@ extern "C" int ngt_gated_fwd(const void* x, int64_t x_stride, const void* w_gate
   if (!x || !w_gate || !w_up || !y) return set_error(NGT_ERR_ARG, "%s: null x, w or y", fn);
   if (x_stride < n_in) return set_error(NGT_ERR_ARG, "%s: x rows overlap", fn);
   if (!aligned16(keep)) return set_error(NGT_ERR_ARG, "%s: keep must be 16-byte aligned", fn);
-  const size_t need = fwd_bytes(n_rows, n_out, n_in);
-  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+  const FwdPlan p = plan_fwd(n_rows, n_out, n_in);
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes || !aligned16(workspace)))
     return set_error(NGT_ERR_WORKSPACE, "%s: workspace %zu < %zu or not 16-byte aligned", fn,
-                     workspace_bytes, need);
+                     workspace_bytes, p.bytes);
   GatedArgs a{};
   a.x = static_cast<const uint16_t*>(x), a.x_stride = x_stride;
   a.wg = static_cast<const uint16_t*>(w_gate), a.wu = static_cast<const uint16_t*>(w_up);
@@ -846,11 +819,21 @@ extern "C" int ngt_gated_fwd(const void* x, int64_t x_stride, const void* w_gate
   a.tiles_m = (a.M + 63) / 64, a.tiles_n = (a.N + 63) / 64;
   hipStream_t st = static_cast<hipStream_t>(stream);
   KernelTimer timer_("gated_fwd", st);
-  const bool aligned = n_in % 8 == 0 && x_stride % 8 == 0 && all_aligned16({x, w_gate, w_up});
+  if (p.packed) {
+    Packed to;
+    NGT_CHECK_OK(launch_pack({{a.x, a.wg, a.wu},
+                              {n_rows, n_out, n_out},
+                              x_stride,
+                              reinterpret_cast<uint16_t*>(static_cast<char*>(workspace) + p.pack),
+                              n_in},
+                             st, &to));
+    a.x = to.x, a.wg = to.wg, a.wu = to.wu, a.K = up8(n_in), a.x_stride = a.K;
+  }
+  const bool aligned = a.K % 8 == 0 && a.x_stride % 8 == 0 && all_aligned16({a.x, a.wg, a.wu});
   // 1 and 64 rows, us, here and in the tiles of 64 rows: 768 -> 2,048 7, 9 and 14, 14; 2,048 -> 8,192
   // 17, 24 and 31, 31.
   if (aligned && n_rows <= kFewRows) {
-    const Split s = few_split(n_rows, n_out, n_in);
+    const Split s = few_split(n_rows, n_out, a.K);
     a.splits = s.splits, a.per_split = s.per_split;
     auto run = [&](auto mt) {
       constexpr int MT = decltype(mt)::value;
@@ -870,14 +853,16 @@ extern "C" int ngt_gated_fwd(const void* x, int64_t x_stride, const void* w_gate
     else if (n_rows <= 48) run(std::integral_constant<int, 3>{});
     else run(std::integral_constant<int, 4>{});
   } else {
-    const Split s = tile_split(n_rows, n_out, n_in);
+    const Split s = tile_split(n_rows, n_out, a.K);
     a.splits = s.splits, a.per_split = s.per_split;
-    if (aligned && tiled(n_out, n_in) && x_stride < kFar && all_aligned16({b_gate, b_up, y, keep})) {
+    if (aligned && a.x_stride < kFar) {
       auto run = [&](auto fm) {
         constexpr int FM = decltype(fm)::value;
         a.tiles_m = (a.M + 64 * FM - 1) / (64 * FM);
         const int64_t blocks = (int64_t(a.tiles_m) * a.tiles_n * (FM == 1 ? a.splits : 1) + 7) / 8 * 8;
-        hipLaunchKernelGGL(k_gated<FM>, dim3(unsigned(blocks)), dim3(256), 0, st, a);
+        const bool whole = n_out % 8 == 0 && aligned16(y);
+        hipLaunchKernelGGL((whole ? &k_gated<FM, true> : &k_gated<FM, false>), dim3(unsigned(blocks)),
+                           dim3(256), 0, st, a);
       };
       // The tallest tile that leaves 384 blocks, three quarters of what the CUs hold (us with 256,
       // 128 and 64 rows: 2,048 -> 8,192 at 512 rows 46, 41, 49, at 1,024 66, 79, 93; 768 -> 2,048 at
@@ -904,9 +889,7 @@ extern "C" int ngt_gated_bwd_workspace_bytes(int64_t n_rows, int32_t n_out, int3
   const char* fn = "ngt_gated_bwd_workspace_bytes";
   NGT_CHECK_OK(check_sizes(fn, n_rows, n_out, n_in));
   if (!bytes) return set_error(NGT_ERR_ARG, "%s: null bytes", fn);
-  BwdPlan p;
-  NGT_CHECK_OK(plan_bwd(n_rows, n_out, n_in, &p));
-  *bytes = p.bytes;
+  *bytes = plan_bwd(n_rows, n_out, n_in).bytes;
   return NGT_OK;
 }
 
@@ -929,8 +912,7 @@ extern "C" int ngt_gated_bwd(const void* dy, const void* keep, const void* x, co
       return set_error(NGT_ERR_ARG, "%s: gradient dtype %d", fn, t.second);
   if (!all_aligned16({dy, keep, x, w_gate, w_up, g.dx, g.dw_gate, g.dw_up}))
     return set_error(NGT_ERR_ARG, "%s: matrices must be 16-byte aligned", fn);
-  BwdPlan p;
-  NGT_CHECK_OK(plan_bwd(n_rows, n_out, n_in, &p));
+  const BwdPlan p = plan_bwd(n_rows, n_out, n_in);
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes || !aligned16(workspace)))
     return set_error(NGT_ERR_WORKSPACE, "%s: workspace %zu < %zu or not 16-byte aligned", fn,
                      workspace_bytes, p.bytes);
@@ -939,15 +921,33 @@ extern "C" int ngt_gated_bwd(const void* dy, const void* keep, const void* x, co
   auto* dz = reinterpret_cast<uint16_t*>(ws + p.dz);
   auto* part = reinterpret_cast<float*>(ws + p.part);
   auto* part_b = reinterpret_cast<float*>(ws + p.part_b);
-  const auto *wg = static_cast<const uint16_t*>(w_gate), *wu = static_cast<const uint16_t*>(w_up);
-  const auto M = static_cast<int32_t>(n_rows);
-  const GatedBwd products{dz, static_cast<const uint16_t*>(x), wg, wu, static_cast<uint16_t*>(g.dx),
-                          {g.dw_gate, g.dw_up}, part, n_rows, n_out, n_in,
-                          {g.dw_gate_dtype == NGT_F32, g.dw_up_dtype == NGT_F32}};
+  GatedBwd products{dz,
+                    static_cast<const uint16_t*>(x),
+                    static_cast<const uint16_t*>(w_gate),
+                    static_cast<const uint16_t*>(w_up),
+                    static_cast<uint16_t*>(g.dx),
+                    {g.dw_gate, g.dw_up},
+                    part,
+                    n_rows,
+                    n_out,
+                    up8(n_in),
+                    {g.dw_gate_dtype == NGT_F32, g.dw_up_dtype == NGT_F32},
+                    p.packed};
+  if (p.packed && n_rows > 0 && (g.dx || want_w)) {
+    KernelTimer timer_("gated_pack", st);
+    Packed to;
+    NGT_CHECK_OK(launch_pack({{products.x, products.wg, products.wu},
+                              {want_w ? n_rows : 0, g.dx ? n_out : 0, g.dx ? n_out : 0},
+                              n_in,
+                              reinterpret_cast<uint16_t*>(ws + p.pack),
+                              n_in},
+                             st, &to));
+    products.x = to.x, products.wg = to.wg, products.wu = to.wu;
+  }
   if (n_rows > 0) {
     KernelTimer timer_("gated_dz", st);
     const int32_t tiles_n = (n_out + 255) / 256;
-    hipLaunchKernelGGL(p.tiled ? &k_gated_dz<true> : &k_gated_dz<false>,
+    hipLaunchKernelGGL(n_out % 8 == 0 ? &k_gated_dz<true> : &k_gated_dz<false>,
                        dim3(unsigned(p.chunks * tiles_n)), dim3(256), 0, st,
                        static_cast<const uint16_t*>(dy), const_cast<void*>(keep), n_rows, n_out,
                        tiles_n, p.chunk_rows, dz, want_b ? part_b : nullptr);
@@ -955,35 +955,20 @@ extern "C" int ngt_gated_bwd(const void* dy, const void* keep, const void* x, co
   }
   if (n_rows > 0 && g.dx) {
     KernelTimer timer_("gated_dx", st);
-    if (p.tiled) {
-      NGT_CHECK_OK(launch_gated_dx(products, p.dx, st));
-    } else {
-      const int32_t tiles_k = (n_in + 63) / 64;
-      const int64_t tiles = (n_rows + 63) / 64 * tiles_k;
-      DxArgs a{dz, wg, wu, static_cast<uint16_t*>(g.dx), p.dx.splits > 1 ? part : nullptr, M, n_out,
-               n_in, tiles_k, static_cast<int32_t>(tiles), p.dx.per_split};
-      hipLaunchKernelGGL(k_gated_dx_any, dim3(unsigned(tiles * p.dx.splits)), dim3(256), 0, st, a);
-      NGT_HIP_CHECK(hipGetLastError());
-    }
-    if (p.dx.splits > 1) {
-      const int64_t blocks = (n_rows * (up8(n_in) / 8) + 255) / 256;
+    NGT_CHECK_OK(launch_gated_dx(products, p.dx, st));
+    if (p.dx.splits > 1 || p.packed) {
+      const int64_t blocks = (n_rows * (products.K / 8) + 255) / 256;
       hipLaunchKernelGGL(k_gated_join_dx, dim3(unsigned(blocks)), dim3(256), 0, st, part, p.dx.splits,
-                         M, n_in, static_cast<uint16_t*>(g.dx));
+                         n_rows, n_in, products.dx);
       NGT_HIP_CHECK(hipGetLastError());
     }
   }
-  int32_t splits = p.dw.splits;
   if (want_w && n_rows > 0) {
-    if (p.tiled) {
-      KernelTimer timer_("gated_dw", st);
-      NGT_CHECK_OK(launch_gated_dw(products, p.dw, st));
-    } else {
-      NGT_CHECK_OK(ngt_wgrad_bf16(x, dz, n_rows, 2 * n_out, n_in, part, nullptr, ws + p.wgrad,
-                                  p.bytes - p.wgrad, stream));
-    }
+    KernelTimer timer_("gated_dw", st);
+    NGT_CHECK_OK(launch_gated_dw(products, p.dw, st));
   }
-  if (n_rows == 0) splits = 0;
-  const bool join_w = want_w && !(p.tiled && p.dw.splits == 1 && n_rows > 0);
+  const int32_t splits = n_rows > 0 ? p.dw.splits : 0;
+  const bool join_w = want_w && (splits != 1 || p.packed);
   if (join_w || want_b) {
     KernelTimer timer_("gated_join", st);
     JoinArgs j{};
@@ -991,9 +976,9 @@ extern "C" int ngt_gated_bwd(const void* dy, const void* keep, const void* x, co
     j.dw[0] = g.dw_gate, j.dw[1] = g.dw_up, j.db[0] = g.db_gate, j.db[1] = g.db_up;
     j.dw_f32[0] = g.dw_gate_dtype == NGT_F32, j.dw_f32[1] = g.dw_up_dtype == NGT_F32;
     j.db_f32[0] = g.db_gate_dtype == NGT_F32, j.db_f32[1] = g.db_up_dtype == NGT_F32;
-    j.nk = int64_t(n_out) * n_in, j.n = n_out, j.splits = splits;
+    j.nk = int64_t(n_out) * n_in, j.n = n_out, j.k = n_in, j.splits = splits;
     j.chunks = static_cast<int32_t>(p.chunks);
-    j.blocks_w = join_w ? static_cast<int32_t>((2 * j.nk + 1023) / 1024) : 0;
+    j.blocks_w = join_w ? static_cast<int32_t>((2 * int64_t(n_out) * products.K + 1023) / 1024) : 0;
     const int blocks_b = want_b ? (2 * n_out + 31) / 32 : 0;
     hipLaunchKernelGGL(k_gated_join, dim3(unsigned(j.blocks_w + blocks_b)), dim3(256), 0, st, j);
     NGT_HIP_CHECK(hipGetLastError());

@@ -165,7 +165,7 @@ __global__ __launch_bounds__(256, 1) void k_gated_bwd(BwdArgs args) {
           }
         }
       };
-      const bool parts = args.shape.splits > 1;
+      const bool parts = args.shape.splits > 1 || g.parts;
       if constexpr (MODE == kDx) {
         if (m < g.M) put(parts ? static_cast<void*>(g.part) : g.dx, parts ? at.split * g.M + m : m, parts);
       } else {

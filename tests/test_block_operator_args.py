@@ -75,7 +75,8 @@ def test_gated_refusals_touch_no_gpu():
                       (dict(act=-1), 1), (dict(x=None), 1), (dict(wg=None), 1), (dict(wu=None), 1),
                       (dict(y=None), 1), (dict(xs=7), 1), (dict(keep=P + 8), 1),
                       (dict(rows=(1 << 30) + 1), 2), (dict(rows=1 << 30, n_out=1 << 12), 2),
-                      (dict(n_out=(1 << 29) + 1), 2)):
+                      (dict(n_out=(1 << 29) + 1), 2), (dict(n_out=1 << 20), 2),
+                      (dict(xs=1 << 21, n_in=1 << 21), 2)):
         assert fwd(**bad) == code, bad
         assert b"ngt_gated_fwd" in lib.ngt_last_error()
     assert fwd(rows=0, x=None, y=None) == 0

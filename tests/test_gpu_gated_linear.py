@@ -118,7 +118,9 @@ def test_tiles(dev, M, N, K, act, bias):
 
 
 @pytest.mark.parametrize("M,N,K", [(512, 72, 136), (513, 264, 520), (600, 8, 8), (5000, 136, 264),
-                                   (511, 264, 520), (70000, 40, 24), (777, 1000, 1288)])
+                                   (511, 264, 520), (70000, 40, 24), (777, 1000, 1288),
+                                   (3001, 513, 264), (2000, 264, 1031), (1025, 769, 769), (70001, 41, 23),
+                                   (900, 1001, 3), (64, 7, 2049)])
 def test_gradients_of_whole_pieces_with_edges(dev, M, N, K):
     _case(dev, M, N, K, "silu", seed=M)
 
