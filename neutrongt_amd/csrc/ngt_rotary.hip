@@ -184,15 +184,6 @@ __global__ __launch_bounds__(kThreads, BWD ? bwd_blocks(V * sizeof(T), sizeof(T)
   for (int tile = block / r.splits; tile < r.tiles; tile += per_round) {
     const int64_t row0 = int64_t(tile) * r.tile_rows;
     const int rows = a.n_rows - row0 < r.tile_rows ? int(a.n_rows - row0) : r.tile_rows;
-    __syncthreads();
-    for (int e = tid; e < rows * pairs; e += kThreads) {
-      const int row = e / pairs;
-      const double p = a.pos64 ? static_cast<double>(static_cast<const int64_t*>(a.positions)[row0 + row])
-                               : static_cast<double>(static_cast<const int32_t*>(a.positions)[row0 + row]);
-      const float2 cs = cos_sin(p * a.turns[e - row * pairs]);
-      table[e] = make_float2(cs.x * a.by_cos, cs.y * a.by_sin);
-    }
-    __syncthreads();
     const int items = rows * r.n_heads, step = groups * r.splits;
     // (below 2^17, so the quotient, half an item off the next whole number, is exact)
     auto row_of = [&](int item) { return static_cast<int>((item + 0.5f) * by_heads); };
@@ -214,9 +205,18 @@ __global__ __launch_bounds__(kThreads, BWD ? bwd_blocks(V * sizeof(T), sizeof(T)
         }
       return h;
     };
-    // the next head is on its way while one is computed
+    // the next head is on its way while one is computed, the first one while the cosines are
     int item = slot * groups + group;
     Head next = fetch(item);
+    __syncthreads();
+    for (int e = tid; e < rows * pairs; e += kThreads) {
+      const int row = e / pairs;
+      const double p = a.pos64 ? static_cast<double>(static_cast<const int64_t*>(a.positions)[row0 + row])
+                               : static_cast<double>(static_cast<const int32_t*>(a.positions)[row0 + row]);
+      const float2 cs = cos_sin(p * a.turns[e - row * pairs]);
+      table[e] = make_float2(cs.x * a.by_cos, cs.y * a.by_sin);
+    }
+    __syncthreads();
     for (; item < items; item += step) {
       const Head now = next;
       next = fetch(item + step);
