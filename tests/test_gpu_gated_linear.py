@@ -198,6 +198,22 @@ def test_no_rows(dev, act):
     assert y.shape == (0, 8) and dx.shape == (0, 16) and not any(g.any() for g in gs)
 
 
+@pytest.mark.parametrize("N", [32768, 32767])
+def test_offsets_behind_2_to_the_31(dev, N):
+    """70,000 rows: the last rows' results, and the last outputs' weights' gradients."""
+    M, K = 70000, 16
+    x, (_, wg, wu, *_) = _inputs(M, 1, K, False, 1)[0], _inputs(1, N, K, False, 2)
+    g = torch.Generator(device=dev).manual_seed(2)
+    gy = torch.randn(M, N, dtype=BF16, device=dev, generator=g)
+    leaves = [t.to(dev).requires_grad_() for t in (x, wg, wu)]
+    y = gated_linear(*leaves)
+    dx, dg, du = torch.autograd.grad(y, leaves, gy)
+    ref = _ref(x[-3:], wg, wu, None, None, gy[-3:].cpu(), "silu")
+    _check([y[-3:].detach(), dx[-3:]], ref[:2], "last rows")
+    ref = _ref(x, wg[-2:], wu[-2:], None, None, gy[:, -2:].cpu(), "silu")
+    _check([dg[-2:], du[-2:]], ref[2:4], "last outputs")
+
+
 def test_only_some_gradients_and_one_bias(dev):
     x, wg, wu, bg, bu, gy = (t.to(dev) for t in _inputs(40, 24, 32, True, 6))
     leaves = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
