@@ -273,8 +273,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_gated_few(GatedArgs a) {
   constexpr int kTiles = 2 * NT * MT;
   __shared__ __align__(16) float red[WAVES][kTiles][16][20];  // [x row][output], padded
   const int lane = tid_x() & 63, wave = packed::wave_id(), quad = lane >> 4, l16 = lane & 15;
-  const int blocks = (a.N + 16 * NT - 1) / (16 * NT), split = wg_x() / blocks;
-  const int n0 = (wg_x() - split * blocks) * 16 * NT;
+  const int split = __builtin_amdgcn_workgroup_id_y(), n0 = wg_x() * 16 * NT;
   const int first = split * a.per_split, end = min(first + a.per_split, a.K);
   f32x4 acc[2][NT][MT];
 #pragma unroll
@@ -300,7 +299,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_gated_few(GatedArgs a) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int c = k + 32 * h + 8 * quad;
-      const bool there = c < a.K;
+      const bool there = c < end;
       auto read = [&](const uint16_t* row) {
         return there ? *reinterpret_cast<const u32x4*>(row + c) : u32x4{0u, 0u, 0u, 0u};
       };
@@ -713,7 +712,7 @@ BwdPlan plan_bwd(int64_t M, int32_t N, int32_t K) {
 // are written and read again (about 4 TB/s), so the best number is a square root, as in the
 // backward; none below 4 stages of 64 each, nor where it saves less than the second launch and a
 // block's start and end again, 8 us.  us, one split / several: 1,024 outputs of 4,096 at 64 rows 27 /
-// 22, at 65 43 / 19, at 1,200 48 / 43; 64 of 8,192 at 1 row 21 / 13, at 300 78 / 19; 255 of 8,191 at 65
+// 17, at 65 43 / 19, at 1,200 48 / 43; 64 of 8,192 at 1 row 21 / 13, at 300 78 / 19; 255 of 8,191 at 65
 // 118 / 26.
 struct Split {
   int32_t splits, per_split;
@@ -842,10 +841,10 @@ extern "C" int ngt_gated_fwd(const void* x, int64_t x_stride, const void* w_gate
       const int blocks = (n_out + 15) / 16;
       if (blocks >= 512)
         hipLaunchKernelGGL((k_gated_few<MT, 2, MT < 3 ? 8 : 4>),
-                           dim3(unsigned((n_out + 31) / 32) * a.splits), dim3(MT < 3 ? 512 : 256), 0,
+                           dim3(unsigned((n_out + 31) / 32), a.splits), dim3(MT < 3 ? 512 : 256), 0,
                            st, a);
       else
-        hipLaunchKernelGGL((k_gated_few<MT, 1, 8>), dim3(unsigned(blocks) * a.splits), dim3(512), 0, st,
+        hipLaunchKernelGGL((k_gated_few<MT, 1, 8>), dim3(unsigned(blocks), a.splits), dim3(512), 0, st,
                            a);
     };
     if (n_rows <= 16) run(std::integral_constant<int, 1>{});

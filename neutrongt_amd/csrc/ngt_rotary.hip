@@ -14,8 +14,8 @@
 // formed once for all heads of a row, in LDS: the angle in fp64 turns, of which only the
 // part behind the quarter turn enters the fp32 functions, so that a far position
 // costs no precision.
-// bf16: 12,289 rows of 32 + 8 heads of 128 48 us, 5.3 TB/s; 32,768 rows of 32 + 32 heads of 24
-// 40 forward, 5.0 TB/s, and 67 backward, 4.5 TB/s (its sums take the registers of two
+// bf16: 12,289 rows of 32 + 8 heads of 128 47 us, 5.4 TB/s; 32,768 rows of 32 + 32 heads of 24
+// 40 forward, 5.0 TB/s, and 64 backward, 4.7 TB/s (its sums take the registers of two
 // of the eight waves that the forward has on a SIMD).
 #include "ngt_common.h"
 
