@@ -263,7 +263,8 @@ def test_special_values_stay_in_their_row_and_column(dev):
         assert torch.equal(got.nan_to_num(1.0, 2.0, 3.0) + 0, want.nan_to_num(1.0, 2.0, 3.0) + 0)
 
 
-@pytest.mark.parametrize("M,N,K", [(3000, 640, 256), (20, 640, 256), (70, 61, 33)])
+@pytest.mark.parametrize("M,N,K", [(3000, 640, 256), (20, 640, 256), (70, 61, 33), (40, 64, 4096),
+                                   (100, 33, 2049), (600, 513, 520)])
 def test_the_same_bits_every_time_on_another_stream_and_captured(dev, M, N, K):
     x, wg, wu, bg, bu, gy = (t.to(dev) for t in _inputs(M, N, K, True, 7))
     leaves = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
