@@ -873,7 +873,7 @@ int ngt_norm_rotary_bwd(int dtype, const ngt_head_rows* q, const ngt_head_rows* 
  * The 2-norm over many gradients, and the gradients scaled by min(1, max_norm / norm).
  * tensors: host array of n_tensors; elements are of dtype (NGT_F32 or NGT_BF16), in
  * one run of memory each, aligned to their type.  Sums are fp64 in a fixed order; *norm (device)
- * is the fp32 norm.  A norm that is not finite scales nothing.  A tensor's result goes
+ * is the fp32 norm.  A *norm that is not finite (so also one above fp32's range) scales nothing.  A tensor's result goes
  * to out (in out_dtype) or, where out is null, back to x, whose memory is left alone
  * where the factor is 1.  max_norm < 0: the norm alone.
  * No two results may overlap, nor a result another tensor's x.  workspace: 16-byte

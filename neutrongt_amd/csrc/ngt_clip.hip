@@ -140,9 +140,9 @@ __global__ __launch_bounds__(kThreads) void k_squares(const TableIn t, double* _
   if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
 
-// What the gradients are scaled by.
+// What the gradients are scaled by: 1 where the norm, as the caller gets it, is not finite.
 __device__ __forceinline__ float factor_of(double norm, double max_norm) {
-  return norm < INFINITY && norm > max_norm ? static_cast<float>(max_norm / norm) : 1.f;
+  return static_cast<float>(norm) < INFINITY && norm > max_norm ? static_cast<float>(max_norm / norm) : 1.f;
 }
 
 // The norm and the factor, of more parts than k_scale adds by itself or of a norm alone.

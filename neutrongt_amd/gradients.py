@@ -108,8 +108,9 @@ def clip_gradients(parameters, max_norm: float, out=None) -> torch.Tensor:
     one run of memory.  ``out``: tensors that take the scaled gradients instead, one
     for each gradient, of its shape and strides, fp32 or bf16 (e.g. fp32 gradients of
     bf16 ones for the optimizer).  The norm is summed in fp64 in a fixed order.  Where
-    it is not finite (a gradient holds a NaN or an infinity) nothing is scaled, and
-    where it is at most max_norm the gradients' memory is left alone."""
+    the one returned is not finite (a gradient holds a NaN or an infinity, or the norm is
+    above fp32's range) nothing is scaled, and where it is at most max_norm the gradients'
+    memory is left alone."""
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")

@@ -1,0 +1,31 @@
+"""clip_gradients where its norm or its factor leaves fp32's range, and where its
+partial sums are more than one kernel adds by itself, against float64
+(tests/test_gpu_clip_gradients.py derives the bounds)."""
+import math
+
+import pytest
+import torch
+
+from neutrongt_amd import clip_gradients, gradient_norm
+from tests.test_gpu_clip_gradients import BF16, F32, U, _check, _norm, _params, node  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("apart", [False, True])
+def test_a_norm_that_fp32_cannot_hold_scales_nothing(dev, node, dtype, apart):
+    """Two gradients of 3e38 have a norm of 4.2e38: returned as an infinity, so nothing is
+    scaled; one of them alone is."""
+    grads = [torch.full((2,), 3e38, dtype=dtype, device=dev), torch.ones(50, device=dev)]
+    before = [t.clone() for t in grads]
+    out = [torch.zeros_like(t) for t in grads] if apart else None
+    assert clip_gradients(_params(grads), 1.0, out=out).item() == math.inf
+    assert all(torch.equal(a, b) for a, b in zip(grads, before))
+    assert not apart or all(torch.equal(a, b) for a, b in zip(out, before))
+    assert gradient_norm(_params(grads)).item() == math.inf
+    grads[0][1] = 0.0
+    before, norm = [t.clone() for t in grads], _norm(grads)
+    got = clip_gradients(_params(grads), 1.0, out=out)
+    assert math.isfinite(got.item()) and abs(got.item() - norm) <= 1.01 * U * norm
+    _check(out or grads, before, 1.0 / norm)
