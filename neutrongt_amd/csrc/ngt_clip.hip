@@ -140,15 +140,28 @@ __global__ __launch_bounds__(kThreads) void k_squares(const TableIn t, double* _
   if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
 
-// What the gradients are scaled by: 1 where the norm, as the caller gets it, is not finite.
-__device__ __forceinline__ float factor_of(double norm, double max_norm) {
-  return static_cast<float>(norm) < INFINITY && norm > max_norm ? static_cast<float>(max_norm / norm) : 1.f;
+// What the gradients are scaled by: `by`, and where that would be below fp32's normal range a
+// power of two more (its numbers there have fewer bits, or are 0).  An element times a `by` of
+// 2^-120 does not overflow, and where it loses bits the result is below 2^-126 too.
+struct Factor {
+  float by;
+  int32_t shift;
+  __device__ __forceinline__ float operator()(float x) const { return ldexpf(x * by, shift); }
+};
+// 1 where the norm, as the caller gets it, is not finite.
+__device__ __forceinline__ Factor factor_of(double norm, double max_norm) {
+  if (!(static_cast<float>(norm) < INFINITY && norm > max_norm)) return {1.f, 0};
+  const double f = max_norm / norm;
+  if (f >= 0x1p-126 || f == 0.0) return {static_cast<float>(f), 0};
+  int e;
+  const double m = frexp(f, &e);
+  return {static_cast<float>(ldexp(m, -120)), e + 120};
 }
 
 // The norm and the factor, of more parts than k_scale adds by itself or of a norm alone.
 __global__ __launch_bounds__(1024) void k_norm(const double* __restrict__ part, int32_t n,
                                                double max_norm, float* __restrict__ norm,
-                                               float* __restrict__ factor) {
+                                               Factor* __restrict__ factor) {
   __shared__ double red[1024 / kWave];
   double s = 0.0;
   for (int i = threadIdx.x; i < n; i += 1024) s += part[i];
@@ -160,7 +173,7 @@ __global__ __launch_bounds__(1024) void k_norm(const double* __restrict__ part, 
 
 template <typename T, typename O>
 __device__ __forceinline__ void scaled(const void* base, void* result, const Part& p, bool wide,
-                                       float by) {
+                                       const Factor& by) {
   const T* x = static_cast<const T*>(base);
   O* o = static_cast<O*>(result);
   int64_t i = p.from;
@@ -168,13 +181,13 @@ __device__ __forceinline__ void scaled(const void* base, void* result, const Par
     i = pieces(x, p.from, p.to, [&](int64_t at, const uint4& w) {
       Piece<T> v = piece_of<T>(w);
 #pragma unroll
-      for (int k = 0; k < Piece<T>::V; ++k) v.v[k] *= by;
+      for (int k = 0; k < Piece<T>::V; ++k) v.v[k] = by(v.v[k]);
       if constexpr (sizeof(T) == 4 && sizeof(O) == 2)
         *reinterpret_cast<uint2*>(o + at) = make_uint2(pack2_bf16(v.v[0], v.v[1]), pack2_bf16(v.v[2], v.v[3]));
       else
         store_row<O, Piece<T>::V>(o + at, v.v);
     });
-  for (i += threadIdx.x; i < p.to; i += kThreads) elem<O>::store(o + i, elem<T>::load(x + i) * by);
+  for (i += threadIdx.x; i < p.to; i += kThreads) elem<O>::store(o + i, by(elem<T>::load(x + i)));
 }
 
 // parts > 0: the factor from so many sums, which all blocks add in the same order (the first
@@ -184,10 +197,10 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void k_scale(const T t, const double* __restrict__ part,
                                                     int32_t parts, double max_norm,
                                                     float* __restrict__ norm,
-                                                    const float* __restrict__ factor) {
+                                                    const Factor* __restrict__ factor) {
   constexpr bool kOut = std::is_same_v<T, TableOut>;
   __shared__ double red[kThreads / kWave];
-  float by;
+  Factor by;
   if (parts > 0) {
     double s = 0.0;
     for (int i = threadIdx.x; i < parts; i += kThreads) s += part[i];
@@ -197,7 +210,7 @@ __global__ __launch_bounds__(kThreads) void k_scale(const T t, const double* __r
   } else {
     by = *factor;
   }
-  if (!kOut && by == 1.f) return;  // left alone
+  if (!kOut && by.by == 1.f) return;  // left alone
   for (int chunk = t.first[t.count] - 1 - blockIdx.x; chunk >= 0; chunk -= gridDim.x) {
     const Part p = part_of(t, chunk);
     const bool wide = t.kind[p.run] & 4;
@@ -334,7 +347,7 @@ extern "C" int ngt_clip_gradients(const ngt_gradient* tensors, int32_t n_tensors
     return set_error(NGT_ERR_WORKSPACE, "%s: workspace %zu < %zu or not 16-byte aligned", fn,
                      workspace_bytes, need);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  float* factor = static_cast<float*>(workspace);
+  auto* factor = static_cast<Factor*>(workspace);
   double* part = reinterpret_cast<double*>(static_cast<char*>(workspace) + 16);
   int32_t done = 0;
   NGT_CHECK_OK((each_launch<kRuns, false>(runs, [&](const TableIn& t, int32_t chunks) -> int {

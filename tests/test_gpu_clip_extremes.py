@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from neutrongt_amd import clip_gradients, gradient_norm
-from tests.test_gpu_clip_gradients import BF16, F32, U, _check, _norm, _params, node  # noqa: F401
+from tests.test_gpu_clip_gradients import BF16, F32, HALF, U, _check, _norm, _params, node  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +29,22 @@ def test_a_norm_that_fp32_cannot_hold_scales_nothing(dev, node, dtype, apart):
     got = clip_gradients(_params(grads), 1.0, out=out)
     assert math.isfinite(got.item()) and abs(got.item() - norm) <= 1.01 * U * norm
     _check(out or grads, before, 1.0 / norm)
+
+
+@pytest.mark.parametrize("dtype,out_dtype", [(F32, None), (BF16, None), (BF16, F32), (F32, BF16)])
+@pytest.mark.parametrize("size,limit", [(1e30, 1e-30), (3e38, 1e-2), (3e38, 3.0), (2e38, 1e-38),
+                                        (1e20, 1e-20), (1e20, 1e-300)])
+def test_a_factor_below_the_range_of_fp32(dev, node, size, limit, dtype, out_dtype):
+    """Besides its roundings a result may be off by what its type's subnormal numbers, 2^-149
+    and 2^-133 apart, lose: two halves of that, of the product and of its shift."""
+    grads = [torch.tensor([size, -size / 3, size * 1e-7, 1.0, 0.0] * 3 + [0.5 * size], dtype=dtype,
+                          device=dev) * 0.25, torch.ones(3, dtype=dtype, device=dev)]
+    before, norm = [t.clone() for t in grads], _norm(grads)
+    out = [torch.full_like(t, 7.0, dtype=out_dtype) for t in grads] if out_dtype else None
+    got = clip_gradients(_params(grads), limit, out=out)
+    assert abs(got.item() - norm) <= 1.01 * U * norm
+    for t, g in zip(out or grads, before):
+        want = g.double().cpu() * (limit / norm)
+        half = HALF[t.dtype]
+        bound = want.abs() * (2.1 * U + half * (1 + 2.1 * U)) + (2.0 ** -149 if t.dtype == F32 else 2.0 ** -133)
+        assert ((t.double().cpu() - want).abs() <= bound).all()
