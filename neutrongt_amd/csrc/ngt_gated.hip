@@ -168,6 +168,10 @@ __global__ __launch_bounds__(256) void k_gated_join_fwd(GatedArgs a) {
   finish8(a, m, (i - m * across) * 8, s[0], s[1]);
 }
 
+// The most blocks of a launch that grows with the matrices' elements, which may be more than the
+// 2^32 threads that a launch stays below: with more to do each block takes several pieces.
+constexpr int64_t kMostBlocks = 1 << 20;
+
 // x, Wg and Wu with their rows filled up to 8s with zeros, one after another (of widths that are
 // no multiple of 8: 2 x 8,193 rows of 2,049 25 us, 5 TB/s).
 struct PackArgs {
@@ -176,30 +180,35 @@ struct PackArgs {
   int64_t x_stride;
   uint16_t* to;
   int32_t k;
+  int32_t blocks;
 };
 __global__ __launch_bounds__(256) void k_gated_pack(PackArgs a) {
   const int across = up8(a.k) / 8, together = across < 256 ? 256 / across : 1;
   const int r = tid_x() / across;
-  int64_t row = int64_t(wg_x()) * together + (across < 256 ? r : 0);
   if (across < 256 && r >= together) return;
-  uint16_t* to = a.to + row * across * 8;
-  int which = 0;
+  const int64_t all = a.rows[0] + a.rows[1] + a.rows[2];
+  for (int64_t at = int64_t(wg_x()) * together + (across < 256 ? r : 0); at < all;
+       at += int64_t(a.blocks) * together) {
+    uint16_t* to = a.to + at * across * 8;
+    int64_t row = at;
+    int which = 0;
 #pragma unroll
-  for (int i = 0; i < 3; ++i)
-    if (which == i && row >= a.rows[i]) row -= a.rows[i], ++which;
-  if (which > 2) return;
-  const uint16_t* from = (which == 0 ? a.from[0] : which == 1 ? a.from[1] : a.from[2]) + row * (which == 0 ? a.x_stride : a.k);
-  for (int c = across < 256 ? tid_x() - r * across : tid_x(); c < across; c += 256)
-    *reinterpret_cast<u32x4*>(to + 8 * c) = load8<false>(from, 8 * c, a.k);
+    for (int i = 0; i < 3; ++i)
+      if (which == i && row >= a.rows[i]) row -= a.rows[i], ++which;
+    const uint16_t* from = (which == 0 ? a.from[0] : which == 1 ? a.from[1] : a.from[2]) + row * (which == 0 ? a.x_stride : a.k);
+    for (int c = across < 256 ? tid_x() - r * across : tid_x(); c < across; c += 256)
+      *reinterpret_cast<u32x4*>(to + 8 * c) = load8<false>(from, 8 * c, a.k);
+  }
 }
 // What of it in its workspace is what.
 struct Packed {
   const uint16_t *x, *wg, *wu;
 };
-int launch_pack(const PackArgs& a, hipStream_t st, Packed* to) {
+int launch_pack(PackArgs a, hipStream_t st, Packed* to) {
   const int across = up8(a.k) / 8, together = across < 256 ? 256 / across : 1;
   const int64_t rows = a.rows[0] + a.rows[1] + a.rows[2];
-  hipLaunchKernelGGL(k_gated_pack, dim3(unsigned((rows + together - 1) / together)), dim3(256), 0, st, a);
+  a.blocks = static_cast<int32_t>(std::min((rows + together - 1) / together, kMostBlocks));
+  hipLaunchKernelGGL(k_gated_pack, dim3(unsigned(a.blocks)), dim3(256), 0, st, a);
   NGT_HIP_CHECK(hipGetLastError());
   to->x = a.to, to->wg = a.to + a.rows[0] * up8(a.k), to->wu = to->wg + a.rows[1] * up8(a.k);
   return NGT_OK;
@@ -824,7 +833,7 @@ extern "C" int ngt_gated_fwd(const void* x, int64_t x_stride, const void* w_gate
                               {n_rows, n_out, n_out},
                               x_stride,
                               reinterpret_cast<uint16_t*>(static_cast<char*>(workspace) + p.pack),
-                              n_in},
+                              n_in, 0},
                              st, &to));
     a.x = to.x, a.wg = to.wg, a.wu = to.wu, a.K = up8(n_in), a.x_stride = a.K;
   }
@@ -939,7 +948,7 @@ extern "C" int ngt_gated_bwd(const void* dy, const void* keep, const void* x, co
                               {want_w ? n_rows : 0, g.dx ? n_out : 0, g.dx ? n_out : 0},
                               n_in,
                               reinterpret_cast<uint16_t*>(ws + p.pack),
-                              n_in},
+                              n_in, 0},
                              st, &to));
     products.x = to.x, products.wg = to.wg, products.wu = to.wu;
   }
