@@ -462,33 +462,34 @@ __global__ __launch_bounds__(256) void k_gated_join(JoinArgs a) {
   __shared__ float red[8][32];
   if (wg_x() < a.blocks_w) {
     const int pitch = up8(a.k);
-    const int64_t at = (int64_t(wg_x()) * 256 + tid_x()) * 4, all = 2 * int64_t(a.n) * pitch;
-    if (at >= all) return;
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    const int64_t all = 2 * int64_t(a.n) * pitch;
+    for (int64_t at = (int64_t(wg_x()) * 256 + tid_x()) * 4; at < all; at += int64_t(a.blocks_w) * 1024) {
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int c = 0; c < a.splits; ++c) {
-      const float4 v = *reinterpret_cast<const float4*>(a.part + c * all + at);
-      s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
-    }
-    // the element of the weights, and how many of the four there are
-    int64_t i = at;
-    int there = 4;
-    if (pitch != a.k) {
-      const int64_t row = at / pitch;
-      const int c = static_cast<int>(at - row * pitch);
-      i = row * a.k + c, there = min(a.k - c, 4);
-    }
+      for (int c = 0; c < a.splits; ++c) {
+        const float4 v = *reinterpret_cast<const float4*>(a.part + c * all + at);
+        s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
+      }
+      // the element of the weights, and how many of the four there are
+      int64_t i = at;
+      int there = 4;
+      if (pitch != a.k) {
+        const int64_t row = at / pitch;
+        const int c = static_cast<int>(at - row * pitch);
+        i = row * a.k + c, there = min(a.k - c, 4);
+      }
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      if (!a.dw[w]) continue;
-      const int64_t o = i - w * a.nk;
-      const bool f32 = a.dw_f32[w];
-      if (pitch == a.k && o >= 0 && o + 4 <= a.nk) {
-        if (f32) *reinterpret_cast<float4*>(static_cast<float*>(a.dw[w]) + o) = make_float4(s[0], s[1], s[2], s[3]);
-        else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.dw[w]) + o) = make_uint2(pack2_bf16(s[0], s[1]), pack2_bf16(s[2], s[3]));
-      } else {
-        for (int t = 0; t < there; ++t)
-          if (o + t >= 0 && o + t < a.nk) put(a.dw[w], o + t, f32, s[t]);
+      for (int w = 0; w < 2; ++w) {
+        if (!a.dw[w]) continue;
+        const int64_t o = i - w * a.nk;
+        const bool f32 = a.dw_f32[w];
+        if (pitch == a.k && o >= 0 && o + 4 <= a.nk) {
+          if (f32) *reinterpret_cast<float4*>(static_cast<float*>(a.dw[w]) + o) = make_float4(s[0], s[1], s[2], s[3]);
+          else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.dw[w]) + o) = make_uint2(pack2_bf16(s[0], s[1]), pack2_bf16(s[2], s[3]));
+        } else {
+          for (int t = 0; t < there; ++t)
+            if (o + t >= 0 && o + t < a.nk) put(a.dw[w], o + t, f32, s[t]);
+        }
       }
     }
     return;
@@ -986,7 +987,7 @@ extern "C" int ngt_gated_bwd(const void* dy, const void* keep, const void* x, co
     j.db_f32[0] = g.db_gate_dtype == NGT_F32, j.db_f32[1] = g.db_up_dtype == NGT_F32;
     j.nk = int64_t(n_out) * n_in, j.n = n_out, j.k = n_in, j.splits = splits;
     j.chunks = static_cast<int32_t>(p.chunks);
-    j.blocks_w = join_w ? static_cast<int32_t>((2 * int64_t(n_out) * products.K + 1023) / 1024) : 0;
+    j.blocks_w = join_w ? static_cast<int32_t>(std::min((2 * int64_t(n_out) * products.K + 1023) / 1024, kMostBlocks)) : 0;
     const int blocks_b = want_b ? (2 * n_out + 31) / 32 : 0;
     hipLaunchKernelGGL(k_gated_join, dim3(unsigned(j.blocks_w + blocks_b)), dim3(256), 0, st, j);
     NGT_HIP_CHECK(hipGetLastError());

@@ -50,3 +50,35 @@ def test_as_many_filled_up_rows_as_a_launch_has_blocks_at_most(dev):
     assert _others_are_zero(y, at)
     del x, y
     torch.cuda.empty_cache()
+
+
+def test_weights_of_more_sums_than_a_launch_has_threads(dev):
+    """The join of two weights of 2^33 elements, 4 a thread, would be 2^32 threads.  No rows:
+    all of the gradient is written as zeros."""
+    N, K = 1 << 16, 1 << 17
+    w = torch.empty(N, K, dtype=BF16, device=dev).requires_grad_()
+    x = torch.empty(0, K, dtype=BF16, device=dev)
+    filler = torch.full((N, K), 3.0, dtype=BF16, device=dev)
+    del filler  # the gradient's memory, most likely, holds something
+    y = gated_linear(x, w, w.detach())
+    dw, = torch.autograd.grad(y, w, torch.empty_like(y))
+    assert dw.shape == (N, K) and not any(bool(c.any()) for c in dw.split(1 << 12))
+    del dw, w, x, y
+    torch.cuda.empty_cache()
+
+
+def test_weights_whose_joined_sums_share_blocks(dev):
+    """2 x 66,000 x 8,193 sums of odd rows, 1,024 a block, are more than 2^20 blocks."""
+    M, N, K = 3, 66000, 8193
+    x, wg, wu, _, _, gy = _inputs(M, 1, K, False, 5)
+    gy = torch.randn(M, N, generator=torch.Generator().manual_seed(6)).to(BF16)
+    g = torch.Generator(device=dev).manual_seed(7)
+    wg, wu = (torch.randn(N, K, device=dev, dtype=BF16, generator=g).mul_(K ** -0.5).requires_grad_()
+              for _ in range(2))
+    dg, du = torch.autograd.grad(gated_linear(x.to(dev), wg, wu), (wg, wu), gy.to(dev))
+    with torch.device(dev):  # the reference on the GPU, for its size
+        ref = _ref(x.to(dev), wg.detach(), wu.detach(), None, None, gy.to(dev), "silu")
+    for got, (want, bound) in zip((dg, du), ref[2:4]):
+        assert ((got.double() - want).abs() <= bound).all()
+    del ref, want, bound
+    torch.cuda.empty_cache()
