@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define NGT_ABI_VERSION 14
+#define NGT_ABI_VERSION 15
 
 #define NGT_F32 0
 #define NGT_BF16 1
@@ -821,6 +821,10 @@ int ngt_gated_fwd(const void* x, int64_t x_stride, const void* w_gate, const voi
                   int32_t activation, void* y, void* keep, void* workspace, size_t workspace_bytes,
                   void* stream);
 int ngt_gated_bwd_workspace_bytes(int64_t n_rows, int32_t n_out, int32_t n_in, size_t* bytes);
+/* How the backward's products are cut: the columns of a block's tile (128, 192 or 256) and the
+ * parts of the contraction, of dx and then of the weights' gradients. */
+int ngt_gated_bwd_tiles(int64_t n_rows, int32_t n_out, int32_t n_in, int32_t columns[2],
+                        int32_t splits[2]);
 int ngt_gated_bwd(const void* dy, const void* keep, const void* x, const void* w_gate,
                   const void* w_up, int64_t n_rows, int32_t n_out, int32_t n_in,
                   const ngt_gated_grads* grads, void* workspace, size_t workspace_bytes,

@@ -13,7 +13,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libngt_attn.so"
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 NGT_F32 = 0
 NGT_BF16 = 1
@@ -241,6 +241,7 @@ SIGNATURES = {
     "ngt_gated_fwd_workspace_bytes": [_i64, _i32, _i32, _psz],
     "ngt_gated_fwd": [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _sz, _vp],
     "ngt_gated_bwd_workspace_bytes": [_i64, _i32, _i32, _psz],
+    "ngt_gated_bwd_tiles": [_i64, _i32, _i32, _pi32, _pi32],
     "ngt_gated_bwd": [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _pgg, _vp, _sz, _vp],
     "ngt_norm_rotary_fwd": [_i32, _phr, _phr, _i64, _i32, _prot, _f32, _vp],
     "ngt_norm_rotary_bwd_workspace_bytes": [_i64, _i32, _psz],

@@ -902,6 +902,17 @@ extern "C" int ngt_gated_bwd_workspace_bytes(int64_t n_rows, int32_t n_out, int3
   return NGT_OK;
 }
 
+extern "C" int ngt_gated_bwd_tiles(int64_t n_rows, int32_t n_out, int32_t n_in, int32_t columns[2],
+                                   int32_t splits[2]) {
+  const char* fn = "ngt_gated_bwd_tiles";
+  NGT_CHECK_OK(check_sizes(fn, n_rows, n_out, n_in));
+  if (!columns || !splits) return set_error(NGT_ERR_ARG, "%s: null columns or splits", fn);
+  const BwdPlan p = plan_bwd(n_rows, n_out, n_in);
+  columns[0] = 64 * p.dx.fn, splits[0] = p.dx.splits;
+  columns[1] = 64 * p.dw.fn, splits[1] = p.dw.splits;
+  return NGT_OK;
+}
+
 extern "C" int ngt_gated_bwd(const void* dy, const void* keep, const void* x, const void* w_gate,
                              const void* w_up, int64_t n_rows, int32_t n_out, int32_t n_in,
                              const ngt_gated_grads* grads, void* workspace, size_t workspace_bytes,
