@@ -48,3 +48,62 @@ def test_a_factor_below_the_range_of_fp32(dev, node, size, limit, dtype, out_dty
         half = HALF[t.dtype]
         bound = want.abs() * (2.1 * U + half * (1 + 2.1 * U)) + (2.0 ** -149 if t.dtype == F32 else 2.0 ** -133)
         assert ((t.double().cpu() - want).abs() <= bound).all()
+
+
+def _apart(dev, count, size, dtype, seed):
+    """Gradients in memory of their own each, as autograd makes them, all of other sizes."""
+    g = torch.Generator(device=dev).manual_seed(seed)
+    return [torch.randn(size + i % 3, device=dev, generator=g).to(dtype) for i in range(count)]
+
+
+# one sum each of 2,500 tensors; 3,200 sums of two launches of 2,000 and 1,200 blocks
+@pytest.mark.parametrize("dtype,out_dtype", [(F32, None), (BF16, None), (BF16, F32), (F32, BF16)])
+@pytest.mark.parametrize("count,size", [(2500, 1), (400, 60000)])
+def test_more_sums_than_a_block_adds(dev, node, count, size, dtype, out_dtype):
+    grads = _apart(dev, count, size, dtype, count)
+    before, norm, ps = [t.clone() for t in grads], _norm(grads), _params(grads)
+    assert abs(gradient_norm(ps).item() - norm) <= 1.01 * U * norm
+    out = [torch.empty_like(t, dtype=out_dtype) for t in grads] if out_dtype else None
+    for limit in (2 * norm, 0.25 * norm):
+        got = clip_gradients(ps, limit, out=out)
+        assert abs(got.item() - norm) <= 1.01 * U * norm
+        _check(out or grads, before, min(1.0, limit / norm))
+        if out or limit > norm:
+            assert all(torch.equal(a, b) for a, b in zip(grads, before))
+    for bad in (math.nan, math.inf):
+        for t, b in zip(grads, before):
+            t.copy_(b)
+        grads[count // 2][0] = bad
+        assert not math.isfinite(clip_gradients(ps, 0.5, out=out).item())
+        for t, b in zip(out or grads, before):
+            if t is not (out or grads)[count // 2]:
+                assert torch.equal(t, b.to(t.dtype))
+
+
+def test_more_sums_than_a_block_adds_captured(dev, node):
+    grads = _apart(dev, 2300, 5, F32, 1)
+    ps = _params(grads)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = clip_gradients(ps, 1.0)
+    for i in range(3):
+        for t in grads:
+            t.normal_().mul_(i + 1)
+        before, want = [t.clone() for t in grads], _norm(grads)
+        other = clip_gradients(_params([t.clone() for t in grads]), 1.0)  # eager work between
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(norm, other) and abs(norm.item() - want) <= 1.01 * U * want
+        _check(grads, before, 1 / want)
+
+
+@pytest.mark.parametrize("count", [10, 2500])
+def test_some_results_in_their_gradients_memory(dev, node, count):
+    grads = _apart(dev, count, 9, F32, count)
+    before, norm = [t.clone() for t in grads], _norm(grads)
+    out = [t if i % 2 else torch.empty_like(t, dtype=BF16) for i, t in enumerate(grads)]
+    for limit in (2 * norm, 0.5 * norm):
+        got = clip_gradients(_params(grads), limit, out=out)
+        assert abs(got.item() - norm) <= 1.01 * U * norm
+        _check(out, before, min(1.0, limit / norm))
+    assert all(torch.equal(a, b) for a, b in zip(grads[::2], before[::2]))
