@@ -797,7 +797,8 @@ int ngt_wgrad_bf16(const void* x, const void* dy, int64_t n_rows, int32_t n_out,
  * (nullable), summed in fp32 and rounded once; any alignment, n_out below 2^20, n_in 2^21.
  * keep, where not null, receives what the backward needs (zu act'(zg) and act(zg), each to
  * 12 bits of mantissa): ngt_gated_keep_bytes, 16-byte aligned.  workspace: 16-byte aligned,
- * ngt_gated_fwd_workspace_bytes (0: none).
+ * ngt_gated_fwd_workspace_bytes (0: none; few blocks that share a long contraction need one, and
+ * many n_in that are no multiple of 8).
  * ngt_gated_bwd: from dy, what was kept and x (dy and x contiguous) the gradients that are not
  * null: dx [n_rows, n_in] bf16, and those of weights and biases in their own types, from
  * fp32 sums in a fixed order.  All matrices and the workspace are 16-byte aligned.

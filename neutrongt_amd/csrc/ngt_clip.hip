@@ -7,7 +7,10 @@
 // number of elements that does not depend on how they are cut.
 // us of norm and scaling, by rocprofv3: 42.6 M fp32 (170 MB, 198 tensors) into fp32 28 + 57, 6.0
 // TB/s with what the last-level cache keeps; 303 M bf16 (606 MB) into fp32 153 + 370, 4.0 and 4.9
-// TB/s; 66 M fp32 below the limit 41 + 5; the slim preset's 70 tensors 4 + 4.
+// TB/s; 66 M fp32 below the limit 41 + 5; the slim preset's 70 tensors 4 + 4.  With the library's
+// timer, which adds 2 to 3 us a launch, the 42.6 M in place 29 + 56, in 198 allocations 30 + 57;
+// into results that lie apart 31 + 60, and 49 + 68 where one element before them leaves no run aligned
+// to 16 bytes: such a run goes element by element.
 #include "ngt_common.h"
 
 #include <new>

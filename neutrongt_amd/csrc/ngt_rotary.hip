@@ -31,6 +31,11 @@ constexpr int kTableBytes = 16384;  // cosines and sines of a block's rows
 // Blocks of a backward that a CU holds, by the registers of its sums, for pieces of `bytes`; a
 // launch has about as many, each with a partial sum (bf16, 32,768 rows of 32 + 32 heads of 24:
 // 1,024 blocks 76 us, 1,280 71, 1,536 67; 12,289 of 32 + 8 of 128: 768 86 us, 1,024 85, 1,280 90).
+// The heads of 24 were measured with interleaved pairs.  In halves the kernel of 8-byte pieces of
+// bf16 needs 4 registers more than six blocks leave it; it keeps them in scratch memory, two of
+// them read once a head (32 + 32 heads of 24 68 us for 63, 16 + 16 of 40 67 for 65, both with the
+// library's timer).  fp32 with a norm, five blocks: 16 + 16 heads of 24 62 us, 4.9 TB/s; of 64 167,
+// 4.8 TB/s.
 constexpr int bwd_blocks(int bytes, int es) { return bytes <= 8 ? 6 : es == 2 ? 4 : 5; }
 constexpr int kBwdBlocks = 6 * 256;
 inline size_t sums_bytes(int32_t d) { return size_t(kBwdBlocks + 2) * d * sizeof(float); }

@@ -477,7 +477,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     gated feed-forward block (linear_epilogue is the second): x [..., n_in], weights
     [n_out, n_in] and biases [n_out] as two nn.Linear hold them, or the halves of a
     joint one; activation "silu" (z / (1 + e^-z)), "gelu" (the erf form), "relu" or None.
-    fp32 inputs are rounded to bf16 as autocast does; the sums, the activation and the
+    fp32 inputs are rounded to bf16 at each call, as autocast does; the sums, the activation and the
     product are fp32 and the result is rounded once.  The gradients have the inputs'
     types; those of weights and biases are fp32 sums in a fixed order.
     Differentiable once."""
