@@ -541,8 +541,8 @@ __global__ __launch_bounds__(256) void k_gated_join_dx(const float* __restrict__
 // 185 (its products and LDS reads alone 146, its loads alone 111), the rest arithmetic and 470 MB
 // of stores, which the loops of other blocks do not hide.  Measured at the first size: 256 rows
 // by 128 outputs in 8 waves with two buffers 175 us, 192 by 64 in two blocks with two buffers 168.
-// At FM = 4 the loop takes all 256 registers that two blocks leave a lane: 4 or 5 of the results'
-// addresses wait in scratch memory, written before the loop and read once after it.
+// At FM = 4 the loop takes all 256 registers that two blocks leave a lane: 4 or 5 that the results
+// need wait in scratch memory, written before the loop and read once after it.
 template <int FM, bool WHOLE>
 __global__ __launch_bounds__(256, 2) void k_gated(GatedArgs a) {
   constexpr int BM = 64 * FM, kRowsBytes = BM * 128;
